@@ -64,6 +64,65 @@ class Params(ctypes.Structure):
     ]
 
 
+i64 = ctypes.c_int64
+FHE_F32, FHE_BF16, FHE_F16 = 0, 1, 2
+
+
+class SsmScanArgs(ctypes.Structure):
+    _fields_ = [
+        ("device", i32), ("dtype", i32),
+        ("batch", u32), ("length", u32), ("heads", u32), ("head_dim", u32), ("d_state", u32), ("groups", u32),
+        ("x", vp), ("x_stride", i64 * 3),
+        ("write", vp), ("write_stride", i64 * 3),
+        ("log_decay", vp), ("log_decay_stride", i64 * 3),
+        ("b", vp), ("b_stride", i64 * 3),
+        ("c", vp), ("c_stride", i64 * 3),
+        ("d", vp), ("initial_state", vp), ("lengths", vp), ("y", vp), ("final_state", vp),
+        ("workspace", vp), ("workspace_bytes", u64), ("stream", vp),
+    ]
+
+
+class SsmScanGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("f", SsmScanArgs),
+        ("dy", vp), ("dfinal", vp), ("dx", vp), ("dwrite", vp), ("dlog_decay", vp), ("db", vp), ("dc", vp),
+        ("dd", vp), ("dinitial", vp), ("workspace", vp), ("workspace_bytes", u64), ("stream", vp),
+    ]
+
+
+class CausalConvArgs(ctypes.Structure):
+    _fields_ = [
+        ("device", i32), ("dtype", i32),
+        ("batch", u32), ("length", u32), ("channels", u32), ("taps", u32), ("silu", i32), ("reserved", u32),
+        ("x", vp), ("x_stride", i64 * 2),
+        ("weight", vp), ("bias", vp), ("initial_state", vp), ("lengths", vp), ("y", vp), ("final_state", vp),
+        ("stream", vp),
+    ]
+
+
+class CausalConvGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("f", CausalConvArgs),
+        ("dy", vp), ("dfinal", vp), ("dx", vp), ("dweight", vp), ("dbias", vp), ("dinitial", vp),
+        ("workspace", vp), ("workspace_bytes", u64), ("stream", vp),
+    ]
+
+
+class TokenLogprobsArgs(ctypes.Structure):
+    _fields_ = [
+        ("device", i32), ("dtype", i32), ("rows", u32), ("vocab", u32), ("top_k", u32), ("reserved", u32),
+        ("logits", vp), ("logits_stride", i64), ("targets", vp), ("logprob", vp), ("entropy", vp),
+        ("top_logprobs", vp), ("top_ids", vp), ("lse", vp), ("stream", vp),
+    ]
+
+
+class TokenLogprobsGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("f", TokenLogprobsArgs),
+        ("dlogprob", vp), ("dentropy", vp), ("dtop_logprobs", vp), ("dlogits", vp), ("stream", vp),
+    ]
+
+
 # name -> (argtypes); all return int status.
 SIGNATURES = {
     "fhe_last_error": [ctypes.c_char_p, ctypes.c_size_t],
@@ -158,6 +217,16 @@ SIGNATURES = {
     "fhe_mul_i": [vp, vp, ctypes.POINTER(vp)],
     "fhe_ct_set_scale": [vp, vp, f64],
     "fhe_chebyshev": [vp, vp, PD, u32, f64, f64, ctypes.POINTER(vp)],
+    # plaintext Mamba-2 operators
+    "fhe_ssm_scan_workspace": [ctypes.POINTER(SsmScanArgs), P64],
+    "fhe_ssm_scan": [ctypes.POINTER(SsmScanArgs)],
+    "fhe_ssm_scan_backward_workspace": [ctypes.POINTER(SsmScanGradArgs), P64],
+    "fhe_ssm_scan_backward": [ctypes.POINTER(SsmScanGradArgs)],
+    "fhe_causal_conv": [ctypes.POINTER(CausalConvArgs)],
+    "fhe_causal_conv_backward_workspace": [ctypes.POINTER(CausalConvGradArgs), P64],
+    "fhe_causal_conv_backward": [ctypes.POINTER(CausalConvGradArgs)],
+    "fhe_token_logprobs": [ctypes.POINTER(TokenLogprobsArgs)],
+    "fhe_token_logprobs_backward": [ctypes.POINTER(TokenLogprobsGradArgs)],
 }
 
 _lock = threading.Lock()

@@ -18,6 +18,7 @@
 #include "program.h"
 #include "shard.h"
 #include "launch_count.h"
+#include "mamba_ops.h"
 
 namespace fhe {
 void rescale_noalloc(Context& c, const uint64_t* in, uint32_t ncomp, uint32_t nq, uint64_t* out);
@@ -1221,6 +1222,70 @@ int fhe_chebyshev(fhe_ctx* ctx, const fhe_ct* a, const double* coeffs, uint32_t 
     fhe::Ckks& k = ckks(ctx);
     fhe::require(coeffs != nullptr && n >= 1, "need at least one coefficient");
     put_ct(out, k.chebyshev(ct_of(a), std::vector<double>(coeffs, coeffs + n), lo, hi));
+  });
+}
+
+// Plaintext Mamba-2 operators.
+int fhe_ssm_scan_workspace(const fhe_ssm_scan_args* args, uint64_t* bytes) {
+  return guarded([&] {
+    fhe::require(args != nullptr && bytes != nullptr, "null argument");
+    *bytes = fhe::ssm_scan_workspace(*args);
+  });
+}
+
+int fhe_ssm_scan(const fhe_ssm_scan_args* args) {
+  return guarded([&] {
+    fhe::require(args != nullptr, "null argument");
+    fhe::ssm_scan(*args);
+  });
+}
+
+int fhe_ssm_scan_backward_workspace(const fhe_ssm_scan_grad_args* args, uint64_t* bytes) {
+  return guarded([&] {
+    fhe::require(args != nullptr && bytes != nullptr, "null argument");
+    *bytes = fhe::ssm_scan_backward_workspace(*args);
+  });
+}
+
+int fhe_ssm_scan_backward(const fhe_ssm_scan_grad_args* args) {
+  return guarded([&] {
+    fhe::require(args != nullptr, "null argument");
+    fhe::ssm_scan_backward(*args);
+  });
+}
+
+int fhe_causal_conv(const fhe_causal_conv_args* args) {
+  return guarded([&] {
+    fhe::require(args != nullptr, "null argument");
+    fhe::causal_conv(*args);
+  });
+}
+
+int fhe_causal_conv_backward_workspace(const fhe_causal_conv_grad_args* args, uint64_t* bytes) {
+  return guarded([&] {
+    fhe::require(args != nullptr && bytes != nullptr, "null argument");
+    *bytes = fhe::causal_conv_backward_workspace(*args);
+  });
+}
+
+int fhe_causal_conv_backward(const fhe_causal_conv_grad_args* args) {
+  return guarded([&] {
+    fhe::require(args != nullptr, "null argument");
+    fhe::causal_conv_backward(*args);
+  });
+}
+
+int fhe_token_logprobs(const fhe_token_logprobs_args* args) {
+  return guarded([&] {
+    fhe::require(args != nullptr, "null argument");
+    fhe::token_logprobs(*args);
+  });
+}
+
+int fhe_token_logprobs_backward(const fhe_token_logprobs_grad_args* args) {
+  return guarded([&] {
+    fhe::require(args != nullptr, "null argument");
+    fhe::token_logprobs_backward(*args);
   });
 }
 

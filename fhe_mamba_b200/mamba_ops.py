@@ -1,0 +1,358 @@
+"""The plaintext Mamba-2 operators as torch functions: the state recurrence
+(``ssm_scan``, ``ssm_step``), the causal convolution (``causal_conv``,
+``causal_conv_step``) and token scoring (``token_logprobs``).
+
+They run on CUDA tensors through the C ABI (fhe_ssm_scan and the others in
+include/fhe_b200.h), on the current stream of the tensors' device, and can be
+captured into CUDA graphs; the scan, the convolution and the scores have
+gradients (to capture a backward pass, hold no eager autograd graph of the same
+leaves: torch would make the capture wait for that graph's stream, and refuses).
+Activations are float32, bfloat16 or float16; gates, states and
+scores are float32.  Arguments that do not fit raise ValueError before any GPU
+work.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import call
+
+_TYPES = {torch.float32: _lib.FHE_F32, torch.bfloat16: _lib.FHE_BF16, torch.float16: _lib.FHE_F16}
+MAX_HEAD_DIM, MAX_STATE, MAX_TAPS, MAX_TOP = 128, 256, 8, 64
+
+
+def _need(ok, message):
+    if not ok:
+        raise ValueError(message)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _inner(t):
+    """t with its innermost axis contiguous (itself if it is)."""
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _check_devices(op, first, *rest):
+    _need(first.is_cuda, f"{op}: CUDA tensors expected")
+    for t in rest:
+        _need(t is None or t.device == first.device, f"{op}: tensors on different devices")
+
+
+def _check(op, name, t, shape, dtype):
+    _need(tuple(t.shape) == tuple(shape), f"{op}: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    _need(t.dtype == dtype, f"{op}: {name} must be {dtype}, got {t.dtype}")
+
+
+def _workspace(name, args, device):
+    n = ctypes.c_uint64()
+    call(name, ctypes.byref(args), ctypes.byref(n))
+    return torch.empty(n.value, dtype=torch.uint8, device=device) if n.value else None
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+# ---- state recurrence ---------------------------------------------------------------------------
+
+
+def _check_scan(op, x, write, log_decay, B, C, D, state, lengths, state_name="initial_state"):
+    _need(x.dim() == 4, f"{op}: x must be [batch, length, heads, head_dim]")
+    b, l, h, p = x.shape
+    _need(x.dtype in _TYPES, f"{op}: x must be float32, bfloat16 or float16")
+    _need(B.dim() == 4, f"{op}: B must be [batch, length, groups, d_state]")
+    k, n = B.shape[2], B.shape[3]
+    _need(k >= 1 and h >= 1 and h % k == 0, f"{op}: heads ({h}) must be a positive multiple of groups ({k})")
+    _need(1 <= p <= MAX_HEAD_DIM, f"{op}: head_dim must be in [1, {MAX_HEAD_DIM}]")
+    _need(1 <= n <= MAX_STATE, f"{op}: d_state must be in [1, {MAX_STATE}]")
+    _check(op, "B", B, (b, l, k, n), x.dtype)
+    _check(op, "C", C, (b, l, k, n), x.dtype)
+    _check(op, "write", write, (b, l, h), torch.float32)
+    _check(op, "log_decay", log_decay, (b, l, h), torch.float32)
+    if D is not None:
+        _check(op, "D", D, (h,), torch.float32)
+    if state is not None:
+        _check(op, state_name, state, (b, h, p, n), torch.float32)
+    if lengths is not None:
+        _check(op, "lengths", lengths, (b,), torch.int32)
+    _check_devices(op, x, write, log_decay, B, C, D, state, lengths)
+
+
+def _scan_args(x, write, log_decay, B, C, D, state, lengths, y, final):
+    b, l, h, p = x.shape
+    return _lib.SsmScanArgs(
+        x.device.index, _TYPES[x.dtype], b, l, h, p, B.shape[3], B.shape[2],
+        x.data_ptr(), x.stride()[:3], write.data_ptr(), write.stride(), log_decay.data_ptr(), log_decay.stride(),
+        B.data_ptr(), B.stride()[:3], C.data_ptr(), C.stride()[:3],
+        _ptr(D), _ptr(state), _ptr(lengths), _ptr(y), _ptr(final), None, 0, _stream(x.device))
+
+
+def _scan_forward(x, write, log_decay, B, C, D, state, lengths, y, final):
+    a = _scan_args(x, write, log_decay, B, C, D, state, lengths, y, final)
+    if x.shape[1] != 1:
+        ws = _workspace("fhe_ssm_scan_workspace", a, x.device)
+        if ws is not None:
+            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    call("fhe_ssm_scan", ctypes.byref(a))
+
+
+class _SsmScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, write, log_decay, B, C, D, state, lengths):
+        b, l, h, p = x.shape
+        y = torch.empty((b, l, h, p), dtype=x.dtype, device=x.device)
+        final = torch.empty((b, h, p, B.shape[3]), dtype=torch.float32, device=x.device)
+        _scan_forward(x, write, log_decay, B, C, D, state, lengths, y, final)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, write, log_decay, B, C, D, state, lengths)
+        return y, final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dfinal):
+        x, write, log_decay, B, C, D, state, lengths = ctx.saved_tensors
+        b, l, h, p = x.shape
+        k, n = B.shape[2], B.shape[3]
+        dy = torch.zeros((b, l, h, p), dtype=x.dtype, device=x.device) if dy is None else dy.contiguous()
+        dfinal = None if dfinal is None else dfinal.contiguous()
+        new = lambda shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=x.device)  # noqa: E731
+        dx, db, dc = new((b, l, h, p), x.dtype), new((b, l, k, n), x.dtype), new((b, l, k, n), x.dtype)
+        dw, dla = new((b, l, h)), new((b, l, h))
+        dd = new((h,)) if D is not None and ctx.needs_input_grad[5] else None
+        ds = new((b, h, p, n)) if state is not None and ctx.needs_input_grad[6] else None
+        g = _lib.SsmScanGradArgs(
+            _scan_args(x, write, log_decay, B, C, D, state, lengths, None, None),
+            dy.data_ptr(), _ptr(dfinal), dx.data_ptr(), dw.data_ptr(), dla.data_ptr(), db.data_ptr(), dc.data_ptr(),
+            _ptr(dd), _ptr(ds), None, 0, _stream(x.device))
+        ws = _workspace("fhe_ssm_scan_backward_workspace", g, x.device)
+        if ws is not None:
+            g.workspace, g.workspace_bytes = ws.data_ptr(), ws.numel()
+        call("fhe_ssm_scan_backward", ctypes.byref(g))
+        return dx, dw, dla, db, dc, dd, ds, None
+
+
+def ssm_scan(x, write, log_decay, B, C, D=None, initial_state=None, lengths=None):
+    """Mamba-2's recurrence over a padded batch of token rows:
+
+        S_t = exp(log_decay_t) S_(t-1) + write_t x_t (x) B_t,   y_t = S_t C_t + D x_t
+
+    x [batch, length, heads, head_dim]; write, log_decay [batch, length, heads]
+    float32 (the layer's dt and A dt); B, C [batch, length, groups, d_state] in
+    x's type, shared by heads/groups consecutive heads; D [heads];
+    initial_state [batch, heads, head_dim, d_state] float32, zeros if None;
+    lengths [batch] int32, full rows if None.  Returns (y, final_state).
+
+    Tokens at or past a row's length are not read, leave the state and get
+    y = 0 (a length is clamped to [0, length]).  log_decay = -inf clears the
+    state before its token, so several texts may share a row.  x, B and C may
+    be slices of one activation tensor (only the last axis must be contiguous,
+    else it is copied).  Gradients reach every floating-point argument."""
+    _check_scan("ssm_scan", x, write, log_decay, B, C, D, initial_state, lengths)
+    D, initial_state, lengths = (None if t is None else t.contiguous() for t in (D, initial_state, lengths))
+    return _SsmScan.apply(_inner(x), write, log_decay, _inner(B), _inner(C), D, initial_state, lengths)
+
+
+def _no_grad(op, instead, *tensors):
+    _need(not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)),
+          f"{op} has no gradient (use {instead})")
+
+
+def ssm_step(state, x, write, log_decay, B, C, D=None, out=None):
+    """One token of each sequence: ``ssm_scan`` without the length axis (x
+    [batch, heads, head_dim], write and log_decay [batch, heads], B and C
+    [batch, groups, d_state]).  The new state is written to `out` ([batch,
+    heads, head_dim, d_state] float32, contiguous), or over `state` if None.
+    Returns (y, new state)."""
+    op = "ssm_step"
+    _need(x.dim() == 3 and B.dim() == 3 and C.dim() == 3 and write.dim() == 2 and log_decay.dim() == 2,
+          f"{op}: one token of each sequence, without a length axis")
+    _no_grad(op, "ssm_scan", state, x, write, log_decay, B, C, D)
+    x, write, log_decay, B, C = (t.unsqueeze(1) for t in (x, write, log_decay, B, C))
+    _check_scan(op, x, write, log_decay, B, C, D, state, None, "state")
+    out = state if out is None else out
+    _check(op, "out", out, state.shape, torch.float32)
+    _need(state.is_contiguous() and out.is_contiguous(), f"{op}: state and out must be contiguous")
+    _check_devices(op, x, out)
+    _need(out.data_ptr() == state.data_ptr() or not _overlap(out, state), f"{op}: out overlaps part of state")
+    y = torch.empty((x.shape[0], 1) + tuple(x.shape[2:]), dtype=x.dtype, device=x.device)
+    _scan_forward(_inner(x), write, log_decay, _inner(B), _inner(C), None if D is None else D.contiguous(), state,
+                  None, y, out)
+    return y[:, 0], out
+
+
+def _overlap(a, b):
+    """Whether two contiguous tensors share memory."""
+    a0, b0 = a.data_ptr(), b.data_ptr()
+    return a0 < b0 + b.numel() * b.element_size() and b0 < a0 + a.numel() * a.element_size()
+
+
+# ---- causal convolution -------------------------------------------------------------------------
+
+
+def _check_conv(op, x, weight, bias, state, lengths, activation, state_name="initial_state"):
+    _need(x.dim() == 3, f"{op}: x must be [batch, length, channels]")
+    b, _, c = x.shape
+    _need(x.dtype in _TYPES, f"{op}: x must be float32, bfloat16 or float16")
+    _need(c >= 1, f"{op}: channels must be positive")
+    _need(weight.dim() == 2 and 1 <= weight.shape[1] <= MAX_TAPS, f"{op}: weight must be [channels, 1 to {MAX_TAPS} taps]")
+    k = weight.shape[1]
+    _check(op, "weight", weight, (c, k), x.dtype)
+    if bias is not None:
+        _check(op, "bias", bias, (c,), x.dtype)
+    if state is not None:
+        _check(op, state_name, state, (b, k - 1, c), x.dtype)
+    if lengths is not None:
+        _check(op, "lengths", lengths, (b,), torch.int32)
+    _need(activation in (None, "silu"), f"{op}: activation must be None or 'silu'")
+    _check_devices(op, x, weight, bias, state, lengths)
+
+
+def _conv_args(x, weight, bias, state, lengths, silu, y, final):
+    b, l, c = x.shape
+    return _lib.CausalConvArgs(
+        x.device.index, _TYPES[x.dtype], b, l, c, weight.shape[1], silu, 0, x.data_ptr(), x.stride()[:2],
+        weight.data_ptr(), _ptr(bias), _ptr(state), _ptr(lengths), _ptr(y), _ptr(final), _stream(x.device))
+
+
+class _CausalConv(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, state, lengths, silu):
+        b, l, c = x.shape
+        y = torch.empty((b, l, c), dtype=x.dtype, device=x.device)
+        final = torch.empty((b, weight.shape[1] - 1, c), dtype=x.dtype, device=x.device)
+        call("fhe_causal_conv", ctypes.byref(_conv_args(x, weight, bias, state, lengths, silu, y, final)))
+        ctx.set_materialize_grads(False)
+        ctx.silu = silu
+        ctx.save_for_backward(x, weight, bias, state, lengths)
+        return y, final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dfinal):
+        x, weight, bias, state, lengths = ctx.saved_tensors
+        b, l, c = x.shape
+        dy = torch.zeros((b, l, c), dtype=x.dtype, device=x.device) if dy is None else dy.contiguous()
+        dfinal = None if dfinal is None else dfinal.contiguous()
+        dx = torch.empty((b, l, c), dtype=x.dtype, device=x.device)
+        dw = torch.empty_like(weight)
+        db = torch.empty_like(bias) if bias is not None else None
+        ds = torch.empty_like(state) if state is not None and ctx.needs_input_grad[3] else None
+        g = _lib.CausalConvGradArgs(
+            _conv_args(x, weight, bias, state, lengths, ctx.silu, None, None), dy.data_ptr(), _ptr(dfinal),
+            dx.data_ptr(), dw.data_ptr(), _ptr(db), _ptr(ds), None, 0, _stream(x.device))
+        ws = _workspace("fhe_causal_conv_backward_workspace", g, x.device)
+        if ws is not None:
+            g.workspace, g.workspace_bytes = ws.data_ptr(), ws.numel()
+        call("fhe_causal_conv_backward", ctypes.byref(g))
+        return dx, dw, db, ds, None, None
+
+
+def causal_conv(x, weight, bias=None, initial_state=None, lengths=None, activation="silu"):
+    """Causal depthwise convolution over the tokens of a padded batch:
+
+        y_t = act(bias + sum_i weight[:, i] row_(t+i)),   row = [initial_state; x]
+
+    x [batch, length, channels] (a slice of a wider tensor will do); weight
+    [channels, taps], the last tap on the present token; bias [channels];
+    initial_state [batch, taps - 1, channels], the tokens before the row,
+    oldest first, zeros if None; lengths [batch] int32; activation "silu" or
+    None.  All in x's type.  Returns (y, final_state): y is 0 at and past a
+    row's length, final_state is the window behind its last token.  Gradients
+    reach every floating-point argument."""
+    _check_conv("causal_conv", x, weight, bias, initial_state, lengths, activation)
+    weight, bias, initial_state, lengths = (None if t is None else t.contiguous()
+                                            for t in (weight, bias, initial_state, lengths))
+    return _CausalConv.apply(_inner(x), weight, bias, initial_state, lengths, activation == "silu")
+
+
+def causal_conv_step(state, x, weight, bias=None, activation="silu", out=None):
+    """One token of each sequence: x [batch, channels], state [batch, taps - 1,
+    channels].  The moved window is written to `out`, or over `state` if None.
+    Returns (y, new state)."""
+    op = "causal_conv_step"
+    _need(x.dim() == 2, f"{op}: one token of each sequence, without a length axis")
+    _no_grad(op, "causal_conv", state, x, weight, bias)
+    x = x.unsqueeze(1)
+    _check_conv(op, x, weight, bias, state, None, activation, "state")
+    out = state if out is None else out
+    _check(op, "out", out, state.shape, x.dtype)
+    _need(state.is_contiguous() and out.is_contiguous(), f"{op}: state and out must be contiguous")
+    _check_devices(op, x, out)
+    _need(out.data_ptr() == state.data_ptr() or not _overlap(out, state), f"{op}: out overlaps part of state")
+    y = torch.empty((x.shape[0], 1, x.shape[2]), dtype=x.dtype, device=x.device)
+    call("fhe_causal_conv", ctypes.byref(_conv_args(_inner(x), weight.contiguous(),
+                                                    None if bias is None else bias.contiguous(), state, None,
+                                                    activation == "silu", y, out)))
+    return y[:, 0], out
+
+
+# ---- token scores -------------------------------------------------------------------------------
+
+
+class TokenLogprobs(NamedTuple):
+    logprob: torch.Tensor       # [rows] float32
+    entropy: torch.Tensor       # [rows] float32, in nats
+    top_logprobs: torch.Tensor  # [rows, top_k] float32
+    top_ids: torch.Tensor       # [rows, top_k] int64
+
+
+def _logprob_args(logits, targets, top_k, logprob, entropy, top_logprobs, top_ids, lse):
+    return _lib.TokenLogprobsArgs(
+        logits.device.index, _TYPES[logits.dtype], logits.shape[0], logits.shape[1], top_k, 0, logits.data_ptr(),
+        logits.stride(0), targets.data_ptr(), _ptr(logprob), _ptr(entropy), _ptr(top_logprobs), _ptr(top_ids),
+        lse.data_ptr(), _stream(logits.device))
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, top_k):
+        r = logits.shape[0]
+        logprob, entropy, lse = (torch.empty(r, dtype=torch.float32, device=logits.device) for _ in range(3))
+        top = torch.empty((r, top_k), dtype=torch.float32, device=logits.device)
+        ids = torch.empty((r, top_k), dtype=torch.int64, device=logits.device)
+        call("fhe_token_logprobs",
+             ctypes.byref(_logprob_args(logits, targets, top_k, logprob, entropy, top, ids, lse)))
+        ctx.mark_non_differentiable(ids)
+        ctx.set_materialize_grads(False)
+        ctx.top_k = top_k
+        ctx.save_for_backward(logits, targets, entropy, ids, lse)
+        return logprob, entropy, top, ids
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dlogprob, dentropy, dtop, _):
+        logits, targets, entropy, ids, lse = ctx.saved_tensors
+        dlogprob, dentropy, dtop = (None if g is None else g.contiguous() for g in (dlogprob, dentropy, dtop))
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        a = _lib.TokenLogprobsGradArgs(
+            _logprob_args(logits, targets, ctx.top_k, None, entropy, None, ids, lse), _ptr(dlogprob),
+            _ptr(dentropy), _ptr(dtop) if ctx.top_k else None, out.data_ptr(), _stream(logits.device))
+        call("fhe_token_logprobs_backward", ctypes.byref(a))
+        return out, None, None
+
+
+def token_logprobs(logits, targets, top_k=0):
+    """Scores of one token per row under softmax(logits): its log-probability,
+    the row's entropy and its top_k (at most 64) most probable tokens, the
+    lower index first among equals.
+
+    logits [rows, vocab] float32, bfloat16 or float16; targets [rows] int64,
+    negative for a row whose token is not scored (log-probability 0); a target
+    past the vocabulary scores NaN.  Entries of -inf are impossible tokens.
+    Returns a ``TokenLogprobs``; gradients of its floating-point parts reach
+    the logits."""
+    op = "token_logprobs"
+    _need(logits.dim() == 2 and logits.dtype in _TYPES, f"{op}: logits must be [rows, vocab] float32, bfloat16 or float16")
+    _need(logits.shape[1] >= 1, f"{op}: an empty vocabulary")
+    _check(op, "targets", targets, (logits.shape[0],), torch.int64)
+    _need(0 <= top_k <= min(MAX_TOP, logits.shape[1]), f"{op}: top_k must be in [0, {min(MAX_TOP, logits.shape[1])}]")
+    _check_devices(op, logits, targets)
+    return TokenLogprobs(*_TokenLogprobs.apply(_inner(logits), targets.contiguous(), int(top_k)))

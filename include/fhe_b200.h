@@ -508,6 +508,147 @@ int fhe_chebyshev(fhe_ctx* ctx, const fhe_ct* a, const double* coeffs, uint32_t 
  * word a call reads was written earlier by the same call. */
 int fhe_rescale_noalloc(fhe_ctx* ctx, const uint64_t* in, uint32_t ncomp, uint32_t n_limbs, uint64_t* out);
 
+/* --- plaintext Mamba-2 operators (state scan, convolution, scoring) -------
+ *
+ * The recurrence, causal convolution and token scoring of the plaintext model
+ * beside the encrypted loop (calibration, scoring, fine-tuning, the client's
+ * selection), on device tensors the caller owns.  They need no context: every
+ * call takes the device ordinal and the cudaStream_t (as void*) its work is
+ * ordered on, allocates nothing and keeps nothing; scratch is the caller's
+ * `workspace` (256-byte aligned, at least the size the matching _workspace
+ * function reports for the same arguments; calls that may run at the same
+ * time need workspaces of their own).  Strides count elements; the innermost
+ * axis is contiguous.  `dtype` is the type of x, b, c, y, the logits and the
+ * convolution's tensors; gates, states, sums and scores are fp32. */
+#define FHE_F32 0
+#define FHE_BF16 1
+#define FHE_F16 2
+
+/* Mamba-2's state recurrence over a padded batch of sequences, per batch row
+ * and head (ssm_scan, src/fhemamba/reference.py:69-115):
+ *   S_t = exp(log_decay_t) S_(t-1) + write_t x_t (x) b_t,   y_t = S_t c_t + d x_t.
+ * Heads [i*heads/groups, (i+1)*heads/groups) share b and c of group i.
+ * log_decay = -inf clears the state before its token.  Tokens at or past
+ * lengths[batch] (clamped to [0, length]) change no state, are not read, and
+ * get y = 0.  head_dim <= 128, d_state <= 256. */
+typedef struct fhe_ssm_scan_args {
+  int32_t device, dtype;
+  uint32_t batch, length, heads, head_dim, d_state, groups;
+  const void* x;              /* [batch][length][heads][head_dim] */
+  int64_t x_stride[3];        /* batch, token, head */
+  const float* write;         /* [batch][length][heads] */
+  int64_t write_stride[3];
+  const float* log_decay;     /* [batch][length][heads] */
+  int64_t log_decay_stride[3];
+  const void* b;              /* [batch][length][groups][d_state] */
+  int64_t b_stride[3];
+  const void* c;              /* [batch][length][groups][d_state] */
+  int64_t c_stride[3];
+  const float* d;             /* [heads], or NULL for no skip term */
+  const float* initial_state; /* [batch][heads][head_dim][d_state], or NULL for zeros */
+  const int32_t* lengths;     /* [batch], or NULL for full rows */
+  void* y;                    /* [batch][length][heads][head_dim], contiguous */
+  float* final_state;         /* as initial_state; may be the same memory */
+  void* workspace;
+  uint64_t workspace_bytes;
+  void* stream;
+} fhe_ssm_scan_args;
+int fhe_ssm_scan_workspace(const fhe_ssm_scan_args* args, uint64_t* bytes);
+int fhe_ssm_scan(const fhe_ssm_scan_args* args);
+
+/* Gradients of fhe_ssm_scan: `f` holds the forward call's inputs (its y,
+ * final_state and workspace are not used).  Every output is contiguous and
+ * written whole; sums run in a fixed order. */
+typedef struct fhe_ssm_scan_grad_args {
+  fhe_ssm_scan_args f;
+  const void* dy;             /* [batch][length][heads][head_dim], contiguous */
+  const float* dfinal;        /* as initial_state, or NULL for zeros */
+  void* dx;                   /* [batch][length][heads][head_dim] */
+  float* dwrite;              /* [batch][length][heads] */
+  float* dlog_decay;          /* [batch][length][heads] */
+  void* db;                   /* [batch][length][groups][d_state] */
+  void* dc;                   /* [batch][length][groups][d_state] */
+  float* dd;                  /* [heads], or NULL */
+  float* dinitial;            /* as initial_state, or NULL */
+  void* workspace;
+  uint64_t workspace_bytes;
+  void* stream;
+} fhe_ssm_scan_grad_args;
+int fhe_ssm_scan_backward_workspace(const fhe_ssm_scan_grad_args* args, uint64_t* bytes);
+int fhe_ssm_scan_backward(const fhe_ssm_scan_grad_args* args);
+
+/* Causal depthwise convolution over the tokens of a padded batch, taps 1 to 8:
+ *   y_t = act(bias + sum_i weight[.][i] row_(t+i)),  row = [initial_state; x],
+ * with act the identity or SiLU.  Tokens at or past lengths[batch] get y = 0;
+ * final_state holds the taps - 1 rows before the end of the sequence (oldest
+ * first), the window a following call starts from. */
+typedef struct fhe_causal_conv_args {
+  int32_t device, dtype;
+  uint32_t batch, length, channels, taps;
+  int32_t silu;
+  uint32_t reserved;
+  const void* x;              /* [batch][length][channels] */
+  int64_t x_stride[2];        /* batch, token */
+  const void* weight;         /* [channels][taps] */
+  const void* bias;           /* [channels], or NULL */
+  const void* initial_state;  /* [batch][taps-1][channels], or NULL for zeros */
+  const int32_t* lengths;     /* [batch], or NULL */
+  void* y;                    /* [batch][length][channels], contiguous */
+  void* final_state;          /* [batch][taps-1][channels]; may be initial_state's memory only if length == 1 */
+  void* stream;
+} fhe_causal_conv_args;
+int fhe_causal_conv(const fhe_causal_conv_args* args);
+
+typedef struct fhe_causal_conv_grad_args {
+  fhe_causal_conv_args f;     /* the forward call's inputs */
+  const void* dy;             /* [batch][length][channels], contiguous */
+  const void* dfinal;         /* [batch][taps-1][channels], or NULL for zeros */
+  void* dx;                   /* [batch][length][channels] */
+  void* dweight;              /* [channels][taps] */
+  void* dbias;                /* [channels], or NULL */
+  void* dinitial;             /* [batch][taps-1][channels], or NULL */
+  void* workspace;
+  uint64_t workspace_bytes;
+  void* stream;
+} fhe_causal_conv_grad_args;
+int fhe_causal_conv_backward_workspace(const fhe_causal_conv_grad_args* args, uint64_t* bytes);
+int fhe_causal_conv_backward(const fhe_causal_conv_grad_args* args);
+
+/* Log-probability of one target per row under softmax(logits), the entropy of
+ * the row and its top_k (<= 64, <= vocab) largest entries with their
+ * log-probabilities, in one read of the logits.  Ties go to the lower index.
+ * A negative target is ignored (log-probability 0); a target >= vocab gives
+ * NaN.  Rows of -inf alone have log-probabilities -inf and entropy 0; a NaN or
+ * +inf logit makes the row's scores NaN (a NaN ranks below every number). */
+typedef struct fhe_token_logprobs_args {
+  int32_t device, dtype;
+  uint32_t rows, vocab, top_k, reserved;
+  const void* logits;         /* [rows][vocab] */
+  int64_t logits_stride;      /* between rows */
+  const int64_t* targets;     /* [rows] */
+  float* logprob;             /* [rows] */
+  float* entropy;             /* [rows] */
+  float* top_logprobs;        /* [rows][top_k], or NULL if top_k == 0 */
+  int64_t* top_ids;           /* [rows][top_k], or NULL if top_k == 0 */
+  float* lse;                 /* [rows]: log of the sum of exponentials */
+  void* stream;
+} fhe_token_logprobs_args;
+int fhe_token_logprobs(const fhe_token_logprobs_args* args);
+
+/* dlogits (contiguous, dtype) from the gradients of logprob, entropy and
+ * top_logprobs (each NULL for zeros); `f` as in the forward call, with its
+ * entropy, top_ids and lse outputs as inputs.  An ignored or out-of-range
+ * target passes no gradient, a row of -inf alone gets zeros. */
+typedef struct fhe_token_logprobs_grad_args {
+  fhe_token_logprobs_args f;
+  const float* dlogprob;      /* [rows] */
+  const float* dentropy;      /* [rows] */
+  const float* dtop_logprobs; /* [rows][top_k] */
+  void* dlogits;              /* [rows][vocab] */
+  void* stream;
+} fhe_token_logprobs_grad_args;
+int fhe_token_logprobs_backward(const fhe_token_logprobs_grad_args* args);
+
 #ifdef __cplusplus
 }
 #endif
