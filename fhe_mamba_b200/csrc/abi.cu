@@ -19,6 +19,7 @@
 #include "shard.h"
 #include "launch_count.h"
 #include "mamba_ops.h"
+#include "mamba_scan.h"
 
 namespace fhe {
 void rescale_noalloc(Context& c, const uint64_t* in, uint32_t ncomp, uint32_t nq, uint64_t* out);
@@ -779,7 +780,7 @@ int fhe_ctx_set_giant_hoisting(fhe_ctx* ctx, int32_t on) {
 int fhe_tc_timeouts(uint64_t* count) {
   return guarded([&] {
     fhe::require(count != nullptr, "null count");
-    *count = fhe::tc_conversion_timeouts();
+    *count = fhe::tc_conversion_timeouts() + fhe::scan_tc_timeouts();
   });
 }
 

@@ -31,29 +31,46 @@ __device__ __forceinline__ int clamp_length(const int32_t* lengths, uint32_t b, 
   return min(max(lengths[b], 0), (int)length);
 }
 
-__device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + expf(-v)); }
+// 1 / (1 + exp(-v)) with the special-function exponential and reciprocal: a
+// few units in the last place of fp32, at a quarter of the instructions of
+// expf and a division, which would bound the 16-bit forms.
+template <int V>
+__device__ __forceinline__ void sigmoid(float (&o)[V], const float (&v)[V]) {
+  float k[V], one[V];
+  vset(k, -1.4426950408889634f);
+  vset(one, 1.f);
+  vmul(o, v, k);
+#pragma unroll
+  for (int i = 0; i < V; ++i) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(o[i]) : "f"(o[i]));
+  vadd(o, o, one);
+#pragma unroll
+  for (int i = 0; i < V; ++i) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(o[i]) : "f"(o[i]));
+}
 
 // Row element: t < 0 is the initial state's entry t + K - 1.
 template <class T, int V, int K>
 __device__ __forceinline__ void load_row(const T* x, const T* init, int64_t sl, uint32_t channels, int t,
                                          float (&o)[V]) {
   const T* p = t >= 0 ? x + (int64_t)t * sl : init ? init + (int64_t)(t + K - 1) * channels : nullptr;
-  if (!p) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) o[v] = 0.f;
-    return;
-  }
-  const Pack<T, V> k = *reinterpret_cast<const Pack<T, V>*>(p);
-#pragma unroll
-  for (int v = 0; v < V; ++v) o[v] = to_f(k.v[v]);
+  if (p) unpack(*reinterpret_cast<const Pack<T, V>*>(p), o);
+  else vset(o, 0.f);
 }
 
+// w[i]: tap i of V channels; the taps of V channels lie together.
 template <class T, int V, int K>
-__device__ __forceinline__ void load_taps(const void* weight, uint32_t c, float (&w)[V][K]) {
+__device__ __forceinline__ void load_taps(const void* weight, uint32_t c, float (&w)[K][V]) {
+  const T* p = static_cast<const T*>(weight) + (int64_t)c * K;
 #pragma unroll
-  for (int v = 0; v < V; ++v)
+  for (int j = 0; j < K; ++j) {
+    const Pack<T, V> k = *reinterpret_cast<const Pack<T, V>*>(p + j * V);
 #pragma unroll
-    for (int i = 0; i < K; ++i) w[v][i] = to_f(static_cast<const T*>(weight)[(int64_t)(c + v) * K + i]);
+    for (int v = 0; v < V; ++v) w[(j * V + v) % K][(j * V + v) / K] = to_f(k.v[v]);
+  }
+}
+template <class T, int V>
+__device__ __forceinline__ void load_bias(const void* bias, uint32_t c, float (&o)[V]) {
+  if (bias) unpack(*reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(bias) + c), o);
+  else vset(o, 0.f);
 }
 
 // Thread = V channels x one run of tokens, channels fastest.  `STEP` (one
@@ -83,38 +100,62 @@ __global__ void __launch_bounds__(kThreads) k_conv(const ConvArgs g) {
   const int t0 = run * g.run, t1 = min(t0 + g.run, g.length);
   const T* x = static_cast<const T*>(g.x) + (int64_t)b * g.sb + c;
   const T* init = g.initial ? static_cast<const T*>(g.initial) + (int64_t)b * (K - 1) * g.channels + c : nullptr;
-  float w[V][K], bias[V], win[K][V];
-  load_taps<T, V, K>(g.weight, c, w);
-#pragma unroll
-  for (int v = 0; v < V; ++v) bias[v] = g.bias ? to_f(static_cast<const T*>(g.bias)[c + v]) : 0.f;
+  float w[K][V], bias[V], win[K][V];
 #pragma unroll
   for (int i = 0; i < K - 1; ++i) {
     const int t = t0 + i - (K - 1);
     if (t < len) load_row<T, V, K>(x, init, g.sl, g.channels, t, win[i + 1]);
   }
+  load_taps<T, V, K>(g.weight, c, w);
+  load_bias<T, V>(g.bias, c, bias);
   T* y = static_cast<T*>(g.y) + ((int64_t)b * g.length + t0) * g.channels + c;
-#pragma unroll 4
-  for (int t = t0; t < t1; ++t, y += g.channels) {
-    Pack<T, V> o;
-    if (t < len) {
+  auto token = [&](const Pack<T, V>& in) {  // win moves on by one token
+    float o[V];
 #pragma unroll
-      for (int i = 0; i < K - 1; ++i)
+    for (int i = 0; i < K - 1; ++i)
 #pragma unroll
-        for (int v = 0; v < V; ++v) win[i][v] = win[i + 1][v];
-      load_row<T, V, K>(x, init, g.sl, g.channels, t, win[K - 1]);
+      for (int v = 0; v < V; ++v) win[i][v] = win[i + 1][v];
+    unpack(in, win[K - 1]);
+    vfma(o, w[0], win[0], bias);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float p = bias[v];
-#pragma unroll
-        for (int i = 0; i < K; ++i) p = fmaf(w[v][i], win[i][v], p);
-        o.v[v] = from_f<T>(SILU ? p * sigmoid(p) : p);
-      }
-    } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) o.v[v] = from_f<T>(0.f);
+    for (int i = 1; i < K; ++i) vfma(o, w[i], win[i], o);
+    if constexpr (SILU) {
+      float e[V];
+      sigmoid(e, o);
+      vmul(o, o, e);
     }
-    *reinterpret_cast<Pack<T, V>*>(y) = o;
+    *reinterpret_cast<Pack<T, V>*>(y) = pack<T>(o);
+    y += g.channels;
+  };
+  int t = t0;
+  const int t_live = min(t1, len);
+  const T* xt = x + (int64_t)t * g.sl;
+  if constexpr (!STEP) {
+    // kAhead tokens are used while the next kAhead are on their way
+    constexpr int kAhead = 4;
+    auto fetch = [&](Pack<T, V> (&in)[kAhead]) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j, xt += g.sl) in[j] = *reinterpret_cast<const Pack<T, V>*>(xt);
+    };
+    if (t + kAhead <= t_live) {
+      Pack<T, V> now[kAhead], next[kAhead];
+      fetch(now);
+      for (; t + 2 * kAhead <= t_live; t += kAhead) {
+        fetch(next);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) token(now[j]);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) now[j] = next[j];
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) token(now[j]);
+      t += kAhead;
+    }
   }
+  for (; t < t_live; ++t, xt += g.sl) token(*reinterpret_cast<const Pack<T, V>*>(xt));
+  float zero[V];
+  vset(zero, 0.f);
+  for (; t < t1; ++t, y += g.channels) *reinterpret_cast<Pack<T, V>*>(y) = pack<T>(zero);
   if constexpr (STEP && K > 1) {
     // an empty sequence keeps its window (win[1..K-1]), else it moved by one (also win[1..K-1] after the shift)
     T* f = static_cast<T*>(g.final_state) + (int64_t)b * (K - 1) * g.channels + c;
@@ -150,83 +191,122 @@ __global__ void __launch_bounds__(kThreads) k_conv_grad(const ConvGradArgs a) {
   const uint32_t run = id % g.runs, b = id / g.runs;
   const int len = clamp_length(g.lengths, b, g.length);
   const int t0 = run * g.run, t1 = min(t0 + g.run, g.length);
-  const bool last = run + 1 == g.runs;
   const T* x = static_cast<const T*>(g.x) + (int64_t)b * g.sb + c;
   const T* init = g.initial ? static_cast<const T*>(g.initial) + (int64_t)b * (K - 1) * g.channels + c : nullptr;
   const T* dy = static_cast<const T*>(a.dy) + (int64_t)b * g.length * g.channels + c;
   const T* dfinal = a.dfinal ? static_cast<const T*>(a.dfinal) + (int64_t)b * (K - 1) * g.channels + c : nullptr;
   T* dx = static_cast<T*>(a.dx) + (int64_t)b * g.length * g.channels + c;
   T* dinit = a.dinitial ? static_cast<T*>(a.dinitial) + (int64_t)b * (K - 1) * g.channels + c : nullptr;
-  float w[V][K], bias[V], win[K][V], dp[K][V], dw[V][K], db[V];
+  float w[K][V], bias[V], win[K][V], dp[K][V], dw[K][V], db[V];
   load_taps<T, V, K>(g.weight, c, w);
+  load_bias<T, V>(g.bias, c, bias);
+  vset(db, 0.f);
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    bias[v] = g.bias ? to_f(static_cast<const T*>(g.bias)[c + v]) : 0.f;
-    db[v] = 0.f;
-#pragma unroll
-    for (int i = 0; i < K; ++i) dw[v][i] = dp[i][v] = win[i][v] = 0.f;
+  for (int i = 0; i < K; ++i) {
+    vset(dw[i], 0.f);
+    vset(dp[i], 0.f);
+    vset(win[i], 0.f);
   }
 #pragma unroll
   for (int i = 0; i < K - 1; ++i) {
     const int t = t0 + i - (K - 1);
     if (t < len) load_row<T, V, K>(x, init, g.sl, g.channels, t, win[i + 1]);
   }
-  (void)last;
-#pragma unroll 2
-  for (int t = t0; t < t1 + K - 1; ++t) {
+  // A token's dpre enters the window; its own tokens also add to the taps'
+  // gradients; the row element taps - 1 before it leaves.
+  auto slope = [&](const Pack<T, V>& xin, const Pack<T, V>& din) {
 #pragma unroll
     for (int i = 0; i < K - 1; ++i)
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        win[i][v] = win[i + 1][v];
-        dp[i][v] = dp[i + 1][v];
-      }
+      for (int v = 0; v < V; ++v) win[i][v] = win[i + 1][v];
+    unpack(xin, win[K - 1]);
+    unpack(din, dp[K - 1]);
+    if constexpr (SILU) {  // slope e (1 + p (1 - e)) of p e, e = sigmoid(p)
+      float p[V], e[V], one[V], f[V];
+      vset(one, 1.f);
+      vfma(p, w[0], win[0], bias);
 #pragma unroll
-    for (int v = 0; v < V; ++v) dp[K - 1][v] = 0.f;
-    if (t < len) {
-      load_row<T, V, K>(x, init, g.sl, g.channels, t, win[K - 1]);
-      const Pack<T, V> d = *reinterpret_cast<const Pack<T, V>*>(dy + (int64_t)t * g.channels);
+      for (int i = 1; i < K; ++i) vfma(p, w[i], win[i], p);
+      sigmoid(e, p);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float s = to_f(d.v[v]);
-        if constexpr (SILU) {
-          float p = bias[v];
-#pragma unroll
-          for (int i = 0; i < K; ++i) p = fmaf(w[v][i], win[i][v], p);
-          const float e = sigmoid(p);
-          s *= e * fmaf(p, 1.f - e, 1.f);
-        }
-        dp[K - 1][v] = s;
-        if (t < t1) {
-          db[v] += s;
-#pragma unroll
-          for (int i = 0; i < K; ++i) dw[v][i] = fmaf(s, win[i][v], dw[v][i]);
-        }
-      }
+      for (int v = 0; v < V; ++v) f[v] = -p[v];
+      vfma(f, f, e, p);  // p - p e
+      vadd(f, f, one);
+      vmul(f, f, e);
+      vmul(dp[K - 1], dp[K - 1], f);
     }
-    // dp[j] holds dpre of token t - (K - 1) + j; the row element of token u = t - (K - 1)
-    const int u = t - (K - 1);
-    if (u < t0 && !(t0 == 0 && dinit)) continue;
-    Pack<T, V> o;
+  };
+  auto shift = [&] {
+#pragma unroll
+    for (int i = 0; i < K - 1; ++i)
+#pragma unroll
+      for (int v = 0; v < V; ++v) dp[i][v] = dp[i + 1][v];
+  };
+  auto taps = [&] {
+    vadd(db, db, dp[K - 1]);
+#pragma unroll
+    for (int i = 0; i < K; ++i) vfma(dw[i], dp[K - 1], win[i], dw[i]);
+  };
+  // dp[j] holds dpre of token u + j; the gradient of row element u (a token, or below 0 of the initial state)
+  auto leave = [&](int u) {
+    float o[V];
     const int j = u + (K - 1) - len;
-    Pack<T, V> df;
-    const bool tail = dfinal && j >= 0 && j < K - 1;
-    if (tail) df = *reinterpret_cast<const Pack<T, V>*>(dfinal + (int64_t)j * g.channels);
+    if (dfinal && j >= 0 && j < K - 1) unpack(*reinterpret_cast<const Pack<T, V>*>(dfinal + (int64_t)j * g.channels), o);
+    else vset(o, 0.f);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float s = tail ? to_f(df.v[v]) : 0.f;
-#pragma unroll
-      for (int i = 0; i < K; ++i) s = fmaf(w[v][i], dp[K - 1 - i][v], s);
-      o.v[v] = from_f<T>(s);
-    }
+    for (int i = 0; i < K; ++i) vfma(o, w[i], dp[K - 1 - i], o);
     T* out = u >= 0 ? dx + (int64_t)u * g.channels : dinit + (int64_t)(u + K - 1) * g.channels;
-    *reinterpret_cast<Pack<T, V>*>(out) = o;
+    *reinterpret_cast<Pack<T, V>*>(out) = pack<T>(o);
+  };
+  const int t2 = t1 + K - 1, t_live = min(t2, len);
+  const T *xt = x + (int64_t)t0 * g.sl, *dt = dy + (int64_t)t0 * g.channels;
+  auto one = [&](int t) {  // any token
+    shift();
+    if (t < t_live) {
+      slope(*reinterpret_cast<const Pack<T, V>*>(xt), *reinterpret_cast<const Pack<T, V>*>(dt));
+      if (t < t1) taps();
+    } else {
+      vset(dp[K - 1], 0.f);
+    }
+    xt += g.sl;
+    dt += g.channels;
+    const int u = t - (K - 1);
+    if (u >= t0 || (t0 == 0 && dinit)) leave(u);
+  };
+  int t = t0;
+  for (; t < min(t0 + K - 1, t2); ++t) one(t);
+  // whole batches of the run's own live tokens, none of whose row elements takes a final state's gradient
+  constexpr int kAhead = 4;
+  auto fetch = [&](Pack<T, V> (&xin)[kAhead], Pack<T, V> (&din)[kAhead]) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j, xt += g.sl, dt += g.channels) {
+      xin[j] = *reinterpret_cast<const Pack<T, V>*>(xt);
+      din[j] = *reinterpret_cast<const Pack<T, V>*>(dt);
+    }
+  };
+  const int t_main = min(t1, len);
+  for (; t + kAhead <= t_main; t += kAhead) {
+    Pack<T, V> xin[kAhead], din[kAhead];
+    fetch(xin, din);
+    T* out = dx + (int64_t)(t - (K - 1)) * g.channels;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j, out += g.channels) {
+      shift();
+      slope(xin[j], din[j]);
+      taps();
+      float o[V];
+      vmul(o, w[0], dp[K - 1]);
+#pragma unroll
+      for (int i = 1; i < K; ++i) vfma(o, w[i], dp[K - 1 - i], o);
+      *reinterpret_cast<Pack<T, V>*>(out) = pack<T>(o);
+    }
   }
+  for (; t < t2; ++t) one(t);
   float* part = a.part + ((int64_t)b * g.runs + run) * (K + 1) * g.channels + c;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
 #pragma unroll
-    for (int i = 0; i < K; ++i) part[(int64_t)i * g.channels + v] = dw[v][i];
+    for (int i = 0; i < K; ++i) part[(int64_t)i * g.channels + v] = dw[i][v];
     part[(int64_t)K * g.channels + v] = db[v];
   }
 }
@@ -297,12 +377,14 @@ ConvArgs conv_args(const fhe_causal_conv_args& a, uint32_t vec, uint32_t least_r
   return g;
 }
 
-// Channels per thread: a 16-byte word forward (8 or 4), 4 backward (whose
-// registers hold twice as much), 1 where channels or alignment do not divide.
+// Channels per thread: 4 (8 or 16 bytes a load: with 8 channels the window and
+// taps leave three warps to a scheduler, 71 against 61 us at 8 x 4096 tokens of
+// 1792 bfloat16 channels), 1 where channels or alignment do not divide.
 uint32_t conv_vec(const fhe_causal_conv_args& a, uint32_t want, const void* p0, const void* p1, const void* p2) {
   const uint32_t e = elem_size(a.dtype);
   const bool ok = a.channels % want == 0 && a.x_stride[0] % want == 0 && a.x_stride[1] % want == 0 &&
-                  aligned(a.x, want * e) && aligned(a.initial_state, want * e) && aligned(p0, want * e) &&
+                  aligned(a.x, want * e) && aligned(a.initial_state, want * e) && aligned(a.weight, want * e) &&
+                  aligned(a.bias, want * e) && aligned(p0, want * e) &&
                   aligned(p1, want * e) && aligned(p2, want * e);
   return ok ? want : 1;
 }
@@ -323,7 +405,7 @@ void causal_conv(const fhe_causal_conv_args& a) {
   cudaStream_t st = static_cast<cudaStream_t>(a.stream);
   with_type(a.dtype, [&](auto tv) {
     using T = decltype(tv);
-    constexpr int kVec = sizeof(T) == 4 ? 4 : 8;
+    constexpr int kVec = 4;
     const uint32_t vec = conv_vec(a, kVec, a.y, a.length == 1 ? a.final_state : nullptr, nullptr);
     ConvArgs g = conv_args(a, vec, 4);
     const bool step = a.length == 1;

@@ -85,6 +85,90 @@ struct alignas(sizeof(T) * N) Pack {
   T v[N];
 };
 
+// Two fp32 operations per instruction (sm_100): elementwise over arrays of V,
+// pairs packed when V is even.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// o = a * b + c, o = a * b, o = a + b
+template <int V>
+__device__ __forceinline__ void vfma(float (&o)[V], const float (&a)[V], const float (&b)[V], const float (&c)[V]) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int v = 0; v < V; v += 2)
+      unpair(fma2(pair(a[v], a[v + 1]), pair(b[v], b[v + 1]), pair(c[v], c[v + 1])), o[v], o[v + 1]);
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) o[v] = fmaf(a[v], b[v], c[v]);
+  }
+}
+template <int V>
+__device__ __forceinline__ void vmul(float (&o)[V], const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int v = 0; v < V; v += 2) unpair(mul2(pair(a[v], a[v + 1]), pair(b[v], b[v + 1])), o[v], o[v + 1]);
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) o[v] = a[v] * b[v];
+  }
+}
+template <int V>
+__device__ __forceinline__ void vadd(float (&o)[V], const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int v = 0; v < V; v += 2) unpair(add2(pair(a[v], a[v + 1]), pair(b[v], b[v + 1])), o[v], o[v + 1]);
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) o[v] = a[v] + b[v];
+  }
+}
+template <int V>
+__device__ __forceinline__ void vset(float (&o)[V], float a) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) o[v] = a;
+}
+template <class T, int V>
+__device__ __forceinline__ void unpack(const Pack<T, V>& p, float (&o)[V]) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) o[v] = to_f(p.v[v]);
+}
+template <class T, int V>
+__device__ __forceinline__ Pack<T, V> pack(const float (&o)[V]) {
+  Pack<T, V> p;
+  if constexpr (V % 2 == 0 && std::is_same_v<T, __nv_bfloat16>) {
+#pragma unroll
+    for (int v = 0; v < V; v += 2)
+      *reinterpret_cast<__nv_bfloat162*>(&p.v[v]) = __floats2bfloat162_rn(o[v], o[v + 1]);
+  } else if constexpr (V % 2 == 0 && std::is_same_v<T, __half>) {
+#pragma unroll
+    for (int v = 0; v < V; v += 2) *reinterpret_cast<__half2*>(&p.v[v]) = __floats2half2_rn(o[v], o[v + 1]);
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) p.v[v] = from_f<T>(o[v]);
+  }
+  return p;
+}
+
 // Calls f with a value of the element type `dtype` names.
 template <class F>
 void with_type(int32_t dtype, F&& f) {

@@ -22,6 +22,7 @@
 
 #include "launch_count.h"
 #include "mamba_ops.h"
+#include "mamba_scan.h"
 
 namespace fhe {
 namespace {
@@ -29,44 +30,7 @@ namespace {
 constexpr int kThreads = 128;
 constexpr int kRowTile = 32;  // rows of S per block: 4 warps x 4 row pairs
 constexpr int kTok = 16;      // tokens staged per step
-
-struct Src {
-  const void* p;
-  int64_t sb, sl, sh;  // batch, token, head (or group)
-  uint32_t share;      // heads per index of the head axis
-  template <class T>
-  __device__ const T* at(uint32_t b, uint32_t h) const {
-    return static_cast<const T*>(p) + (int64_t)b * sb + (int64_t)(h / share) * sh;
-  }
-};
-
-struct Gate {
-  const float* p;
-  int64_t sb, sl, sh;
-};
-
-struct RecArgs {
-  Src r, k, q;
-  Gate write, log_decay;  // write.p == nullptr: 1
-  const int32_t* lengths;
-  uint32_t length, heads, rows, cols, seglen, nseg;
-  const float* d;         // OUT 1, 2
-  Gate out_scale;         // OUT 2: o is scaled by it
-  const float* state_in;  // slot base, or nullptr for zeros
-  float* state_out;       // or nullptr
-  // element (b, h, segment, row, col) of the states
-  int64_t in_bh, in_seg, out_bh, out_seg, st_row, st_col;
-  float* seg_decay;  // STATE pass: product of the segment's decays [bh][nseg]
-  void* out;
-  bool vec;  // r, k and q may be read four elements at a time
-};
-
-enum { kOutNone = 0, kOutY = 1, kOutDx = 2, kOutRaw = 3 };
-
-__device__ __forceinline__ int clamp_length(const int32_t* lengths, uint32_t b, uint32_t length) {
-  if (!lengths) return (int)length;
-  return min(max(lengths[b], 0), (int)length);
-}
+constexpr uint32_t kTcTokens = 64;  // shortest rows the tensor-core form takes
 
 // Four consecutive elements of a row of `width` at column col, zeros outside.
 template <class T>
@@ -120,16 +84,21 @@ __global__ void __launch_bounds__(kThreads) k_rec(const RecArgs g) {
   const float* wbase = g.write.p ? g.write.p + (int64_t)b * g.write.sb + (int64_t)h * g.write.sh : nullptr;
   const float* abase = g.log_decay.p + (int64_t)b * g.log_decay.sb + (int64_t)h * g.log_decay.sh;
 
-  float s[2][CW];
+  uint64_t s[2][CW / 2];  // two columns each
   const int64_t bh = (int64_t)b * g.heads + h;
 #pragma unroll
   for (int j = 0; j < 2; ++j)
 #pragma unroll
-    for (int i = 0; i < CW; ++i) {
-      const int row = row0 + rp + j, col = c0 + (i / 4) * 32 + (i & 3);
-      s[j][i] = (OUT != kOutNone && g.state_in && row < (int)g.rows && col < (int)g.cols)
+    for (int i = 0; i < CW; i += 2) {
+      float v[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+      const int row = row0 + rp + j, col = c0 + (i / 4) * 32 + (i & 3) + u;
+      v[u] = (OUT != kOutNone && g.state_in && row < (int)g.rows && col < (int)g.cols)
                     ? g.state_in[bh * g.in_bh + seg * g.in_seg + row * g.st_row + col * g.st_col]
                     : 0.f;
+      }
+      s[j][i / 2] = pair(v[0], v[1]);
     }
   float decay = 1.f;  // thread 0 of a STATE pass
 
@@ -177,38 +146,37 @@ __global__ void __launch_bounds__(kThreads) k_rec(const RecArgs g) {
       const int t = REV ? kTok - 1 - i : i;
       const float a = as[t], w = wsm[t];
       const float2 r2 = *reinterpret_cast<const float2*>(&rs[t][rp]);
-      const float r0 = r2.x * w, r1 = r2.y * w;
-      float o0 = 0.f, o1 = 0.f;
+      const uint64_t aa = pair(a, a), r0 = pair(r2.x * w, r2.x * w), r1 = pair(r2.y * w, r2.y * w);
+      uint64_t p0 = 0, p1 = 0;  // two columns at a time (f32x2)
 #pragma unroll
       for (int v = 0; v < CW / 4; ++v) {
-        const float4 k4 = *reinterpret_cast<const float4*>(&ks[t][c0 + 32 * v]);
-        const float kk[4] = {k4.x, k4.y, k4.z, k4.w};
-        float4 q4 = make_float4(0, 0, 0, 0);
-        if constexpr (OUT != kOutNone) q4 = *reinterpret_cast<const float4*>(&qs[t][c0 + 32 * v]);
-        const float qq[4] = {q4.x, q4.y, q4.z, q4.w};
+        const ulonglong2 k4 = *reinterpret_cast<const ulonglong2*>(&ks[t][c0 + 32 * v]);
+        ulonglong2 q4 = make_ulonglong2(0, 0);
+        if constexpr (OUT != kOutNone) q4 = *reinterpret_cast<const ulonglong2*>(&qs[t][c0 + 32 * v]);
+        const uint64_t kk[2] = {k4.x, k4.y}, qq[2] = {q4.x, q4.y};
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          float &x0 = s[0][4 * v + u], &x1 = s[1][4 * v + u];
-          if constexpr (!REV) {
-            x0 = fmaf(r0, kk[u], x0 * a);
-            x1 = fmaf(r1, kk[u], x1 * a);
-          } else {
-            x0 = fmaf(r0, kk[u], x0);
-            x1 = fmaf(r1, kk[u], x1);
-          }
+        for (int u = 0; u < 2; ++u) {
+          uint64_t &x0 = s[0][2 * v + u], &x1 = s[1][2 * v + u];
+          x0 = fma2(r0, kk[u], REV ? x0 : mul2(x0, aa));
+          x1 = fma2(r1, kk[u], REV ? x1 : mul2(x1, aa));
           if constexpr (OUT != kOutNone) {
-            o0 = fmaf(x0, qq[u], o0);
-            o1 = fmaf(x1, qq[u], o1);
+            p0 = fma2(x0, qq[u], p0);
+            p1 = fma2(x1, qq[u], p1);
           }
           if constexpr (REV) {
-            x0 *= a;
-            x1 *= a;
+            x0 = mul2(x0, aa);
+            x1 = mul2(x1, aa);
           }
         }
       }
       if constexpr (OUT == kOutNone) {
         decay *= a;
       } else {
+        float o0, o1, e0, e1;
+        unpair(p0, o0, e0);
+        unpair(p1, o1, e1);
+        o0 += e0;
+        o1 += e1;
         // lanes with bit 2 clear finish row 0, the others row 1
         const bool up = lane & 4;
         float o = (up ? o1 : o0) + __shfl_xor_sync(~0u, up ? o0 : o1, 4);
@@ -242,10 +210,15 @@ __global__ void __launch_bounds__(kThreads) k_rec(const RecArgs g) {
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int i = 0; i < CW; ++i) {
-        const int row = row0 + rp + j, col = c0 + (i / 4) * 32 + (i & 3);
-        if (row < (int)g.rows && col < (int)g.cols)
-          g.state_out[bh * g.out_bh + seg * g.out_seg + row * g.st_row + col * g.st_col] = s[j][i];
+      for (int i = 0; i < CW; i += 2) {
+        float v[2];
+        unpair(s[j][i / 2], v[0], v[1]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int row = row0 + rp + j, col = c0 + (i / 4) * 32 + (i & 3) + u;
+          if (row < (int)g.rows && col < (int)g.cols)
+            g.state_out[bh * g.out_bh + seg * g.out_seg + row * g.st_row + col * g.st_col] = v[u];
+        }
       }
   }
   if (OUT == kOutNone && tile == 0 && tid == 0) g.seg_decay[bh * g.nseg + seg] = decay;
@@ -557,6 +530,8 @@ void launch_step(const StepArgs& g, cudaStream_t st) {
 
 template <class T, bool REV, int OUT>
 void launch_rec(RecArgs g, uint32_t batch, cudaStream_t st) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>)
+    if (g.length >= kTcTokens && scan_tc_ok(g, OUT != kOutNone)) return launch_scan_tc(g, REV, OUT, batch, st);
   const uint64_t tiles = (g.rows + kRowTile - 1) / kRowTile;
   const uint64_t blocks = tiles * g.nseg * g.heads * batch;
   require(blocks < (1ull << 31), "too many blocks");
@@ -603,10 +578,12 @@ Cut forward_cut(const fhe_ssm_scan_args& a) {
   return {seglen, std::max(1u, (a.length + seglen - 1) / seglen)};
 }
 
-// The backward pass starts its running sums anew at least every 256 tokens.
+// The backward pass starts its running sums anew at every segment: of 128
+// tokens for the tensor-core form, whose products carry more rounding, of at
+// most 256 else.
 Cut backward_cut(const fhe_ssm_scan_args& a) {
   Cut c = forward_cut(a);
-  c.seglen = std::min(c.seglen, 256u);
+  c.seglen = a.dtype == FHE_BF16 && a.length >= kTcTokens ? 128u : std::min(c.seglen, 256u);
   c.nseg = std::max(1u, (a.length + c.seglen - 1) / c.seglen);
   return c;
 }
@@ -792,6 +769,7 @@ void ssm_scan_backward(const fhe_ssm_scan_grad_args& g) {
       RecArgs r = base;
       r.r = c; r.k = dy; r.q = x;
       r.state_in = s.d_slots + size;
+      r.out_scale = write;  // for the tensor-core form's roundings alone
       r.out = s.u;
       launch_rec<T, true, kOutRaw>(r, a.batch, st);
     }

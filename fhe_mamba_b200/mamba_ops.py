@@ -57,11 +57,40 @@ def _workspace(name, args, device):
     return torch.empty(n.value, dtype=torch.uint8, device=device) if n.value else None
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+# the current stream's handle of a device index, without making a Stream object
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _wants_grad(*tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _dense(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 # ---- state recurrence ---------------------------------------------------------------------------
+
+
+def _scan_fits(x, write, log_decay, B, C, D, state, lengths):
+    """Whether the arguments pass every test of ``_check_scan``, which names the one that fails."""
+    if x.dim() != 4 or B.dim() != 4:
+        return False
+    b, l, h, p = x.shape
+    k, n = B.shape[2:]
+    t, d, f, gates = x.dtype, x.device, torch.float32, (b, l, h)
+    return (t in _TYPES and x.is_cuda and k >= 1 and h >= 1 and h % k == 0 and 1 <= p <= MAX_HEAD_DIM
+            and 1 <= n <= MAX_STATE and B.shape == C.shape == (b, l, k, n) and B.dtype == C.dtype == t
+            and write.shape == log_decay.shape == gates and write.dtype == log_decay.dtype == f
+            and B.device == C.device == write.device == log_decay.device == d
+            and (D is None or (D.shape == (h,) and D.dtype == f and D.device == d))
+            and (state is None or (state.shape == (b, h, p, n) and state.dtype == f and state.device == d))
+            and (lengths is None or (lengths.shape == (b,) and lengths.dtype == torch.int32 and lengths.device == d)))
 
 
 def _check_scan(op, x, write, log_decay, B, C, D, state, lengths, state_name="initial_state"):
@@ -92,25 +121,30 @@ def _scan_args(x, write, log_decay, B, C, D, state, lengths, y, final):
         x.device.index, _TYPES[x.dtype], b, l, h, p, B.shape[3], B.shape[2],
         x.data_ptr(), x.stride()[:3], write.data_ptr(), write.stride(), log_decay.data_ptr(), log_decay.stride(),
         B.data_ptr(), B.stride()[:3], C.data_ptr(), C.stride()[:3],
-        _ptr(D), _ptr(state), _ptr(lengths), _ptr(y), _ptr(final), None, 0, _stream(x.device))
+        _ptr(D), _ptr(state), _ptr(lengths), _ptr(y), _ptr(final), None, 0, _stream_of(x.device.index))
 
 
 def _scan_forward(x, write, log_decay, B, C, D, state, lengths, y, final):
     a = _scan_args(x, write, log_decay, B, C, D, state, lengths, y, final)
-    if x.shape[1] != 1:
+    if x.shape[1] >= 128:  # shorter rows are never cut into segments
         ws = _workspace("fhe_ssm_scan_workspace", a, x.device)
         if ws is not None:
             a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
     call("fhe_ssm_scan", ctypes.byref(a))
 
 
+def _run_scan(x, write, log_decay, B, C, D, state, lengths):
+    b, _, h, p = x.shape
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    final = torch.empty((b, h, p, B.shape[3]), dtype=torch.float32, device=x.device)
+    _scan_forward(x, write, log_decay, B, C, D, state, lengths, y, final)
+    return y, final
+
+
 class _SsmScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, write, log_decay, B, C, D, state, lengths):
-        b, l, h, p = x.shape
-        y = torch.empty((b, l, h, p), dtype=x.dtype, device=x.device)
-        final = torch.empty((b, h, p, B.shape[3]), dtype=torch.float32, device=x.device)
-        _scan_forward(x, write, log_decay, B, C, D, state, lengths, y, final)
+        y, final = _run_scan(x, write, log_decay, B, C, D, state, lengths)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, write, log_decay, B, C, D, state, lengths)
         return y, final
@@ -131,7 +165,7 @@ class _SsmScan(torch.autograd.Function):
         g = _lib.SsmScanGradArgs(
             _scan_args(x, write, log_decay, B, C, D, state, lengths, None, None),
             dy.data_ptr(), _ptr(dfinal), dx.data_ptr(), dw.data_ptr(), dla.data_ptr(), db.data_ptr(), dc.data_ptr(),
-            _ptr(dd), _ptr(ds), None, 0, _stream(x.device))
+            _ptr(dd), _ptr(ds), None, 0, _stream_of(x.device.index))
         ws = _workspace("fhe_ssm_scan_backward_workspace", g, x.device)
         if ws is not None:
             g.workspace, g.workspace_bytes = ws.data_ptr(), ws.numel()
@@ -155,14 +189,25 @@ def ssm_scan(x, write, log_decay, B, C, D=None, initial_state=None, lengths=None
     state before its token, so several texts may share a row.  x, B and C may
     be slices of one activation tensor (only the last axis must be contiguous,
     else it is copied).  Gradients reach every floating-point argument."""
-    _check_scan("ssm_scan", x, write, log_decay, B, C, D, initial_state, lengths)
-    D, initial_state, lengths = (None if t is None else t.contiguous() for t in (D, initial_state, lengths))
-    return _SsmScan.apply(_inner(x), write, log_decay, _inner(B), _inner(C), D, initial_state, lengths)
+    if not _scan_fits(x, write, log_decay, B, C, D, initial_state, lengths):
+        _check_scan("ssm_scan", x, write, log_decay, B, C, D, initial_state, lengths)
+    args = (_inner(x), write, log_decay, _inner(B), _inner(C), _dense(D), _dense(initial_state), _dense(lengths))
+    if _wants_grad(x, write, log_decay, B, C, D, initial_state):
+        return _SsmScan.apply(*args)
+    return _run_scan(*args)
 
 
-def _no_grad(op, instead, *tensors):
-    _need(not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)),
-          f"{op} has no gradient (use {instead})")
+def _check_state_out(op, state, out):
+    """Where a step writes the new state: over the old one if `out` is None."""
+    _need(state.is_contiguous(), op + ": state and out must be contiguous")
+    if out is None or out is state:
+        return state
+    if out.shape != state.shape or out.dtype != state.dtype:
+        _check(op, "out", out, state.shape, state.dtype)
+    _need(out.is_contiguous(), op + ": state and out must be contiguous")
+    _need(out.device == state.device, op + ": tensors on different devices")
+    _need(out.data_ptr() == state.data_ptr() or not _overlap(out, state), op + ": out overlaps part of state")
+    return out
 
 
 def ssm_step(state, x, write, log_decay, B, C, D=None, out=None):
@@ -173,19 +218,16 @@ def ssm_step(state, x, write, log_decay, B, C, D=None, out=None):
     Returns (y, new state)."""
     op = "ssm_step"
     _need(x.dim() == 3 and B.dim() == 3 and C.dim() == 3 and write.dim() == 2 and log_decay.dim() == 2,
-          f"{op}: one token of each sequence, without a length axis")
-    _no_grad(op, "ssm_scan", state, x, write, log_decay, B, C, D)
+          "ssm_step: one token of each sequence, without a length axis")
+    if _wants_grad(state, x, write, log_decay, B, C, D):
+        _need(False, f"{op} has no gradient (use ssm_scan)")
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     x, write, log_decay, B, C = (t.unsqueeze(1) for t in (x, write, log_decay, B, C))
-    _check_scan(op, x, write, log_decay, B, C, D, state, None, "state")
-    out = state if out is None else out
-    _check(op, "out", out, state.shape, torch.float32)
-    _need(state.is_contiguous() and out.is_contiguous(), f"{op}: state and out must be contiguous")
-    _check_devices(op, x, out)
-    _need(out.data_ptr() == state.data_ptr() or not _overlap(out, state), f"{op}: out overlaps part of state")
-    y = torch.empty((x.shape[0], 1) + tuple(x.shape[2:]), dtype=x.dtype, device=x.device)
-    _scan_forward(_inner(x), write, log_decay, _inner(B), _inner(C), None if D is None else D.contiguous(), state,
-                  None, y, out)
-    return y[:, 0], out
+    if not _scan_fits(x, write, log_decay, B, C, D, state, None):
+        _check_scan(op, x, write, log_decay, B, C, D, state, None, "state")
+    out = _check_state_out(op, state, out)
+    _scan_forward(_inner(x), write, log_decay, _inner(B), _inner(C), _dense(D), state, None, y, out)
+    return y, out
 
 
 def _overlap(a, b):
@@ -195,6 +237,20 @@ def _overlap(a, b):
 
 
 # ---- causal convolution -------------------------------------------------------------------------
+
+
+def _conv_fits(x, weight, bias, state, lengths, activation):
+    """Whether the arguments pass every test of ``_check_conv``."""
+    if x.dim() != 3 or weight.dim() != 2:
+        return False
+    b, _, c = x.shape
+    k, t, d = weight.shape[1], x.dtype, x.device
+    return (t in _TYPES and x.is_cuda and c >= 1 and 1 <= k <= MAX_TAPS and weight.shape == (c, k)
+            and weight.dtype == t and weight.device == d
+            and (bias is None or (bias.shape == (c,) and bias.dtype == t and bias.device == d))
+            and (state is None or (state.shape == (b, k - 1, c) and state.dtype == t and state.device == d))
+            and (lengths is None or (lengths.shape == (b,) and lengths.dtype == torch.int32 and lengths.device == d))
+            and (activation is None or activation == "silu"))
 
 
 def _check_conv(op, x, weight, bias, state, lengths, activation, state_name="initial_state"):
@@ -219,16 +275,20 @@ def _conv_args(x, weight, bias, state, lengths, silu, y, final):
     b, l, c = x.shape
     return _lib.CausalConvArgs(
         x.device.index, _TYPES[x.dtype], b, l, c, weight.shape[1], silu, 0, x.data_ptr(), x.stride()[:2],
-        weight.data_ptr(), _ptr(bias), _ptr(state), _ptr(lengths), _ptr(y), _ptr(final), _stream(x.device))
+        weight.data_ptr(), _ptr(bias), _ptr(state), _ptr(lengths), _ptr(y), _ptr(final), _stream_of(x.device.index))
+
+
+def _run_conv(x, weight, bias, state, lengths, silu):
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    final = torch.empty((x.shape[0], weight.shape[1] - 1, x.shape[2]), dtype=x.dtype, device=x.device)
+    call("fhe_causal_conv", ctypes.byref(_conv_args(x, weight, bias, state, lengths, silu, y, final)))
+    return y, final
 
 
 class _CausalConv(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, state, lengths, silu):
-        b, l, c = x.shape
-        y = torch.empty((b, l, c), dtype=x.dtype, device=x.device)
-        final = torch.empty((b, weight.shape[1] - 1, c), dtype=x.dtype, device=x.device)
-        call("fhe_causal_conv", ctypes.byref(_conv_args(x, weight, bias, state, lengths, silu, y, final)))
+        y, final = _run_conv(x, weight, bias, state, lengths, silu)
         ctx.set_materialize_grads(False)
         ctx.silu = silu
         ctx.save_for_backward(x, weight, bias, state, lengths)
@@ -247,7 +307,7 @@ class _CausalConv(torch.autograd.Function):
         ds = torch.empty_like(state) if state is not None and ctx.needs_input_grad[3] else None
         g = _lib.CausalConvGradArgs(
             _conv_args(x, weight, bias, state, lengths, ctx.silu, None, None), dy.data_ptr(), _ptr(dfinal),
-            dx.data_ptr(), dw.data_ptr(), _ptr(db), _ptr(ds), None, 0, _stream(x.device))
+            dx.data_ptr(), dw.data_ptr(), _ptr(db), _ptr(ds), None, 0, _stream_of(x.device.index))
         ws = _workspace("fhe_causal_conv_backward_workspace", g, x.device)
         if ws is not None:
             g.workspace, g.workspace_bytes = ws.data_ptr(), ws.numel()
@@ -267,10 +327,12 @@ def causal_conv(x, weight, bias=None, initial_state=None, lengths=None, activati
     None.  All in x's type.  Returns (y, final_state): y is 0 at and past a
     row's length, final_state is the window behind its last token.  Gradients
     reach every floating-point argument."""
-    _check_conv("causal_conv", x, weight, bias, initial_state, lengths, activation)
-    weight, bias, initial_state, lengths = (None if t is None else t.contiguous()
-                                            for t in (weight, bias, initial_state, lengths))
-    return _CausalConv.apply(_inner(x), weight, bias, initial_state, lengths, activation == "silu")
+    if not _conv_fits(x, weight, bias, initial_state, lengths, activation):
+        _check_conv("causal_conv", x, weight, bias, initial_state, lengths, activation)
+    args = (_inner(x), _dense(weight), _dense(bias), _dense(initial_state), _dense(lengths), activation == "silu")
+    if _wants_grad(x, weight, bias, initial_state):
+        return _CausalConv.apply(*args)
+    return _run_conv(*args)
 
 
 def causal_conv_step(state, x, weight, bias=None, activation="silu", out=None):
@@ -278,20 +340,17 @@ def causal_conv_step(state, x, weight, bias=None, activation="silu", out=None):
     channels].  The moved window is written to `out`, or over `state` if None.
     Returns (y, new state)."""
     op = "causal_conv_step"
-    _need(x.dim() == 2, f"{op}: one token of each sequence, without a length axis")
-    _no_grad(op, "causal_conv", state, x, weight, bias)
+    _need(x.dim() == 2, "causal_conv_step: one token of each sequence, without a length axis")
+    if _wants_grad(state, x, weight, bias):
+        _need(False, f"{op} has no gradient (use causal_conv)")
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     x = x.unsqueeze(1)
-    _check_conv(op, x, weight, bias, state, None, activation, "state")
-    out = state if out is None else out
-    _check(op, "out", out, state.shape, x.dtype)
-    _need(state.is_contiguous() and out.is_contiguous(), f"{op}: state and out must be contiguous")
-    _check_devices(op, x, out)
-    _need(out.data_ptr() == state.data_ptr() or not _overlap(out, state), f"{op}: out overlaps part of state")
-    y = torch.empty((x.shape[0], 1, x.shape[2]), dtype=x.dtype, device=x.device)
-    call("fhe_causal_conv", ctypes.byref(_conv_args(_inner(x), weight.contiguous(),
-                                                    None if bias is None else bias.contiguous(), state, None,
+    if not _conv_fits(x, weight, bias, state, None, activation):
+        _check_conv(op, x, weight, bias, state, None, activation, "state")
+    out = _check_state_out(op, state, out)
+    call("fhe_causal_conv", ctypes.byref(_conv_args(_inner(x), _dense(weight), _dense(bias), state, None,
                                                     activation == "silu", y, out)))
-    return y[:, 0], out
+    return y, out
 
 
 # ---- token scores -------------------------------------------------------------------------------
@@ -308,18 +367,23 @@ def _logprob_args(logits, targets, top_k, logprob, entropy, top_logprobs, top_id
     return _lib.TokenLogprobsArgs(
         logits.device.index, _TYPES[logits.dtype], logits.shape[0], logits.shape[1], top_k, 0, logits.data_ptr(),
         logits.stride(0), targets.data_ptr(), _ptr(logprob), _ptr(entropy), _ptr(top_logprobs), _ptr(top_ids),
-        lse.data_ptr(), _stream(logits.device))
+        lse.data_ptr(), _stream_of(logits.device.index))
+
+
+def _run_logprobs(logits, targets, top_k):
+    r, d = logits.shape[0], logits.device
+    logprob = torch.empty(r, dtype=torch.float32, device=d)
+    entropy, lse = torch.empty_like(logprob), torch.empty_like(logprob)
+    top = torch.empty((r, top_k), dtype=torch.float32, device=d)
+    ids = torch.empty((r, top_k), dtype=torch.int64, device=d)
+    call("fhe_token_logprobs", ctypes.byref(_logprob_args(logits, targets, top_k, logprob, entropy, top, ids, lse)))
+    return logprob, entropy, top, ids, lse
 
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top_k):
-        r = logits.shape[0]
-        logprob, entropy, lse = (torch.empty(r, dtype=torch.float32, device=logits.device) for _ in range(3))
-        top = torch.empty((r, top_k), dtype=torch.float32, device=logits.device)
-        ids = torch.empty((r, top_k), dtype=torch.int64, device=logits.device)
-        call("fhe_token_logprobs",
-             ctypes.byref(_logprob_args(logits, targets, top_k, logprob, entropy, top, ids, lse)))
+        logprob, entropy, top, ids, lse = _run_logprobs(logits, targets, top_k)
         ctx.mark_non_differentiable(ids)
         ctx.set_materialize_grads(False)
         ctx.top_k = top_k
@@ -334,7 +398,7 @@ class _TokenLogprobs(torch.autograd.Function):
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         a = _lib.TokenLogprobsGradArgs(
             _logprob_args(logits, targets, ctx.top_k, None, entropy, None, ids, lse), _ptr(dlogprob),
-            _ptr(dentropy), _ptr(dtop) if ctx.top_k else None, out.data_ptr(), _stream(logits.device))
+            _ptr(dentropy), _ptr(dtop) if ctx.top_k else None, out.data_ptr(), _stream_of(logits.device.index))
         call("fhe_token_logprobs_backward", ctypes.byref(a))
         return out, None, None
 
@@ -349,10 +413,17 @@ def token_logprobs(logits, targets, top_k=0):
     past the vocabulary scores NaN.  Entries of -inf are impossible tokens.
     Returns a ``TokenLogprobs``; gradients of its floating-point parts reach
     the logits."""
-    op = "token_logprobs"
-    _need(logits.dim() == 2 and logits.dtype in _TYPES, f"{op}: logits must be [rows, vocab] float32, bfloat16 or float16")
-    _need(logits.shape[1] >= 1, f"{op}: an empty vocabulary")
-    _check(op, "targets", targets, (logits.shape[0],), torch.int64)
-    _need(0 <= top_k <= min(MAX_TOP, logits.shape[1]), f"{op}: top_k must be in [0, {min(MAX_TOP, logits.shape[1])}]")
-    _check_devices(op, logits, targets)
-    return TokenLogprobs(*_TokenLogprobs.apply(_inner(logits), targets.contiguous(), int(top_k)))
+    op, most = "token_logprobs", min(MAX_TOP, logits.shape[-1] if logits.dim() else 0)
+    if not (logits.dim() == 2 and logits.dtype in _TYPES and targets.shape == logits.shape[:1]
+            and targets.dtype == torch.int64 and 0 <= top_k <= most and most >= 1 and logits.is_cuda
+            and targets.device == logits.device):
+        _need(logits.dim() == 2 and logits.dtype in _TYPES,
+              f"{op}: logits must be [rows, vocab] float32, bfloat16 or float16")
+        _need(most >= 1, f"{op}: an empty vocabulary")
+        _check(op, "targets", targets, (logits.shape[0],), torch.int64)
+        _need(0 <= top_k <= most, f"{op}: top_k must be in [0, {most}]")
+        _check_devices(op, logits, targets)
+    logits, targets, top_k = _inner(logits), _dense(targets), int(top_k)
+    if _wants_grad(logits):
+        return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, top_k))
+    return TokenLogprobs(*_run_logprobs(logits, targets, top_k)[:4])

@@ -362,7 +362,8 @@ int fhe_ctx_set_keyswitch_fusion(fhe_ctx* ctx, int32_t fused);
  * EvalLinearTransform performs.  Results agree within the key switching
  * noise, not word for word. */
 int fhe_ctx_set_giant_hoisting(fhe_ctx* ctx, int32_t on);
-/* Number of tensor-core conversion blocks whose bounded wait for their MMA
+/* Number of tensor-core blocks (basis conversions, state scans) whose bounded
+ * wait for their MMA
  * ran out (their outputs were skipped); 0 on a healthy device. */
 int fhe_tc_timeouts(uint64_t* count);
 
