@@ -17,12 +17,15 @@
 // bfloat16 terms (2^-16).  E o w o r, whose sum is the fp32 state, always
 // enters as two terms.
 //
-// One CTA walks one (batch, head, 64 rows, segment).  Shared memory holds q,
-// k, r and S0 in 128-byte-swizzled tiles of 64 columns; the scaled r takes
+// One CTA walks one (batch, head, tile of rows, segment).  Shared memory holds
+// q, k, r and S0 in 128-byte-swizzled tiles of 64 columns; the scaled r takes
 // q's place once q has been used, which keeps two CTAs on an SM, so that one
 // computes while the other waits for its loads or its products.  Tensor
-// memory: G (its columns become the A operand G o L o w), O and S'.  The state
-// itself stays in registers.
+// memory: G (its columns become the A operand G o L o w), O (which starts from
+// the scaled q S0^T) and S'.  The state itself stays in registers.
+//
+// A walk that carries no state on (CARRY false: the gradients', a segment of
+// one chunk each) leaves S' out and takes 128 rows where there are as many.
 #include <algorithm>
 
 #include "launch_count.h"
@@ -33,10 +36,9 @@ namespace fhe {
 namespace {
 
 constexpr uint32_t kQ = 128;            // tokens per chunk (MMA M)
-constexpr uint32_t kRowsTc = 64;        // rows per CTA (MMA N)
 constexpr uint32_t kThreadsTc = 256;
 constexpr uint32_t kTile = kQ * 128;    // bytes of a 128 x 64 tile
-constexpr uint32_t kTmemCols = 256;     // G 128, O 64, S' 64
+constexpr uint32_t kTmemCols = 256;     // G 128; O 64 and S' 64, or O 128
 constexpr uint32_t kColO = 128, kColS = 192;
 // More than a third of an SM's shared memory: at most two CTAs are resident,
 // whose tensor memory (2 x 256 columns) fits.
@@ -117,6 +119,15 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&u)[16]
       "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const float (&v)[32]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t u[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(v[16 * h + i]);
+    tmem_st16(addr + 16 * h, u);
+  }
+}
 __device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // 16 bytes to shared memory, the first `bytes` of them from src and zeros after.
@@ -124,82 +135,165 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t b
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+__device__ __forceinline__ uint32_t pack2(uint64_t p) {
+  float a, b;
+  unpair(p, a, b);
   uint32_t v;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(b), "f"(a));
   return v;
 }
-__device__ __forceinline__ float low(uint32_t v) { return __uint_as_float(v << 16); }
-__device__ __forceinline__ float high(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
+__device__ __forceinline__ uint64_t unpack2(uint32_t v) {
+  return pair(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
 // The two bfloat16 terms of a pair of floats.
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = pack2(a, b);
-  lo = pack2(a - low(hi), b - high(hi));
+__device__ __forceinline__ void split2(uint64_t p, uint32_t& hi, uint32_t& lo) {
+  hi = pack2(p);
+  lo = pack2(fma2(unpack2(hi), pair(-1.f, -1.f), p));
+}
+
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one;
 }
 
 // Byte offset of 16-byte word `word` of row `row` in a 128-byte-swizzled tile.
 __device__ __forceinline__ uint32_t swz(uint32_t row, uint32_t word) { return row * 128 + ((word ^ (row & 7)) << 4); }
 
+// Products of decays of one chunk, over blocks of 32 tokens and of 8.
 struct Gates {
   float a[kQ], w[kQ];    // decay and write of each token
   float head[kQ];        // product over its block of 32 up to and with the token
-  float tail[kQ];        // product over its block after the token
-  float col[kQ];         // the column factor times w: tail (forward) or head (reversed)
-  float total[4];        // product over each block
+  float tail[kQ];        // product over its block of 32 after the token
+  float col[kQ];         // column factor for rows of other blocks of 32: tail (reversed: head) times w
+  float col8[kQ];        // and for rows of other blocks of 8 in its block of 32
+  float total[4];        // product over each block of 32
 };
 
-// One block of 32 columns of G o L o w for one row, in place in v; `own` is
-// the row's own block.  `scale` multiplies the row (it is in `row` already).
+// Warps 0-3, one token per thread.
 template <bool REV>
-__device__ __forceinline__ void weigh(float (&v)[32], const Gates& g, uint32_t blk, bool own, uint32_t lane, float row,
-                                      float scale) {
-  const uint32_t s0 = blk * 32;
-  if (!own) {
+__device__ __forceinline__ void put_gates(Gates& g, uint32_t t, uint32_t lane, float a, float w) {
+  const float after = __shfl_down_sync(~0u, a, 1);
+  const int in = lane & 7;
+  float head = a, head8 = a, tail = lane == 31 ? 1.f : after, tail8 = in == 7 ? 1.f : after;
 #pragma unroll
-    for (int i = 0; i < 32; i += 4) {
-      const float4 c = *reinterpret_cast<const float4*>(&g.col[s0 + i]);
-      v[i] *= row * c.x;
-      v[i + 1] *= row * c.y;
-      v[i + 2] *= row * c.z;
-      v[i + 3] *= row * c.w;
+  for (int o = 1; o < 32; o <<= 1) {
+    const float u = __shfl_up_sync(~0u, head, o), d = __shfl_down_sync(~0u, tail, o);
+    if ((int)lane >= o) head *= u;
+    if ((int)lane + o < 32) tail *= d;
+    if (o < 8) {
+      const float u8 = __shfl_up_sync(~0u, head8, o), d8 = __shfl_down_sync(~0u, tail8, o);
+      if (in >= o) head8 *= u8;
+      if (in + o < 8) tail8 *= d8;
     }
-    return;
   }
-  float p = 1.f;
+  g.a[t] = a;
+  g.w[t] = w;
+  g.head[t] = head;
+  g.tail[t] = tail;
+  g.col[t] = (REV ? head : tail) * w;
+  g.col8[t] = (REV ? head8 : tail8) * w;
+  if (lane == 31) g.total[t >> 5] = head;
+}
+
+// A row's factors within its own block of 32, times `scale`: `own` for the
+// columns of its block of 8 (zero off the triangle), `row` for the columns of
+// the other blocks of 8, times their col8.
+struct OwnBlock {
+  float own[8], row[4];
+};
+template <bool REV>
+__device__ __forceinline__ OwnBlock own_block(const Gates& g, uint32_t t, uint32_t lane, float scale) {
+  OwnBlock o;
+  const uint32_t s0 = t & ~7u;
+  const int sub = lane >> 3, in = lane & 7;
+  float a[8], w[8];
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    if constexpr (!REV) {
-      const int i = 31 - j;  // p = product of a over (i, lane]
-      if (i < 31) p = i < (int)lane ? p * g.a[s0 + i + 1] : 1.f;
-      v[i] = i <= (int)lane ? v[i] * (scale * (p * g.w[s0 + i])) : 0.f;
-    } else {
-      const int i = j;       // p = product of a over (lane, i]
-      p = i > (int)lane ? p * g.a[s0 + i] : 1.f;
-      v[i] = i >= (int)lane ? v[i] * (scale * (p * g.w[s0 + i])) : 0.f;
+  for (int i = 0; i < 8; i += 4) {
+    const float4 x = *reinterpret_cast<const float4*>(&g.a[s0 + i]), y = *reinterpret_cast<const float4*>(&g.w[s0 + i]);
+    a[i] = x.x, a[i + 1] = x.y, a[i + 2] = x.z, a[i + 3] = x.w;
+    w[i] = y.x, w[i + 1] = y.y, w[i + 2] = y.z, w[i + 3] = y.w;
+  }
+  float p = scale, all = 1.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int i = REV ? j : 7 - j;
+    // scale times the product of a over (i, in], or over (in, i]
+    if constexpr (REV) p = i > in ? p * a[i] : scale;
+    else if (i < 7) p = i < in ? p * a[i + 1] : scale;
+    o.own[i] = (REV ? i >= in : i <= in) ? p * w[i] : 0.f;
+    all *= a[i];
+  }
+  const float edge = REV ? p : p * a[0];  // to the end (the start, with the token) of its block of 8
+  float tot[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) tot[j] = __shfl_sync(~0u, all, 8 * j);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float r = edge;
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+      if (REV ? (m > sub && m < j) : (m > j && m < sub)) r *= tot[m];
+    o.row[j] = (REV ? j > sub : j < sub) ? r : 0.f;
+  }
+  return o;
+}
+
+// 32 columns of G o L o w for one row, in place: columns of another block of
+// 32, and of the row's own.
+__device__ __forceinline__ void weigh(float (&v)[32], const float* col, float row) {
+  const uint64_t rr = pair(row, row);
+#pragma unroll
+  for (int i = 0; i < 32; i += 4) {
+    const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(col + i);
+    unpair(mul2(pair(v[i], v[i + 1]), mul2(rr, c.x)), v[i], v[i + 1]);
+    unpair(mul2(pair(v[i + 2], v[i + 3]), mul2(rr, c.y)), v[i + 2], v[i + 3]);
+  }
+}
+__device__ __forceinline__ void weigh_own(float (&v)[32], const float* col8, const OwnBlock& o, uint32_t lane) {
+  const int sub = lane >> 3;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint64_t rr = pair(o.row[j], o.row[j]);
+    const bool mine = sub == j;
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(col8 + 8 * j + i);
+      float f[4];
+      unpair(mul2(rr, c.x), f[0], f[1]);
+      unpair(mul2(rr, c.y), f[2], f[3]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = mine ? o.own[i + e] : f[e];
+      float* x = v + 8 * j + i;
+      unpair(mul2(pair(x[0], x[1]), pair(f[0], f[1])), x[0], x[1]);
+      unpair(mul2(pair(x[2], x[3]), pair(f[2], f[3])), x[2], x[3]);
     }
   }
 }
 
-// COLS: columns held, 64 or 128 (those past g.cols are zeros).
-template <int COLS, bool REV, int OUT, bool PRECISE>
+// COLS: columns held, 64 or 128 (those past g.cols are zeros); ROWS: rows per
+// CTA, 64 or 128 (128 only without CARRY).
+template <int COLS, int ROWS, bool REV, int OUT, bool PRECISE, bool CARRY>
 __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g) {
-  constexpr uint32_t kHalves = COLS / 64;
+  static_assert(CARRY ? ROWS == 64 : OUT != kOutNone, "shapes");
+  constexpr uint32_t kHalves = COLS / 64, kRowTiles = ROWS / 64;
+  constexpr uint32_t kBytesQ = CARRY ? 2 * kTile : kHalves * kTile;  // q, then the scaled r (two terms)
   constexpr uint32_t kBytesK = kHalves * kTile;
-  constexpr uint32_t kBytesS = COLS * 128;
+  constexpr uint32_t kBytesR = kRowTiles * kTile;
+  constexpr uint32_t kTileS = COLS * 128, kBytesS = kRowTiles * kTileS;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ Gates gate;
+  __shared__ __align__(16) Gates gate;
   __shared__ __align__(8) uint64_t bars[3];  // G and q S0, S', O
   __shared__ uint32_t tslot;
-  const uint32_t sq = smem_u32(smem);            // q, then the scaled r (two terms)
-  const uint32_t sk = sq + 2 * kTile;
-  const uint32_t sr = sk + kBytesK;
-  const uint32_t ss = sr + kTile;                // S0 (two terms with PRECISE)
+  const uint32_t sq = smem_u32(smem), sk = sq + kBytesQ, sr = sk + kBytesK;
+  const uint32_t ss = sr + kBytesR;  // S0 (two terms with PRECISE)
   const uint32_t bar_g = smem_u32(&bars[0]), bar_s = bar_g + 8, bar_o = bar_g + 16;
 
-  const uint32_t tiles = (g.rows + kRowsTc - 1) / kRowsTc;
+  const uint32_t tiles = (g.rows + ROWS - 1) / ROWS;
   uint32_t id = blockIdx.x;
-  const uint32_t row0 = id % tiles * kRowsTc;
+  const uint32_t row0 = id % tiles * ROWS;
   id /= tiles;
   const uint32_t h = id % g.heads;
   id /= g.heads;
@@ -207,6 +301,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g) {
   const int64_t bh = (int64_t)b * g.heads + h;
   const int len = clamp_length(g.lengths, b, g.length);
   const int t_lo = seg * g.seglen, t_hi = min(t_lo + (int)g.seglen, (int)g.length);
+  const int t_end = min(t_hi, len);  // live tokens: [t_lo, t_end)
   const int chunks = (t_hi - t_lo + (int)kQ - 1) / (int)kQ;
 
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -227,87 +322,100 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g) {
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
 
-  auto first = [&](int i) { return REV ? t_hi - (int)kQ * (i + 1) : t_lo + (int)kQ * i; };
-  auto live = [&](int tok) { return tok >= t_lo && tok < t_hi && tok < len; };
-  // A [128][COLS] tile: 16-byte words, columns past `cols` and dead tokens zero.
-  auto load_cols = [&](uint32_t dst, const T* p, int64_t sl, int t0) {
+  auto first = [&](int i) { return t_lo + (int)kQ * (REV ? chunks - 1 - i : i); };
+  // 128 tokens of 16-byte words; words past `width` elements and dead tokens zero.
+  auto load = [&](uint32_t dst, const T* p, int64_t sl, int width, int t0, auto words) {
+    constexpr uint32_t kWords = decltype(words)::value, kStep = kThreadsTc / kWords;
+    const uint32_t word = tid % kWords, row = tid / kWords;
+    const int n = min(max((width - (int)word * 8) * 2, 0), 16);
+    int tok = t0 + (int)row;
+    const T* src = p + (int64_t)tok * sl + word * 8;
+    uint32_t to = dst + (word >> 3) * kTile + swz(row, word & 7);
 #pragma unroll
-    for (uint32_t e = tid; e < kQ * COLS / 8; e += kThreadsTc) {
-      const uint32_t row = e / (COLS / 8), word = e % (COLS / 8);
-      const int tok = t0 + (int)row, col = (int)word * 8;
-      const int n = live(tok) ? min(max(((int)g.cols - col) * 2, 0), 16) : 0;
-      copy16(dst + (word >> 3) * kTile + swz(row, word & 7), n ? p + (int64_t)tok * sl + col : p, n);
+    for (uint32_t i = 0; i < kQ / kStep; ++i) {
+      const bool in = n > 0 && tok < t_end;
+      copy16(to, in ? src : p, in ? n : 0);
+      src += (int64_t)kStep * sl;
+      to += kStep * 128;
+      tok += kStep;
     }
   };
   auto load_rows = [&](int t0) {
-#pragma unroll
-    for (uint32_t e = tid; e < kQ * 8; e += kThreadsTc) {
-      const uint32_t row = e / 8, word = e % 8;
-      const int tok = t0 + (int)row, col = (int)word * 8;
-      const int n = live(tok) ? min(max(((int)g.rows - (int)row0 - col) * 2, 0), 16) : 0;
-      copy16(sr + swz(row, word), n ? rp + (int64_t)tok * g.r.sl + col : rp, n);
-    }
+    load(sr, rp, g.r.sl, (int)g.rows - (int)row0, t0, std::integral_constant<uint32_t, ROWS / 8>{});
   };
   auto load_kq = [&](int t0) {
-    load_cols(sk, kp, g.k.sl, t0);
-    if constexpr (OUT != kOutNone) load_cols(sq, qp, g.q.sl, t0);
+    load(sk, kp, g.k.sl, (int)g.cols, t0, std::integral_constant<uint32_t, COLS / 8>{});
+    if constexpr (OUT != kOutNone)
+      load(sq, qp, g.q.sl, (int)g.cols, t0, std::integral_constant<uint32_t, COLS / 8>{});
   };
-
-  // The state: column t of rows half * 32 + i.
-  float s[32];
-#pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    const uint32_t row = row0 + half * 32 + i;
-    s[i] = (OUT != kOutNone && g.state_in && row < g.rows && t < g.cols)
-               ? g.state_in[bh * g.in_bh + seg * g.in_seg + row * g.st_row + t * g.st_col]
-               : 0.f;
-  }
-  auto put_state = [&] {  // S0 as the B operand [column][row]
-    if (t >= (uint32_t)COLS) return;
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      uint4 hi, lo;
-      split2(s[8 * v], s[8 * v + 1], hi.x, lo.x);
-      split2(s[8 * v + 2], s[8 * v + 3], hi.y, lo.y);
-      split2(s[8 * v + 4], s[8 * v + 5], hi.z, lo.z);
-      split2(s[8 * v + 6], s[8 * v + 7], hi.w, lo.w);
-      const uint32_t at = ss - sq + swz(t, half * 4 + v);
-      *reinterpret_cast<uint4*>(smem + at) = hi;
-      if constexpr (PRECISE) *reinterpret_cast<uint4*>(smem + at + kBytesS) = lo;
-    }
-  };
-  if constexpr (OUT != kOutNone) put_state();
   load_kq(first(0));
   load_rows(first(0));
 
   const float* wp = g.write.p ? g.write.p + (int64_t)b * g.write.sb + (int64_t)h * g.write.sh : nullptr;
   const float* ap = g.log_decay.p + (int64_t)b * g.log_decay.sb + (int64_t)h * g.log_decay.sh;
+  float next_a = 0.f, next_w = 0.f;  // warps 0-3: the gates of the chunk to come
+  auto load_gates = [&](int t0) {
+    const int tok = t0 + (int)t;
+    const bool l = tid < kQ && tok < t_end;
+    next_a = l ? ap[(int64_t)tok * g.log_decay.sl] : 0.f;
+    next_w = l ? (wp ? wp[(int64_t)tok * g.write.sl] : 1.f) : 0.f;
+  };
+  load_gates(first(0));
+  const float skip = (OUT == kOutY || OUT == kOutDx) && g.d ? g.d[h] : 0.f;
+
+  // The state: column t of 32 rows, in pairs; without CARRY only on its way to
+  // shared memory, where it is the B operand [column][row].
+  uint64_t s[16];
+  auto put_state = [&](uint32_t piece) {
+    if (t >= (uint32_t)COLS) return;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (PRECISE) split2(s[4 * v + e], hi[e], lo[e]);
+        else hi[e] = pack2(s[4 * v + e]);
+      }
+      const uint32_t at = ss - sq + (piece >> 1) * kTileS + swz(t, (piece & 1) * 4 + v);
+      *reinterpret_cast<uint4*>(smem + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      if constexpr (PRECISE) *reinterpret_cast<uint4*>(smem + at + kBytesS) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+  };
+  const float* s_in = OUT != kOutNone && g.state_in && t < g.cols
+                          ? g.state_in + bh * g.in_bh + seg * g.in_seg + (int64_t)t * g.st_col : nullptr;
+#pragma unroll
+  for (uint32_t u = 0; u < kRowTiles; ++u) {
+    const uint32_t piece = half * kRowTiles + u;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t row = row0 + piece * 32 + 2 * i;
+      s[i] = pair(s_in && row < g.rows ? s_in[row * g.st_row] : 0.f,
+                  s_in && row + 1 < g.rows ? s_in[(row + 1) * g.st_row] : 0.f);
+    }
+    if constexpr (OUT != kOutNone) put_state(piece);
+  }
+
   float decay = 1.f;
   uint32_t tmem = 0;
+  const uint32_t lanes = (quarter * 32) << 16;
   bool ok = true;
   int done = 0;  // chunks whose products were issued
   for (int i = 0; i < chunks; ++i) {
-    const int t0 = first(i);
+    const int t0 = first(i), tok = t0 + (int)t;
+    const bool live = tok < t_end;
     const uint32_t par = i & 1;
-    if (tid < kQ) {  // warps 0-3: the block's decays and their products
-      const int tok = t0 + (int)t;
-      const bool l = live(tok);
-      const float a = l ? expf(ap[(int64_t)tok * g.log_decay.sl]) : 1.f;
-      const float w = l ? (wp ? wp[(int64_t)tok * g.write.sl] : 1.f) : 0.f;
-      float head = a, tail = __shfl_down_sync(~0u, a, 1);
-      if (lane == 31) tail = 1.f;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const float u = __shfl_up_sync(~0u, head, o), d = __shfl_down_sync(~0u, tail, o);
-        if ((int)lane >= o) head *= u;
-        if ((int)lane + o < 32) tail *= d;
+    if (tid < kQ) put_gates<REV>(gate, t, lane, expf(next_a), next_w);
+    // Row scale of this token's products: w of dx; for U of the gradients the
+    // mantissa of w, so that its products are rounded at w_t times their value
+    // as those of dC_h are, up to a power of two.  alpha and beta, whose
+    // difference is summed, then carry the same roundings and the sum loses them.
+    float rho = 1.f;
+    if constexpr (OUT == kOutDx || (REV && OUT == kOutRaw)) {
+      rho = live ? g.out_scale.p[b * g.out_scale.sb + tok * g.out_scale.sl + h * g.out_scale.sh] : 1.f;
+      if constexpr (OUT == kOutRaw) {
+        const uint32_t bits = __float_as_uint(rho);
+        rho = (bits >> 23 & 0xff) - 1u < 0xfeu ? __uint_as_float((bits & 0x7fffffu) | 0x3f800000u) : 1.f;
       }
-      gate.a[t] = a;
-      gate.w[t] = w;
-      gate.head[t] = head;
-      gate.tail[t] = tail;
-      gate.col[t] = (REV ? head : tail) * w;
-      if (lane == 31) gate.total[quarter] = head;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     fence_async();
@@ -316,8 +424,8 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g) {
     fence_after();
     if (!ok) break;
     tmem = tslot;
-    if constexpr (OUT != kOutNone) {
-      if (tid == 0) {
+    if (OUT != kOutNone && warp == 0) {
+      if (elect_one()) {
 #pragma unroll
         for (uint32_t j = 0; j < COLS / 16; ++j) {
           const uint32_t at = (j >> 2) * kTile + (j & 3) * 32;
@@ -326,101 +434,94 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g) {
 #pragma unroll
         for (uint32_t j = 0; j < COLS / 16; ++j) {
           const uint32_t at = (j >> 2) * kTile + (j & 3) * 32;
-          mma_ss(tmem + kColO, desc(sq + at, 16), desc(ss + j * 2048, 0), idesc(kRowsTc, false, true), j);
+          mma_ss(tmem + kColO, desc(sq + at, 16), desc(ss + j * 2048, kTileS), idesc(ROWS, false, true), j);
           if constexpr (PRECISE)
-            mma_ss(tmem + kColO, desc(sq + at, 16), desc(ss + kBytesS + j * 2048, 0), idesc(kRowsTc, false, true), 1);
+            mma_ss(tmem + kColO, desc(sq + at, 16), desc(ss + kBytesS + j * 2048, kTileS), idesc(ROWS, false, true), 1);
         }
         commit(bar_g);
       }
+      __syncwarp();
     }
-    // products over blocks around this row's and token's own
+    if (i + 1 < chunks) load_gates(first(i + 1));
+    // products over the blocks around this row's own
     float before = 1.f, after = 1.f;
 #pragma unroll
     for (uint32_t u = 0; u < 4; ++u) {
       if (u < quarter) before *= gate.total[u];
       if (u > quarter) after *= gate.total[u];
     }
-    const float head = gate.head[t], tail = gate.tail[t], w = gate.w[t];
-    const float pt = REV ? tail * after : head * before;
-    const float et = (REV ? head * before : tail * after) * w;
+    const float head = gate.head[t], tail = gate.tail[t];
+    const float pt = (REV ? tail * after : head * before) * rho;
+    const float et = (REV ? head * before : tail * after) * gate.w[t];
     const float all = gate.total[0] * gate.total[1] * gate.total[2] * gate.total[3];
     decay *= all;
-    const uint32_t lanes = (quarter * 32) << 16;
-    float acc[OUT == kOutNone ? 1 : 32];
+    const uint32_t blk_own = quarter;
+    const bool owner = half == (quarter == 1 || quarter == 2 ? 1u : 0u);  // half 0: blocks 0 and 3, half 1: 1 and 2
+    OwnBlock ob;
     if constexpr (OUT != kOutNone) {
-      __syncwarp();
+      if (owner) ob = own_block<REV>(gate, t, lane, rho);
       ok = __all_sync(~0u, wait(bar_g, par));
       done = i + 1;
       fence_after();
-      if (ok) {
-        tmem_ld32(tmem + lanes + kColO + half * 32, acc);
-        ld_wait();
-      }
     }
-    const float skip = (OUT == kOutY || OUT == kOutDx) && g.d ? g.d[h] : 0.f;
-    float oscale = 1.f;
-    // U of the gradients: its products are rounded at w_t times their value, as
-    // those of dC_h are, with the power of two of w_t left out.  alpha and beta,
-    // whose difference is summed, then carry the same roundings and the sum
-    // loses them.
-    float mant = 1.f;
-    if constexpr (REV && OUT == kOutRaw) {
-      const int tok = t0 + (int)t;
-      const float ws = live(tok) ? g.out_scale.p[b * g.out_scale.sb + tok * g.out_scale.sl + h * g.out_scale.sh] : 1.f;
-      const uint32_t bits = __float_as_uint(ws);
-      if ((bits >> 23 & 0xff) - 1u < 0xfeu) mant = __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
-      oscale = 1.f / mant;
-    }
-    if constexpr (OUT == kOutDx) {
-      const int tok = t0 + (int)t;
-      oscale = live(tok) ? g.out_scale.p[b * g.out_scale.sb + tok * g.out_scale.sl + h * g.out_scale.sh] : 0.f;
-    }
-    // the scaled r in two terms, over q; with it P_t (q S0) and the skip term
     if (ok) {
+      // O starts from P_t (q S0) and the skip term; the scaled r, in two terms, goes over q
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const uint32_t at = swz(t, half * 4 + v);
-        const uint4 x = *reinterpret_cast<const uint4*>(smem + (sr - sq) + at);
-        const uint32_t u[4] = {x.x, x.y, x.z, x.w};
-        uint32_t hi[4], lo[4];
+      for (uint32_t u = 0; u < kRowTiles; ++u) {
+        const uint32_t piece = half * kRowTiles + u;
+        float v[32];
+        if constexpr (OUT != kOutNone) {
+          tmem_ld32(tmem + lanes + kColO + piece * 32, v);
+          ld_wait();
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float x0 = low(u[e]), x1 = high(u[e]);
-          split2(et * x0, et * x1, hi[e], lo[e]);
-          if constexpr (OUT != kOutNone) {
-            float &o0 = acc[8 * v + 2 * e], &o1 = acc[8 * v + 2 * e + 1];
-            o0 *= pt;
-            o1 *= pt;
-            if constexpr (OUT == kOutDx) {
-              o0 *= oscale;
-              o1 *= oscale;
+          const uint32_t at = (piece >> 1) * kTile + swz(t, (piece & 1) * 4 + e);
+          uint32_t x[4] = {0, 0, 0, 0};
+          if constexpr (CARRY || OUT == kOutY || OUT == kOutDx) {
+            const uint4 q4 = *reinterpret_cast<const uint4*>(smem + (sr - sq) + at);
+            x[0] = q4.x, x[1] = q4.y, x[2] = q4.z, x[3] = q4.w;
+          }
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int f = 0; f < 4; ++f) {
+            const uint64_t xx = unpack2(x[f]);
+            if constexpr (CARRY) split2(mul2(pair(et, et), xx), hi[f], lo[f]);
+            if constexpr (OUT != kOutNone) {
+              float *o = v + 8 * e + 2 * f;
+              uint64_t a = mul2(pair(pt, pt), pair(o[0], o[1]));
+              if constexpr (OUT == kOutY || OUT == kOutDx) a = fma2(pair(skip, skip), xx, a);
+              unpair(a, o[0], o[1]);
             }
-            o0 = fmaf(skip, x0, o0);
-            o1 = fmaf(skip, x1, o1);
+          }
+          if constexpr (CARRY) {
+            *reinterpret_cast<uint4*>(smem + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(smem + kTile + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
           }
         }
-        *reinterpret_cast<uint4*>(smem + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(smem + kTile + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        if constexpr (OUT != kOutNone) tmem_st32(tmem + lanes + kColO + piece * 32, v);
       }
       if constexpr (OUT != kOutNone) {
 #pragma unroll
         for (uint32_t u = 0; u < 2; ++u) {
-          const uint32_t blk = half * 2 + u;
+          const uint32_t blk = half ? 1 + u : 3 * u;
           const bool zero = REV ? blk < quarter : blk > quarter;
           uint32_t hi[16], lo[16];
           if (!zero) {
             float v[32];
             tmem_ld32(tmem + lanes + blk * 32, v);
-            ld_wait();
-            float row = (REV ? tail : head) * mant;  // times the blocks between
+            float row = (REV ? tail : head) * rho;  // times the blocks between
 #pragma unroll
             for (uint32_t m = 0; m < 4; ++m)
               if (REV ? (m > quarter && m < blk) : (m > blk && m < quarter)) row *= gate.total[m];
-            weigh<REV>(v, gate, blk, blk == quarter, lane, row, mant);
+            ld_wait();
+            if (blk == blk_own) weigh_own(v, &gate.col8[blk * 32], ob, lane);
+            else weigh(v, &gate.col[blk * 32], row);
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              if constexpr (PRECISE) split2(v[2 * e], v[2 * e + 1], hi[e], lo[e]);
-              else hi[e] = pack2(v[2 * e], v[2 * e + 1]);
+              const uint64_t p = pair(v[2 * e], v[2 * e + 1]);
+              if constexpr (PRECISE) split2(p, hi[e], lo[e]);
+              else hi[e] = pack2(p);
             }
           } else {
 #pragma unroll
@@ -437,36 +538,46 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g) {
     ok = __syncthreads_and(ok);
     fence_after();
     if (!ok) break;
-    if (tid == 0) {
-      const uint32_t lead = kHalves == 2 ? kTile : 0;
+    if (warp == 0) {
+      if (elect_one()) {
+        if constexpr (CARRY) {
+          const uint32_t lead = kHalves == 2 ? kTile : 0;
 #pragma unroll
-      for (uint32_t j = 0; j < kQ / 16; ++j) {
-        const uint64_t a = desc(sk + j * 2048, lead);
-        mma_ss(tmem + kColS, a, desc(sq + j * 2048, 0), idesc(kRowsTc, true, true), j);
-        mma_ss(tmem + kColS, a, desc(sq + kTile + j * 2048, 0), idesc(kRowsTc, true, true), 1);
-      }
-      commit(bar_s);
-      if constexpr (OUT != kOutNone) {
-#pragma unroll
-        for (uint32_t j = 0; j < kQ / 16; ++j) {
-          const uint32_t a = tmem + (j >> 1) * 32 + (j & 1) * 8;
-          mma_ts(tmem + kColO, a, desc(sr + j * 2048, 0), idesc(kRowsTc, false, true), j);
-          if constexpr (PRECISE) mma_ts(tmem + kColO, a + 16, desc(sr + j * 2048, 0), idesc(kRowsTc, false, true), 1);
+          for (uint32_t j = 0; j < kQ / 16; ++j) {
+            const uint64_t a = desc(sk + j * 2048, lead);
+            mma_ss(tmem + kColS, a, desc(sq + j * 2048, 0), idesc(64, true, true), j);
+            mma_ss(tmem + kColS, a, desc(sq + kTile + j * 2048, 0), idesc(64, true, true), 1);
+          }
+          commit(bar_s);
         }
-        commit(bar_o);
-      }
-    }
-    __syncwarp();
-    ok = __all_sync(~0u, wait(bar_s, par));
-    fence_after();
-    if (ok) {
-      if (i + 1 < chunks) load_kq(first(i + 1));  // q's and k's places are free
-      float v[32];
-      tmem_ld32(tmem + lanes + kColS + half * 32, v);
-      ld_wait();
+        if constexpr (OUT != kOutNone) {
 #pragma unroll
-      for (int e = 0; e < 32; ++e) s[e] = fmaf(all, s[e], v[e]);
-      if constexpr (OUT != kOutNone) put_state();
+          for (uint32_t j = 0; j < kQ / 16; ++j) {
+            const uint32_t a = tmem + (j >> 1) * 32 + (j & 1) * 8;
+            mma_ts(tmem + kColO, a, desc(sr + j * 2048, kTile), idesc(ROWS, false, true), 1);
+            if constexpr (PRECISE)
+              mma_ts(tmem + kColO, a + 16, desc(sr + j * 2048, kTile), idesc(ROWS, false, true), 1);
+          }
+          commit(bar_o);
+        }
+      }
+      __syncwarp();
+    }
+    if constexpr (CARRY) {
+      ok = __all_sync(~0u, wait(bar_s, par));
+      done = i + 1;
+      fence_after();
+      if (ok) {
+        if (i + 1 < chunks) load_kq(first(i + 1));  // q's and k's places are free
+        float v[32];
+        tmem_ld32(tmem + lanes + kColS + half * 32, v);
+        ld_wait();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = fma2(pair(all, all), s[e], pair(v[2 * e], v[2 * e + 1]));
+        if constexpr (OUT != kOutNone) {
+          if (i + 1 < chunks) put_state(half);
+        }
+      }
     }
     if constexpr (OUT == kOutNone) {
       if (ok && i + 1 < chunks) load_rows(first(i + 1));
@@ -474,29 +585,35 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g) {
       ok = __all_sync(~0u, wait(bar_o, par)) && ok;
       fence_after();
       if (ok) {
-        if (i + 1 < chunks) load_rows(first(i + 1));
-        float v[32];
-        tmem_ld32(tmem + lanes + kColO + half * 32, v);
-        ld_wait();
-        const int tok = t0 + (int)t;
-        const uint32_t row = row0 + half * 32;
-        if (tok >= t_lo && tok < t_hi && row < g.rows && (OUT != kOutRaw || tok < len)) {
-          const bool l = tok < len;
-          const int64_t at = (((int64_t)b * g.length + tok) * g.heads + h) * g.rows + row;
+        if (i + 1 < chunks) {
+          if constexpr (!CARRY) load_kq(first(i + 1));
+          load_rows(first(i + 1));
+        }
+        const float inv = OUT == kOutRaw && REV ? 1.f / rho : 1.f;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = l ? fmaf(oscale, v[e], acc[e]) : 0.f;
-          if constexpr (OUT == kOutRaw) {
-            float* o = static_cast<float*>(g.out) + at;
+        for (uint32_t u = 0; u < kRowTiles; ++u) {
+          const uint32_t piece = half * kRowTiles + u, row = row0 + piece * 32;
+          float v[32];
+          tmem_ld32(tmem + lanes + kColO + piece * 32, v);
+          ld_wait();
+          if (tok < t_hi && row < g.rows && (OUT != kOutRaw || live)) {
+            const int64_t at = (((int64_t)b * g.length + tok) * g.heads + h) * g.rows + row;
+            if constexpr (OUT == kOutRaw) {
+              float* o = static_cast<float*>(g.out) + at;
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              if (row + e < g.rows) *reinterpret_cast<float4*>(o + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-          } else {
-            T* o = static_cast<T*>(g.out) + at;
+              for (int e = 0; e < 32; e += 4)
+                if (row + e < g.rows)
+                  *reinterpret_cast<float4*>(o + e) = make_float4(inv * v[e], inv * v[e + 1], inv * v[e + 2], inv * v[e + 3]);
+            } else {
+              T* o = static_cast<T*>(g.out) + at;
 #pragma unroll
-            for (int e = 0; e < 32; e += 8)
-              if (row + e < g.rows)
-                *reinterpret_cast<uint4*>(o + e) = make_uint4(pack2(v[e], v[e + 1]), pack2(v[e + 2], v[e + 3]),
-                                                              pack2(v[e + 4], v[e + 5]), pack2(v[e + 6], v[e + 7]));
+              for (int e = 0; e < 32; e += 8) {
+                uint32_t x[4];
+#pragma unroll
+                for (int f = 0; f < 4; ++f) x[f] = live ? pack2(pair(v[e + 2 * f], v[e + 2 * f + 1])) : 0u;
+                if (row + e < g.rows) *reinterpret_cast<uint4*>(o + e) = make_uint4(x[0], x[1], x[2], x[3]);
+              }
+            }
           }
         }
       }
@@ -504,12 +621,15 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g) {
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
   if (ok) {
-    if (g.state_out) {
+    if (CARRY && g.state_out && t < g.cols) {
+      float* o = g.state_out + bh * g.out_bh + seg * g.out_seg + (int64_t)t * g.st_col;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const uint32_t row = row0 + half * 32 + i;
-        if (row < g.rows && t < g.cols)
-          g.state_out[bh * g.out_bh + seg * g.out_seg + row * g.st_row + t * g.st_col] = s[i];
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t row = row0 + half * 32 + 2 * i;
+        float a, c;
+        unpair(s[i], a, c);
+        if (row < g.rows) o[row * g.st_row] = a;
+        if (row + 1 < g.rows) o[(row + 1) * g.st_row] = c;
       }
     }
     if (OUT == kOutNone && row0 == 0 && tid == 0) g.seg_decay[bh * g.nseg + seg] = decay;
@@ -518,9 +638,9 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g) {
     atomicAdd(&g_scan_timeouts, 1u);
     if (done) {
       const uint32_t par = (done - 1) & 1;
-      wait(bar_g, par);
-      wait(bar_s, par);
-      wait(bar_o, par);
+      if (OUT != kOutNone) wait(bar_g, par);
+      if (CARRY) wait(bar_s, par);
+      if (OUT != kOutNone) wait(bar_o, par);
     }
   }
   fence_before();
@@ -530,15 +650,16 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tslot), "r"(kTmemCols));
 }
 
-template <int COLS, bool REV, int OUT, bool PRECISE>
+template <int COLS, int ROWS, bool REV, int OUT, bool PRECISE, bool CARRY>
 void launch(const RecArgs& g, uint32_t batch, cudaStream_t st) {
-  const uint32_t need = 1024 + 2 * kTile + COLS / 64 * kTile + kTile + COLS * 128 * (PRECISE ? 2 : 1);
+  const uint32_t need = 1024 + (CARRY ? 2 : COLS / 64) * kTile + COLS / 64 * kTile + ROWS / 64 * kTile +
+                        COLS * 128 * (ROWS / 64) * (PRECISE ? 2 : 1);
   const uint32_t smem = std::max(need, kLeastSmem);
-  FHE_CUDA(cudaFuncSetAttribute(k_scan_tc<COLS, REV, OUT, PRECISE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)smem));
-  const uint64_t blocks = (uint64_t)((g.rows + kRowsTc - 1) / kRowsTc) * g.heads * g.nseg * batch;
+  auto* kernel = k_scan_tc<COLS, ROWS, REV, OUT, PRECISE, CARRY>;
+  FHE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  const uint64_t blocks = (uint64_t)((g.rows + ROWS - 1) / ROWS) * g.heads * g.nseg * batch;
   require(blocks < (1ull << 31), "too many blocks");
-  k_scan_tc<COLS, REV, OUT, PRECISE><<<(uint32_t)blocks, kThreadsTc, smem, st>>>(g);
+  kernel<<<(uint32_t)blocks, kThreadsTc, smem, st>>>(g);
   note_launch();
   FHE_CUDA(cudaGetLastError());
 }
@@ -556,14 +677,20 @@ bool scan_tc_ok(const RecArgs& g, bool needs_q) {
 void launch_scan_tc(const RecArgs& g, bool rev, int out, uint32_t batch, cudaStream_t st) {
   auto go = [&](auto cols) {
     constexpr int C = decltype(cols)::value;
-    if (!rev && out == kOutNone) launch<C, false, kOutNone, false>(g, batch, st);
-    else if (!rev && out == kOutY) launch<C, false, kOutY, false>(g, batch, st);
-    else if (!rev && out == kOutRaw) launch<C, false, kOutRaw, true>(g, batch, st);
-    else if (rev && out == kOutNone) launch<C, true, kOutNone, false>(g, batch, st);
-    else if (rev && out == kOutDx) launch<C, true, kOutDx, false>(g, batch, st);
-    else if (rev && out == kOutRaw) launch<C, true, kOutRaw, true>(g, batch, st);
-    else require(false, "unknown walk", FHE_ERR_INTERNAL);
+    if (!rev && out == kOutNone) launch<C, 64, false, kOutNone, false, true>(g, batch, st);
+    else if (!rev && out == kOutY) launch<C, 64, false, kOutY, false, true>(g, batch, st);
+    else if (rev && out == kOutNone) launch<C, 64, true, kOutNone, false, true>(g, batch, st);
+    else if (rev && out == kOutDx) launch<C, 64, true, kOutDx, false, false>(g, batch, st);
+    else if (out == kOutRaw && g.rows <= 64) {
+      if (rev) launch<C, 64, true, kOutRaw, true, false>(g, batch, st);
+      else launch<C, 64, false, kOutRaw, true, false>(g, batch, st);
+    } else if (out == kOutRaw) {
+      if (rev) launch<C, 128, true, kOutRaw, true, false>(g, batch, st);
+      else launch<C, 128, false, kOutRaw, true, false>(g, batch, st);
+    } else require(false, "unknown walk", FHE_ERR_INTERNAL);
   };
+  // without a carried state a segment is one chunk
+  require(out == kOutNone || out == kOutY || g.seglen == kQ, "segment of more than one chunk", FHE_ERR_INTERNAL);
   if (g.cols <= 64) go(std::integral_constant<int, 64>{});
   else go(std::integral_constant<int, 128>{});
 }
