@@ -531,7 +531,7 @@ void launch_step(const StepArgs& g, cudaStream_t st) {
 template <class T, bool REV, int OUT>
 void launch_rec(RecArgs g, uint32_t batch, cudaStream_t st) {
   if constexpr (std::is_same_v<T, __nv_bfloat16>)
-    if (g.length >= kTcTokens && scan_tc_ok(g, OUT != kOutNone)) return launch_scan_tc(g, REV, OUT, batch, st);
+    if (g.length >= kTcTokens && launch_scan_tc(g, REV, OUT, batch, st)) return;
   const uint64_t tiles = (g.rows + kRowTile - 1) / kRowTile;
   const uint64_t blocks = tiles * g.nseg * g.heads * batch;
   require(blocks < (1ull << 31), "too many blocks");
@@ -567,8 +567,20 @@ struct Cut {
   uint32_t seglen, nseg;
 };
 
+bool tc_type(const fhe_ssm_scan_args& a) { return a.dtype == FHE_BF16 && a.length >= kTcTokens; }
+
 // Rows are cut when the (batch, head, row tile) blocks alone leave SMs idle.
 Cut forward_cut(const fhe_ssm_scan_args& a) {
+  if (tc_type(a)) {
+    // two CTAs of 64 rows to an SM; segments of whole chunks of 128 tokens
+    const uint64_t blocks = (uint64_t)a.batch * a.heads * ((a.head_dim + 63) / 64);
+    const uint32_t chunks = (a.length + 127) / 128;
+    uint32_t nseg = 1;
+    if (blocks < 148) nseg = (uint32_t)std::min<uint64_t>(296 / std::max<uint64_t>(blocks, 1), std::max(1u, chunks / 2));
+    nseg = std::max(1u, nseg);
+    const uint32_t seglen = (chunks + nseg - 1) / nseg * 128;
+    return {seglen, std::max(1u, (a.length + seglen - 1) / seglen)};
+  }
   const uint64_t blocks = (uint64_t)a.batch * a.heads * ((a.head_dim + kRowTile - 1) / kRowTile);
   uint32_t nseg = 1;
   if (blocks < 148 * 2) nseg = (uint32_t)(148 * 4 / std::max<uint64_t>(blocks, 1));
@@ -583,7 +595,7 @@ Cut forward_cut(const fhe_ssm_scan_args& a) {
 // most 256 else.
 Cut backward_cut(const fhe_ssm_scan_args& a) {
   Cut c = forward_cut(a);
-  c.seglen = a.dtype == FHE_BF16 && a.length >= kTcTokens ? 128u : std::min(c.seglen, 256u);
+  c.seglen = tc_type(a) ? 128u : std::min(c.seglen, 256u);
   c.nseg = std::max(1u, (a.length + c.seglen - 1) / c.seglen);
   return c;
 }

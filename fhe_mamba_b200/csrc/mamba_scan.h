@@ -42,9 +42,9 @@ __device__ __forceinline__ int clamp_length(const int32_t* lengths, uint32_t b, 
   return min(max(lengths[b], 0), (int)length);
 }
 
-// The tensor-core form (mamba_scan_tc.cu), bfloat16 only.
-bool scan_tc_ok(const RecArgs& g, bool needs_q);
-void launch_scan_tc(const RecArgs& g, bool rev, int out, uint32_t batch, cudaStream_t st);
+// The tensor-core form (mamba_scan_tc.cu), bfloat16 only; false, with nothing
+// launched, for sizes and layouts that it does not take.
+bool launch_scan_tc(const RecArgs& g, bool rev, int out, uint32_t batch, cudaStream_t st);
 unsigned scan_tc_timeouts();
 
 }  // namespace fhe

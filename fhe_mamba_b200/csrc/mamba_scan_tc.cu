@@ -27,6 +27,7 @@
 // A walk that carries no state on (CARRY false: the gradients', a segment of
 // one chunk each) leaves S' out and takes 128 rows where there are as many.
 #include <algorithm>
+#include <cuda.h>
 
 #include "launch_count.h"
 #include "mamba_ops.h"
@@ -130,9 +131,22 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const float (&v)[32]) {
 }
 __device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 16 bytes to shared memory, the first `bytes` of them from src and zeros after.
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+// Tensor maps of q, k and r: [batch][token][head or group][column or row], a
+// box of 64 columns x 128 tokens.  The tensor's extents end at the row's
+// length, columns and rows, past which a box is filled with zeros.
+struct Maps {
+  CUtensorMap q, k, r;
+};
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int col, int head, int tok, int batch,
+                                         uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(dst),
+      "l"(map), "r"(col), "r"(head), "r"(tok), "r"(batch), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 
 __device__ __forceinline__ uint32_t pack2(uint64_t p) {
@@ -275,7 +289,7 @@ __device__ __forceinline__ void weigh_own(float (&v)[32], const float* col8, con
 // COLS: columns held, 64 or 128 (those past g.cols are zeros); ROWS: rows per
 // CTA, 64 or 128 (128 only without CARRY).
 template <int COLS, int ROWS, bool REV, int OUT, bool PRECISE, bool CARRY>
-__global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g) {
+__global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, const __grid_constant__ Maps maps) {
   static_assert(CARRY ? ROWS == 64 : OUT != kOutNone, "shapes");
   constexpr uint32_t kHalves = COLS / 64, kRowTiles = ROWS / 64;
   constexpr uint32_t kBytesQ = CARRY ? 2 * kTile : kHalves * kTile;  // q, then the scaled r (two terms)
@@ -285,11 +299,12 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ __align__(16) Gates gate;
-  __shared__ __align__(8) uint64_t bars[3];  // G and q S0, S', O
+  __shared__ __align__(8) uint64_t bars[5];  // G and q S0, S', O; k and q have arrived, r has
   __shared__ uint32_t tslot;
   const uint32_t sq = smem_u32(smem), sk = sq + kBytesQ, sr = sk + kBytesK;
   const uint32_t ss = sr + kBytesR;  // S0 (two terms with PRECISE)
-  const uint32_t bar_g = smem_u32(&bars[0]), bar_s = bar_g + 8, bar_o = bar_g + 16;
+  const uint32_t bar_g = smem_u32(&bars[0]), bar_s = bar_g + 8, bar_o = bar_g + 16, bar_kq = bar_g + 24,
+                 bar_r = bar_g + 32;
 
   const uint32_t tiles = (g.rows + ROWS - 1) / ROWS;
   uint32_t id = blockIdx.x;
@@ -308,9 +323,6 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g) {
   const uint32_t quarter = warp & 3, half = warp >> 2;
   const uint32_t t = quarter * 32 + lane;  // this thread's token, and column of S
   using T = __nv_bfloat16;
-  const T* rp = g.r.at<T>(b, h) + row0;
-  const T* kp = g.k.at<T>(b, h);
-  const T* qp = g.q.at<T>(b, h);
 
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tslot)),
@@ -318,38 +330,37 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g) {
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   if (tid == 0) {
-    for (int i = 0; i < 3; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar_g + 8 * i));
+    for (int i = 0; i < 5; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar_g + 8 * i));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
 
   auto first = [&](int i) { return t_lo + (int)kQ * (REV ? chunks - 1 - i : i); };
-  // 128 tokens of 16-byte words; words past `width` elements and dead tokens zero.
-  auto load = [&](uint32_t dst, const T* p, int64_t sl, int width, int t0, auto words) {
-    constexpr uint32_t kWords = decltype(words)::value, kStep = kThreadsTc / kWords;
-    const uint32_t word = tid % kWords, row = tid / kWords;
-    const int n = min(max((width - (int)word * 8) * 2, 0), 16);
-    int tok = t0 + (int)row;
-    const T* src = p + (int64_t)tok * sl + word * 8;
-    uint32_t to = dst + (word >> 3) * kTile + swz(row, word & 7);
-#pragma unroll
-    for (uint32_t i = 0; i < kQ / kStep; ++i) {
-      const bool in = n > 0 && tok < t_end;
-      copy16(to, in ? src : p, in ? n : 0);
-      src += (int64_t)kStep * sl;
-      to += kStep * 128;
-      tok += kStep;
-    }
-  };
+  // One thread: the boxes of a chunk.
   auto load_rows = [&](int t0) {
-    load(sr, rp, g.r.sl, (int)g.rows - (int)row0, t0, std::integral_constant<uint32_t, ROWS / 8>{});
+    expect(bar_r, kBytesR);
+#pragma unroll
+    for (uint32_t j = 0; j < kRowTiles; ++j) load_box(sr + j * kTile, &maps.r, row0 + 64 * j, h / g.r.share, t0, b, bar_r);
   };
   auto load_kq = [&](int t0) {
-    load(sk, kp, g.k.sl, (int)g.cols, t0, std::integral_constant<uint32_t, COLS / 8>{});
-    if constexpr (OUT != kOutNone)
-      load(sq, qp, g.q.sl, (int)g.cols, t0, std::integral_constant<uint32_t, COLS / 8>{});
+    expect(bar_kq, kBytesK * (OUT != kOutNone ? 2 : 1));
+#pragma unroll
+    for (uint32_t j = 0; j < kHalves; ++j) {
+      load_box(sk + j * kTile, &maps.k, 64 * j, h / g.k.share, t0, b, bar_kq);
+      if constexpr (OUT != kOutNone) load_box(sq + j * kTile, &maps.q, 64 * j, h / g.q.share, t0, b, bar_kq);
+    }
   };
-  load_kq(first(0));
-  load_rows(first(0));
+  // Tokens past the sequence's end that lie within the row were loaded too:
+  // this thread's words of them become zeros.
+  auto clear = [&](uint32_t tile, uint32_t count) {
+    for (uint32_t j = 0; j < count; ++j)
+#pragma unroll
+      for (uint32_t v = 0; v < 4; ++v)
+        *reinterpret_cast<uint4*>(smem + (tile - sq) + j * kTile + swz(t, half * 4 + v)) = make_uint4(0, 0, 0, 0);
+  };
+  if (tid == 0) {
+    load_kq(first(0));
+    load_rows(first(0));
+  }
 
   const float* wp = g.write.p ? g.write.p + (int64_t)b * g.write.sb + (int64_t)h * g.write.sh : nullptr;
   const float* ap = g.log_decay.p + (int64_t)b * g.log_decay.sb + (int64_t)h * g.log_decay.sh;
@@ -417,12 +428,28 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g) {
         rho = (bits >> 23 & 0xff) - 1u < 0xfeu ? __uint_as_float((bits & 0x7fffffu) | 0x3f800000u) : 1.f;
       }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (i > 0) {  // (the barriers are initialised before the first)
+      ok = __all_sync(~0u, wait(bar_kq, par)) && ok;
+      if (!live) {
+        clear(sk, kHalves);
+        if constexpr (OUT != kOutNone) clear(sq, kHalves);
+      }
+    }
     fence_async();
     fence_before();
     ok = __syncthreads_and(ok);
     fence_after();
     if (!ok) break;
+    if (i == 0) {
+      ok = __all_sync(~0u, wait(bar_kq, par));
+      if (!live) {
+        clear(sk, kHalves);
+        if constexpr (OUT != kOutNone) clear(sq, kHalves);
+      }
+      fence_async();
+      ok = __syncthreads_and(ok);
+      if (!ok) break;
+    }
     tmem = tslot;
     if (OUT != kOutNone && warp == 0) {
       if (elect_one()) {
@@ -464,6 +491,8 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g) {
       done = i + 1;
       fence_after();
     }
+    ok = __all_sync(~0u, wait(bar_r, par)) && ok;
+    if (!live) clear(sr, kRowTiles);
     if (ok) {
       // O starts from P_t (q S0) and the skip term; the scaled r, in two terms, goes over q
 #pragma unroll
@@ -568,7 +597,8 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g) {
       done = i + 1;
       fence_after();
       if (ok) {
-        if (i + 1 < chunks) load_kq(first(i + 1));  // q's and k's places are free
+        if (i + 1 < chunks && tid == 0) load_kq(first(i + 1));  // q's and k's places are free
+        __syncwarp();
         float v[32];
         tmem_ld32(tmem + lanes + kColS + half * 32, v);
         ld_wait();
@@ -580,15 +610,13 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g) {
       }
     }
     if constexpr (OUT == kOutNone) {
-      if (ok && i + 1 < chunks) load_rows(first(i + 1));
+      if (ok && i + 1 < chunks && tid == 0) load_rows(first(i + 1));
     } else {
       ok = __all_sync(~0u, wait(bar_o, par)) && ok;
       fence_after();
       if (ok) {
-        if (i + 1 < chunks) {
-          if constexpr (!CARRY) load_kq(first(i + 1));
-          load_rows(first(i + 1));
-        }
+        if (i + 1 < chunks && tid == 0) load_rows(first(i + 1));
+        __syncwarp();
         const float inv = OUT == kOutRaw && REV ? 1.f / rho : 1.f;
 #pragma unroll
         for (uint32_t u = 0; u < kRowTiles; ++u) {
@@ -604,22 +632,45 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g) {
               for (int e = 0; e < 32; e += 4)
                 if (row + e < g.rows)
                   *reinterpret_cast<float4*>(o + e) = make_float4(inv * v[e], inv * v[e + 1], inv * v[e + 2], inv * v[e + 3]);
-            } else {
-              T* o = static_cast<T*>(g.out) + at;
+            }
+          }
+          if constexpr (OUT != kOutRaw) {
+            // Four lanes hold 64 bytes of four tokens each; transposed among
+            // them, every store covers whole 64-byte runs of eight tokens.
+            uint32_t x[4][4];
 #pragma unroll
-              for (int e = 0; e < 32; e += 8) {
-                uint32_t x[4];
+            for (int e = 0; e < 4; ++e)
 #pragma unroll
-                for (int f = 0; f < 4; ++f) x[f] = live ? pack2(pair(v[e + 2 * f], v[e + 2 * f + 1])) : 0u;
-                if (row + e < g.rows) *reinterpret_cast<uint4*>(o + e) = make_uint4(x[0], x[1], x[2], x[3]);
+              for (int f = 0; f < 4; ++f) x[e][f] = live ? pack2(pair(v[8 * e + 2 * f], v[8 * e + 2 * f + 1])) : 0u;
+#pragma unroll
+            for (int d = 1; d < 4; d *= 2) {
+              const bool up = lane & d;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if (e & d) continue;
+#pragma unroll
+                for (int f = 0; f < 4; ++f) {
+                  const uint32_t send = up ? x[e][f] : x[e + d][f];
+                  const uint32_t got = __shfl_xor_sync(~0u, send, d);
+                  if (up) x[e][f] = got;
+                  else x[e + d][f] = got;
+                }
               }
+            }
+            // x[e]: word lane & 3 of the token 4 (lane / 4) + e of the warp's 32
+            const uint32_t col = row + 8 * (lane & 3);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int tk = t0 + (int)(quarter * 32 + (lane & ~3u) + e);
+              if (tk < t_hi && col < g.rows)
+                *reinterpret_cast<uint4*>(static_cast<T*>(g.out) + (((int64_t)b * g.length + tk) * g.heads + h) * g.rows +
+                                          col) = make_uint4(x[e][0], x[e][1], x[e][2], x[e][3]);
             }
           }
         }
       }
     }
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
   if (ok) {
     if (CARRY && g.state_out && t < g.cols) {
       float* o = g.state_out + bh * g.out_bh + seg * g.out_seg + (int64_t)t * g.st_col;
@@ -642,6 +693,11 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g) {
       if (CARRY) wait(bar_s, par);
       if (OUT != kOutNone) wait(bar_o, par);
     }
+    // phases of the loads: the last issued completes with either parity seen
+    wait(bar_kq, 0);
+    wait(bar_kq, 1);
+    wait(bar_r, 0);
+    wait(bar_r, 1);
   }
   fence_before();
   __syncthreads();
@@ -650,8 +706,42 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tslot), "r"(kTmemCols));
 }
 
+using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                            const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                            CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+Encode encoder() {
+  static const Encode fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<Encode>(p);
+  }();
+  return fn;
+}
+
+// The map of one operand; false if its layout has none.
+bool make_map(CUtensorMap& m, const Src& s, uint32_t width, const RecArgs& g, uint32_t batch) {
+  const Encode fn = encoder();
+  if (!fn) return false;
+  const uint64_t dims[4] = {width, g.heads / s.share, g.length, batch};
+  const int64_t at[3] = {s.sh, s.sl, s.sb};
+  uint64_t strides[3];
+  for (int i = 0; i < 3; ++i) {
+    if (dims[i + 1] > 1 && (at[i] <= 0 || at[i] % 8 != 0)) return false;
+    strides[i] = dims[i + 1] > 1 ? (uint64_t)at[i] * 2 : 16;  // an axis of one element never moves
+  }
+  const cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]}, st[3] = {strides[0], strides[1], strides[2]};
+  const cuuint32_t box[4] = {64, 1, kQ, 1}, step[4] = {1, 1, 1, 1};
+  return reinterpret_cast<uintptr_t>(s.p) % 16 == 0 &&
+         fn(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(s.p), d, st, box, step,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int COLS, int ROWS, bool REV, int OUT, bool PRECISE, bool CARRY>
-void launch(const RecArgs& g, uint32_t batch, cudaStream_t st) {
+void launch(const RecArgs& g, const Maps& maps, uint32_t batch, cudaStream_t st) {
   const uint32_t need = 1024 + (CARRY ? 2 : COLS / 64) * kTile + COLS / 64 * kTile + ROWS / 64 * kTile +
                         COLS * 128 * (ROWS / 64) * (PRECISE ? 2 : 1);
   const uint32_t smem = std::max(need, kLeastSmem);
@@ -659,40 +749,38 @@ void launch(const RecArgs& g, uint32_t batch, cudaStream_t st) {
   FHE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   const uint64_t blocks = (uint64_t)((g.rows + ROWS - 1) / ROWS) * g.heads * g.nseg * batch;
   require(blocks < (1ull << 31), "too many blocks");
-  kernel<<<(uint32_t)blocks, kThreadsTc, smem, st>>>(g);
+  kernel<<<(uint32_t)blocks, kThreadsTc, smem, st>>>(g, maps);
   note_launch();
   FHE_CUDA(cudaGetLastError());
 }
 
 }  // namespace
 
-bool scan_tc_ok(const RecArgs& g, bool needs_q) {
-  auto aligned = [](const Src& s) {
-    return reinterpret_cast<uintptr_t>(s.p) % 16 == 0 && s.sb % 8 == 0 && s.sl % 8 == 0 && s.sh % 8 == 0;
-  };
-  return g.cols <= 128 && g.rows % 8 == 0 && aligned(g.r) && aligned(g.k) && (!needs_q || aligned(g.q)) &&
-         reinterpret_cast<uintptr_t>(g.out) % 16 == 0;
-}
-
-void launch_scan_tc(const RecArgs& g, bool rev, int out, uint32_t batch, cudaStream_t st) {
+bool launch_scan_tc(const RecArgs& g, bool rev, int out, uint32_t batch, cudaStream_t st) {
+  Maps maps{};
+  if (g.cols > 128 || g.rows % 8 != 0 || g.seglen % kQ != 0 || reinterpret_cast<uintptr_t>(g.out) % 16 != 0 ||
+      !make_map(maps.k, g.k, g.cols, g, batch) || !make_map(maps.r, g.r, g.rows, g, batch) ||
+      (out != kOutNone && !make_map(maps.q, g.q, g.cols, g, batch)))
+    return false;
   auto go = [&](auto cols) {
     constexpr int C = decltype(cols)::value;
-    if (!rev && out == kOutNone) launch<C, 64, false, kOutNone, false, true>(g, batch, st);
-    else if (!rev && out == kOutY) launch<C, 64, false, kOutY, false, true>(g, batch, st);
-    else if (rev && out == kOutNone) launch<C, 64, true, kOutNone, false, true>(g, batch, st);
-    else if (rev && out == kOutDx) launch<C, 64, true, kOutDx, false, false>(g, batch, st);
+    if (!rev && out == kOutNone) launch<C, 64, false, kOutNone, false, true>(g, maps, batch, st);
+    else if (!rev && out == kOutY) launch<C, 64, false, kOutY, false, true>(g, maps, batch, st);
+    else if (rev && out == kOutNone) launch<C, 64, true, kOutNone, false, true>(g, maps, batch, st);
+    else if (rev && out == kOutDx) launch<C, 64, true, kOutDx, false, false>(g, maps, batch, st);
     else if (out == kOutRaw && g.rows <= 64) {
-      if (rev) launch<C, 64, true, kOutRaw, true, false>(g, batch, st);
-      else launch<C, 64, false, kOutRaw, true, false>(g, batch, st);
+      if (rev) launch<C, 64, true, kOutRaw, true, false>(g, maps, batch, st);
+      else launch<C, 64, false, kOutRaw, true, false>(g, maps, batch, st);
     } else if (out == kOutRaw) {
-      if (rev) launch<C, 128, true, kOutRaw, true, false>(g, batch, st);
-      else launch<C, 128, false, kOutRaw, true, false>(g, batch, st);
+      if (rev) launch<C, 128, true, kOutRaw, true, false>(g, maps, batch, st);
+      else launch<C, 128, false, kOutRaw, true, false>(g, maps, batch, st);
     } else require(false, "unknown walk", FHE_ERR_INTERNAL);
   };
   // without a carried state a segment is one chunk
   require(out == kOutNone || out == kOutY || g.seglen == kQ, "segment of more than one chunk", FHE_ERR_INTERNAL);
   if (g.cols <= 64) go(std::integral_constant<int, 64>{});
   else go(std::integral_constant<int, 128>{});
+  return true;
 }
 
 unsigned scan_tc_timeouts() {
