@@ -325,12 +325,22 @@ __global__ void k_join(float* slots, const float* seg_decay, const float* start,
 }
 
 // gamma[bh][s] = <gradient, state> at the end of segment s.
-__global__ void k_anchor(const float* s_slots, const float* d_slots, float* gamma, uint32_t nseg, uint32_t size) {
+__global__ void __launch_bounds__(256) k_anchor(const float* s_slots, const float* d_slots, float* gamma, uint32_t nseg,
+                                                uint32_t size) {
   const int64_t bh = blockIdx.x / nseg;
   const uint32_t seg = blockIdx.x % nseg;
   const int64_t at = (bh * (nseg + 1) + seg + 1) * (int64_t)size;
   float v = 0.f;
-  for (uint32_t i = threadIdx.x; i < size; i += blockDim.x) v = fmaf(s_slots[at + i], d_slots[at + i], v);
+  if (size % 4 == 0) {  // the slots start 256-byte aligned
+    const float4 *s = reinterpret_cast<const float4*>(s_slots + at), *d = reinterpret_cast<const float4*>(d_slots + at);
+#pragma unroll 8
+    for (uint32_t i = threadIdx.x; i < size / 4; i += 256) {
+      const float4 x = s[i], y = d[i];
+      v = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, v))));
+    }
+  } else {
+    for (uint32_t i = threadIdx.x; i < size; i += 256) v = fmaf(s_slots[at + i], d_slots[at + i], v);
+  }
   __shared__ float part[8];
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
@@ -354,80 +364,109 @@ struct SumArgs {
   float* skip;  // [b][length][heads]: <dy, x>, or nullptr
 };
 
-// One block per token: sums U and dC_h over the heads of each group in a
-// fixed order and forms the per-head products.  Memory-bound: it reads the
-// two per-head arrays once.
-constexpr int kSumWarps = 8;
-template <class T>
-__global__ void __launch_bounds__(32 * kSumWarps) k_sum(const SumArgs g) {
-  __shared__ float part[2][kSumWarps][256];
-  const uint32_t t = blockIdx.x % g.length, b = blockIdx.x / g.length;
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// Sums COUNT values of every lane over the warp; lane i ends with the sum of
+// value i % COUNT (a power of two): each step halves the values a lane holds.
+template <int COUNT>
+__device__ __forceinline__ float sum_each(float (&v)[COUNT], uint32_t lane) {
+#pragma unroll
+  for (int n = COUNT / 2; n >= 1; n /= 2) {
+    const bool up = lane & n;
+#pragma unroll
+    for (int i = 0; i < n; ++i) v[i] = (up ? v[i + n] : v[i]) + __shfl_xor_sync(~0u, up ? v[i] : v[i + n], n);
+  }
+  float r = v[0];
+#pragma unroll
+  for (int o = COUNT; o < 32; o <<= 1) r += __shfl_xor_sync(~0u, r, o);
+  return r;
+}
+
+// One warp per token: sums U and dC_h over the heads of each group in order
+// and forms the per-head products.  Memory-bound: it reads the two per-head
+// arrays once, H heads at a time with all their loads in flight.  A lane holds
+// V neighbouring columns of every 32 V, NP of those.
+template <class T, int V, int NP, int H>
+__global__ void __launch_bounds__(128) k_sum(const SumArgs g, uint32_t tokens) {
+  const uint32_t id = (blockIdx.x * 128 + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+  if (id >= tokens) return;
+  const uint32_t t = id % g.length, b = id / g.length;
   const bool live = (int)t < clamp_length(g.lengths, b, g.length);
   const uint32_t each = g.heads / g.groups, N = g.d_state, P = g.head_dim;
-  const int64_t tok = (int64_t)b * g.length + t;
+  const int64_t tok = id;
   for (uint32_t grp = 0; grp < g.groups; ++grp) {
     const T* bp = g.b.at<T>(b, grp * each) + (int64_t)t * g.b.sl;
     const T* cp = g.c.at<T>(b, grp * each) + (int64_t)t * g.c.sl;
-    float sb[8], sc[8], bv[8], cv[8];
+    float bv[NP][V], cv[NP][V], sb[NP][V], sc[NP][V];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t n = lane + 32 * i;
-      sb[i] = sc[i] = 0.f;
-      bv[i] = live && n < N ? to_f(bp[n]) : 0.f;
-      cv[i] = live && n < N ? to_f(cp[n]) : 0.f;
-    }
-    for (uint32_t hh = warp; hh < each; hh += kSumWarps) {
-      const uint32_t h = grp * each + hh;
-      const int64_t at = tok * g.heads + h;
-      float dw = 0.f, alpha = 0.f, skip = 0.f, w = 0.f;
-      if (live) {
-        w = g.write.p[b * g.write.sb + t * g.write.sl + h * g.write.sh];
+    for (int i = 0; i < NP; ++i)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t n = lane + 32 * i;
-          if (n < N) {
-            const float u = g.u[at * N + n], dch = g.dch[at * N + n];
-            dw = fmaf(bv[i], u, dw);
-            alpha = fmaf(cv[i], dch, alpha);
-            sb[i] = fmaf(w, u, sb[i]);
-            sc[i] += dch;
+      for (int v = 0; v < V; ++v) {
+        const uint32_t n = (i * 32 + lane) * V + v;
+        bv[i][v] = live && n < N ? to_f(bp[n]) : 0.f;
+        cv[i][v] = live && n < N ? to_f(cp[n]) : 0.f;
+        sb[i][v] = sc[i][v] = 0.f;
+      }
+    for (uint32_t h0 = 0; h0 < each; h0 += H) {
+      Pack<float, V> u[H][NP], dc[H][NP];
+      // lane j < H: write of head h0 + j
+      const uint32_t mine = grp * each + h0 + lane % H;
+      const bool has = live && h0 + lane % H < each;
+      const float wl = has ? g.write.p[b * g.write.sb + t * g.write.sl + mine * g.write.sh] : 0.f;
+#pragma unroll
+      for (int j = 0; j < H; ++j)
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const uint32_t n = (i * 32 + lane) * V;
+          const int64_t at = (tok * g.heads + grp * each + h0 + j) * N + n;
+#pragma unroll
+          for (int v = 0; v < V; ++v) u[j][i].v[v] = dc[j][i].v[v] = 0.f;
+          if (live && h0 + j < each && n < N) {  // N is a multiple of V
+            u[j][i] = *reinterpret_cast<const Pack<float, V>*>(g.u + at);
+            dc[j][i] = *reinterpret_cast<const Pack<float, V>*>(g.dch + at);
           }
         }
-        if (g.skip) {
-          const T* xp = g.x.at<T>(b, h) + (int64_t)t * g.x.sl;
-          const T* dyp = static_cast<const T*>(g.dy) + at * P;
-          for (uint32_t p = lane; p < P; p += 32) skip = fmaf(to_f(xp[p]), to_f(dyp[p]), skip);
-        }
-        for (int o = 16; o; o >>= 1) {
-          dw += __shfl_xor_sync(~0u, dw, o);
-          alpha += __shfl_xor_sync(~0u, alpha, o);
-          skip += __shfl_xor_sync(~0u, skip, o);
-        }
-      }
-      if (lane == 0) {
-        g.dwrite[at] = dw;
-        g.diff[at] = alpha - w * dw;
-        if (g.skip) g.skip[at] = skip;
-      }
-    }
-    __syncthreads();  // the previous group's sums have been read
+      float dot[2 * H], skip[H];  // <b, U>, then <c, dC_h>; <x, dy>
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      part[0][warp][lane + 32 * i] = sb[i];
-      part[1][warp][lane + 32 * i] = sc[i];
-    }
-    __syncthreads();
-    const uint32_t n = threadIdx.x;
-    if (n < N) {
-      float vb = 0.f, vc = 0.f;
-      for (int i = 0; i < kSumWarps; ++i) {
-        vb += part[0][i][n];
-        vc += part[1][i][n];
+      for (int j = 0; j < H; ++j) {
+        const float w = __shfl_sync(~0u, wl, j);
+        dot[j] = dot[j + H] = skip[j] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            dot[j] = fmaf(bv[i][v], u[j][i].v[v], dot[j]);
+            dot[j + H] = fmaf(cv[i][v], dc[j][i].v[v], dot[j + H]);
+            sb[i][v] = fmaf(w, u[j][i].v[v], sb[i][v]);
+            sc[i][v] += dc[j][i].v[v];
+          }
+        if (g.skip && live && h0 + j < each) {
+          const uint32_t h = grp * each + h0 + j;
+          const T* xp = g.x.at<T>(b, h) + (int64_t)t * g.x.sl;
+          const T* dyp = static_cast<const T*>(g.dy) + (tok * g.heads + h) * P;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t p = lane + 32 * i;
+            if (p < P) skip[j] = fmaf(to_f(xp[p]), to_f(dyp[p]), skip[j]);
+          }
+        }
       }
-      const int64_t at = (tok * g.groups + grp) * N + n;
-      static_cast<T*>(g.db)[at] = from_f<T>(vb);
-      static_cast<T*>(g.dc)[at] = from_f<T>(vc);
+      const float d = sum_each(dot, lane);  // lane j: <b, U> of head j, lane j + H: alpha
+      const float alpha = __shfl_down_sync(~0u, d, H);
+      const float sk = g.skip ? sum_each(skip, lane) : 0.f;
+      if (lane < H && h0 + lane < each) {
+        const int64_t at = tok * g.heads + mine;
+        g.dwrite[at] = d;
+        g.diff[at] = alpha - wl * d;
+        if (g.skip) g.skip[at] = sk;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const uint32_t n = (i * 32 + lane) * V;
+      if (n < N) {
+        const int64_t at = (tok * g.groups + grp) * N + n;
+        *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(g.db) + at) = pack<T>(sb[i]);
+        *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(g.dc) + at) = pack<T>(sc[i]);
+      }
     }
   }
 }
@@ -795,7 +834,12 @@ void ssm_scan_backward(const fhe_ssm_scan_grad_args& g) {
     }
     SumArgs u{x, b, c, write, g.dy, a.lengths, a.length, a.heads, a.head_dim, a.d_state, a.groups,
               s.u, s.dch, g.db, g.dc, g.dwrite, s.diff, g.dd ? s.skip : nullptr};
-    k_sum<T><<<a.batch * a.length, 32 * kSumWarps, 0, st>>>(u);
+    const uint32_t tokens = a.batch * a.length, grid = (tokens + 3) / 4;
+    const bool wide = a.d_state % 4 == 0 && reinterpret_cast<uintptr_t>(g.db) % 16 == 0 &&
+                      reinterpret_cast<uintptr_t>(g.dc) % 16 == 0;
+    if (wide && a.d_state <= 128) k_sum<T, 4, 1, 8><<<grid, 128, 0, st>>>(u, tokens);
+    else if (wide) k_sum<T, 4, 2, 4><<<grid, 128, 0, st>>>(u, tokens);
+    else k_sum<T, 1, 8, 4><<<grid, 128, 0, st>>>(u, tokens);
     note_launch();
   });
   const uint32_t count = bh * cut.nseg;

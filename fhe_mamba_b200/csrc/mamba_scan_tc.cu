@@ -290,7 +290,7 @@ __device__ __forceinline__ void weigh_own(float (&v)[32], const float* col8, con
 // CTA, 64 or 128 (128 only without CARRY).
 template <int COLS, int ROWS, bool REV, int OUT, bool PRECISE, bool CARRY>
 __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, const __grid_constant__ Maps maps) {
-  static_assert(CARRY ? ROWS == 64 : OUT != kOutNone, "shapes");
+  static_assert((CARRY ? OUT != kOutRaw : OUT != kOutNone) && (ROWS == 64 || OUT == kOutRaw), "shapes");
   constexpr uint32_t kHalves = COLS / 64, kRowTiles = ROWS / 64;
   constexpr uint32_t kBytesQ = CARRY ? 2 * kTile : kHalves * kTile;  // q, then the scaled r (two terms)
   constexpr uint32_t kBytesK = kHalves * kTile;
@@ -374,10 +374,10 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
   load_gates(first(0));
   const float skip = (OUT == kOutY || OUT == kOutDx) && g.d ? g.d[h] : 0.f;
 
-  // The state: column t of 32 rows, in pairs; without CARRY only on its way to
-  // shared memory, where it is the B operand [column][row].
+  // The state: column t of 32 rows, in pairs; in shared memory it is the B
+  // operand [column][row].
   uint64_t s[16];
-  auto put_state = [&](uint32_t piece) {
+  [[maybe_unused]] auto put_state = [&](uint32_t piece) {
     if (t >= (uint32_t)COLS) return;
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
@@ -392,18 +392,33 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
       if constexpr (PRECISE) *reinterpret_cast<uint4*>(smem + at + kBytesS) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
   };
-  const float* s_in = OUT != kOutNone && g.state_in && t < g.cols
+  if constexpr (OUT == kOutRaw) {
+    // rows run along memory here (st_row 1): a warp takes a column's 128 rows
+    // at a time, four to a lane
+    const float* in = g.state_in + bh * g.in_bh + seg * g.in_seg;
+#pragma unroll
+    for (uint32_t j = 0; j < COLS * ROWS / 4 / kThreadsTc; ++j) {
+      const uint32_t e = j * kThreadsTc + tid, per = ROWS / 4;  // groups of four rows
+      const uint32_t c = e / per, n = e % per * 4, row = row0 + n;
+      float4 x = make_float4(0, 0, 0, 0);
+      if (c < g.cols && row < g.rows) x = *reinterpret_cast<const float4*>(in + (int64_t)c * g.st_col + row);
+      uint2 hi, lo;
+      split2(pair(x.x, x.y), hi.x, lo.x);
+      split2(pair(x.z, x.w), hi.y, lo.y);
+      const uint32_t at = ss - sq + (n >> 6) * kTileS + swz(c, n >> 3 & 7) + (n & 4) * 2;
+      *reinterpret_cast<uint2*>(smem + at) = hi;
+      if constexpr (PRECISE) *reinterpret_cast<uint2*>(smem + at + kBytesS) = lo;
+    }
+  } else {
+    const float* in = OUT != kOutNone && g.state_in && t < g.cols
                           ? g.state_in + bh * g.in_bh + seg * g.in_seg + (int64_t)t * g.st_col : nullptr;
 #pragma unroll
-  for (uint32_t u = 0; u < kRowTiles; ++u) {
-    const uint32_t piece = half * kRowTiles + u;
-#pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const uint32_t row = row0 + piece * 32 + 2 * i;
-      s[i] = pair(s_in && row < g.rows ? s_in[row * g.st_row] : 0.f,
-                  s_in && row + 1 < g.rows ? s_in[(row + 1) * g.st_row] : 0.f);
+      const uint32_t row = row0 + half * 32 + 2 * i;
+      s[i] = pair(in && row < g.rows ? in[row * g.st_row] : 0.f,
+                  in && row + 1 < g.rows ? in[(row + 1) * g.st_row] : 0.f);
     }
-    if constexpr (OUT != kOutNone) put_state(piece);
+    if constexpr (OUT != kOutNone) put_state(half);
   }
 
   float decay = 1.f;
@@ -758,6 +773,7 @@ void launch(const RecArgs& g, const Maps& maps, uint32_t batch, cudaStream_t st)
 
 bool launch_scan_tc(const RecArgs& g, bool rev, int out, uint32_t batch, cudaStream_t st) {
   Maps maps{};
+  if (out == kOutRaw && (g.st_row != 1 || g.st_col % 4 != 0 || reinterpret_cast<uintptr_t>(g.state_in) % 16 != 0)) return false;
   if (g.cols > 128 || g.rows % 8 != 0 || g.seglen % kQ != 0 || reinterpret_cast<uintptr_t>(g.out) % 16 != 0 ||
       !make_map(maps.k, g.k, g.cols, g, batch) || !make_map(maps.r, g.r, g.rows, g, batch) ||
       (out != kOutNone && !make_map(maps.q, g.q, g.cols, g, batch)))
