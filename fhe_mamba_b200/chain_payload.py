@@ -1120,13 +1120,19 @@ class EncryptedChain:
         return self.cc.Decrypt(ct).GetRealPackedValue()[:self.p.d_model]
 
 
-def select_token(payload: ChainPayload, hidden) -> int:
-    """Client greedy selection over the (tied or untied) LM head
-    (stage1_mamba2_decode_fideslib.cpp:4551-4575)."""
+def client_logits(payload: ChainPayload, hidden):
+    """The (tied or untied) LM head over a decrypted hidden vector."""
     head = payload.client_lm_head_w if payload.client_lm_head_w is not None else payload.client_embedding_w
     logits = head @ hidden
     if payload.client_lm_head_b is not None:
         logits = logits + payload.client_lm_head_b
+    return logits
+
+
+def select_token(payload: ChainPayload, hidden) -> int:
+    """Client greedy selection over the LM head
+    (stage1_mamba2_decode_fideslib.cpp:4551-4575)."""
+    logits = client_logits(payload, hidden)
     if not np.all(np.isfinite(logits)):
         raise PayloadError("non-finite autoregressive client logit")
     return int(np.argmax(logits))
@@ -1135,7 +1141,7 @@ def select_token(payload: ChainPayload, hidden) -> int:
 def run_chain(cc, payload: ChainPayload, tokens: int, tolerance: float = 5e-2,
               autoregressive_client_loop: bool = False, passes: int = 2, cache_gb: float = 8.0,
               meta_bts: bool | None = None, meta_bts_residual_layers=(), debug_layer_errors: bool = False,
-              rotation_keys: str = "full", rotation_key_gib: float = 45.0):
+              rotation_keys: str = "full", rotation_key_gib: float = 45.0, client_alternatives: int = 0):
     """The decode's chain mode: encrypt each test (or client-selected) token's
     embedding, evaluate, decrypt, and compare with the polynomial-circuit
     reference (``chain_expected_poly_final``, or the last layer's
@@ -1143,12 +1149,19 @@ def run_chain(cc, payload: ChainPayload, tokens: int, tolerance: float = 5e-2,
     exact model.  `cc` holds the secret, relinearisation and bootstrapping
     keys; the layers' rotation keys are generated here.  debug_layer_errors
     also decrypts every layer's output and compares it with that layer's
-    polynomial reference (the decode's --debug-layer-errors).  Returns the
+    polynomial reference (the decode's --debug-layer-errors).
+    client_alternatives > 0 adds the client loop's scores (log-probability,
+    entropy and that many alternatives of every selection, on the context's
+    GPU) as ``autoregressive_selected_scores``.  Returns the
     result document of the reference's decode (stage1_mamba2_decode_fideslib.cpp:
     4823-5060, the fields this backend has)."""
     p = payload
     if tokens < 1:
         raise PayloadError("--tokens must be positive")
+    if not 0 <= client_alternatives <= 64:
+        raise PayloadError("--client-alternatives must be in [0, 64]")
+    if client_alternatives and not autoregressive_client_loop:
+        raise PayloadError("--client-alternatives needs the autoregressive client loop")
     if autoregressive_client_loop:
         if p.autoregressive is None:
             raise PayloadError("autoregressive-client-loop requested but payload has no assets")
@@ -1179,6 +1192,7 @@ def run_chain(cc, payload: ChainPayload, tokens: int, tolerance: float = 5e-2,
     cc.EvalRotateKeyGen(chain.rotation_steps())
     setup = time.perf_counter() - t0
     per_token, per_token_exact, ok, selected, outputs, per_layer = [], [], [], [], [], []
+    selected_logits = []
     next_embedding = None
     t1 = time.perf_counter()
     for t in range(tokens):
@@ -1205,12 +1219,19 @@ def run_chain(cc, payload: ChainPayload, tokens: int, tolerance: float = 5e-2,
         if autoregressive_client_loop and t >= prompt - 1:
             sel = select_token(p, got)
             selected.append(sel)
+            if client_alternatives:
+                selected_logits.append(client_logits(p, got))
             next_embedding = p.client_embedding_w[sel]
     seconds = time.perf_counter() - t1
     max_error = max(per_token)
     tokens_match = (not autoregressive_client_loop) or selected == expected_ids
     passed = max_error <= tolerance and tokens_match
     w = p.layers[0].weights
+    scores = {}
+    if selected_logits:
+        from .plain_model import client_scores
+        scores["autoregressive_selected_scores"] = client_scores(np.stack(selected_logits), selected,
+                                                                 client_alternatives, cc.device)
     return {
         "schema": "fhemamba-stage1-mamba2-result-v1",
         "backend": "fhe_b200",
@@ -1233,6 +1254,7 @@ def run_chain(cc, payload: ChainPayload, tokens: int, tolerance: float = 5e-2,
             "autoregressive_selected_ids": selected,
             "autoregressive_expected_ids": expected_ids,
             "autoregressive_tokens_match": tokens_match,
+            **scores,
             "token0_decrypted_sample": [float(v) for v in outputs[0][:8]],
             "token0_expected_sample": [float(v) for v in reference[0][:8]],
             "token0_exact_sample": [float(v) for v in exact_ref[0][:8]],

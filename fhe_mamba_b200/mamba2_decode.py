@@ -9,7 +9,8 @@ stage1_mamba2_config.hpp:20-211):
         [--num-large-digits 0] [--bootstrap-level-budget-cts 5]
         [--bootstrap-level-budget-stc 5] [--security 128-classic|not-set]
         [--secret-key-dist uniform-ternary|sparse-encapsulated]
-        [--autoregressive-client-loop 0|1] [--tolerance 5e-2] [--refresh-passes 2]
+        [--autoregressive-client-loop 0|1] [--client-alternatives K]
+        [--tolerance 5e-2] [--refresh-passes 2]
         [--meta-bts 0|1] [--meta-bts-alpha 12] [--meta-bts-residual-layers 20,21]
         [--pt-cache-gib 5] [--seed S] [--debug-layer-errors 0|1]
         [--rotation-keys full|compact|balanced] [--rotation-key-gib 45]
@@ -28,6 +29,10 @@ DIR/server and the encrypted test inputs to DIR/exchange; server-eval loads
 only DIR/server, evaluates and writes DIR/exchange/output_t*.ct; client-decrypt
 decrypts them and checks them against the payload's reference.  Each role is
 its own process with the same parameter flags.
+
+With --client-alternatives K the client loop's result also holds, for every
+selected token, its log-probability, the entropy and the K most probable
+tokens (``autoregressive_selected_scores``).
 
 The result document goes to --output-json; the exit code is 0 when the
 decrypted outputs are within --tolerance of the payload's polynomial-circuit
@@ -81,6 +86,8 @@ def parse_args(argv=None):
     ap.add_argument("--security", choices=("128-classic", "not-set"), default="128-classic")
     ap.add_argument("--secret-key-dist", default="uniform-ternary")
     ap.add_argument("--autoregressive-client-loop", type=_bool, default=False)
+    ap.add_argument("--client-alternatives", type=int, default=0,
+                    help="score the client loop's selections: log-probability, entropy and this many alternatives")
     ap.add_argument("--tolerance", type=float, default=5e-2)
     ap.add_argument("--refresh-passes", type=int, choices=(1, 2), default=2)
     ap.add_argument("--meta-bts", type=_bool, default=None)
@@ -135,6 +142,10 @@ def run(args, context_factory=None) -> dict:
     if args.secret_key_dist not in ("uniform-ternary", "sparse-encapsulated"):
         raise PayloadError(f"unsupported --secret-key-dist {args.secret_key_dist} "
                            "(uniform-ternary or sparse-encapsulated)")
+    if args.client_alternatives and not args.autoregressive_client_loop:
+        raise PayloadError("--client-alternatives needs the autoregressive client loop")
+    if not 0 <= args.client_alternatives <= 64:
+        raise PayloadError("--client-alternatives must be in [0, 64]")
     log_n = int(args.ring_dim).bit_length() - 1
     audit = None
     if args.security == "128-classic":
@@ -188,7 +199,8 @@ def run(args, context_factory=None) -> dict:
                               else 0)
         cc.EvalBootstrapKeyGen()
         result = run_chain(cc, payload, args.tokens, args.tolerance, args.autoregressive_client_loop,
-                           debug_layer_errors=args.debug_layer_errors, **chain_options)
+                           debug_layer_errors=args.debug_layer_errors,
+                           client_alternatives=args.client_alternatives, **chain_options)
     else:
         result = run_role(args, payload, factory, budget, chain_options)
     result["parameters"].update({"multiplicative_depth": args.multiplicative_depth,

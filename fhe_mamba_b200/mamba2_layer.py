@@ -889,6 +889,14 @@ class Mamba2Model:
                 "max_bound_ratio": max(v["max"] for v in ratio.values()),
                 "max_domain_position": max(v["max"] for v in dom.values())}
 
+    def plain_sequences(self, device="cuda", dtype=None):
+        """The layers with the exact nonlinearities over whole sequences on the
+        GPU (``plain_model.PlainMamba2``): scoring, prefill, gradients."""
+        import torch
+
+        from .plain_model import PlainMamba2
+        return PlainMamba2(self, device, dtype or torch.float32)
+
     def initial_state(self):
         return [([np.zeros(W.conv_dim) for _ in range(W.conv_kernel - 1)], None) for W in self.layers]
 
@@ -947,6 +955,12 @@ class EncryptedMamba2Model:
         self.tokens.append(int(order[0]))
         self.margins.append(float(logits[order[0]] - logits[order[1]]))
         return int(order[0]), hf
+
+    def client_scores(self, hidden, tokens, top_k=5):
+        """Client: how likely the model holds `tokens` (one per decrypted hidden
+        vector, as ``select`` returns them), with entropy and alternatives."""
+        from .plain_model import client_scores
+        return client_scores(np.asarray(hidden) @ self.m.embedding.T, tokens, top_k, self.cc.device)
 
     def refreshes(self):
         return sum(layer.refreshes for layer in self.layers)

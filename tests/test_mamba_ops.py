@@ -128,3 +128,13 @@ def test_backward_c_refusals():
     for name in ("fhe_ssm_scan", "fhe_ssm_scan_backward", "fhe_causal_conv", "fhe_causal_conv_backward",
                  "fhe_token_logprobs", "fhe_token_logprobs_backward"):
         assert getattr(lib, name)(None) == _lib.FHE_ERR_INVALID and "null" in _lib.last_error()
+
+
+def test_client_alternatives_refusals(tmp_path):
+    import json
+
+    from fhe_mamba_b200 import mamba2_decode
+    out = tmp_path / "r.json"
+    for extra in (["--client-alternatives", "3"], ["--client-alternatives", "65", "--autoregressive-client-loop", "1"]):
+        assert mamba2_decode.main(["--input-chain", "missing", "--output-json", str(out)] + extra) == 2
+        assert "--client-alternatives" in json.loads(out.read_text())["error"]
