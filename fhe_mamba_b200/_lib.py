@@ -276,7 +276,9 @@ def check(code: int, fn: str) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(load(), name)(*args), name)
+    code = getattr(_lib or load(), name)(*args)
+    if code:
+        check(code, name)
 
 
 def kernel_launches() -> int:

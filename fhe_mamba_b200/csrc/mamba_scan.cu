@@ -63,6 +63,7 @@ __global__ void __launch_bounds__(kThreads) k_rec(const RecArgs g) {
   __shared__ __align__(16) float os[OUT == kOutNone ? 1 : kTok][kRowTile + 1];
   __shared__ float as[kTok], wsm[kTok];
 
+  if (g.only_if && *g.only_if == 0) return;
   const uint32_t tiles = (g.rows + kRowTile - 1) / kRowTile;
   uint32_t id = blockIdx.x;
   const uint32_t tile = id % tiles;
@@ -308,7 +309,8 @@ __global__ void __launch_bounds__(kThreads) k_step(const StepArgs g) {
 // slot nseg the final state's gradient.  `end` receives the last slot written.
 template <bool REV>
 __global__ void k_join(float* slots, const float* seg_decay, const float* start, float* end, uint32_t nseg,
-                       uint32_t size) {
+                       uint32_t size, const int* only_if) {
+  if (only_if && *only_if == 0) return;
   const uint32_t e = blockIdx.x * blockDim.x + threadIdx.x;
   const int64_t bh = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
   if (e >= size) return;
@@ -567,10 +569,11 @@ void launch_step(const StepArgs& g, cudaStream_t st) {
   FHE_CUDA(cudaGetLastError());
 }
 
+// One walk; whether the tensor-core form took it.  `fp32` keeps to the fp32 form.
 template <class T, bool REV, int OUT>
-void launch_rec(RecArgs g, uint32_t batch, cudaStream_t st) {
-  if constexpr (std::is_same_v<T, __nv_bfloat16>)
-    if (g.length >= kTcTokens && launch_scan_tc(g, REV, OUT, batch, st)) return;
+bool launch_rec(RecArgs g, uint32_t batch, cudaStream_t st, bool fp32) {
+  if constexpr (sizeof(T) == 2)
+    if (!fp32 && g.length >= kTcTokens && launch_scan_tc<T>(g, REV, OUT, batch, st)) return true;
   const uint64_t tiles = (g.rows + kRowTile - 1) / kRowTile;
   const uint64_t blocks = tiles * g.nseg * g.heads * batch;
   require(blocks < (1ull << 31), "too many blocks");
@@ -582,10 +585,11 @@ void launch_rec(RecArgs g, uint32_t batch, cudaStream_t st) {
   else k_rec<T, 32, REV, OUT><<<grid, kThreads, 0, st>>>(g);
   note_launch();
   FHE_CUDA(cudaGetLastError());
+  return false;
 }
 
 void launch_join(bool rev, float* slots, const float* dec, const float* start, float* end, uint32_t nseg,
-                 uint32_t size, uint32_t bh, cudaStream_t st) {
+                 uint32_t size, uint32_t bh, const int* only_if, cudaStream_t st) {
   const uint32_t y = std::min(bh, 32768u);
   // bh < 2^24; whole rows of y blocks, then the rest
   for (uint32_t at = 0; at < bh; at += y) {
@@ -595,8 +599,8 @@ void launch_join(bool rev, float* slots, const float* dec, const float* start, f
     const float* de = dec + (int64_t)at * nseg;
     const float* b0 = start ? start + (int64_t)at * size : nullptr;
     float* e0 = end ? end + (int64_t)at * size : nullptr;
-    if (rev) k_join<true><<<grid, 256, 0, st>>>(sl, de, b0, e0, nseg, size);
-    else k_join<false><<<grid, 256, 0, st>>>(sl, de, b0, e0, nseg, size);
+    if (rev) k_join<true><<<grid, 256, 0, st>>>(sl, de, b0, e0, nseg, size, only_if);
+    else k_join<false><<<grid, 256, 0, st>>>(sl, de, b0, e0, nseg, size, only_if);
     note_launch();
   }
   FHE_CUDA(cudaGetLastError());
@@ -606,7 +610,7 @@ struct Cut {
   uint32_t seglen, nseg;
 };
 
-bool tc_type(const fhe_ssm_scan_args& a) { return a.dtype == FHE_BF16 && a.length >= kTcTokens; }
+bool tc_type(const fhe_ssm_scan_args& a) { return a.dtype != FHE_F32 && a.length >= kTcTokens; }
 
 // Rows are cut when the (batch, head, row tile) blocks alone leave SMs idle.
 Cut forward_cut(const fhe_ssm_scan_args& a) {
@@ -652,15 +656,30 @@ RecArgs rec_args(const fhe_ssm_scan_args& a, const Cut& cut) {
 
 }  // namespace
 
+namespace {
+struct ForwardSpace {
+  int* bad;
+  float *slots, *dec;
+  uint64_t bytes;
+};
+ForwardSpace forward_space(const fhe_ssm_scan_args& a, const Cut& cut, void* base) {
+  const uint64_t bh = (uint64_t)a.batch * a.heads;
+  Carver w(base);
+  ForwardSpace s{};
+  if (a.dtype == FHE_F16 && tc_type(a)) s.bad = w.take<int>(1);
+  if (cut.nseg > 1) {
+    s.slots = w.take<float>(bh * (cut.nseg + 1) * a.head_dim * a.d_state);
+    s.dec = w.take<float>(bh * cut.nseg);
+  }
+  s.bytes = w.used;
+  return s;
+}
+}  // namespace
+
 uint64_t ssm_scan_workspace(const fhe_ssm_scan_args& a) {
   check_scan(a);
-  const Cut cut = forward_cut(a);
-  if (cut.nseg == 1) return 0;
-  const uint64_t bh = (uint64_t)a.batch * a.heads;
-  Carver w(nullptr);
-  w.take<float>(bh * (cut.nseg + 1) * a.head_dim * a.d_state);
-  w.take<float>(bh * cut.nseg);
-  return w.used;
+  if (a.batch == 0 || a.length == 0) return 0;
+  return forward_space(a, forward_cut(a), nullptr).bytes;
 }
 
 void ssm_scan(const fhe_ssm_scan_args& a) {
@@ -697,30 +716,45 @@ void ssm_scan(const fhe_ssm_scan_args& a) {
   with_type(a.dtype, [&](auto v) {
     using T = decltype(v);
     if (a.length == 1 && step_ok(a, one)) return launch_step<T>(one, st);
-    if (cut.nseg > 1) {
-      Carver w(a.workspace);
-      float* slots = w.take<float>((uint64_t)bh * (cut.nseg + 1) * size);
-      g.seg_decay = w.take<float>((uint64_t)bh * cut.nseg);
-      g.out_bh = (int64_t)(cut.nseg + 1) * size;
-      g.out_seg = size;
-      g.state_out = slots + size;
-      launch_rec<T, false, kOutNone>(g, a.batch, st);
-      launch_join(false, slots, g.seg_decay, a.initial_state, a.final_state, cut.nseg, size, bh, st);
-      g.state_in = slots;
-      g.in_bh = g.out_bh;
-      g.in_seg = size;
-      g.state_out = nullptr;
+    const ForwardSpace sp = forward_space(a, cut, a.workspace);
+    auto walk = [&](bool fp32, const int* only_if) {
+      RecArgs r = g;
+      r.only_if = only_if;
+      r.bad = sp.bad;
+      bool tc = false;
+      if (cut.nseg > 1) {
+        r.seg_decay = sp.dec;
+        r.out_bh = (int64_t)(cut.nseg + 1) * size;
+        r.out_seg = size;
+        r.state_out = sp.slots + size;
+        tc |= launch_rec<T, false, kOutNone>(r, a.batch, st, fp32);
+        launch_join(false, sp.slots, sp.dec, a.initial_state, a.final_state, cut.nseg, size, bh, only_if, st);
+        r.state_in = sp.slots;
+        r.in_bh = r.out_bh;
+        r.in_seg = size;
+        r.state_out = nullptr;
+      } else {
+        r.state_in = a.initial_state;
+        r.state_out = a.final_state;
+        r.in_bh = r.out_bh = size;
+      }
+      tc |= launch_rec<T, false, kOutY>(r, a.batch, st, fp32);
+      return tc;
+    };
+    if (!sp.bad) {
+      walk(false, nullptr);
+    } else if (a.initial_state == a.final_state) {
+      walk(true, nullptr);  // a second walk would start from the first one's end
     } else {
-      g.state_in = a.initial_state;
-      g.state_out = a.final_state;
-      g.in_bh = g.out_bh = size;
+      FHE_CUDA(cudaMemsetAsync(sp.bad, 0, sizeof(int), st));
+      if (walk(false, nullptr)) walk(true, sp.bad);
     }
-    launch_rec<T, false, kOutY>(g, a.batch, st);
   });
 }
 
 namespace {
 struct BackwardSpace {
+  int* bad;
   float *s_slots, *d_slots, *dec_f, *dec_r, *gamma, *u, *dch, *diff, *skip, *dd_part;
   uint64_t bytes;
 };
@@ -740,6 +774,7 @@ BackwardSpace backward_space(const fhe_ssm_scan_grad_args& g, const Cut& cut, vo
   s.diff = w.take<float>(tok);
   s.skip = w.take<float>(tok);
   s.dd_part = w.take<float>(bh * cut.nseg);
+  if (a.dtype == FHE_F16 && tc_type(a)) s.bad = w.take<int>(1);
   s.bytes = w.used;
   return s;
 }
@@ -777,61 +812,69 @@ void ssm_scan_backward(const fhe_ssm_scan_grad_args& g) {
   const int64_t slot_bh = (int64_t)(cut.nseg + 1) * size;
   with_type(a.dtype, [&](auto v) {
     using T = decltype(v);
-    RecArgs base = rec_args(a, cut);
-    base.in_bh = base.out_bh = slot_bh;
-    base.in_seg = base.out_seg = size;
-    base.rows = a.head_dim;
-    base.cols = a.d_state;
-    base.st_row = a.d_state;
-    base.st_col = 1;
-    {  // states at the segments' ends
-      RecArgs r = base;
-      r.r = x; r.k = b; r.q = c;
-      r.write = write;
-      r.state_out = s.s_slots + size;
-      r.seg_decay = s.dec_f;
-      launch_rec<T, false, kOutNone>(r, a.batch, st);
-      launch_join(false, s.s_slots, s.dec_f, a.initial_state, nullptr, cut.nseg, size, bh, st);
-    }
-    {  // gradients of the states before the segments
-      RecArgs r = base;
-      r.r = dy; r.k = c; r.q = b;
-      r.state_out = s.d_slots;
-      r.seg_decay = s.dec_r;
-      launch_rec<T, true, kOutNone>(r, a.batch, st);
-      launch_join(true, s.d_slots, s.dec_r, g.dfinal, g.dinitial, cut.nseg, size, bh, st);
-    }
+    auto walks = [&](bool fp32, const int* only_if) {
+      bool tc = false;
+      RecArgs base = rec_args(a, cut);
+      base.only_if = only_if;
+      base.bad = s.bad;
+      base.in_bh = base.out_bh = slot_bh;
+      base.in_seg = base.out_seg = size;
+      base.rows = a.head_dim;
+      base.cols = a.d_state;
+      base.st_row = a.d_state;
+      base.st_col = 1;
+      {  // states at the segments' ends
+        RecArgs r = base;
+        r.r = x; r.k = b; r.q = c;
+        r.write = write;
+        r.state_out = s.s_slots + size;
+        r.seg_decay = s.dec_f;
+        tc |= launch_rec<T, false, kOutNone>(r, a.batch, st, fp32);
+        launch_join(false, s.s_slots, s.dec_f, a.initial_state, nullptr, cut.nseg, size, bh, only_if, st);
+      }
+      {  // gradients of the states before the segments
+        RecArgs r = base;
+        r.r = dy; r.k = c; r.q = b;
+        r.state_out = s.d_slots;
+        r.seg_decay = s.dec_r;
+        tc |= launch_rec<T, true, kOutNone>(r, a.batch, st, fp32);
+        launch_join(true, s.d_slots, s.dec_r, g.dfinal, g.dinitial, cut.nseg, size, bh, only_if, st);
+      }
+      {
+        RecArgs r = base;
+        r.r = dy; r.k = c; r.q = b;
+        r.state_in = s.d_slots + size;
+        r.out_scale = write;
+        r.d = a.d;
+        r.out = g.dx;
+        tc |= launch_rec<T, true, kOutDx>(r, a.batch, st, fp32);
+      }
+      base.rows = a.d_state;
+      base.cols = a.head_dim;
+      base.st_row = 1;
+      base.st_col = a.d_state;
+      {
+        RecArgs r = base;
+        r.r = c; r.k = dy; r.q = x;
+        r.state_in = s.d_slots + size;
+        r.out_scale = write;  // for the tensor-core form's roundings alone
+        r.out = s.u;
+        tc |= launch_rec<T, true, kOutRaw>(r, a.batch, st, fp32);
+      }
+      {
+        RecArgs r = base;
+        r.r = b; r.k = x; r.q = dy;
+        r.write = write;
+        r.state_in = s.s_slots;
+        r.out = s.dch;
+        tc |= launch_rec<T, false, kOutRaw>(r, a.batch, st, fp32);
+      }
+      return tc;
+    };
+    if (s.bad) FHE_CUDA(cudaMemsetAsync(s.bad, 0, sizeof(int), st));
+    if (walks(false, nullptr) && s.bad) walks(true, s.bad);
     k_anchor<<<bh * cut.nseg, 256, 0, st>>>(s.s_slots, s.d_slots, s.gamma, cut.nseg, size);
     note_launch();
-    {
-      RecArgs r = base;
-      r.r = dy; r.k = c; r.q = b;
-      r.state_in = s.d_slots + size;
-      r.out_scale = write;
-      r.d = a.d;
-      r.out = g.dx;
-      launch_rec<T, true, kOutDx>(r, a.batch, st);
-    }
-    base.rows = a.d_state;
-    base.cols = a.head_dim;
-    base.st_row = 1;
-    base.st_col = a.d_state;
-    {
-      RecArgs r = base;
-      r.r = c; r.k = dy; r.q = x;
-      r.state_in = s.d_slots + size;
-      r.out_scale = write;  // for the tensor-core form's roundings alone
-      r.out = s.u;
-      launch_rec<T, true, kOutRaw>(r, a.batch, st);
-    }
-    {
-      RecArgs r = base;
-      r.r = b; r.k = x; r.q = dy;
-      r.write = write;
-      r.state_in = s.s_slots;
-      r.out = s.dch;
-      launch_rec<T, false, kOutRaw>(r, a.batch, st);
-    }
     SumArgs u{x, b, c, write, g.dy, a.lengths, a.length, a.heads, a.head_dim, a.d_state, a.groups,
               s.u, s.dch, g.db, g.dc, g.dwrite, s.diff, g.dd ? s.skip : nullptr};
     const uint32_t tokens = a.batch * a.length, grid = (tokens + 3) / 4;

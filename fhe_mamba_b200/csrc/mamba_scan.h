@@ -33,6 +33,8 @@ struct RecArgs {
   float* seg_decay;  // STATE pass: product of the segment's decays [bh][nseg]
   void* out;
   bool vec;  // r, k and q may be read four elements at a time
+  int* bad;            // set by the float16 tensor-core form when a product overflowed
+  const int* only_if;  // the fp32 walk does nothing while it is 0 (nullptr: always runs)
 };
 
 enum { kOutNone = 0, kOutY = 1, kOutDx = 2, kOutRaw = 3 };
@@ -42,8 +44,9 @@ __device__ __forceinline__ int clamp_length(const int32_t* lengths, uint32_t b, 
   return min(max(lengths[b], 0), (int)length);
 }
 
-// The tensor-core form (mamba_scan_tc.cu), bfloat16 only; false, with nothing
-// launched, for sizes and layouts that it does not take.
+// The tensor-core form (mamba_scan_tc.cu) for bfloat16 and float16; false, with
+// nothing launched, for sizes and layouts that it does not take.
+template <class T>
 bool launch_scan_tc(const RecArgs& g, bool rev, int out, uint32_t batch, cudaStream_t st);
 unsigned scan_tc_timeouts();
 

@@ -1,4 +1,4 @@
-// Mamba-2 state recurrence for bfloat16 activations on the tensor cores
+// Mamba-2 state recurrence for 16-bit activations on the tensor cores
 // (tcgen05.mma kind::f16), 128 tokens at a time.
 //
 // The walk of mamba_scan.cu, o_t = S_t q_t with S_t = a_t S_(t-1) + w_t r_t (x) k_t,
@@ -11,11 +11,15 @@
 // Every factor is a product of at most 128 decays in its own order, never a
 // quotient, so decays of zero or near it lose nothing.
 //
-// Roundings.  q, k and r are bfloat16 as given; G, O and S accumulate in
-// fp32.  G o L o w and S0 enter their products as bfloat16, half a step of
-// 2^-8 of each term, as y's own rounding; with PRECISE they enter as two
-// bfloat16 terms (2^-16).  E o w o r, whose sum is the fp32 state, always
-// enters as two terms.
+// Roundings.  q, k and r are as given; G, O and S accumulate in fp32.
+// G o L o w and S0 enter their products in the activations' type, half a step
+// of each term (2^-8 for bfloat16) as y's own rounding; with PRECISE they
+// enter as two terms of that type (2^-16).  E o w o r, whose sum is the fp32
+// state, always enters as two terms.
+// For float16 the factors are scaled by powers of two (the chunk's largest w to
+// about 8, the state by 16) to use its range; where an operand overflows all
+// the same, a product is not finite, the kernel says so in *bad, and the
+// caller's launches of the fp32 walk, idle otherwise, take the work over.
 //
 // One CTA walks one (batch, head, tile of rows, segment).  Shared memory holds
 // q, k, r and S0 in 128-byte-swizzled tiles of 64 columns; the scaled r takes
@@ -61,10 +65,12 @@ __device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lead) {
          ((uint64_t)(1024u >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
-// kind::f16, bfloat16 operands, fp32 accumulator; a_mn / b_mn: the operand's
+// kind::f16, operands of type T, fp32 accumulator; a_mn / b_mn: the operand's
 // M / N axis is contiguous.
+template <class T>
 constexpr uint32_t idesc(uint32_t n, bool a_mn, bool b_mn) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((n >> 3) << 17) |
+  constexpr uint32_t type = std::is_same_v<T, __half> ? 0u : 1u;
+  return (1u << 4) | (type << 7) | (type << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((n >> 3) << 17) |
          ((kQ >> 4) << 24);
 }
 
@@ -149,20 +155,35 @@ __device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 
+template <class T>
 __device__ __forceinline__ uint32_t pack2(uint64_t p) {
   float a, b;
   unpair(p, a, b);
   uint32_t v;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(b), "f"(a));
+  if constexpr (std::is_same_v<T, __half>) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(b), "f"(a));
+  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(b), "f"(a));
   return v;
 }
+template <class T>
 __device__ __forceinline__ uint64_t unpack2(uint32_t v) {
-  return pair(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  if constexpr (std::is_same_v<T, __half>) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
+    return pair(f.x, f.y);
+  } else {
+    return pair(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  }
 }
-// The two bfloat16 terms of a pair of floats.
+// The two terms of T of a pair of floats.
+template <class T>
 __device__ __forceinline__ void split2(uint64_t p, uint32_t& hi, uint32_t& lo) {
-  hi = pack2(p);
-  lo = pack2(fma2(unpack2(hi), pair(-1.f, -1.f), p));
+  hi = pack2<T>(p);
+  lo = pack2<T>(fma2(unpack2<T>(hi), pair(-1.f, -1.f), p));
+}
+
+// The power of two that brings |v| into [1, 2), 1 for 0, denormals and above 2^100.
+__device__ __forceinline__ float scale_of(float v) {
+  const uint32_t e = __float_as_uint(v) >> 23 & 0xff;
+  return e - 1u < 226u ? __uint_as_float((254u - e) << 23) : 1.f;
 }
 
 // One lane of a converged warp.
@@ -183,6 +204,7 @@ struct Gates {
   float col[kQ];         // column factor for rows of other blocks of 32: tail (reversed: head) times w
   float col8[kQ];        // and for rows of other blocks of 8 in its block of 32
   float total[4];        // product over each block of 32
+  float most[4];         // largest |w| in each block of 32 (float16)
 };
 
 // Warps 0-3, one token per thread.
@@ -209,6 +231,8 @@ __device__ __forceinline__ void put_gates(Gates& g, uint32_t t, uint32_t lane, f
   g.col[t] = (REV ? head : tail) * w;
   g.col8[t] = (REV ? head8 : tail8) * w;
   if (lane == 31) g.total[t >> 5] = head;
+  const uint32_t most = __reduce_max_sync(~0u, __float_as_uint(fabsf(w)));
+  if (lane == 0) g.most[t >> 5] = __uint_as_float(most);
 }
 
 // A row's factors within its own block of 32, times `scale`: `own` for the
@@ -288,7 +312,7 @@ __device__ __forceinline__ void weigh_own(float (&v)[32], const float* col8, con
 
 // COLS: columns held, 64 or 128 (those past g.cols are zeros); ROWS: rows per
 // CTA, 64 or 128 (128 only without CARRY).
-template <int COLS, int ROWS, bool REV, int OUT, bool PRECISE, bool CARRY>
+template <class T, int COLS, int ROWS, bool REV, int OUT, bool PRECISE, bool CARRY>
 __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, const __grid_constant__ Maps maps) {
   static_assert((CARRY ? OUT != kOutRaw : OUT != kOutNone) && (ROWS == 64 || OUT == kOutRaw), "shapes");
   constexpr uint32_t kHalves = COLS / 64, kRowTiles = ROWS / 64;
@@ -322,7 +346,9 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t quarter = warp & 3, half = warp >> 2;
   const uint32_t t = quarter * 32 + lane;  // this thread's token, and column of S
-  using T = __nv_bfloat16;
+  constexpr bool kHalf = std::is_same_v<T, __half>;
+  constexpr float kStateScale = kHalf ? 16.f : 1.f;  // of S0 in shared memory
+  uint64_t poison = 0;  // a sum of 0 times every product: NaN once one is not finite (float16)
 
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tslot)),
@@ -384,8 +410,9 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if constexpr (PRECISE) split2(s[4 * v + e], hi[e], lo[e]);
-        else hi[e] = pack2(s[4 * v + e]);
+        const uint64_t x = kHalf ? mul2(s[4 * v + e], pair(kStateScale, kStateScale)) : s[4 * v + e];
+        if constexpr (PRECISE) split2<T>(x, hi[e], lo[e]);
+        else hi[e] = pack2<T>(x);
       }
       const uint32_t at = ss - sq + (piece >> 1) * kTileS + swz(t, (piece & 1) * 4 + v);
       *reinterpret_cast<uint4*>(smem + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
@@ -403,8 +430,8 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
       float4 x = make_float4(0, 0, 0, 0);
       if (c < g.cols && row < g.rows) x = *reinterpret_cast<const float4*>(in + (int64_t)c * g.st_col + row);
       uint2 hi, lo;
-      split2(pair(x.x, x.y), hi.x, lo.x);
-      split2(pair(x.z, x.w), hi.y, lo.y);
+      split2<T>(pair(kStateScale * x.x, kStateScale * x.y), hi.x, lo.x);
+      split2<T>(pair(kStateScale * x.z, kStateScale * x.w), hi.y, lo.y);
       const uint32_t at = ss - sq + (n >> 6) * kTileS + swz(c, n >> 3 & 7) + (n & 4) * 2;
       *reinterpret_cast<uint2*>(smem + at) = hi;
       if constexpr (PRECISE) *reinterpret_cast<uint2*>(smem + at + kBytesS) = lo;
@@ -434,13 +461,17 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
     // Row scale of this token's products: w of dx; for U of the gradients the
     // mantissa of w, so that its products are rounded at w_t times their value
     // as those of dC_h are, up to a power of two.  alpha and beta, whose
-    // difference is summed, then carry the same roundings and the sum loses them.
-    float rho = 1.f;
+    // difference is summed, then carry the same roundings and the sum loses
+    // them.  `up` undoes what the row scale took too much.
+    float rho = 1.f, up = 1.f;
     if constexpr (OUT == kOutDx || (REV && OUT == kOutRaw)) {
-      rho = live ? g.out_scale.p[b * g.out_scale.sb + tok * g.out_scale.sl + h * g.out_scale.sh] : 1.f;
+      const float w = live ? g.out_scale.p[b * g.out_scale.sb + tok * g.out_scale.sl + h * g.out_scale.sh] : 1.f;
+      rho = OUT == kOutRaw || kHalf ? w * scale_of(w) : w;
       if constexpr (OUT == kOutRaw) {
-        const uint32_t bits = __float_as_uint(rho);
-        rho = (bits >> 23 & 0xff) - 1u < 0xfeu ? __uint_as_float((bits & 0x7fffffu) | 0x3f800000u) : 1.f;
+        if (fabsf(rho) < 1.f) rho = 1.f;  // 0 or denormal
+        up = 1.f / rho;
+      } else if constexpr (kHalf) {
+        up = 1.f / scale_of(w);
       }
     }
     if (i > 0) {  // (the barriers are initialised before the first)
@@ -471,14 +502,14 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
 #pragma unroll
         for (uint32_t j = 0; j < COLS / 16; ++j) {
           const uint32_t at = (j >> 2) * kTile + (j & 3) * 32;
-          mma_ss(tmem, desc(sq + at, 16), desc(sk + at, 16), idesc(kQ, false, false), j);
+          mma_ss(tmem, desc(sq + at, 16), desc(sk + at, 16), idesc<T>(kQ, false, false), j);
         }
 #pragma unroll
         for (uint32_t j = 0; j < COLS / 16; ++j) {
           const uint32_t at = (j >> 2) * kTile + (j & 3) * 32;
-          mma_ss(tmem + kColO, desc(sq + at, 16), desc(ss + j * 2048, kTileS), idesc(ROWS, false, true), j);
+          mma_ss(tmem + kColO, desc(sq + at, 16), desc(ss + j * 2048, kTileS), idesc<T>(ROWS, false, true), j);
           if constexpr (PRECISE)
-            mma_ss(tmem + kColO, desc(sq + at, 16), desc(ss + kBytesS + j * 2048, kTileS), idesc(ROWS, false, true), 1);
+            mma_ss(tmem + kColO, desc(sq + at, 16), desc(ss + kBytesS + j * 2048, kTileS), idesc<T>(ROWS, false, true), 1);
         }
         commit(bar_g);
       }
@@ -493,8 +524,15 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
       if (u > quarter) after *= gate.total[u];
     }
     const float head = gate.head[t], tail = gate.tail[t];
-    const float pt = (REV ? tail * after : head * before) * rho;
-    const float et = (REV ? head * before : tail * after) * gate.w[t];
+    if constexpr (kHalf) {  // w of the chunk scaled to at most 16
+      const float sw = 8.f * scale_of(fmaxf(fmaxf(gate.most[0], gate.most[1]), fmaxf(gate.most[2], gate.most[3])));
+      rho *= sw;
+      up /= sw;
+    }
+    const float back = kHalf ? 1.f / (8.f * scale_of(fmaxf(fmaxf(gate.most[0], gate.most[1]), fmaxf(gate.most[2], gate.most[3])))) : 1.f;
+    const float pt = (REV ? tail * after : head * before) * (rho / kStateScale);
+    const float et = (REV ? head * before : tail * after) * gate.w[t] / back;
+    const float keep = skip / up;  // the skip term in the products' scale
     const float all = gate.total[0] * gate.total[1] * gate.total[2] * gate.total[3];
     decay *= all;
     const uint32_t blk_own = quarter;
@@ -529,12 +567,12 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
           uint32_t hi[4], lo[4];
 #pragma unroll
           for (int f = 0; f < 4; ++f) {
-            const uint64_t xx = unpack2(x[f]);
-            if constexpr (CARRY) split2(mul2(pair(et, et), xx), hi[f], lo[f]);
+            const uint64_t xx = unpack2<T>(x[f]);
+            if constexpr (CARRY) split2<T>(mul2(pair(et, et), xx), hi[f], lo[f]);
             if constexpr (OUT != kOutNone) {
               float *o = v + 8 * e + 2 * f;
               uint64_t a = mul2(pair(pt, pt), pair(o[0], o[1]));
-              if constexpr (OUT == kOutY || OUT == kOutDx) a = fma2(pair(skip, skip), xx, a);
+              if constexpr (OUT == kOutY || OUT == kOutDx) a = fma2(pair(keep, keep), xx, a);
               unpair(a, o[0], o[1]);
             }
           }
@@ -564,8 +602,8 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
               const uint64_t p = pair(v[2 * e], v[2 * e + 1]);
-              if constexpr (PRECISE) split2(p, hi[e], lo[e]);
-              else hi[e] = pack2(p);
+              if constexpr (PRECISE) split2<T>(p, hi[e], lo[e]);
+              else hi[e] = pack2<T>(p);
             }
           } else {
 #pragma unroll
@@ -589,8 +627,8 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
 #pragma unroll
           for (uint32_t j = 0; j < kQ / 16; ++j) {
             const uint64_t a = desc(sk + j * 2048, lead);
-            mma_ss(tmem + kColS, a, desc(sq + j * 2048, 0), idesc(64, true, true), j);
-            mma_ss(tmem + kColS, a, desc(sq + kTile + j * 2048, 0), idesc(64, true, true), 1);
+            mma_ss(tmem + kColS, a, desc(sq + j * 2048, 0), idesc<T>(64, true, true), j);
+            mma_ss(tmem + kColS, a, desc(sq + kTile + j * 2048, 0), idesc<T>(64, true, true), 1);
           }
           commit(bar_s);
         }
@@ -598,9 +636,9 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
 #pragma unroll
           for (uint32_t j = 0; j < kQ / 16; ++j) {
             const uint32_t a = tmem + (j >> 1) * 32 + (j & 1) * 8;
-            mma_ts(tmem + kColO, a, desc(sr + j * 2048, kTile), idesc(ROWS, false, true), 1);
+            mma_ts(tmem + kColO, a, desc(sr + j * 2048, kTile), idesc<T>(ROWS, false, true), 1);
             if constexpr (PRECISE)
-              mma_ts(tmem + kColO, a + 16, desc(sr + j * 2048, kTile), idesc(ROWS, false, true), 1);
+              mma_ts(tmem + kColO, a + 16, desc(sr + j * 2048, kTile), idesc<T>(ROWS, false, true), 1);
           }
           commit(bar_o);
         }
@@ -618,7 +656,14 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
         tmem_ld32(tmem + lanes + kColS + half * 32, v);
         ld_wait();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = fma2(pair(all, all), s[e], pair(v[2 * e], v[2 * e + 1]));
+        for (int e = 0; e < 16; ++e) {
+          uint64_t x = pair(v[2 * e], v[2 * e + 1]);
+          if constexpr (kHalf) {
+            poison = fma2(x, 0, poison);
+            x = mul2(x, pair(back, back));
+          }
+          s[e] = fma2(pair(all, all), s[e], x);
+        }
         if constexpr (OUT != kOutNone) {
           if (i + 1 < chunks) put_state(half);
         }
@@ -632,13 +677,20 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
       if (ok) {
         if (i + 1 < chunks && tid == 0) load_rows(first(i + 1));
         __syncwarp();
-        const float inv = OUT == kOutRaw && REV ? 1.f / rho : 1.f;
 #pragma unroll
         for (uint32_t u = 0; u < kRowTiles; ++u) {
           const uint32_t piece = half * kRowTiles + u, row = row0 + piece * 32;
           float v[32];
           tmem_ld32(tmem + lanes + kColO + piece * 32, v);
           ld_wait();
+          if constexpr (kHalf || (OUT == kOutRaw && REV)) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const uint64_t x = pair(v[e], v[e + 1]);
+              if constexpr (kHalf) poison = fma2(x, 0, poison);
+              unpair(mul2(x, pair(up, up)), v[e], v[e + 1]);
+            }
+          }
           if (tok < t_hi && row < g.rows && (OUT != kOutRaw || live)) {
             const int64_t at = (((int64_t)b * g.length + tok) * g.heads + h) * g.rows + row;
             if constexpr (OUT == kOutRaw) {
@@ -646,7 +698,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
 #pragma unroll
               for (int e = 0; e < 32; e += 4)
                 if (row + e < g.rows)
-                  *reinterpret_cast<float4*>(o + e) = make_float4(inv * v[e], inv * v[e + 1], inv * v[e + 2], inv * v[e + 3]);
+                  *reinterpret_cast<float4*>(o + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
             }
           }
           if constexpr (OUT != kOutRaw) {
@@ -656,7 +708,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
-              for (int f = 0; f < 4; ++f) x[e][f] = live ? pack2(pair(v[8 * e + 2 * f], v[8 * e + 2 * f + 1])) : 0u;
+              for (int f = 0; f < 4; ++f) x[e][f] = live ? pack2<T>(pair(v[8 * e + 2 * f], v[8 * e + 2 * f + 1])) : 0u;
 #pragma unroll
             for (int d = 1; d < 4; d *= 2) {
               const bool up = lane & d;
@@ -685,6 +737,11 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
         }
       }
     }
+  }
+  if constexpr (kHalf) {
+    float a, c;
+    unpair(poison, a, c);
+    if (!(a == 0.f && c == 0.f)) *g.bad = 1;
   }
   if (ok) {
     if (CARRY && g.state_out && t < g.cols) {
@@ -737,7 +794,7 @@ Encode encoder() {
 }
 
 // The map of one operand; false if its layout has none.
-bool make_map(CUtensorMap& m, const Src& s, uint32_t width, const RecArgs& g, uint32_t batch) {
+bool make_map(CUtensorMap& m, const Src& s, uint32_t width, const RecArgs& g, uint32_t batch, bool half) {
   const Encode fn = encoder();
   if (!fn) return false;
   const uint64_t dims[4] = {width, g.heads / s.share, g.length, batch};
@@ -750,17 +807,17 @@ bool make_map(CUtensorMap& m, const Src& s, uint32_t width, const RecArgs& g, ui
   const cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]}, st[3] = {strides[0], strides[1], strides[2]};
   const cuuint32_t box[4] = {64, 1, kQ, 1}, step[4] = {1, 1, 1, 1};
   return reinterpret_cast<uintptr_t>(s.p) % 16 == 0 &&
-         fn(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(s.p), d, st, box, step,
+         fn(&m, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(s.p), d, st, box, step,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int COLS, int ROWS, bool REV, int OUT, bool PRECISE, bool CARRY>
+template <class T, int COLS, int ROWS, bool REV, int OUT, bool PRECISE, bool CARRY>
 void launch(const RecArgs& g, const Maps& maps, uint32_t batch, cudaStream_t st) {
   const uint32_t need = 1024 + (CARRY ? 2 : COLS / 64) * kTile + COLS / 64 * kTile + ROWS / 64 * kTile +
                         COLS * 128 * (ROWS / 64) * (PRECISE ? 2 : 1);
   const uint32_t smem = std::max(need, kLeastSmem);
-  auto* kernel = k_scan_tc<COLS, ROWS, REV, OUT, PRECISE, CARRY>;
+  auto* kernel = k_scan_tc<T, COLS, ROWS, REV, OUT, PRECISE, CARRY>;
   FHE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   const uint64_t blocks = (uint64_t)((g.rows + ROWS - 1) / ROWS) * g.heads * g.nseg * batch;
   require(blocks < (1ull << 31), "too many blocks");
@@ -771,25 +828,27 @@ void launch(const RecArgs& g, const Maps& maps, uint32_t batch, cudaStream_t st)
 
 }  // namespace
 
+template <class T>
 bool launch_scan_tc(const RecArgs& g, bool rev, int out, uint32_t batch, cudaStream_t st) {
+  constexpr bool kHalf = std::is_same_v<T, __half>;
   Maps maps{};
   if (out == kOutRaw && (g.st_row != 1 || g.st_col % 4 != 0 || reinterpret_cast<uintptr_t>(g.state_in) % 16 != 0)) return false;
   if (g.cols > 128 || g.rows % 8 != 0 || g.seglen % kQ != 0 || reinterpret_cast<uintptr_t>(g.out) % 16 != 0 ||
-      !make_map(maps.k, g.k, g.cols, g, batch) || !make_map(maps.r, g.r, g.rows, g, batch) ||
-      (out != kOutNone && !make_map(maps.q, g.q, g.cols, g, batch)))
+      !make_map(maps.k, g.k, g.cols, g, batch, kHalf) || !make_map(maps.r, g.r, g.rows, g, batch, kHalf) ||
+      (out != kOutNone && !make_map(maps.q, g.q, g.cols, g, batch, kHalf)))
     return false;
   auto go = [&](auto cols) {
     constexpr int C = decltype(cols)::value;
-    if (!rev && out == kOutNone) launch<C, 64, false, kOutNone, false, true>(g, maps, batch, st);
-    else if (!rev && out == kOutY) launch<C, 64, false, kOutY, false, true>(g, maps, batch, st);
-    else if (rev && out == kOutNone) launch<C, 64, true, kOutNone, false, true>(g, maps, batch, st);
-    else if (rev && out == kOutDx) launch<C, 64, true, kOutDx, false, false>(g, maps, batch, st);
+    if (!rev && out == kOutNone) launch<T, C, 64, false, kOutNone, false, true>(g, maps, batch, st);
+    else if (!rev && out == kOutY) launch<T, C, 64, false, kOutY, false, true>(g, maps, batch, st);
+    else if (rev && out == kOutNone) launch<T, C, 64, true, kOutNone, false, true>(g, maps, batch, st);
+    else if (rev && out == kOutDx) launch<T, C, 64, true, kOutDx, false, false>(g, maps, batch, st);
     else if (out == kOutRaw && g.rows <= 64) {
-      if (rev) launch<C, 64, true, kOutRaw, true, false>(g, maps, batch, st);
-      else launch<C, 64, false, kOutRaw, true, false>(g, maps, batch, st);
+      if (rev) launch<T, C, 64, true, kOutRaw, true, false>(g, maps, batch, st);
+      else launch<T, C, 64, false, kOutRaw, true, false>(g, maps, batch, st);
     } else if (out == kOutRaw) {
-      if (rev) launch<C, 128, true, kOutRaw, true, false>(g, maps, batch, st);
-      else launch<C, 128, false, kOutRaw, true, false>(g, maps, batch, st);
+      if (rev) launch<T, C, 128, true, kOutRaw, true, false>(g, maps, batch, st);
+      else launch<T, C, 128, false, kOutRaw, true, false>(g, maps, batch, st);
     } else require(false, "unknown walk", FHE_ERR_INTERNAL);
   };
   // without a carried state a segment is one chunk
@@ -798,6 +857,9 @@ bool launch_scan_tc(const RecArgs& g, bool rev, int out, uint32_t batch, cudaStr
   else go(std::integral_constant<int, 128>{});
   return true;
 }
+
+template bool launch_scan_tc<__nv_bfloat16>(const RecArgs&, bool, int, uint32_t, cudaStream_t);
+template bool launch_scan_tc<__half>(const RecArgs&, bool, int, uint32_t, cudaStream_t);
 
 unsigned scan_tc_timeouts() {
   unsigned v = 0;

@@ -126,7 +126,7 @@ def _scan_args(x, write, log_decay, B, C, D, state, lengths, y, final):
 
 def _scan_forward(x, write, log_decay, B, C, D, state, lengths, y, final):
     a = _scan_args(x, write, log_decay, B, C, D, state, lengths, y, final)
-    if x.shape[1] >= 128:  # shorter rows are never cut into segments
+    if x.shape[1] >= 64:  # shorter rows need no workspace
         ws = _workspace("fhe_ssm_scan_workspace", a, x.device)
         if ws is not None:
             a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
@@ -221,12 +221,23 @@ def ssm_step(state, x, write, log_decay, B, C, D=None, out=None):
           "ssm_step: one token of each sequence, without a length axis")
     if _wants_grad(state, x, write, log_decay, B, C, D):
         _need(False, f"{op} has no gradient (use ssm_scan)")
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    x, write, log_decay, B, C = (t.unsqueeze(1) for t in (x, write, log_decay, B, C))
-    if not _scan_fits(x, write, log_decay, B, C, D, state, None):
-        _check_scan(op, x, write, log_decay, B, C, D, state, None, "state")
+    b, h, p = x.shape
+    k, n = B.shape[1:]
+    t, d, f = x.dtype, x.device, torch.float32
+    if not (t in _TYPES and x.is_cuda and k >= 1 and h >= 1 and h % k == 0 and 1 <= p <= MAX_HEAD_DIM
+            and 1 <= n <= MAX_STATE and B.shape == C.shape == (b, k, n) and B.dtype == C.dtype == t
+            and write.shape == log_decay.shape == (b, h) and write.dtype == log_decay.dtype == state.dtype == f
+            and state.shape == (b, h, p, n) and B.device == C.device == write.device == log_decay.device == d
+            and state.device == d and (D is None or (D.shape == (h,) and D.dtype == f and D.device == d))):
+        _check_scan(op, *(v.unsqueeze(1) for v in (x, write, log_decay, B, C)), D, state, None, "state")
     out = _check_state_out(op, state, out)
-    _scan_forward(_inner(x), write, log_decay, _inner(B), _inner(C), _dense(D), state, None, y, out)
+    x, B, C, D = _inner(x), _inner(B), _inner(C), _dense(D)
+    y = torch.empty(x.shape, dtype=t, device=d)
+    gates = tuple((v.data_ptr(), (v.stride(0), 0, v.stride(1))) for v in (x, write, log_decay, B, C))
+    (xp, xs), (wp, ws), (ap, as_), (bp, bs), (cp, cs) = gates
+    a = _lib.SsmScanArgs(d.index, _TYPES[t], b, 1, h, p, n, k, xp, xs, wp, ws, ap, as_, bp, bs, cp, cs, _ptr(D),
+                         state.data_ptr(), None, y.data_ptr(), out.data_ptr(), None, 0, _stream_of(d.index))
+    call("fhe_ssm_scan", ctypes.byref(a))
     return y, out
 
 

@@ -184,6 +184,29 @@ def test_lengths_are_clamped(ops):
     assert torch.equal(y, y2) and torch.equal(s, s2) and torch.equal(s[1], i["initial_state"][1])
 
 
+def test_scan_float16_products_past_its_range(ops):
+    """Products of B and C that float16 cannot hold, with outputs that it can: the fp32 walk takes over, forward and
+    backward, so no operand's rounding is left."""
+    i = scan_inputs(17, 2, 200, 2, 64, 128, 1, torch.float16, strided=False)
+    i["B"], i["C"] = i["B"] * 200, i["C"] * 200
+    i["write"] = i["write"] * 1e-5
+    i["initial_state"] = i["initial_state"] * 1e-3
+    assert (i["B"].float() @ i["C"].float().transpose(-1, -2)).abs().max() > 65504
+    y, s = ops.ssm_scan(**i)
+    wy, ws, _ = reference(i)
+    my, ms, _ = reference(i, absolute=True)
+    close(y, wy, my, scan_k(i), "y")
+    close(s, ws, ms, scan_k(i), "state")
+    check_scan(ops, i)
+
+
+def test_scan_float16_small_factors(ops):
+    """Weights and states near the bottom of float16's range lose nothing to it."""
+    i = scan_inputs(18, 2, 300, 2, 64, 128, 1, torch.float16)
+    i["write"], i["initial_state"], i["D"] = i["write"] * 1e-6, i["initial_state"] * 1e-4, None
+    check_scan(ops, i)
+
+
 @pytest.mark.parametrize("b, l", [(0, 5), (2, 0), (0, 0)])
 def test_scan_empty(ops, b, l):
     i = scan_inputs(9, b, l, 2, 8, 16, 1, torch.float32)
