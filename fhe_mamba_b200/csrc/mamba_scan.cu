@@ -28,7 +28,6 @@ namespace fhe {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kRowTile = 32;  // rows of S per block: 4 warps x 4 row pairs
 constexpr int kTok = 16;      // tokens staged per step
 constexpr uint32_t kTcTokens = 64;  // shortest rows the tensor-core form takes
 
@@ -47,20 +46,23 @@ __device__ __forceinline__ float4 unpack4(const Pack<T, 4>& v) {
   return make_float4(to_f(v.v[0]), to_f(v.v[1]), to_f(v.v[2]), to_f(v.v[3]));
 }
 
-// One block walks one segment of one (batch, head) for a tile of 32 rows.
-// A thread holds 2 rows x CW columns: lane bits 0-2 choose the columns
-// 4 (lane & 7) + 32 i, lane bits 3-4 and the warp the row pair.  The 8 lanes
-// of a row pair add their parts of S q with three shuffles for both rows.
+// One block walks one segment of one (batch, head) for a tile of 16 R rows.
+// A thread holds R rows x CW columns: lane bits 0-2 choose the columns
+// 4 (lane & 7) + 32 i, lane bits 3-4 and the warp the rows.  S q of 16 / R
+// tokens is left in 16 partial sums per lane, which the 8 lanes of a row then
+// add with 14 shuffles for all of them (one token's alone would take three,
+// each waited for: 113 instructions a token against 80, and the latency).
 // The next tokens are fetched into registers while the present ones are used.
-template <class T, int CW, bool REV, int OUT>
+template <class T, int CW, int R, bool REV, int OUT>
 __global__ void __launch_bounds__(kThreads) k_rec(const RecArgs g) {
+  constexpr int kRowTile = 16 * R, kGroup = 16 / R;  // rows per block, tokens per round of sums
   constexpr int W = CW * 8;
   constexpr int kFetch = kTok * W / 4 / kThreads;  // 4-element loads per thread, k and q each
   static_assert(kFetch >= 1 && kTok * W / 4 % kThreads == 0, "tile");
   __shared__ __align__(16) float ks[kTok][W];
   __shared__ __align__(16) float qs[OUT == kOutNone ? 1 : kTok][W];
   __shared__ __align__(16) float rs[kTok][kRowTile];
-  __shared__ __align__(16) float os[OUT == kOutNone ? 1 : kTok][kRowTile + 1];
+  __shared__ __align__(16) float os[OUT == kOutNone ? 1 : kTok][kRowTile + 2];
   __shared__ float as[kTok], wsm[kTok];
 
   if (g.only_if && *g.only_if == 0) return;
@@ -78,32 +80,33 @@ __global__ void __launch_bounds__(kThreads) k_rec(const RecArgs g) {
 
   const int tid = threadIdx.x, lane = tid & 31;
   const int c0 = 4 * (lane & 7);
-  const int rp = 2 * ((tid >> 5) * 4 + (lane >> 3));  // row pair within the tile
+  const int rp = R * ((tid >> 5) * 4 + (lane >> 3));  // first row within the tile
   const T* rbase = g.r.at<T>(b, h) + row0;
   const T* kbase = g.k.at<T>(b, h);
   const T* qbase = g.q.at<T>(b, h);
   const float* wbase = g.write.p ? g.write.p + (int64_t)b * g.write.sb + (int64_t)h * g.write.sh : nullptr;
   const float* abase = g.log_decay.p + (int64_t)b * g.log_decay.sb + (int64_t)h * g.log_decay.sh;
 
-  uint64_t s[2][CW / 2];  // two columns each
+  uint64_t s[R][CW / 2];  // two columns each
   const int64_t bh = (int64_t)b * g.heads + h;
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+  for (int j = 0; j < R; ++j)
 #pragma unroll
     for (int i = 0; i < CW; i += 2) {
       float v[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-      const int row = row0 + rp + j, col = c0 + (i / 4) * 32 + (i & 3) + u;
-      v[u] = (OUT != kOutNone && g.state_in && row < (int)g.rows && col < (int)g.cols)
-                    ? g.state_in[bh * g.in_bh + seg * g.in_seg + row * g.st_row + col * g.st_col]
-                    : 0.f;
+        const int row = row0 + rp + j, col = c0 + (i / 4) * 32 + (i & 3) + u;
+        v[u] = (OUT != kOutNone && g.state_in && row < (int)g.rows && col < (int)g.cols)
+                   ? g.state_in[bh * g.in_bh + seg * g.in_seg + row * g.st_row + col * g.st_col]
+                   : 0.f;
       }
       s[j][i / 2] = pair(v[0], v[1]);
     }
   float decay = 1.f;  // thread 0 of a STATE pass
 
-  Pack<T, 4> pk[kFetch], pq[kFetch], pr;
+  constexpr int kFetchR = kTok * kRowTile / 4 / kThreads;
+  Pack<T, 4> pk[kFetch], pq[kFetch], pr[kFetchR];
   float pa = 1.f, pw = 0.f;
   auto first = [&](int step) { return REV ? t_hi - kTok * (step + 1) : t_lo + kTok * step; };
   auto fetch = [&](int step) {
@@ -115,9 +118,10 @@ __global__ void __launch_bounds__(kThreads) k_rec(const RecArgs g) {
       pk[i] = load4(kbase + (int64_t)t * g.k.sl, col, g.cols, g.vec, live(t));
       if constexpr (OUT != kOutNone) pq[i] = load4(qbase + (int64_t)t * g.q.sl, col, g.cols, g.vec, live(t));
     }
-    {
-      const int t = t0 + tid / 8, col = 4 * (tid % 8);
-      pr = load4(rbase + (int64_t)t * g.r.sl, col, (int)g.rows - row0, g.vec, live(t));
+#pragma unroll
+    for (int i = 0; i < kFetchR; ++i) {
+      const int e = tid + i * kThreads, t = t0 + e / (kRowTile / 4), col = 4 * (e % (kRowTile / 4));
+      pr[i] = load4(rbase + (int64_t)t * g.r.sl, col, (int)g.rows - row0, g.vec, live(t));
     }
     if (tid < kTok) {
       const int t = t0 + tid;
@@ -135,55 +139,70 @@ __global__ void __launch_bounds__(kThreads) k_rec(const RecArgs g) {
       *reinterpret_cast<float4*>(&ks[t][col]) = unpack4(pk[i]);
       if constexpr (OUT != kOutNone) *reinterpret_cast<float4*>(&qs[t][col]) = unpack4(pq[i]);
     }
-    *reinterpret_cast<float4*>(&rs[tid / 8][4 * (tid % 8)]) = unpack4(pr);
+#pragma unroll
+    for (int i = 0; i < kFetchR; ++i) {
+      const int e = tid + i * kThreads;
+      *reinterpret_cast<float4*>(&rs[e / (kRowTile / 4)][4 * (e % (kRowTile / 4))]) = unpack4(pr[i]);
+    }
     if (tid < kTok) {
       as[tid] = pa;
       wsm[tid] = pw;
     }
     __syncthreads();
     if (step + 1 < steps) fetch(step + 1);
-#pragma unroll 4
-    for (int i = 0; i < kTok; ++i) {
-      const int t = REV ? kTok - 1 - i : i;
-      const float a = as[t], w = wsm[t];
-      const float2 r2 = *reinterpret_cast<const float2*>(&rs[t][rp]);
-      const uint64_t aa = pair(a, a), r0 = pair(r2.x * w, r2.x * w), r1 = pair(r2.y * w, r2.y * w);
-      uint64_t p0 = 0, p1 = 0;  // two columns at a time (f32x2)
+#pragma unroll 1
+    for (int i0 = 0; i0 < kTok; i0 += kGroup) {
+      float part[16];  // [token of the group][row]
 #pragma unroll
-      for (int v = 0; v < CW / 4; ++v) {
-        const ulonglong2 k4 = *reinterpret_cast<const ulonglong2*>(&ks[t][c0 + 32 * v]);
-        ulonglong2 q4 = make_ulonglong2(0, 0);
-        if constexpr (OUT != kOutNone) q4 = *reinterpret_cast<const ulonglong2*>(&qs[t][c0 + 32 * v]);
-        const uint64_t kk[2] = {k4.x, k4.y}, qq[2] = {q4.x, q4.y};
+      for (int j = 0; j < kGroup; ++j) {
+        const int t = REV ? kTok - 1 - i0 - j : i0 + j;
+        const float a = as[t], w = wsm[t];
+        const uint64_t aa = pair(a, a);
+        uint64_t rr[R], o[R];  // two columns at a time (f32x2)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          uint64_t &x0 = s[0][2 * v + u], &x1 = s[1][2 * v + u];
-          x0 = fma2(r0, kk[u], REV ? x0 : mul2(x0, aa));
-          x1 = fma2(r1, kk[u], REV ? x1 : mul2(x1, aa));
-          if constexpr (OUT != kOutNone) {
-            p0 = fma2(x0, qq[u], p0);
-            p1 = fma2(x1, qq[u], p1);
-          }
-          if constexpr (REV) {
-            x0 = mul2(x0, aa);
-            x1 = mul2(x1, aa);
-          }
+        for (int r = 0; r < R; r += 2) {
+          const float2 r2 = *reinterpret_cast<const float2*>(&rs[t][rp + r]);
+          rr[r] = pair(r2.x * w, r2.x * w);
+          rr[r + 1] = pair(r2.y * w, r2.y * w);
+          o[r] = o[r + 1] = 0;
+        }
+#pragma unroll
+        for (int v = 0; v < CW / 4; ++v) {
+          const ulonglong2 k4 = *reinterpret_cast<const ulonglong2*>(&ks[t][c0 + 32 * v]);
+          ulonglong2 q4 = make_ulonglong2(0, 0);
+          if constexpr (OUT != kOutNone) q4 = *reinterpret_cast<const ulonglong2*>(&qs[t][c0 + 32 * v]);
+          const uint64_t kk[2] = {k4.x, k4.y}, qq[2] = {q4.x, q4.y};
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+              uint64_t& x = s[r][2 * v + u];
+              x = fma2(rr[r], kk[u], REV ? x : mul2(x, aa));
+              if constexpr (OUT != kOutNone) o[r] = fma2(x, qq[u], o[r]);
+              if constexpr (REV) x = mul2(x, aa);
+            }
+        }
+        if constexpr (OUT == kOutNone) decay *= a;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          float even, odd;
+          unpair(o[r], even, odd);
+          part[j * R + r] = even + odd;
         }
       }
-      if constexpr (OUT == kOutNone) {
-        decay *= a;
-      } else {
-        float o0, o1, e0, e1;
-        unpair(p0, o0, e0);
-        unpair(p1, o1, e1);
-        o0 += e0;
-        o1 += e1;
-        // lanes with bit 2 clear finish row 0, the others row 1
-        const bool up = lane & 4;
-        float o = (up ? o1 : o0) + __shfl_xor_sync(~0u, up ? o0 : o1, 4);
-        o += __shfl_xor_sync(~0u, o, 2);
-        o += __shfl_xor_sync(~0u, o, 1);
-        if ((lane & 3) == 0) os[t][rp + (up ? 1 : 0)] = o;
+      if constexpr (OUT != kOutNone) {
+        // lane bits 2, 1, 0 end with entries 8, 4, 2 x those bits, and the next one
+#pragma unroll
+        for (int n = 8, bit = 4; n >= 2; n /= 2, bit /= 2) {
+          const bool up = lane & bit;
+#pragma unroll
+          for (int e = 0; e < n; ++e) {
+            const float keep = up ? part[e + n] : part[e], give = up ? part[e] : part[e + n];
+            part[e] = keep + __shfl_xor_sync(~0u, give, bit);
+          }
+        }
+        const int e = 2 * (lane & 7), j = e / R, t = REV ? kTok - 1 - i0 - j : i0 + j;
+        *reinterpret_cast<float2*>(&os[t][rp + e % R]) = make_float2(part[0], part[1]);
       }
     }
     if constexpr (OUT != kOutNone) {
@@ -209,7 +228,7 @@ __global__ void __launch_bounds__(kThreads) k_rec(const RecArgs g) {
   }
   if (g.state_out) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < R; ++j)
 #pragma unroll
       for (int i = 0; i < CW; i += 2) {
         float v[2];
@@ -574,15 +593,21 @@ template <class T, bool REV, int OUT>
 bool launch_rec(RecArgs g, uint32_t batch, cudaStream_t st, bool fp32) {
   if constexpr (sizeof(T) == 2)
     if (!fp32 && g.length >= kTcTokens && launch_scan_tc<T>(g, REV, OUT, batch, st)) return true;
-  const uint64_t tiles = (g.rows + kRowTile - 1) / kRowTile;
-  const uint64_t blocks = tiles * g.nseg * g.heads * batch;
-  require(blocks < (1ull << 31), "too many blocks");
-  const dim3 grid((uint32_t)blocks);
   g.vec = vec4_ok(g.r, sizeof(T)) && vec4_ok(g.k, sizeof(T)) && (OUT == kOutNone || vec4_ok(g.q, sizeof(T)));
-  if (g.cols <= 32) k_rec<T, 4, REV, OUT><<<grid, kThreads, 0, st>>>(g);
-  else if (g.cols <= 64) k_rec<T, 8, REV, OUT><<<grid, kThreads, 0, st>>>(g);
-  else if (g.cols <= 128) k_rec<T, 16, REV, OUT><<<grid, kThreads, 0, st>>>(g);
-  else k_rec<T, 32, REV, OUT><<<grid, kThreads, 0, st>>>(g);
+  auto go = [&](auto cw, auto rv) {
+    constexpr int CW = decltype(cw)::value, R = decltype(rv)::value;
+    const uint64_t blocks = (uint64_t)((g.rows + 16 * R - 1) / (16 * R)) * g.nseg * g.heads * batch;
+    require(blocks < (1ull << 31), "too many blocks");
+    k_rec<T, CW, R, REV, OUT><<<(uint32_t)blocks, kThreads, 0, st>>>(g);
+  };
+  using std::integral_constant;
+  // narrow states: four rows to a thread, so that a token's fixed work serves as many elements
+  if (g.cols <= 32 && g.rows > 32) go(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+  else if (g.cols <= 32) go(integral_constant<int, 4>{}, integral_constant<int, 2>{});
+  else if (g.cols <= 64 && g.rows > 32) go(integral_constant<int, 8>{}, integral_constant<int, 4>{});
+  else if (g.cols <= 64) go(integral_constant<int, 8>{}, integral_constant<int, 2>{});
+  else if (g.cols <= 128) go(integral_constant<int, 16>{}, integral_constant<int, 2>{});
+  else go(integral_constant<int, 32>{}, integral_constant<int, 2>{});
   note_launch();
   FHE_CUDA(cudaGetLastError());
   return false;
@@ -624,7 +649,7 @@ Cut forward_cut(const fhe_ssm_scan_args& a) {
     const uint32_t seglen = (chunks + nseg - 1) / nseg * 128;
     return {seglen, std::max(1u, (a.length + seglen - 1) / seglen)};
   }
-  const uint64_t blocks = (uint64_t)a.batch * a.heads * ((a.head_dim + kRowTile - 1) / kRowTile);
+  const uint64_t blocks = (uint64_t)a.batch * a.heads * ((a.head_dim + 31) / 32);
   uint32_t nseg = 1;
   if (blocks < 148 * 2) nseg = (uint32_t)(148 * 4 / std::max<uint64_t>(blocks, 1));
   nseg = std::max(1u, std::min(nseg, a.length / 64));
