@@ -398,6 +398,11 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
     next_w = l ? (wp ? wp[(int64_t)tok * g.write.sl] : 1.f) : 0.f;
   };
   load_gates(first(0));
+  float row_w = 1.f;  // without CARRY: w of this thread's token, for its row scale
+  if constexpr (OUT == kOutDx || (REV && OUT == kOutRaw)) {
+    const int tok = first(0) + (int)t;
+    if (tok < t_end) row_w = g.out_scale.p[b * g.out_scale.sb + tok * g.out_scale.sl + h * g.out_scale.sh];
+  }
   const float skip = (OUT == kOutY || OUT == kOutDx) && g.d ? g.d[h] : 0.f;
 
   // The state: column t of 32 rows, in pairs; in shared memory it is the B
@@ -465,7 +470,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
     // them.  `up` undoes what the row scale took too much.
     float rho = 1.f, up = 1.f;
     if constexpr (OUT == kOutDx || (REV && OUT == kOutRaw)) {
-      const float w = live ? g.out_scale.p[b * g.out_scale.sb + tok * g.out_scale.sl + h * g.out_scale.sh] : 1.f;
+      const float w = row_w;
       rho = OUT == kOutRaw || kHalf ? w * scale_of(w) : w;
       if constexpr (OUT == kOutRaw) {
         if (fabsf(rho) < 1.f) rho = 1.f;  // 0 or denormal
@@ -476,7 +481,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
     }
     if (i > 0) {  // (the barriers are initialised before the first)
       ok = __all_sync(~0u, wait(bar_kq, par)) && ok;
-      if (!live) {
+      if (!live && t_end < t_hi) {
         clear(sk, kHalves);
         if constexpr (OUT != kOutNone) clear(sq, kHalves);
       }
@@ -488,7 +493,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
     if (!ok) break;
     if (i == 0) {
       ok = __all_sync(~0u, wait(bar_kq, par));
-      if (!live) {
+      if (!live && t_end < t_hi) {
         clear(sk, kHalves);
         if constexpr (OUT != kOutNone) clear(sq, kHalves);
       }
@@ -545,7 +550,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
       fence_after();
     }
     ok = __all_sync(~0u, wait(bar_r, par)) && ok;
-    if (!live) clear(sr, kRowTiles);
+    if (!live && t_end < t_hi) clear(sr, kRowTiles);
     if (ok) {
       // O starts from P_t (q S0) and the skip term; the scaled r, in two terms, goes over q
 #pragma unroll
@@ -691,24 +696,9 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
               unpair(mul2(x, pair(up, up)), v[e], v[e + 1]);
             }
           }
-          if (tok < t_hi && row < g.rows && (OUT != kOutRaw || live)) {
-            const int64_t at = (((int64_t)b * g.length + tok) * g.heads + h) * g.rows + row;
-            if constexpr (OUT == kOutRaw) {
-              float* o = static_cast<float*>(g.out) + at;
-#pragma unroll
-              for (int e = 0; e < 32; e += 4)
-                if (row + e < g.rows)
-                  *reinterpret_cast<float4*>(o + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-            }
-          }
-          if constexpr (OUT != kOutRaw) {
-            // Four lanes hold 64 bytes of four tokens each; transposed among
-            // them, every store covers whole 64-byte runs of eight tokens.
-            uint32_t x[4][4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-              for (int f = 0; f < 4; ++f) x[e][f] = live ? pack2<T>(pair(v[8 * e + 2 * f], v[8 * e + 2 * f + 1])) : 0u;
+          // Four lanes hold words of four tokens each; transposed among them,
+          // every store covers whole 64-byte runs of eight tokens.
+          auto transpose = [&](uint32_t (&x)[4][4]) {
 #pragma unroll
             for (int d = 1; d < 4; d *= 2) {
               const bool up = lane & d;
@@ -724,7 +714,32 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
                 }
               }
             }
-            // x[e]: word lane & 3 of the token 4 (lane / 4) + e of the warp's 32
+          };  // x[e]: word lane & 3 of the token 4 (lane / 4) + e of the warp's 32
+          if constexpr (OUT == kOutRaw) {
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {  // 16 rows: four words of four
+              uint32_t x[4][4];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) x[e / 4][e % 4] = __float_as_uint(v[16 * part + e]);
+              transpose(x);
+              const uint32_t col = row + 16 * part + 4 * (lane & 3);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int tk = t0 + (int)(quarter * 32 + (lane & ~3u) + e);
+                if (tk < t_end && col < g.rows)
+                  *reinterpret_cast<uint4*>(static_cast<float*>(g.out) +
+                                            (((int64_t)b * g.length + tk) * g.heads + h) * g.rows + col) =
+                      make_uint4(x[e][0], x[e][1], x[e][2], x[e][3]);
+              }
+            }
+          }
+          if constexpr (OUT != kOutRaw) {
+            uint32_t x[4][4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int f = 0; f < 4; ++f) x[e][f] = live ? pack2<T>(pair(v[8 * e + 2 * f], v[8 * e + 2 * f + 1])) : 0u;
+            transpose(x);
             const uint32_t col = row + 8 * (lane & 3);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
