@@ -73,6 +73,24 @@ __device__ __forceinline__ void load_bias(const void* bias, uint32_t c, float (&
   else vset(o, 0.f);
 }
 
+// A thread's own tokens on their way to it: batches of kAhead packs go to its
+// slots of a ring in shared memory by asynchronous copies, so that RING - 1
+// batches are in flight without holding registers.  No thread reads another's
+// slots, so no barrier is needed.
+constexpr int kAhead = 4;
+template <class T, int V>
+__device__ __forceinline__ void copy_pack(Pack<T, V>* to, const T* from) {
+  constexpr int kBytes = V * sizeof(T);
+  const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+  if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(from), "n"(kBytes) : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+template <class T, int V>
+constexpr bool kCopies = V * sizeof(T) >= 4;  // the smallest asynchronous copy
+
 // Thread = V channels x one run of tokens, channels fastest.  `STEP` (one
 // token): the same thread also writes the window behind it, so the state may
 // be updated in place.
@@ -131,25 +149,29 @@ __global__ void __launch_bounds__(kThreads) k_conv(const ConvArgs g) {
   const int t_live = min(t1, len);
   const T* xt = x + (int64_t)t * g.sl;
   if constexpr (!STEP) {
-    // kAhead tokens are used while the next kAhead are on their way
-    constexpr int kAhead = 4;
-    auto fetch = [&](Pack<T, V> (&in)[kAhead]) {
+    if constexpr (kCopies<T, V>) {
+      constexpr int kRing = 4;
+      __shared__ Pack<T, V> ring[kRing][kAhead][kThreads];
+      const int batches = t_live > t ? (t_live - t) / kAhead : 0;
+      auto fetch = [&](int i) {
+        if (i < batches) {
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j, xt += g.sl) in[j] = *reinterpret_cast<const Pack<T, V>*>(xt);
-    };
-    if (t + kAhead <= t_live) {
-      Pack<T, V> now[kAhead], next[kAhead];
-      fetch(now);
-      for (; t + 2 * kAhead <= t_live; t += kAhead) {
-        fetch(next);
+          for (int j = 0; j < kAhead; ++j, xt += g.sl) copy_pack(&ring[i % kRing][j][threadIdx.x], xt);
+        }
+        copies_done();
+      };
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) token(now[j]);
+      for (int i = 0; i < kRing - 1; ++i) fetch(i);
+      for (int i = 0; i < batches; ++i) {
+        wait_copies<kRing - 2>();
+        Pack<T, V> in[kAhead];
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) now[j] = next[j];
+        for (int j = 0; j < kAhead; ++j) in[j] = ring[i % kRing][j][threadIdx.x];
+        fetch(i + kRing - 1);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) token(in[j]);
       }
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) token(now[j]);
-      t += kAhead;
+      t += batches * kAhead;
     }
   }
   for (; t < t_live; ++t, xt += g.sl) token(*reinterpret_cast<const Pack<T, V>*>(xt));
@@ -276,30 +298,46 @@ __global__ void __launch_bounds__(kThreads) k_conv_grad(const ConvGradArgs a) {
   int t = t0;
   for (; t < min(t0 + K - 1, t2); ++t) one(t);
   // whole batches of the run's own live tokens, none of whose row elements takes a final state's gradient
-  constexpr int kAhead = 4;
-  auto fetch = [&](Pack<T, V> (&xin)[kAhead], Pack<T, V> (&din)[kAhead]) {
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j, xt += g.sl, dt += g.channels) {
-      xin[j] = *reinterpret_cast<const Pack<T, V>*>(xt);
-      din[j] = *reinterpret_cast<const Pack<T, V>*>(dt);
-    }
-  };
   const int t_main = min(t1, len);
-  for (; t + kAhead <= t_main; t += kAhead) {
-    Pack<T, V> xin[kAhead], din[kAhead];
-    fetch(xin, din);
+  if constexpr (kCopies<T, V>) {
+    constexpr int kRing = 3;
+    __shared__ Pack<T, V> ring[2][kRing][kAhead][kThreads];
+    const int batches = t_main > t ? (t_main - t) / kAhead : 0;
+    auto fetch = [&](int i) {
+      if (i < batches) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j, xt += g.sl, dt += g.channels) {
+          copy_pack(&ring[0][i % kRing][j][threadIdx.x], xt);
+          copy_pack(&ring[1][i % kRing][j][threadIdx.x], dt);
+        }
+      }
+      copies_done();
+    };
+#pragma unroll
+    for (int i = 0; i < kRing - 1; ++i) fetch(i);
     T* out = dx + (int64_t)(t - (K - 1)) * g.channels;
+    for (int i = 0; i < batches; ++i) {
+      wait_copies<kRing - 2>();
+      Pack<T, V> xin[kAhead], din[kAhead];
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j, out += g.channels) {
-      shift();
-      slope(xin[j], din[j]);
-      taps();
-      float o[V];
-      vmul(o, w[0], dp[K - 1]);
+      for (int j = 0; j < kAhead; ++j) {
+        xin[j] = ring[0][i % kRing][j][threadIdx.x];
+        din[j] = ring[1][i % kRing][j][threadIdx.x];
+      }
+      fetch(i + kRing - 1);
 #pragma unroll
-      for (int i = 1; i < K; ++i) vfma(o, w[i], dp[K - 1 - i], o);
-      *reinterpret_cast<Pack<T, V>*>(out) = pack<T>(o);
+      for (int j = 0; j < kAhead; ++j, out += g.channels) {
+        shift();
+        slope(xin[j], din[j]);
+        taps();
+        float o[V];
+        vmul(o, w[0], dp[K - 1]);
+#pragma unroll
+        for (int i = 1; i < K; ++i) vfma(o, w[i], dp[K - 1 - i], o);
+        *reinterpret_cast<Pack<T, V>*>(out) = pack<T>(o);
+      }
     }
+    t += batches * kAhead;
   }
   for (; t < t2; ++t) one(t);
   float* part = a.part + ((int64_t)b * g.runs + run) * (K + 1) * g.channels + c;
