@@ -100,7 +100,8 @@ def scan_struct(**kw):
     (dict(dtype=7), "dtype"), (dict(heads=3, groups=2), "multiple of groups"), (dict(groups=0), "multiple of groups"),
     (dict(head_dim=0), "head_dim"), (dict(head_dim=200), "head_dim"), (dict(d_state=300), "d_state"),
     (dict(x=None), "null input"), (dict(y=None), "null output"), (dict(final_state=None), "null output"),
-    (dict(batch=1 << 20, length=1 << 20), "below 2"),
+    (dict(batch=1 << 20, length=1 << 20), "below 2"), (dict(batch=1 << 8, heads=1 << 16), "below 2"),
+    (dict(batch=1, heads=1 << 16, length=1 << 20), "below 2"),
     (dict(length=4096), "workspace too small"), (dict(length=4096, workspace=256 * 3 + 1, workspace_bytes=1 << 40), "aligned"),
 ])
 def test_scan_c_refusals(kw, message):
