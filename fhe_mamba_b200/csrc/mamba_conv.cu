@@ -76,7 +76,9 @@ __device__ __forceinline__ void load_bias(const void* bias, uint32_t c, float (&
 // A thread's own tokens on their way to it: batches of kAhead packs go to its
 // slots of a ring in shared memory by asynchronous copies, so that RING - 1
 // batches are in flight without holding registers.  No thread reads another's
-// slots, so no barrier is needed.
+// slots, so no barrier is needed.  8 x 4096 tokens of 1792 bfloat16 channels, 4
+// taps: 45 us, 5.2 TB/s (60 us with the batches in registers, half of them in
+// flight).
 constexpr int kAhead = 4;
 template <class T, int V>
 __device__ __forceinline__ void copy_pack(Pack<T, V>* to, const T* from) {
@@ -202,6 +204,8 @@ struct ConvGradArgs {
 // tokens more: dpre_t = dy_t act'(pre_t) enters a window of taps values, and
 // drow_u = sum_i w_i dpre_(u-i) (u a row index, u - (K - 1) a token) leaves
 // it.  The taps' and bias's gradients of the run's own tokens go to `part`.
+// 8 x 1001 tokens of 1792 float32 channels: 44 us, 3.9 TB/s; registers (two
+// windows and the taps' sums) keep it to 20 warps an SM.
 template <class T, int V, int K, bool SILU>
 __global__ void __launch_bounds__(kThreads) k_conv_grad(const ConvGradArgs a) {
   const ConvArgs& g = a.f;

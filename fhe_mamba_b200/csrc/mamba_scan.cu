@@ -53,6 +53,9 @@ __device__ __forceinline__ float4 unpack4(const Pack<T, 4>& v) {
 // add with 14 shuffles for all of them (one token's alone would take three,
 // each waited for: 113 instructions a token against 80, and the latency).
 // The next tokens are fetched into registers while the present ones are used.
+// 8 x 509 float32 tokens of 24 heads x 64, state 128: 166 us, 67 at the FMA
+// pipe's rate (three operations an element); the shared-memory loads of k and q
+// and 10 warps an SM bound it.
 template <class T, int CW, int R, bool REV, int OUT>
 __global__ void __launch_bounds__(kThreads) k_rec(const RecArgs g) {
   constexpr int kRowTile = 16 * R, kGroup = 16 / R;  // rows per block, tokens per round of sums
@@ -249,7 +252,8 @@ __global__ void __launch_bounds__(kThreads) k_rec(const RecArgs g) {
 // A row of S lies across G lanes in 16-byte words (NV words per lane); a warp
 // takes kStepRows x 32 / G rows and has all their loads in flight at once.
 // Each element is read and written by one thread: the state may be updated
-// in place.
+// in place.  192 sequences of 24 heads x 64 x 128: 55 us, 5.5 TB/s (85% of a
+// measured copy's rate).
 struct StepArgs {
   Src x, b, c;
   Gate write, log_decay;
@@ -404,7 +408,8 @@ __device__ __forceinline__ float sum_each(float (&v)[COUNT], uint32_t lane) {
 // One warp per token: sums U and dC_h over the heads of each group in order
 // and forms the per-head products.  Memory-bound: it reads the two per-head
 // arrays once, H heads at a time with all their loads in flight.  A lane holds
-// V neighbouring columns of every 32 V, NP of those.
+// V neighbouring columns of every 32 V, NP of those.  4 x 2048 bfloat16 tokens of
+// 24 heads: 94 us, 2.7 TB/s (a block of 8 warps per token: 180 us).
 template <class T, int V, int NP, int H>
 __global__ void __launch_bounds__(128) k_sum(const SumArgs g, uint32_t tokens) {
   const uint32_t id = (blockIdx.x * 128 + threadIdx.x) >> 5, lane = threadIdx.x & 31;

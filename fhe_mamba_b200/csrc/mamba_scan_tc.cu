@@ -28,6 +28,13 @@
 // memory: G (its columns become the A operand G o L o w), O (which starts from
 // the scaled q S0^T) and S'.  The state itself stays in registers.
 //
+// 8 x 4096 bfloat16 tokens of 24 heads x 64, state 128: 225 us, of which memory
+// needs 36 and the products about 60 at full rate; a chunk is a chain of
+// products and element passes that two CTAs to an SM cover in part (issue slots
+// 36% busy).  Loads by tensor maps and stores of 64-byte runs took the load and
+// store unit out of that chain (343 us with 16-byte asynchronous copies and
+// scattered stores).
+//
 // A walk that carries no state on (CARRY false: the gradients', a segment of
 // one chunk each) leaves S' out and takes 128 rows where there are as many.
 #include <algorithm>

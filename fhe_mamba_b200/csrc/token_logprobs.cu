@@ -223,6 +223,10 @@ struct Part {
 // CTA takes a share of the row, and the first puts the shares together over
 // distributed shared memory.  Elements before the row's first 16-byte boundary
 // and after its last go to threads of the first CTA one by one.
+// 2048 bfloat16 rows of 50304: 52 us, 4.0 TB/s; 4095 rows of 50280 with the 8 top
+// entries: 124 us, 3.3 TB/s.  Issue slots (60% busy) and the latency between a
+// row's turns bound it: 9 instructions an element, 4.5 of them the conversion,
+// exponential and sums.
 template <class T, bool TOP>
 __global__ void __launch_bounds__(kThreads, 4) k_logprobs(const fhe_token_logprobs_args g, uint32_t split) {
   using Q = Quad<T>;
@@ -501,6 +505,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(const fhe_token_logpro
 // dlogits = p (-G - g_e (log p + H)) plus, at the target and the top entries,
 // their own gradients; G is the sum of those.  One read, one write, in 16-byte
 // words where logits and dlogits reach a 16-byte boundary at the same element.
+// 2048 bfloat16 rows of 50304: 64 us, 6.4 TB/s, a measured copy's rate.
 template <class T>
 __global__ void __launch_bounds__(kThreads) k_logprobs_grad(const fhe_token_logprobs_grad_args a, uint32_t parts) {
   using Q = Quad<T>;
