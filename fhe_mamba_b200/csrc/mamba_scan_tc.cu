@@ -15,7 +15,8 @@
 // G o L o w and S0 enter their products in the activations' type, half a step
 // of each term (2^-8 for bfloat16) as y's own rounding; with PRECISE they
 // enter as two terms of that type (2^-16).  E o w o r, whose sum is the fp32
-// state, always enters as two terms.
+// state, always enters with 22 bits and more: three terms of bfloat16 or two of
+// float16.
 // For float16 the factors are scaled by powers of two (the chunk's largest w to
 // about 8, the state by 16) to use its range; where an operand overflows all
 // the same, a product is not finite, the kernel says so in *bad, and the
@@ -28,7 +29,7 @@
 // memory: G (its columns become the A operand G o L o w), O (which starts from
 // the scaled q S0^T) and S'.  The state itself stays in registers.
 //
-// 8 x 4096 bfloat16 tokens of 24 heads x 64, state 128: 225 us, of which memory
+// 8 x 4096 bfloat16 tokens of 24 heads x 64, state 128: 199 us, of which memory
 // needs 36 and the products about 60 at full rate; a chunk is a chain of
 // products and element passes that two CTAs to an SM cover in part (issue slots
 // 36% busy).  Loads by tensor maps and stores of 64-byte runs took the load and
@@ -327,6 +328,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
   constexpr uint32_t kBytesK = kHalves * kTile;
   constexpr uint32_t kBytesR = kRowTiles * kTile;
   constexpr uint32_t kTileS = COLS * 128, kBytesS = kRowTiles * kTileS;
+  constexpr bool kThird = CARRY && !std::is_same_v<T, __half>;  // a third term of the scaled r, in S0's place
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ __align__(16) Gates gate;
@@ -576,11 +578,17 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
             const uint4 q4 = *reinterpret_cast<const uint4*>(smem + (sr - sq) + at);
             x[0] = q4.x, x[1] = q4.y, x[2] = q4.z, x[3] = q4.w;
           }
-          uint32_t hi[4], lo[4];
+          uint32_t hi[4], lo[4], third[4];
 #pragma unroll
           for (int f = 0; f < 4; ++f) {
             const uint64_t xx = unpack2<T>(x[f]);
-            if constexpr (CARRY) split2<T>(mul2(pair(et, et), xx), hi[f], lo[f]);
+            if constexpr (CARRY) {
+              const uint64_t scaled = mul2(pair(et, et), xx);
+              split2<T>(scaled, hi[f], lo[f]);
+              if constexpr (kThird)
+                third[f] = pack2<T>(fma2(unpack2<T>(lo[f]), pair(-1.f, -1.f),
+                                         fma2(unpack2<T>(hi[f]), pair(-1.f, -1.f), scaled)));
+            }
             if constexpr (OUT != kOutNone) {
               float *o = v + 8 * e + 2 * f;
               uint64_t a = mul2(pair(pt, pt), pair(o[0], o[1]));
@@ -591,6 +599,8 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
           if constexpr (CARRY) {
             *reinterpret_cast<uint4*>(smem + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
             *reinterpret_cast<uint4*>(smem + kTile + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            if constexpr (kThird)
+              *reinterpret_cast<uint4*>(smem + (ss - sq) + at) = make_uint4(third[0], third[1], third[2], third[3]);
           }
         }
         if constexpr (OUT != kOutNone) tmem_st32(tmem + lanes + kColO + piece * 32, v);
@@ -641,6 +651,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
             const uint64_t a = desc(sk + j * 2048, lead);
             mma_ss(tmem + kColS, a, desc(sq + j * 2048, 0), idesc<T>(64, true, true), j);
             mma_ss(tmem + kColS, a, desc(sq + kTile + j * 2048, 0), idesc<T>(64, true, true), 1);
+            if constexpr (kThird) mma_ss(tmem + kColS, a, desc(ss + j * 2048, 0), idesc<T>(64, true, true), 1);
           }
           commit(bar_s);
         }
@@ -837,7 +848,7 @@ bool make_map(CUtensorMap& m, const Src& s, uint32_t width, const RecArgs& g, ui
 template <class T, int COLS, int ROWS, bool REV, int OUT, bool PRECISE, bool CARRY>
 void launch(const RecArgs& g, const Maps& maps, uint32_t batch, cudaStream_t st) {
   const uint32_t need = 1024 + (CARRY ? 2 : COLS / 64) * kTile + COLS / 64 * kTile + ROWS / 64 * kTile +
-                        COLS * 128 * (ROWS / 64) * (PRECISE ? 2 : 1);
+                        std::max(COLS * 128u * (ROWS / 64) * (PRECISE ? 2 : 1), CARRY ? kTile : 0u);
   const uint32_t smem = std::max(need, kLeastSmem);
   auto* kernel = k_scan_tc<T, COLS, ROWS, REV, OUT, PRECISE, CARRY>;
   FHE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
