@@ -29,7 +29,7 @@
 // memory: G (its columns become the A operand G o L o w), O (which starts from
 // the scaled q S0^T) and S'.  The state itself stays in registers.
 //
-// 8 x 4096 bfloat16 tokens of 24 heads x 64, state 128: 199 us, of which memory
+// 8 x 4096 bfloat16 tokens of 24 heads x 64, state 128: 193 us, of which memory
 // needs 36 and the products about 60 at full rate; a chunk is a chain of
 // products and element passes that two CTAs to an SM cover in part (issue slots
 // 36% busy).  Loads by tensor maps and stores of 64-byte runs took the load and
@@ -215,7 +215,7 @@ struct Gates {
   float most[4];         // largest |w| in each block of 32 (float16)
 };
 
-// Warps 0-3, one token per thread.
+// Four warps, one token per thread.
 template <bool REV>
 __device__ __forceinline__ void put_gates(Gates& g, uint32_t t, uint32_t lane, float a, float w) {
   const float after = __shfl_down_sync(~0u, a, 1);
@@ -399,10 +399,10 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
 
   const float* wp = g.write.p ? g.write.p + (int64_t)b * g.write.sb + (int64_t)h * g.write.sh : nullptr;
   const float* ap = g.log_decay.p + (int64_t)b * g.log_decay.sb + (int64_t)h * g.log_decay.sh;
-  float next_a = 0.f, next_w = 0.f;  // warps 0-3: the gates of the chunk to come
+  float next_a = 0.f, next_w = 0.f;  // warps 4-7 (warp 0 has the products to issue): the gates of the chunk to come
   auto load_gates = [&](int t0) {
     const int tok = t0 + (int)t;
-    const bool l = tid < kQ && tok < t_end;
+    const bool l = tid >= kQ && tok < t_end;
     next_a = l ? ap[(int64_t)tok * g.log_decay.sl] : 0.f;
     next_w = l ? (wp ? wp[(int64_t)tok * g.write.sl] : 1.f) : 0.f;
   };
@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
     const int t0 = first(i), tok = t0 + (int)t;
     const bool live = tok < t_end;
     const uint32_t par = i & 1;
-    if (tid < kQ) put_gates<REV>(gate, t, lane, expf(next_a), next_w);
+    if (tid >= kQ) put_gates<REV>(gate, t, lane, expf(next_a), next_w);
     // Row scale of this token's products: w of dx; for U of the gradients the
     // mantissa of w, so that its products are rounded at w_t times their value
     // as those of dC_h are, up to a power of two.  alpha and beta, whose
