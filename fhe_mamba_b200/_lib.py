@@ -112,7 +112,7 @@ class TokenLogprobsArgs(ctypes.Structure):
     _fields_ = [
         ("device", i32), ("dtype", i32), ("rows", u32), ("vocab", u32), ("top_k", u32), ("reserved", u32),
         ("logits", vp), ("logits_stride", i64), ("targets", vp), ("logprob", vp), ("entropy", vp),
-        ("top_logprobs", vp), ("top_ids", vp), ("lse", vp), ("stream", vp),
+        ("top_logprobs", vp), ("top_ids", vp), ("norm", vp), ("stream", vp),
     ]
 
 

@@ -481,7 +481,9 @@ __global__ void __launch_bounds__(kThreads, 4) k_logprobs(const fhe_token_logpro
       const float h = ls - a.u / a.s;
       g.logprob[row] = lp;
       g.entropy[row] = empty ? 0.f : plain ? kLn2 * h : h;
-      g.lse[row] = empty ? -INFINITY : plain ? kLn2 * (shift_a + ls) : a.m + ls;
+      // the shift's own rounding, left out of m, goes back into the sum
+      g.norm[2 * (int64_t)row] = a.m;
+      g.norm[2 * (int64_t)row + 1] = empty ? 0.f : plain ? kLn2 * (ls + fmaf(-a.m, kLog2e, shift_a)) : ls;
     }
     if constexpr (TOP) {
       for (uint32_t c = tid; c < split * kMaxTop; c += kThreads) {
@@ -517,8 +519,9 @@ __global__ void __launch_bounds__(kThreads) k_logprobs_grad(const fhe_token_logp
   T* dz = static_cast<T*>(a.dlogits) + (int64_t)row * vocab;
   const uint32_t each = (vocab + parts - 1) / parts;  // elements of this part
   const uint32_t e0 = min(part * each, vocab), e1 = min(e0 + each, vocab);
-  const float lse = g.lse[row];
-  if (lse == -INFINITY) {  // nothing is possible: no gradient
+  // log p = (z - m) - log s: neither loses the other's digits at large |m|
+  const float m = g.norm[2 * (int64_t)row], ls = g.norm[2 * (int64_t)row + 1];
+  if (m == -INFINITY) {  // nothing is possible: no gradient
     for (uint32_t e = e0 + tid; e < e1; e += kThreads) dz[e] = from_f<T>(0.f);
     return;
   }
@@ -530,18 +533,18 @@ __global__ void __launch_bounds__(kThreads) k_logprobs_grad(const fhe_token_logp
   for (uint32_t i = 0; i < k; ++i) G += a.dtop_logprobs[(int64_t)row * k + i];
   const float c = -G - ge * H;
   auto base = [&](float v) {
-    const float lp = fmaxf(v - lse, -1e37f), d = exp2_fast(lp * kLog2e) * fmaf(-ge, lp, c);
+    const float lp = fmaxf((v - m) - ls, -1e37f), d = exp2_fast(lp * kLog2e) * fmaf(-ge, lp, c);
     return isnan(v) ? v : v == -INFINITY ? 0.f : d;
   };
   auto scalar = [&](uint32_t lo, uint32_t hi) {
     for (uint32_t e = lo + tid; e < hi; e += kThreads) dz[e] = from_f<T>(base(to_f(z[e])));
   };
   const uint32_t head = min(e1 - e0, (uint32_t)((0 - reinterpret_cast<uintptr_t>(dz + e0)) % 16 / sizeof(T)));
-  if (plain_max<T>(lse) && reinterpret_cast<uintptr_t>(z + e0 + head) % 16 == 0) {
+  if (plain_max<T>(m) && isfinite(ls) && reinterpret_cast<uintptr_t>(z + e0 + head) % 16 == 0) {
     const uint32_t packs = (e1 - e0 - head) / V;
     const T* zb = z + e0 + head;
     T* db = dz + e0 + head;
-    const uint64_t sub = pair(-lse, -lse), l2 = pair(kLog2e, kLog2e), nge = pair(-ge, -ge), cc = pair(c, c);
+    const uint64_t sub = pair(-m, -m), sub2 = pair(-ls, -ls), l2 = pair(kLog2e, kLog2e), nge = pair(-ge, -ge), cc = pair(c, c);
     for (uint32_t i = tid; i < packs; i += kAhead * kThreads) {
       Q p[kAhead];
 #pragma unroll
@@ -553,7 +556,8 @@ __global__ void __launch_bounds__(kThreads) k_logprobs_grad(const fhe_token_logp
         float o[V];
 #pragma unroll
         for (uint32_t v = 0; v < V; v += 2) {
-          const uint64_t lp = add2(pair(fmaxf(p[j].element(v), floor_of<T>()), fmaxf(p[j].element(v + 1), floor_of<T>())), sub);
+          const uint64_t lp = add2(
+              add2(pair(fmaxf(p[j].element(v), floor_of<T>()), fmaxf(p[j].element(v + 1), floor_of<T>())), sub), sub2);
           float x0, x1;
           unpair(mul2(lp, l2), x0, x1);
           unpair(mul2(pair(exp2_fast(x0), exp2_fast(x1)), fma2(nge, lp, cc)), o[v], o[v + 1]);
@@ -596,7 +600,7 @@ void check_logprobs(const fhe_token_logprobs_args& a) {
 void token_logprobs(const fhe_token_logprobs_args& a) {
   check_logprobs(a);
   if (a.rows == 0) return;
-  require(a.logits && a.targets && a.logprob && a.entropy && a.lse, "null input or output");
+  require(a.logits && a.targets && a.logprob && a.entropy && a.norm, "null input or output");
   require(a.top_k == 0 || (a.top_logprobs && a.top_ids), "null top outputs");
   DeviceGuard dev(a.device);
   cudaStream_t st = static_cast<cudaStream_t>(a.stream);
@@ -628,7 +632,7 @@ void token_logprobs(const fhe_token_logprobs_args& a) {
 void token_logprobs_backward(const fhe_token_logprobs_grad_args& a) {
   check_logprobs(a.f);
   if (a.f.rows == 0) return;
-  require(a.f.logits && a.f.targets && a.f.lse && a.dlogits, "null input or output");
+  require(a.f.logits && a.f.targets && a.f.norm && a.dlogits, "null input or output");
   require(!a.dentropy || a.f.entropy, "null entropy");
   require(!a.dtop_logprobs || a.f.top_k == 0 || a.f.top_ids, "null top_ids");
   DeviceGuard dev(a.f.device);

@@ -225,7 +225,7 @@ def ssm_step(state, x, write, log_decay, B, C, D=None, out=None):
     op = "ssm_step"
     _need(x.dim() == 3 and B.dim() == 3 and C.dim() == 3 and write.dim() == 2 and log_decay.dim() == 2,
           "ssm_step: one token of each sequence, without a length axis")
-    if _wants_grad(state, x, write, log_decay, B, C, D):
+    if _wants_grad(state, x, write, log_decay, B, C, D, out):
         _need(False, f"{op} has no gradient (use ssm_scan)")
     b, h, p = x.shape
     k, n = B.shape[1:]
@@ -358,7 +358,7 @@ def causal_conv_step(state, x, weight, bias=None, activation="silu", out=None):
     Returns (y, new state)."""
     op = "causal_conv_step"
     _need(x.dim() == 2, "causal_conv_step: one token of each sequence, without a length axis")
-    if _wants_grad(state, x, weight, bias):
+    if _wants_grad(state, x, weight, bias, out):
         _need(False, f"{op} has no gradient (use causal_conv)")
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     x = x.unsqueeze(1)
@@ -380,41 +380,42 @@ class TokenLogprobs(NamedTuple):
     top_ids: torch.Tensor       # [rows, top_k] int64
 
 
-def _logprob_args(logits, targets, top_k, logprob, entropy, top_logprobs, top_ids, lse):
+def _logprob_args(logits, targets, top_k, logprob, entropy, top_logprobs, top_ids, norm):
     return _lib.TokenLogprobsArgs(
         logits.device.index, _TYPES[logits.dtype], logits.shape[0], logits.shape[1], top_k, 0, logits.data_ptr(),
         logits.stride(0), targets.data_ptr(), _ptr(logprob), _ptr(entropy), _ptr(top_logprobs), _ptr(top_ids),
-        lse.data_ptr(), _stream_of(logits.device.index))
+        norm.data_ptr(), _stream_of(logits.device.index))
 
 
 def _run_logprobs(logits, targets, top_k):
     r, d = logits.shape[0], logits.device
     logprob = torch.empty(r, dtype=torch.float32, device=d)
-    entropy, lse = torch.empty_like(logprob), torch.empty_like(logprob)
+    entropy = torch.empty_like(logprob)
+    norm = torch.empty((r, 2), dtype=torch.float32, device=d)
     top = torch.empty((r, top_k), dtype=torch.float32, device=d)
     ids = torch.empty((r, top_k), dtype=torch.int64, device=d)
-    call("fhe_token_logprobs", ctypes.byref(_logprob_args(logits, targets, top_k, logprob, entropy, top, ids, lse)))
-    return logprob, entropy, top, ids, lse
+    call("fhe_token_logprobs", ctypes.byref(_logprob_args(logits, targets, top_k, logprob, entropy, top, ids, norm)))
+    return logprob, entropy, top, ids, norm
 
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top_k):
-        logprob, entropy, top, ids, lse = _run_logprobs(logits, targets, top_k)
+        logprob, entropy, top, ids, norm = _run_logprobs(logits, targets, top_k)
         ctx.mark_non_differentiable(ids)
         ctx.set_materialize_grads(False)
         ctx.top_k = top_k
-        ctx.save_for_backward(logits, targets, entropy, ids, lse)
+        ctx.save_for_backward(logits, targets, entropy, ids, norm)
         return logprob, entropy, top, ids
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dlogprob, dentropy, dtop, _):
-        logits, targets, entropy, ids, lse = ctx.saved_tensors
+        logits, targets, entropy, ids, norm = ctx.saved_tensors
         dlogprob, dentropy, dtop = (None if g is None else g.contiguous() for g in (dlogprob, dentropy, dtop))
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         a = _lib.TokenLogprobsGradArgs(
-            _logprob_args(logits, targets, ctx.top_k, None, entropy, None, ids, lse), _ptr(dlogprob),
+            _logprob_args(logits, targets, ctx.top_k, None, entropy, None, ids, norm), _ptr(dlogprob),
             _ptr(dentropy), _ptr(dtop) if ctx.top_k else None, out.data_ptr(), _stream_of(logits.device.index))
         call("fhe_token_logprobs_backward", ctypes.byref(a))
         return out, None, None

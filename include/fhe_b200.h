@@ -363,8 +363,8 @@ int fhe_ctx_set_keyswitch_fusion(fhe_ctx* ctx, int32_t fused);
  * noise, not word for word. */
 int fhe_ctx_set_giant_hoisting(fhe_ctx* ctx, int32_t on);
 /* Number of tensor-core blocks (basis conversions, state scans) whose bounded
- * wait for their MMA
- * ran out (their outputs were skipped); 0 on a healthy device. */
+ * wait for their MMA ran out (their outputs were skipped); 0 on a healthy
+ * device. */
 int fhe_tc_timeouts(uint64_t* count);
 
 /* Bootstrapping of the context's slots (full packing N/2, or sparse packing:
@@ -635,14 +635,14 @@ typedef struct fhe_token_logprobs_args {
   float* entropy;             /* [rows] */
   float* top_logprobs;        /* [rows][top_k], or NULL if top_k == 0 */
   int64_t* top_ids;           /* [rows][top_k], or NULL if top_k == 0 */
-  float* lse;                 /* [rows]: log of the sum of exponentials */
+  float* norm;                /* [rows][2]: the row's maximum m, and log of the sum of exp(z - m) */
   void* stream;
 } fhe_token_logprobs_args;
 int fhe_token_logprobs(const fhe_token_logprobs_args* args);
 
 /* dlogits (contiguous, dtype) from the gradients of logprob, entropy and
  * top_logprobs (each NULL for zeros); `f` as in the forward call, with its
- * entropy, top_ids and lse outputs as inputs.  An ignored or out-of-range
+ * entropy, top_ids and norm outputs as inputs.  An ignored or out-of-range
  * target passes no gradient, a row of -inf alone gets zeros. */
 typedef struct fhe_token_logprobs_grad_args {
   fhe_token_logprobs_args f;

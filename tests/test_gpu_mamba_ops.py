@@ -479,6 +479,30 @@ def test_logprobs_masks(ops, dtype):
     assert torch.isfinite(d).all() and (d[4] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_logprobs_lowest_masks(ops, dtype):
+    """Masks of the type's lowest number: impossible beside ordinary entries, uniform among themselves."""
+    z, t = logits_of(4, 4, 2000, dtype)
+    low = torch.finfo(dtype).min
+    z[0, 100:] = low
+    t[0] = 50
+    z[1, :] = low
+    z[2, :] = low
+    z[2, 7] = -math.inf
+    z[3, 5:] = -math.inf
+    z[3, :5] = low
+    t[2], t[3] = 9, 2
+    check_logprobs(ops, z, t, 5)
+
+
+def test_logprobs_far_from_zero(ops):
+    """A common offset changes nothing but the logits' own rounding: scores and gradients keep their digits."""
+    z, t = logits_of(6, 5, 3000, torch.float32)
+    check_logprobs(ops, z + 1e5, t, 4)
+    check_logprobs(ops, z * 1e3 - 1e6, t, 4)
+    check_logprobs(ops, z * 1e36, t, 4)
+
+
 def test_logprobs_ties_and_odd_rows(ops):
     z = torch.zeros(3, 9000, device="cuda")          # every entry equal: more candidates than are kept
     z[1, 5000:] = 1
