@@ -223,12 +223,13 @@ struct Part {
 // CTA takes a share of the row, and the first puts the shares together over
 // distributed shared memory.  Elements before the row's first 16-byte boundary
 // and after its last go to threads of the first CTA one by one.
-// 2048 bfloat16 rows of 50304: 52 us, 4.0 TB/s; 4095 rows of 50280 with the 8 top
-// entries: 124 us, 3.3 TB/s.  Issue slots (60% busy) and the latency between a
+// 2048 bfloat16 rows of 50304: 51 us, 4.0 TB/s; 4095 rows of 50280 with the 8 top
+// entries: 118 us, 3.5 TB/s (126 with four CTAs to an SM, 151 with six and half the
+// loads in flight).  Issue slots (60% busy) and the latency between a
 // row's turns bound it: 9 instructions an element, 4.5 of them the conversion,
 // exponential and sums.
 template <class T, bool TOP>
-__global__ void __launch_bounds__(kThreads, 4) k_logprobs(const fhe_token_logprobs_args g, uint32_t split) {
+__global__ void __launch_bounds__(kThreads, 5) k_logprobs(const fhe_token_logprobs_args g, uint32_t split) {
   using Q = Quad<T>;
   constexpr uint32_t V = Q::kElems;
   __shared__ float red[3][kThreads / 32];

@@ -272,6 +272,34 @@ def test_scan_is_repeatable(ops):
         assert torch.equal(a, b)
 
 
+def test_no_wait_ran_out(ops):
+    import ctypes
+
+    from fhe_mamba_b200 import _lib
+    ops.ssm_scan(**scan_inputs(19, 2, 300, 4, 64, 128, 1, torch.bfloat16))
+    torch.cuda.synchronize()
+    n = ctypes.c_uint64(1)
+    _lib.call("fhe_tc_timeouts", ctypes.byref(n))
+    assert n.value == 0
+
+
+def test_scan_on_a_long_row(ops):
+    """Two rows of 9000 tokens against two of 4500 carried on: the same states and outputs, K u mag apart."""
+    for dtype in DTYPES:
+        i = scan_inputs(20, 2, 9000, 2, 32, 64, 1, dtype)
+        y, s = ops.ssm_scan(**i)
+        half = {n: (v[:, :4500] if n in ("x", "B", "C", "write", "log_decay") else v) for n, v in i.items()}
+        y1, s1 = ops.ssm_scan(**half)
+        half = {n: (v[:, 4500:] if n in ("x", "B", "C", "write", "log_decay") else v) for n, v in i.items()}
+        y2, s2 = ops.ssm_scan(**dict(half, initial_state=s1))
+        # decays of at most 4 per unit of write: contributions older than some 600 tokens are below u; a y is a sum
+        # of at most that many terms of size max |x| |B| |C| w 64 <= the largest |y| a few times over
+        big = y.float().abs().max().item()
+        tol = 8 * (4000 * U + 2 * torch.finfo(dtype).eps) * big if dtype != torch.float32 else 8 * 4000 * U * big
+        assert (torch.cat([y1, y2], 1).float() - y.float()).abs().max().item() <= tol
+        assert (s2 - s).abs().max() <= 8 * 4000 * U * s.abs().max() + 3 * (torch.finfo(dtype).eps / 2) ** 2 * 64
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("b, h, p, n, k", [(1, 1, 1, 1, 1), (3, 4, 64, 128, 1), (2, 6, 33, 100, 2), (5, 2, 128, 256, 1),
                                            (2, 3, 16, 16, 3), (2, 2, 20, 18, 1)])
