@@ -13,10 +13,9 @@
 //
 // Roundings.  q, k and r are as given; G, O and S accumulate in fp32.
 // G o L o w and S0 enter their products in the activations' type, half a step
-// of each term (2^-8 for bfloat16) as y's own rounding; with PRECISE they
-// enter as two terms of that type (2^-16).  E o w o r, whose sum is the fp32
-// state, always enters with 22 bits and more: three terms of bfloat16 or two of
-// float16.
+// of each term (2^-8 for bfloat16) as y's own rounding; with PRECISE, and for
+// E o w o r, whose sum is the fp32 state, always, they enter with 22 bits and
+// more: three terms of bfloat16 or two of float16.
 // For float16 the factors are scaled by powers of two (the chunk's largest w to
 // about 8, the state by 16) to use its range; where an operand overflows all
 // the same, a product is not finite, the kernel says so in *bad, and the
@@ -329,6 +328,10 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
   constexpr uint32_t kBytesR = kRowTiles * kTile;
   constexpr uint32_t kTileS = COLS * 128, kBytesS = kRowTiles * kTileS;
   constexpr bool kThird = CARRY && !std::is_same_v<T, __half>;  // a third term of the scaled r, in S0's place
+  // PRECISE's third terms: of S0 in r's place, which is loaded once q S0 is
+  // done, and of the weighted G as an operand in q's and k's (dwrite of 4 x 2048
+  // bfloat16 tokens 4e-7 off, 2.4e-6 with two; 87 us a pass, 77)
+  constexpr bool kThirds = PRECISE && !std::is_same_v<T, __half>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ __align__(16) Gates gate;
@@ -394,7 +397,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
   };
   if (tid == 0) {
     load_kq(first(0));
-    load_rows(first(0));
+    if constexpr (!kThirds) load_rows(first(0));
   }
 
   const float* wp = g.write.p ? g.write.p + (int64_t)b * g.write.sb + (int64_t)h * g.write.sh : nullptr;
@@ -449,6 +452,12 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
       const uint32_t at = ss - sq + (n >> 6) * kTileS + swz(c, n >> 3 & 7) + (n & 4) * 2;
       *reinterpret_cast<uint2*>(smem + at) = hi;
       if constexpr (PRECISE) *reinterpret_cast<uint2*>(smem + at + kBytesS) = lo;
+      if constexpr (kThirds) {
+        const uint64_t m1 = pair(-1.f, -1.f);
+        *reinterpret_cast<uint2*>(smem + at - (ss - sr)) =
+            make_uint2(pack2<T>(fma2(unpack2<T>(lo.x), m1, fma2(unpack2<T>(hi.x), m1, pair(x.x, x.y)))),
+                       pack2<T>(fma2(unpack2<T>(lo.y), m1, fma2(unpack2<T>(hi.y), m1, pair(x.z, x.w)))));
+      }
     }
   } else {
     const float* in = OUT != kOutNone && g.state_in && t < g.cols
@@ -524,6 +533,8 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
           mma_ss(tmem + kColO, desc(sq + at, 16), desc(ss + j * 2048, kTileS), idesc<T>(ROWS, false, true), j);
           if constexpr (PRECISE)
             mma_ss(tmem + kColO, desc(sq + at, 16), desc(ss + kBytesS + j * 2048, kTileS), idesc<T>(ROWS, false, true), 1);
+          if constexpr (kThirds)
+            mma_ss(tmem + kColO, desc(sq + at, 16), desc(sr + j * 2048, kTileS), idesc<T>(ROWS, false, true), 1);
         }
         commit(bar_g);
       }
@@ -558,8 +569,13 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
       done = i + 1;
       fence_after();
     }
-    ok = __all_sync(~0u, wait(bar_r, par)) && ok;
-    if (!live && t_end < t_hi) clear(sr, kRowTiles);
+    if constexpr (kThirds) {
+      if (ok && tid == 0) load_rows(t0);
+      __syncwarp();
+    } else {
+      ok = __all_sync(~0u, wait(bar_r, par)) && ok;
+      if (!live && t_end < t_hi) clear(sr, kRowTiles);
+    }
     if (ok) {
       // O starts from P_t (q S0) and the skip term; the scaled r, in two terms, goes over q
 #pragma unroll
@@ -610,7 +626,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
         for (uint32_t u = 0; u < 2; ++u) {
           const uint32_t blk = half ? 1 + u : 3 * u;
           const bool zero = REV ? blk < quarter : blk > quarter;
-          uint32_t hi[16], lo[16];
+          uint32_t hi[16], lo[16], third[16];
           if (!zero) {
             float v[32];
             tmem_ld32(tmem + lanes + blk * 32, v);
@@ -626,16 +642,28 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
               const uint64_t p = pair(v[2 * e], v[2 * e + 1]);
               if constexpr (PRECISE) split2<T>(p, hi[e], lo[e]);
               else hi[e] = pack2<T>(p);
+              if constexpr (kThirds)
+                third[e] = pack2<T>(fma2(unpack2<T>(lo[e]), pair(-1.f, -1.f), fma2(unpack2<T>(hi[e]), pair(-1.f, -1.f), p)));
             }
           } else {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) hi[e] = lo[e] = 0;
+            for (int e = 0; e < 16; ++e) hi[e] = lo[e] = third[e] = 0;
+          }
+          if constexpr (kThirds) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<uint4*>(smem + (blk >> 1) * kTile + swz(t, (blk & 1) * 4 + e)) =
+                  make_uint4(third[4 * e], third[4 * e + 1], third[4 * e + 2], third[4 * e + 3]);
           }
           tmem_st16(tmem + lanes + blk * 32, hi);
           if constexpr (PRECISE) tmem_st16(tmem + lanes + blk * 32 + 16, lo);
         }
         st_wait();
       }
+    }
+    if constexpr (kThirds) {
+      ok = __all_sync(~0u, wait(bar_r, par)) && ok;
+      if (!live && t_end < t_hi) clear(sr, kRowTiles);
     }
     fence_async();
     fence_before();
@@ -662,6 +690,9 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
             mma_ts(tmem + kColO, a, desc(sr + j * 2048, kTile), idesc<T>(ROWS, false, true), 1);
             if constexpr (PRECISE)
               mma_ts(tmem + kColO, a + 16, desc(sr + j * 2048, kTile), idesc<T>(ROWS, false, true), 1);
+            if constexpr (kThirds)
+              mma_ss(tmem + kColO, desc(sq + (j >> 2) * kTile + (j & 3) * 32, 16), desc(sr + j * 2048, kTile),
+                     idesc<T>(ROWS, false, true), 1);
           }
           commit(bar_o);
         }

@@ -191,10 +191,9 @@ def ssm_scan(x, write, log_decay, B, C, D=None, initial_state=None, lengths=None
     else it is copied).  Gradients reach every floating-point argument.
 
     Rows of 64 tokens and more in 16 bits run on the tensor cores: y, dx, dB and
-    dC then carry about one more rounding of that type, the final state keeps 22
-    bits and more of every product, the gates' gradients 16 (bfloat16) or 22
-    (float16); in bfloat16 a NaN or an infinity may reach earlier tokens of its
-    128."""
+    dC then carry about one more rounding of that type, the final state and the
+    gates' gradients keep 22 bits and more of every product; in bfloat16 a NaN
+    or an infinity may reach earlier tokens of its 128."""
     if not _scan_fits(x, write, log_decay, B, C, D, initial_state, lengths):
         _check_scan("ssm_scan", x, write, log_decay, B, C, D, initial_state, lengths)
     args = (_inner(x), write, log_decay, _inner(B), _inner(C), _dense(D), _dense(initial_state), _dense(lengths))
