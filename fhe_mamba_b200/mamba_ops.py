@@ -18,6 +18,7 @@ from typing import NamedTuple
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._lib import call
@@ -243,6 +244,7 @@ def ssm_step(state, x, write, log_decay, B, C, D=None, out=None):
     a = _lib.SsmScanArgs(d.index, _TYPES[t], b, 1, h, p, n, k, xp, xs, wp, ws, ap, as_, bp, bs, cp, cs, _ptr(D),
                          state.data_ptr(), None, y.data_ptr(), out.data_ptr(), None, 0, _stream_of(d.index))
     call("fhe_ssm_scan", ctypes.byref(a))
+    increment_version(out)  # a backward pass that saved the old state must not run on the new one
     return y, out
 
 
@@ -366,6 +368,7 @@ def causal_conv_step(state, x, weight, bias=None, activation="silu", out=None):
     out = _check_state_out(op, state, out)
     call("fhe_causal_conv", ctypes.byref(_conv_args(_inner(x), _dense(weight), _dense(bias), state, None,
                                                     activation == "silu", y, out)))
+    increment_version(out)
     return y, out
 
 
