@@ -98,6 +98,8 @@ class PlainMamba2(torch.nn.Module):
         """Each row's tokens 1.. under the model, given the tokens before them:
         a ``TokenLogprobs`` of [batch, length - 1] scores (log-probability 0 at
         and past a row's length)."""
+        if tokens.dim() != 2 or tokens.shape[1] < 1:
+            raise ValueError("tokens must be [batch, at least 1]")
         b, l = tokens.shape
         hidden, _ = self(tokens, state, lengths)
         targets = tokens[:, 1:].long()
@@ -107,9 +109,9 @@ class PlainMamba2(torch.nn.Module):
         return TokenLogprobs(*(v.unflatten(0, (b, l - 1)) for v in out))
 
     def loss(self, tokens, lengths=None):
-        """Mean negative log-probability of the scored tokens."""
+        """Mean negative log-probability of the scored tokens, 0 if there are none."""
         scores = self.score(tokens, lengths=lengths)
-        n = tokens.shape[0] * (tokens.shape[1] - 1) if lengths is None else \
+        n = max(tokens.shape[0] * (tokens.shape[1] - 1), 1) if lengths is None else \
             (lengths.long().clamp(0, tokens.shape[1]) - 1).clamp(min=0).sum().clamp(min=1)
         return -scores.logprob.sum() / n
 

@@ -95,6 +95,20 @@ def test_scores(model):
     assert abs(loss + (want[0].sum() + want[1, :24].sum()) / 63) <= tol
 
 
+def test_rows_with_nothing_to_score(model):
+    """Rows of one token: no scores, a loss of 0 and gradients of 0; rows of none are refused."""
+    net = model.plain_sequences()
+    one = torch.tensor([[3], [5]], device="cuda")
+    assert net.score(one, top_k=4).top_ids.shape == (2, 0, 4)
+    for lengths in (None, torch.tensor([1, 0], dtype=torch.int32, device="cuda")):
+        loss = net.loss(one, lengths)
+        assert loss.item() == 0
+        grad = torch.autograd.grad(loss, net.embedding)[0]
+        assert not grad.any()
+    with pytest.raises(ValueError, match="at least 1"):
+        net.score(one[:, :0])
+
+
 def test_loss_has_the_gradients_of_differences(model):
     """The loss's gradient along a direction against the central difference: the loss is rounded by at most
     2 TOL x (log vocab + spread of the logits) and its curvature along the step is of the size of the loss."""
