@@ -52,21 +52,25 @@ __device__ __forceinline__ float exp2_fast(float v) {
 
 // The running sums are kept in base 2 around a shift derived from the running
 // maximum m: d = log2(e) z - shift, s = sum of 2^d, u = sum of 2^d d.  The
-// shift cancels from every score, so its rounding does not matter.  Entries
-// are raised to the type's floor first, which makes d finite; rows whose
-// maximum lies near the floor, and rows with a NaN or infinite maximum, are
-// summed again entry by entry (exact_stats).
+// shift cancels from every score, so its rounding does not matter as long as
+// 2^d survives it: it follows m between -2^20 and 2^20, where it is off by at
+// most 1/16, and stays at either end beyond (below, all d lie far below 0 and
+// the sums stay 0 until an entry within the range comes).  Entries are raised
+// to the type's floor first, which makes d finite.  Rows whose own maximum
+// lies outside, and rows with a NaN or infinite maximum, are summed again entry
+// by entry (exact_stats).
+constexpr float kFar = 1048576.f;  // 2^20
 template <class T>
 __device__ __forceinline__ float floor_of() {
   return std::is_same_v<T, __half> ? -65504.f : -1e38f;
 }
 template <class T>
-__device__ __forceinline__ float least_max() {  // far enough above the floor
-  return std::is_same_v<T, __half> ? -60000.f : -1e30f;
+__device__ __forceinline__ float least_max() {  // for float16 far enough above its floor
+  return std::is_same_v<T, __half> ? -60000.f : -kFar;
 }
 template <class T>
 __device__ __forceinline__ bool plain_max(float m) {
-  return m > least_max<T>() && m < 1e37f;
+  return m > least_max<T>() && m < kFar;
 }
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -76,7 +80,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // Rounded on its own (never contracted into an fma): equal maxima, equal shifts.
 template <class T>
 __device__ __forceinline__ float shift_of(float m) {
-  return __fmul_rn(kLog2e, fminf(fmaxf(m, least_max<T>()), 1e37f));
+  return __fmul_rn(kLog2e, fminf(fmaxf(m, least_max<T>()), kFar));
 }
 
 template <class T>
