@@ -537,8 +537,11 @@ __global__ void __launch_bounds__(kThreads) k_logprobs_grad(const fhe_token_logp
   float G = gl;
   for (uint32_t i = 0; i < k; ++i) G += a.dtop_logprobs[(int64_t)row * k + i];
   const float c = -G - ge * H;
+  // Entries this far below the maximum have p = 0 and are held there, so that no
+  // multiple of their log p overflows into 0 times infinity.
+  constexpr float kGone = -1e4f;
   auto base = [&](float v) {
-    const float lp = fmaxf((v - m) - ls, -1e37f), d = exp2_fast(lp * kLog2e) * fmaf(-ge, lp, c);
+    const float lp = fmaxf((v - m) - ls, kGone), d = exp2_fast(lp * kLog2e) * fmaf(-ge, lp, c);
     return isnan(v) ? v : v == -INFINITY ? 0.f : d;
   };
   auto scalar = [&](uint32_t lo, uint32_t hi) {
@@ -550,6 +553,7 @@ __global__ void __launch_bounds__(kThreads) k_logprobs_grad(const fhe_token_logp
     const T* zb = z + e0 + head;
     T* db = dz + e0 + head;
     const uint64_t sub = pair(-m, -m), sub2 = pair(-ls, -ls), l2 = pair(kLog2e, kLog2e), nge = pair(-ge, -ge), cc = pair(c, c);
+    const float low = m + kGone;
     for (uint32_t i = tid; i < packs; i += kAhead * kThreads) {
       Q p[kAhead];
 #pragma unroll
@@ -562,7 +566,7 @@ __global__ void __launch_bounds__(kThreads) k_logprobs_grad(const fhe_token_logp
 #pragma unroll
         for (uint32_t v = 0; v < V; v += 2) {
           const uint64_t lp = add2(
-              add2(pair(fmaxf(p[j].element(v), floor_of<T>()), fmaxf(p[j].element(v + 1), floor_of<T>())), sub), sub2);
+              add2(pair(fmaxf(p[j].element(v), low), fmaxf(p[j].element(v + 1), low)), sub), sub2);
           float x0, x1;
           unpair(mul2(lp, l2), x0, x1);
           unpair(mul2(pair(exp2_fast(x0), exp2_fast(x1)), fma2(nge, lp, cc)), o[v], o[v + 1]);

@@ -99,3 +99,20 @@ def test_masks_of_several_sizes(ops, dtype):
     z[3] = size
     t[:] = torch.tensor([0, 39999, 20000, 39999], device="cuda")
     check(ops, z, t, 5)
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("low", [-math.inf, "min"])
+@pytest.mark.parametrize("ge", [1.0, 10.0, 65536.0])
+def test_entropy_gradients_of_masked_rows(ops, dtype, low, ge):
+    """Masked entries take no gradient however large the entropy's own is."""
+    if dtype == torch.float16:
+        ge = min(ge, 100.0)  # the gradients themselves fit float16
+    z, t = rows_of(4, 3, 5003, dtype)
+    z[:, 4800:] = torch.finfo(dtype).min if low == "min" else low
+    z[1, ::2] = z[1, -1]
+    t = t % 4800 | 1
+    check(ops, z, t, 3, ge)
+    odd = torch.zeros(3, 5004, dtype=dtype, device="cuda")[:, 1:]  # rows that 16-byte words do not fit
+    odd.copy_(z)
+    check(ops, odd, t, 3, ge)
