@@ -536,13 +536,13 @@ __global__ void __launch_bounds__(kThreads) k_logprobs_grad(const fhe_token_logp
   const float ge = a.dentropy ? a.dentropy[row] : 0.f, H = a.dentropy ? g.entropy[row] : 0.f;
   float G = gl;
   for (uint32_t i = 0; i < k; ++i) G += a.dtop_logprobs[(int64_t)row * k + i];
-  const float c = -G - ge * H;
+  const float c = isnan(ls) ? ls : -G - ge * H;  // a row without scores has no gradient either
   // Entries this far below the maximum have p = 0 and are held there, so that no
   // multiple of their log p overflows into 0 times infinity.
   constexpr float kGone = -1e4f;
   auto base = [&](float v) {
     const float lp = fmaxf((v - m) - ls, kGone), d = exp2_fast(lp * kLog2e) * fmaf(-ge, lp, c);
-    return isnan(v) ? v : v == -INFINITY ? 0.f : d;
+    return isnan(v) ? v : v == -INFINITY && !isnan(ls) ? 0.f : d;
   };
   auto scalar = [&](uint32_t lo, uint32_t hi) {
     for (uint32_t e = lo + tid; e < hi; e += kThreads) dz[e] = from_f<T>(base(to_f(z[e])));

@@ -643,7 +643,8 @@ int fhe_token_logprobs(const fhe_token_logprobs_args* args);
 /* dlogits (contiguous, dtype) from the gradients of logprob, entropy and
  * top_logprobs (each NULL for zeros); `f` as in the forward call, with its
  * entropy, top_ids and norm outputs as inputs.  An ignored or out-of-range
- * target passes no gradient, a row of -inf alone gets zeros. */
+ * target passes no gradient, a row of -inf alone gets zeros, a row whose scores
+ * are NaN gets NaN. */
 typedef struct fhe_token_logprobs_grad_args {
   fhe_token_logprobs_args f;
   const float* dlogprob;      /* [rows] */

@@ -116,3 +116,15 @@ def test_entropy_gradients_of_masked_rows(ops, dtype, low, ge):
     odd = torch.zeros(3, 5004, dtype=dtype, device="cuda")[:, 1:]  # rows that 16-byte words do not fit
     odd.copy_(z)
     check(ops, odd, t, 3, ge)
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_gradients_of_rows_without_scores(ops, dtype, value):
+    """A row whose scores are not numbers has a gradient that is none either; the rows beside it keep theirs."""
+    z, t = rows_of(5, 3, 5000, dtype)
+    good = z.detach().clone().requires_grad_()
+    z[1, 10] = value
+    z.requires_grad_()
+    got, want = (torch.autograd.grad(ops.token_logprobs(v, t).logprob.sum(), v)[0] for v in (z, good))
+    assert got[1].isnan().all() and torch.equal(got[::2], want[::2])
