@@ -268,7 +268,7 @@ constexpr int kStepRows = 4;
 template <class T, int G, int NV>
 __global__ void __launch_bounds__(kThreads) k_step(const StepArgs g) {
   constexpr uint32_t kRows = kStepRows * 32 / G;  // per warp
-  const uint32_t warp = (blockIdx.x * kThreads + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+  const uint32_t warp = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   const uint32_t per = (g.head_dim + kRows - 1) / kRows;  // warps per head
   const uint32_t bh = warp / per;
   if (bh >= g.batch * g.heads) return;
@@ -412,7 +412,7 @@ __device__ __forceinline__ float sum_each(float (&v)[COUNT], uint32_t lane) {
 // 24 heads: 94 us, 2.7 TB/s (a block of 8 warps per token: 180 us).
 template <class T, int V, int NP, int H>
 __global__ void __launch_bounds__(128) k_sum(const SumArgs g, uint32_t tokens) {
-  const uint32_t id = (blockIdx.x * 128 + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+  const uint32_t id = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;  // threads may pass 2^32
   if (id >= tokens) return;
   const uint32_t t = id % g.length, b = id / g.length;
   const bool live = (int)t < clamp_length(g.lengths, b, g.length);
@@ -500,10 +500,11 @@ __global__ void __launch_bounds__(128) k_sum(const SumArgs g, uint32_t tokens) {
 // One warp per (batch, head, segment): the running sum of alpha - beta from
 // the segment's end (fp64: it is a difference of sums), and the segment's
 // share of dd.
-__global__ void k_log_decay_grad(const float* diff, const float* skip, const float* gamma, Gate log_decay,
-                                 const int32_t* lengths, float* out, float* dd_part, uint32_t length, uint32_t heads,
-                                 uint32_t seglen, uint32_t nseg, uint32_t count) {
-  const uint32_t id = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(128)
+    k_log_decay_grad(const float* diff, const float* skip, const float* gamma, Gate log_decay, const int32_t* lengths,
+                     float* out, float* dd_part, uint32_t length, uint32_t heads, uint32_t seglen, uint32_t nseg,
+                     uint32_t count) {
+  const uint32_t id = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;  // blocks of 128 threads
   if (id >= count) return;
   const uint32_t seg = id % nseg, h = id / nseg % heads, b = id / nseg / heads;
   const int len = clamp_length(lengths, b, length);
