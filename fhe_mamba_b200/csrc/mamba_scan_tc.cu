@@ -12,28 +12,34 @@
 // quotient, so decays of zero or near it lose nothing.
 //
 // Roundings.  q, k and r are as given; G, O and S accumulate in fp32.
-// G o L o w and S0 enter their products in the activations' type, half a step
-// of each term (2^-8 for bfloat16) as y's own rounding; with PRECISE, and for
-// E o w o r, whose sum is the fp32 state, always, they enter with 22 bits and
-// more: three terms of bfloat16 or two of float16.
+// G o L o w and S0 enter their products as two terms of the activations' type
+// (16 bits for bfloat16, 22 for float16: y and dx are off by their own rounding
+// alone; with one term their error was 1.1 times that, and a row of 64 tokens
+// differed from one of 63).  For the raw sums (OUT kOutRaw) and for E o w o r,
+// whose sum is the fp32 state, it is 22 bits and more: three terms of bfloat16
+// or two of float16.
 // For float16 the factors are scaled by powers of two (the chunk's largest w to
 // about 8, the state by 16) to use its range; where an operand overflows all
 // the same, a product is not finite, the kernel says so in *bad, and the
 // caller's launches of the fp32 walk, idle otherwise, take the work over.
 //
 // One CTA walks one (batch, head, tile of rows, segment).  Shared memory holds
-// q, k, r and S0 in 128-byte-swizzled tiles of 64 columns; the scaled r takes
-// q's place once q has been used, which keeps two CTAs on an SM, so that one
-// computes while the other waits for its loads or its products.  Tensor
-// memory: G (its columns become the A operand G o L o w), O (which starts from
-// the scaled q S0^T) and S'.  The state itself stays in registers.
+// q, k, r and S0's two terms in 128-byte-swizzled tiles of 64 columns; the
+// scaled r takes q's place once q has been used, and what tokens read of each
+// other fits 1 KB, which keeps two CTAs on an SM, so that one computes while the
+// other waits for its loads or its products.  Tensor memory: G (its columns
+// become the A operand G o L o w), O (which starts from the scaled q S0^T) and S'
+// (before, q times S0's second term).  The state itself stays in registers; the
+// element passes take 16 columns at a time, since spilled registers cost more
+// than their instructions (what shared memory leaves of the L1 cache is small).
 //
-// 8 x 4096 bfloat16 tokens of 24 heads x 64, state 128: 193 us, of which memory
-// needs 36 and the products about 60 at full rate; a chunk is a chain of
-// products and element passes that two CTAs to an SM cover in part (issue slots
-// 36% busy).  Loads by tensor maps and stores of 64-byte runs took the load and
-// store unit out of that chain (343 us with 16-byte asynchronous copies and
-// scattered stores).
+// 8 x 4096 bfloat16 tokens of 24 heads x 64, state 128: 236 us (198 with one term
+// of G o L o w and S0), of which memory needs 36 and the products about 80 at
+// full rate; a chunk is a chain of products and element passes that two CTAs to
+// an SM cover in part, and 192 CTAs leave 104 of 148 SMs with one (148 CTAs take
+// 176 us, 296 take 236).  Loads by tensor maps and stores of 64-byte runs took the
+// load and store unit out of that chain (343 us with 16-byte asynchronous copies
+// and scattered stores).
 //
 // A walk that carries no state on (CARRY false: the gradients', a segment of
 // one chunk each) leaves S' out and takes 128 rows where there are as many.
@@ -124,6 +130,15 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
         "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
       : "r"(addr));
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+      : "r"(addr));
+}
 __device__ __forceinline__ void ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&u)[16]) {
   asm volatile(
@@ -132,15 +147,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&u)[16]
       "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
       "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
       : "memory");
-}
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const float (&v)[32]) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t u[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(v[16 * h + i]);
-    tmem_st16(addr + 16 * h, u);
-  }
 }
 __device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -203,20 +209,31 @@ __device__ __forceinline__ bool elect_one() {
 // Byte offset of 16-byte word `word` of row `row` in a 128-byte-swizzled tile.
 __device__ __forceinline__ uint32_t swz(uint32_t row, uint32_t word) { return row * 128 + ((word ^ (row & 7)) << 4); }
 
-// Products of decays of one chunk, over blocks of 32 tokens and of 8.
-struct Gates {
-  float a[kQ], w[kQ];    // decay and write of each token
-  float head[kQ];        // product over its block of 32 up to and with the token
-  float tail[kQ];        // product over its block of 32 after the token
-  float col[kQ];         // column factor for rows of other blocks of 32: tail (reversed: head) times w
-  float col8[kQ];        // and for rows of other blocks of 8 in its block of 32
-  float total[4];        // product over each block of 32
-  float most[4];         // largest |w| in each block of 32 (float16)
+// What a chunk's threads read of each other's tokens, with the barriers: 1 KB,
+// which is what two CTAs' tiles leave of an SM's shared memory.
+template <bool REV>
+struct Small {
+  float cols[96];   // column factor for rows of other blocks of 32: tail (reversed: head) times w
+  float col8[kQ];   // and for rows of other blocks of 8 in its block of 32
+  float total[4];   // product over each block of 32
+  float most[4];    // largest |w| in each block of 32 (float16)
+  uint64_t bars[5];  // G and q S0, S', O; k and q have arrived, r has
+  uint32_t tslot;
+  // no row lies beyond the last (reversed: before the first) block of 32
+  __device__ __forceinline__ float* col(uint32_t blk) { return cols + (blk - (REV ? 1u : 0u)) * 32; }
+};
+constexpr uint32_t kSmall = 1024;
+static_assert(sizeof(Small<false>) <= kSmall, "shared memory");
+
+// A token's decay and write, and the products of decays over its block of 32:
+// up to and with the token, and after it.
+struct Token {
+  float a, w, head, tail;
 };
 
-// Four warps, one token per thread.
+// All warps, one token per thread; those of `put` (four) leave the chunk's column factors.
 template <bool REV>
-__device__ __forceinline__ void put_gates(Gates& g, uint32_t t, uint32_t lane, float a, float w) {
+__device__ __forceinline__ Token make_token(Small<REV>& g, uint32_t t, uint32_t lane, float a, float w, bool put) {
   const float after = __shfl_down_sync(~0u, a, 1);
   const int in = lane & 7;
   float head = a, head8 = a, tail = lane == 31 ? 1.f : after, tail8 = in == 7 ? 1.f : after;
@@ -231,15 +248,15 @@ __device__ __forceinline__ void put_gates(Gates& g, uint32_t t, uint32_t lane, f
       if (in + o < 8) tail8 *= d8;
     }
   }
-  g.a[t] = a;
-  g.w[t] = w;
-  g.head[t] = head;
-  g.tail[t] = tail;
-  g.col[t] = (REV ? head : tail) * w;
-  g.col8[t] = (REV ? head8 : tail8) * w;
-  if (lane == 31) g.total[t >> 5] = head;
-  const uint32_t most = __reduce_max_sync(~0u, __float_as_uint(fabsf(w)));
-  if (lane == 0) g.most[t >> 5] = __uint_as_float(most);
+  if (put) {
+    const uint32_t blk = t >> 5;
+    if (REV ? blk > 0 : blk < 3) g.col(blk)[lane] = (REV ? head : tail) * w;
+    g.col8[t] = (REV ? head8 : tail8) * w;
+    if (lane == 31) g.total[blk] = head;
+    const uint32_t most = __reduce_max_sync(~0u, __float_as_uint(fabsf(w)));
+    if (lane == 0) g.most[blk] = __uint_as_float(most);
+  }
+  return Token{a, w, head, tail};
 }
 
 // A row's factors within its own block of 32, times `scale`: `own` for the
@@ -249,16 +266,14 @@ struct OwnBlock {
   float own[8], row[4];
 };
 template <bool REV>
-__device__ __forceinline__ OwnBlock own_block(const Gates& g, uint32_t t, uint32_t lane, float scale) {
+__device__ __forceinline__ OwnBlock own_block(const Token& g, uint32_t lane, float scale) {
   OwnBlock o;
-  const uint32_t s0 = t & ~7u;
   const int sub = lane >> 3, in = lane & 7;
   float a[8], w[8];
 #pragma unroll
-  for (int i = 0; i < 8; i += 4) {
-    const float4 x = *reinterpret_cast<const float4*>(&g.a[s0 + i]), y = *reinterpret_cast<const float4*>(&g.w[s0 + i]);
-    a[i] = x.x, a[i + 1] = x.y, a[i + 2] = x.z, a[i + 3] = x.w;
-    w[i] = y.x, w[i + 1] = y.y, w[i + 2] = y.z, w[i + 3] = y.w;
+  for (int i = 0; i < 8; ++i) {
+    a[i] = __shfl_sync(~0u, g.a, i, 8);
+    w[i] = __shfl_sync(~0u, g.w, i, 8);
   }
   float p = scale, all = 1.f;
 #pragma unroll
@@ -285,23 +300,23 @@ __device__ __forceinline__ OwnBlock own_block(const Gates& g, uint32_t t, uint32
   return o;
 }
 
-// 32 columns of G o L o w for one row, in place: columns of another block of
-// 32, and of the row's own.
-__device__ __forceinline__ void weigh(float (&v)[32], const float* col, float row) {
+// 16 columns of G o L o w for one row, in place: columns of another block of
+// 32, and (from group j of 8 on) of the row's own.
+__device__ __forceinline__ void weigh(float (&v)[16], const float* col, float row) {
   const uint64_t rr = pair(row, row);
 #pragma unroll
-  for (int i = 0; i < 32; i += 4) {
+  for (int i = 0; i < 16; i += 4) {
     const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(col + i);
     unpair(mul2(pair(v[i], v[i + 1]), mul2(rr, c.x)), v[i], v[i + 1]);
     unpair(mul2(pair(v[i + 2], v[i + 3]), mul2(rr, c.y)), v[i + 2], v[i + 3]);
   }
 }
-__device__ __forceinline__ void weigh_own(float (&v)[32], const float* col8, const OwnBlock& o, uint32_t lane) {
+__device__ __forceinline__ void weigh_own(float (&v)[16], const float* col8, const OwnBlock& o, uint32_t lane, int j0) {
   const int sub = lane >> 3;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint64_t rr = pair(o.row[j], o.row[j]);
-    const bool mine = sub == j;
+  for (int j = 0; j < 2; ++j) {
+    const uint64_t rr = pair(o.row[j0 + j], o.row[j0 + j]);
+    const bool mine = sub == j0 + j;
 #pragma unroll
     for (int i = 0; i < 8; i += 4) {
       const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(col8 + 8 * j + i);
@@ -319,7 +334,7 @@ __device__ __forceinline__ void weigh_own(float (&v)[32], const float* col8, con
 
 // COLS: columns held, 64 or 128 (those past g.cols are zeros); ROWS: rows per
 // CTA, 64 or 128 (128 only without CARRY).
-template <class T, int COLS, int ROWS, bool REV, int OUT, bool PRECISE, bool CARRY>
+template <class T, int COLS, int ROWS, bool REV, int OUT, bool CARRY>
 __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, const __grid_constant__ Maps maps) {
   static_assert((CARRY ? OUT != kOutRaw : OUT != kOutNone) && (ROWS == 64 || OUT == kOutRaw), "shapes");
   constexpr uint32_t kHalves = COLS / 64, kRowTiles = ROWS / 64;
@@ -328,18 +343,19 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
   constexpr uint32_t kBytesR = kRowTiles * kTile;
   constexpr uint32_t kTileS = COLS * 128, kBytesS = kRowTiles * kTileS;
   constexpr bool kThird = CARRY && !std::is_same_v<T, __half>;  // a third term of the scaled r, in S0's place
-  // PRECISE's third terms: of S0 in r's place, which is loaded once q S0 is
-  // done, and of the weighted G as an operand in q's and k's (dwrite of 4 x 2048
-  // bfloat16 tokens 4e-7 off, 2.4e-6 with two; 87 us a pass, 77)
-  constexpr bool kThirds = PRECISE && !std::is_same_v<T, __half>;
+  // The raw sums' third terms: of S0 in r's place, and of the weighted G as an
+  // operand in q's and k's (dwrite of 4 x 2048 bfloat16 tokens 4e-7 off, 2.4e-6
+  // with two; 87 us a pass, 77)
+  constexpr bool kThirds = OUT == kOutRaw && !std::is_same_v<T, __half>;
+  // One product gives q times both terms of S0, side by side: the second's takes
+  // the place of S', not needed yet.
+  constexpr bool kPair = OUT != kOutNone && ROWS == 64 && !kThirds;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ __align__(16) Gates gate;
-  __shared__ __align__(8) uint64_t bars[5];  // G and q S0, S', O; k and q have arrived, r has
-  __shared__ uint32_t tslot;
+  Small<REV>& gate = *reinterpret_cast<Small<REV>*>(smem_raw);
+  uint8_t* smem = smem_raw + kSmall;  // the tiles
   const uint32_t sq = smem_u32(smem), sk = sq + kBytesQ, sr = sk + kBytesK;
-  const uint32_t ss = sr + kBytesR;  // S0 (two terms with PRECISE)
-  const uint32_t bar_g = smem_u32(&bars[0]), bar_s = bar_g + 8, bar_o = bar_g + 16, bar_kq = bar_g + 24,
+  const uint32_t ss = sr + kBytesR;  // S0, two terms
+  const uint32_t bar_g = smem_u32(&gate.bars[0]), bar_s = bar_g + 8, bar_o = bar_g + 16, bar_kq = bar_g + 24,
                  bar_r = bar_g + 32;
 
   const uint32_t tiles = (g.rows + ROWS - 1) / ROWS;
@@ -363,7 +379,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
   uint64_t poison = 0;  // a sum of 0 times every product: NaN once one is not finite (float16)
 
   if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tslot)),
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&gate.tslot)),
                  "r"(kTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -402,10 +418,10 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
 
   const float* wp = g.write.p ? g.write.p + (int64_t)b * g.write.sb + (int64_t)h * g.write.sh : nullptr;
   const float* ap = g.log_decay.p + (int64_t)b * g.log_decay.sb + (int64_t)h * g.log_decay.sh;
-  float next_a = 0.f, next_w = 0.f;  // warps 4-7 (warp 0 has the products to issue): the gates of the chunk to come
+  float next_a = 0.f, next_w = 0.f;  // the gates of the chunk to come
   auto load_gates = [&](int t0) {
     const int tok = t0 + (int)t;
-    const bool l = tid >= kQ && tok < t_end;
+    const bool l = tok < t_end;
     next_a = l ? ap[(int64_t)tok * g.log_decay.sl] : 0.f;
     next_w = l ? (wp ? wp[(int64_t)tok * g.write.sl] : 1.f) : 0.f;
   };
@@ -428,12 +444,11 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint64_t x = kHalf ? mul2(s[4 * v + e], pair(kStateScale, kStateScale)) : s[4 * v + e];
-        if constexpr (PRECISE) split2<T>(x, hi[e], lo[e]);
-        else hi[e] = pack2<T>(x);
+        split2<T>(x, hi[e], lo[e]);
       }
       const uint32_t at = ss - sq + (piece >> 1) * kTileS + swz(t, (piece & 1) * 4 + v);
       *reinterpret_cast<uint4*>(smem + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      if constexpr (PRECISE) *reinterpret_cast<uint4*>(smem + at + kBytesS) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      *reinterpret_cast<uint4*>(smem + at + kBytesS) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
   };
   if constexpr (OUT == kOutRaw) {
@@ -451,7 +466,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
       split2<T>(pair(kStateScale * x.z, kStateScale * x.w), hi.y, lo.y);
       const uint32_t at = ss - sq + (n >> 6) * kTileS + swz(c, n >> 3 & 7) + (n & 4) * 2;
       *reinterpret_cast<uint2*>(smem + at) = hi;
-      if constexpr (PRECISE) *reinterpret_cast<uint2*>(smem + at + kBytesS) = lo;
+      *reinterpret_cast<uint2*>(smem + at + kBytesS) = lo;
       if constexpr (kThirds) {
         const uint64_t m1 = pair(-1.f, -1.f);
         *reinterpret_cast<uint2*>(smem + at - (ss - sr)) =
@@ -480,7 +495,8 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
     const int t0 = first(i), tok = t0 + (int)t;
     const bool live = tok < t_end;
     const uint32_t par = i & 1;
-    if (tid >= kQ) put_gates<REV>(gate, t, lane, expf(next_a), next_w);
+    // (column factors by warps 4-7: warp 0 has the products to issue)
+    const Token me = make_token<REV>(gate, t, lane, expf(next_a), next_w, half == 1);
     // Row scale of this token's products: w of dx; for U of the gradients the
     // mantissa of w, so that its products are rounded at w_t times their value
     // as those of dC_h are, up to a power of two.  alpha and beta, whose
@@ -519,7 +535,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
       ok = __syncthreads_and(ok);
       if (!ok) break;
     }
-    tmem = tslot;
+    tmem = gate.tslot;
     if (OUT != kOutNone && warp == 0) {
       if (elect_one()) {
 #pragma unroll
@@ -530,9 +546,12 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
 #pragma unroll
         for (uint32_t j = 0; j < COLS / 16; ++j) {
           const uint32_t at = (j >> 2) * kTile + (j & 3) * 32;
-          mma_ss(tmem + kColO, desc(sq + at, 16), desc(ss + j * 2048, kTileS), idesc<T>(ROWS, false, true), j);
-          if constexpr (PRECISE)
+          if constexpr (kPair) {
+            mma_ss(tmem + kColO, desc(sq + at, 16), desc(ss + j * 2048, kTileS), idesc<T>(128, false, true), j);
+          } else {
+            mma_ss(tmem + kColO, desc(sq + at, 16), desc(ss + j * 2048, kTileS), idesc<T>(ROWS, false, true), j);
             mma_ss(tmem + kColO, desc(sq + at, 16), desc(ss + kBytesS + j * 2048, kTileS), idesc<T>(ROWS, false, true), 1);
+          }
           if constexpr (kThirds)
             mma_ss(tmem + kColO, desc(sq + at, 16), desc(sr + j * 2048, kTileS), idesc<T>(ROWS, false, true), 1);
         }
@@ -548,23 +567,21 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
       if (u < quarter) before *= gate.total[u];
       if (u > quarter) after *= gate.total[u];
     }
-    const float head = gate.head[t], tail = gate.tail[t];
     if constexpr (kHalf) {  // w of the chunk scaled to at most 16
       const float sw = 8.f * scale_of(fmaxf(fmaxf(gate.most[0], gate.most[1]), fmaxf(gate.most[2], gate.most[3])));
       rho *= sw;
       up /= sw;
     }
     const float back = kHalf ? 1.f / (8.f * scale_of(fmaxf(fmaxf(gate.most[0], gate.most[1]), fmaxf(gate.most[2], gate.most[3])))) : 1.f;
-    const float pt = (REV ? tail * after : head * before) * (rho / kStateScale);
-    const float et = (REV ? head * before : tail * after) * gate.w[t] / back;
+    const float pt = (REV ? me.tail * after : me.head * before) * (rho / kStateScale);
+    const float et = (REV ? me.head * before : me.tail * after) * me.w / back;
     const float keep = skip / up;  // the skip term in the products' scale
     const float all = gate.total[0] * gate.total[1] * gate.total[2] * gate.total[3];
     decay *= all;
-    const uint32_t blk_own = quarter;
     const bool owner = half == (quarter == 1 || quarter == 2 ? 1u : 0u);  // half 0: blocks 0 and 3, half 1: 1 and 2
     OwnBlock ob;
     if constexpr (OUT != kOutNone) {
-      if (owner) ob = own_block<REV>(gate, t, lane, rho);
+      if (owner) ob = own_block<REV>(me, lane, rho);
       ok = __all_sync(~0u, wait(bar_g, par));
       done = i + 1;
       fence_after();
@@ -572,23 +589,73 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
     if constexpr (kThirds) {
       if (ok && tid == 0) load_rows(t0);
       __syncwarp();
-    } else {
-      ok = __all_sync(~0u, wait(bar_r, par)) && ok;
-      if (!live && t_end < t_hi) clear(sr, kRowTiles);
     }
+    if constexpr (OUT != kOutNone) {
+      if (ok) {
+#pragma unroll
+        for (uint32_t u = 0; u < 2; ++u) {
+          const uint32_t blk = half ? 1 + u : 3 * u;
+          const bool zero = REV ? blk < quarter : blk > quarter;
+          float row = (REV ? me.tail : me.head) * rho;  // times the blocks between
+#pragma unroll
+          for (uint32_t m = 0; m < 4; ++m)
+            if (REV ? (m > quarter && m < blk) : (m > blk && m < quarter)) row *= gate.total[m];
+#pragma unroll
+          for (uint32_t n = 0; n < 2; ++n) {  // 16 columns: their first terms, then their second
+            const uint32_t at = tmem + lanes + blk * 32 + n * 16;
+            uint32_t x[16], third[8];
+            if (!zero) {
+              float v[16];
+              tmem_ld16(at, v);
+              ld_wait();
+              if (blk == quarter) weigh_own(v, &gate.col8[blk * 32 + n * 16], ob, lane, 2 * n);
+              else weigh(v, gate.col(blk) + n * 16, row);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const uint64_t p = pair(v[2 * e], v[2 * e + 1]);
+                split2<T>(p, x[e], x[8 + e]);
+                if constexpr (kThirds)
+                  third[e] =
+                      pack2<T>(fma2(unpack2<T>(x[8 + e]), pair(-1.f, -1.f), fma2(unpack2<T>(x[e]), pair(-1.f, -1.f), p)));
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) x[e] = x[8 + e] = third[e] = 0;
+            }
+            if constexpr (kThirds) {
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                *reinterpret_cast<uint4*>(smem + (blk >> 1) * kTile + swz(t, (blk & 1) * 4 + n * 2 + e)) =
+                    make_uint4(third[4 * e], third[4 * e + 1], third[4 * e + 2], third[4 * e + 3]);
+            }
+            tmem_st16(at, x);
+          }
+        }
+      }
+    }
+    ok = __all_sync(~0u, wait(bar_r, par)) && ok;
+    if (!live && t_end < t_hi) clear(sr, kRowTiles);
     if (ok) {
       // O starts from P_t (q S0) and the skip term; the scaled r, in two terms, goes over q
 #pragma unroll
-      for (uint32_t u = 0; u < kRowTiles; ++u) {
-        const uint32_t piece = half * kRowTiles + u;
-        float v[32];
+      for (uint32_t u = 0; u < 2 * kRowTiles; ++u) {
+        const uint32_t part = half * 2 * kRowTiles + u;  // 16 rows
+        float v[16];
         if constexpr (OUT != kOutNone) {
-          tmem_ld32(tmem + lanes + kColO + piece * 32, v);
-          ld_wait();
+          tmem_ld16(tmem + lanes + kColO + part * 16, v);
+          if constexpr (kPair) {
+            float low[16];
+            tmem_ld16(tmem + lanes + kColS + part * 16, low);
+            ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) unpair(add2(pair(v[e], v[e + 1]), pair(low[e], low[e + 1])), v[e], v[e + 1]);
+          } else {
+            ld_wait();
+          }
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t at = (piece >> 1) * kTile + swz(t, (piece & 1) * 4 + e);
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t at = (part >> 2) * kTile + swz(t, (part & 3) * 2 + e);
           uint32_t x[4] = {0, 0, 0, 0};
           if constexpr (CARRY || OUT == kOutY || OUT == kOutDx) {
             const uint4 q4 = *reinterpret_cast<const uint4*>(smem + (sr - sq) + at);
@@ -619,51 +686,14 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
               *reinterpret_cast<uint4*>(smem + (ss - sq) + at) = make_uint4(third[0], third[1], third[2], third[3]);
           }
         }
-        if constexpr (OUT != kOutNone) tmem_st32(tmem + lanes + kColO + piece * 32, v);
-      }
-      if constexpr (OUT != kOutNone) {
+        if constexpr (OUT != kOutNone) {
+          uint32_t w[16];
 #pragma unroll
-        for (uint32_t u = 0; u < 2; ++u) {
-          const uint32_t blk = half ? 1 + u : 3 * u;
-          const bool zero = REV ? blk < quarter : blk > quarter;
-          uint32_t hi[16], lo[16], third[16];
-          if (!zero) {
-            float v[32];
-            tmem_ld32(tmem + lanes + blk * 32, v);
-            float row = (REV ? tail : head) * rho;  // times the blocks between
-#pragma unroll
-            for (uint32_t m = 0; m < 4; ++m)
-              if (REV ? (m > quarter && m < blk) : (m > blk && m < quarter)) row *= gate.total[m];
-            ld_wait();
-            if (blk == blk_own) weigh_own(v, &gate.col8[blk * 32], ob, lane);
-            else weigh(v, &gate.col[blk * 32], row);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const uint64_t p = pair(v[2 * e], v[2 * e + 1]);
-              if constexpr (PRECISE) split2<T>(p, hi[e], lo[e]);
-              else hi[e] = pack2<T>(p);
-              if constexpr (kThirds)
-                third[e] = pack2<T>(fma2(unpack2<T>(lo[e]), pair(-1.f, -1.f), fma2(unpack2<T>(hi[e]), pair(-1.f, -1.f), p)));
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) hi[e] = lo[e] = third[e] = 0;
-          }
-          if constexpr (kThirds) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              *reinterpret_cast<uint4*>(smem + (blk >> 1) * kTile + swz(t, (blk & 1) * 4 + e)) =
-                  make_uint4(third[4 * e], third[4 * e + 1], third[4 * e + 2], third[4 * e + 3]);
-          }
-          tmem_st16(tmem + lanes + blk * 32, hi);
-          if constexpr (PRECISE) tmem_st16(tmem + lanes + blk * 32 + 16, lo);
+          for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(v[e]);
+          tmem_st16(tmem + lanes + kColO + part * 16, w);
         }
-        st_wait();
       }
-    }
-    if constexpr (kThirds) {
-      ok = __all_sync(~0u, wait(bar_r, par)) && ok;
-      if (!live && t_end < t_hi) clear(sr, kRowTiles);
+      if constexpr (OUT != kOutNone) st_wait();
     }
     fence_async();
     fence_before();
@@ -686,10 +716,9 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
         if constexpr (OUT != kOutNone) {
 #pragma unroll
           for (uint32_t j = 0; j < kQ / 16; ++j) {
-            const uint32_t a = tmem + (j >> 1) * 32 + (j & 1) * 8;
+            const uint32_t a = tmem + j * 16;
             mma_ts(tmem + kColO, a, desc(sr + j * 2048, kTile), idesc<T>(ROWS, false, true), 1);
-            if constexpr (PRECISE)
-              mma_ts(tmem + kColO, a + 16, desc(sr + j * 2048, kTile), idesc<T>(ROWS, false, true), 1);
+            mma_ts(tmem + kColO, a + 8, desc(sr + j * 2048, kTile), idesc<T>(ROWS, false, true), 1);
             if constexpr (kThirds)
               mma_ss(tmem + kColO, desc(sq + (j >> 2) * kTile + (j & 3) * 32, 16), desc(sr + j * 2048, kTile),
                      idesc<T>(ROWS, false, true), 1);
@@ -734,17 +763,18 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
 #pragma unroll
         for (uint32_t u = 0; u < kRowTiles; ++u) {
           const uint32_t piece = half * kRowTiles + u, row = row0 + piece * 32;
-          float v[32];
-          tmem_ld32(tmem + lanes + kColO + piece * 32, v);
-          ld_wait();
-          if constexpr (kHalf || (OUT == kOutRaw && REV)) {
+          auto load = [&](uint32_t n, float (&v)[16]) {  // 16 of its rows
+            tmem_ld16(tmem + lanes + kColO + piece * 32 + n * 16, v);
+            ld_wait();
+            if constexpr (kHalf || (OUT == kOutRaw && REV)) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const uint64_t x = pair(v[e], v[e + 1]);
-              if constexpr (kHalf) poison = fma2(x, 0, poison);
-              unpair(mul2(x, pair(up, up)), v[e], v[e + 1]);
+              for (int e = 0; e < 16; e += 2) {
+                const uint64_t x = pair(v[e], v[e + 1]);
+                if constexpr (kHalf) poison = fma2(x, 0, poison);
+                unpair(mul2(x, pair(up, up)), v[e], v[e + 1]);
+              }
             }
-          }
+          };
           // Four lanes hold words of four tokens each; transposed among them,
           // every store covers whole 64-byte runs of eight tokens.
           auto transpose = [&](uint32_t (&x)[4][4]) {
@@ -767,9 +797,11 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
           if constexpr (OUT == kOutRaw) {
 #pragma unroll
             for (int part = 0; part < 2; ++part) {  // 16 rows: four words of four
+              float v[16];
+              load(part, v);
               uint32_t x[4][4];
 #pragma unroll
-              for (int e = 0; e < 16; ++e) x[e / 4][e % 4] = __float_as_uint(v[16 * part + e]);
+              for (int e = 0; e < 16; ++e) x[e / 4][e % 4] = __float_as_uint(v[e]);
               transpose(x);
               const uint32_t col = row + 16 * part + 4 * (lane & 3);
 #pragma unroll
@@ -785,9 +817,12 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
           if constexpr (OUT != kOutRaw) {
             uint32_t x[4][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int n = 0; n < 2; ++n) {
+              float v[16];
+              load(n, v);
 #pragma unroll
-              for (int f = 0; f < 4; ++f) x[e][f] = live ? pack2<T>(pair(v[8 * e + 2 * f], v[8 * e + 2 * f + 1])) : 0u;
+              for (int e = 0; e < 8; ++e) x[2 * n + e / 4][e % 4] = live ? pack2<T>(pair(v[2 * e], v[2 * e + 1])) : 0u;
+            }
             transpose(x);
             const uint32_t col = row + 8 * (lane & 3);
 #pragma unroll
@@ -839,7 +874,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
   __syncthreads();
   fence_after();
   if (warp == 0)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tslot), "r"(kTmemCols));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(gate.tslot), "r"(kTmemCols));
 }
 
 using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -876,13 +911,14 @@ bool make_map(CUtensorMap& m, const Src& s, uint32_t width, const RecArgs& g, ui
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <class T, int COLS, int ROWS, bool REV, int OUT, bool PRECISE, bool CARRY>
+template <class T, int COLS, int ROWS, bool REV, int OUT, bool CARRY>
 void launch(const RecArgs& g, const Maps& maps, uint32_t batch, cudaStream_t st) {
-  const uint32_t need = 1024 + (CARRY ? 2 : COLS / 64) * kTile + COLS / 64 * kTile + ROWS / 64 * kTile +
-                        std::max(COLS * 128u * (ROWS / 64) * (PRECISE ? 2 : 1), CARRY ? kTile : 0u);
+  const uint32_t need = kSmall + (CARRY ? 2 : COLS / 64) * kTile + COLS / 64 * kTile + ROWS / 64 * kTile +
+                        (OUT == kOutNone ? kTile : COLS * 128u * (ROWS / 64) * 2);
   const uint32_t smem = std::max(need, kLeastSmem);
-  auto* kernel = k_scan_tc<T, COLS, ROWS, REV, OUT, PRECISE, CARRY>;
+  auto* kernel = k_scan_tc<T, COLS, ROWS, REV, OUT, CARRY>;
   FHE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  FHE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
   const uint64_t blocks = (uint64_t)((g.rows + ROWS - 1) / ROWS) * g.heads * g.nseg * batch;
   require(blocks < (1ull << 31), "too many blocks");
   kernel<<<(uint32_t)blocks, kThreadsTc, smem, st>>>(g, maps);
@@ -903,16 +939,16 @@ bool launch_scan_tc(const RecArgs& g, bool rev, int out, uint32_t batch, cudaStr
     return false;
   auto go = [&](auto cols) {
     constexpr int C = decltype(cols)::value;
-    if (!rev && out == kOutNone) launch<T, C, 64, false, kOutNone, false, true>(g, maps, batch, st);
-    else if (!rev && out == kOutY) launch<T, C, 64, false, kOutY, false, true>(g, maps, batch, st);
-    else if (rev && out == kOutNone) launch<T, C, 64, true, kOutNone, false, true>(g, maps, batch, st);
-    else if (rev && out == kOutDx) launch<T, C, 64, true, kOutDx, false, false>(g, maps, batch, st);
+    if (!rev && out == kOutNone) launch<T, C, 64, false, kOutNone, true>(g, maps, batch, st);
+    else if (!rev && out == kOutY) launch<T, C, 64, false, kOutY, true>(g, maps, batch, st);
+    else if (rev && out == kOutNone) launch<T, C, 64, true, kOutNone, true>(g, maps, batch, st);
+    else if (rev && out == kOutDx) launch<T, C, 64, true, kOutDx, false>(g, maps, batch, st);
     else if (out == kOutRaw && g.rows <= 64) {
-      if (rev) launch<T, C, 64, true, kOutRaw, true, false>(g, maps, batch, st);
-      else launch<T, C, 64, false, kOutRaw, true, false>(g, maps, batch, st);
+      if (rev) launch<T, C, 64, true, kOutRaw, false>(g, maps, batch, st);
+      else launch<T, C, 64, false, kOutRaw, false>(g, maps, batch, st);
     } else if (out == kOutRaw) {
-      if (rev) launch<T, C, 128, true, kOutRaw, true, false>(g, maps, batch, st);
-      else launch<T, C, 128, false, kOutRaw, true, false>(g, maps, batch, st);
+      if (rev) launch<T, C, 128, true, kOutRaw, false>(g, maps, batch, st);
+      else launch<T, C, 128, false, kOutRaw, false>(g, maps, batch, st);
     } else require(false, "unknown walk", FHE_ERR_INTERNAL);
   };
   // without a carried state a segment is one chunk

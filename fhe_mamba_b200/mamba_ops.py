@@ -191,10 +191,11 @@ def ssm_scan(x, write, log_decay, B, C, D=None, initial_state=None, lengths=None
     be slices of one activation tensor (only the last axis must be contiguous,
     else it is copied).  Gradients reach every floating-point argument.
 
-    Rows of 64 tokens and more in 16 bits run on the tensor cores: y, dx, dB and
-    dC then carry about one more rounding of that type, the final state and the
-    gates' gradients keep 22 bits and more of every product; in bfloat16 a NaN
-    or an infinity may reach earlier tokens of its 128."""
+    Rows of 64 tokens and more in 16 bits run on the tensor cores, whose operands
+    are split into two or three terms of that type: outputs of the type are off by
+    their own rounding and 16 bits of each product, the final state and the gates'
+    gradients keep 22 bits and more of every product; in bfloat16 a NaN or an
+    infinity may reach earlier tokens of its 128."""
     if not _scan_fits(x, write, log_decay, B, C, D, initial_state, lengths):
         _check_scan("ssm_scan", x, write, log_decay, B, C, D, initial_state, lengths)
     args = (_inner(x), write, log_decay, _inner(B), _inner(C), _dense(D), _dense(initial_state), _dense(lengths))

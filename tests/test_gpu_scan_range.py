@@ -1,0 +1,122 @@
+"""The state scan where ranges and masks are hard: 16-bit operands, small and large factors, values that are not
+numbers, texts of different sizes in one row, growing decays.  Against 64 bits, token by token.
+
+Tolerances as in test_gpu_mamba_ops (K roundings of u = 2^-24 of the terms' magnitudes `mag`, half a step of the
+output's type), with what an operand's rounding leaves, half = finfo.eps / 2 of the activations' type:
+- outputs of that type (y, dx): an operand of two terms, half^2 mag; dB and dC no more;
+- float32 outputs: three terms of bfloat16 or two of float16, 3 half^3 or 3 half^2 mag;
+and, as an output's own last step can be a subnormal one, half the smallest subnormal of its type.
+"""
+import math
+
+import pytest
+import torch
+
+from test_gpu_mamba_ops import DTYPES, U, reference, scan_inputs, scan_k
+
+pytestmark = pytest.mark.gpu
+HALVES = [torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from fhe_mamba_b200 import mamba_ops
+    return mamba_ops
+
+
+def operand(i, dtype):
+    """What the operands' roundings leave of a term in an output of `dtype`."""
+    t = i["x"].dtype
+    half = torch.finfo(t).eps / 2
+    if t == torch.float32:
+        return 0.0
+    return half ** 2 if dtype == t or t == torch.float16 and dtype != torch.float32 else \
+        3 * half ** (3 if t == torch.bfloat16 else 2)
+
+
+def close(got, want, mag, k, what, factor):
+    assert got.shape == want.shape, what
+    f = torch.finfo(got.dtype)
+    got = got.double()
+    assert torch.isfinite(got).all(), what
+    err = (k * U + factor) * mag
+    tol = err + f.eps / 2 * (want.abs() + err) + f.smallest_normal * f.eps / 2 * (1 + 2.0 ** -20) + 2.0 ** -140
+    worst = ((got - want).abs() / tol).max().item() if got.numel() else 0.0
+    assert worst <= 1.0, f"{what}: {worst:.3g} of the tolerance"
+
+
+def log_decay_mag(i, mag):
+    """Terms behind a token's gradient of log_decay: <dS, S> at the end of its 128 tokens and alpha, beta of those
+    after it among them; a cleared state cuts the sum."""
+    gamma = mag["log_decay"] + i["write"].double() * mag["write"]
+    alive = torch.exp(i["log_decay"].double()) != 0
+    out, l = torch.zeros_like(gamma), gamma.shape[1]
+    acc = torch.zeros_like(gamma[:, 0])
+    for t in reversed(range(l)):
+        if t == l - 1 or t % 128 == 127:
+            acc = gamma[:, t].clone()
+        acc = acc + 2 * gamma[:, t]
+        out[:, t] = acc
+        acc = torch.where(alive[:, t], acc, 0.0)
+    return out
+
+
+def check(ops, i, dy=None, dfinal=None, names=None):
+    """Forward, and the gradients of `names` (all if None) where dy and dfinal are given."""
+    y, s = ops.ssm_scan(**i)
+    wy, ws, _ = reference(i)
+    my, ms, _ = reference(i, absolute=True)
+    k = scan_k(i)
+    close(y, wy, my, k, "y", operand(i, y.dtype))
+    close(s, ws, ms, k, "final state", operand(i, s.dtype))
+    if dy is None:
+        return
+    leaf = {n: v.detach().requires_grad_() for n, v in i.items() if n != "lengths" and v is not None}
+    y, s = ops.ssm_scan(**leaf, lengths=i["lengths"])
+    got = dict(zip(leaf, torch.autograd.grad([y, s], list(leaf.values()), [dy, dfinal])))
+    _, _, want = reference(i, dy, dfinal)
+    _, _, mag = reference(i, dy, dfinal, absolute=True)
+    mag["log_decay"] = log_decay_mag(i, mag)
+    b, l = i["x"].shape[:2]
+    for n in names or got:
+        close(got[n], want[n], mag[n], 2 * k + (b * l if n == "D" else 0), "d" + n, operand(i, got[n].dtype))
+
+
+def upstream(i, seed, dy=1.0, dfinal=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x, n = i["x"], i["B"].shape[3]
+    return ((dy * torch.randn(x.shape, generator=g, device="cuda")).to(x.dtype),
+            dfinal * torch.randn(x.shape[0], x.shape[2], x.shape[3], n, generator=g, device="cuda"))
+
+
+def single(i, c=3):
+    """Inputs whose inner products have one term each, so that an operand's rounding is not averaged away."""
+    for n in ("B", "C"):
+        v = torch.zeros_like(i[n])
+        v[..., c] = i[n][..., c]
+        i[n] = v
+    return i
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("l", [64, 300])
+@pytest.mark.parametrize("n", [8, 64, 128])
+def test_outputs_hold_two_terms(ops, dtype, l, n):
+    """y and dx are one product each (the state is cleared at every token), or the carried state alone: they are off
+    by their own rounding and no operand's beside it."""
+    i = single(scan_inputs(31, 2, l, 2, 64, n, 1, dtype, strided=False))
+    i["D"] = None
+    dy, ds = upstream(i, 1)
+    check(ops, dict(i, log_decay=torch.full_like(i["write"], -math.inf), initial_state=None), dy, ds * 0)
+    keep = i["log_decay"].clone()
+    keep[:] = 0
+    check(ops, dict(i, log_decay=keep, write=torch.zeros_like(keep)))
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("l, p, n, k", [(64, 16, 32, 1), (130, 16, 16, 2), (129, 64, 128, 1), (300, 128, 128, 1),
+                                        (200, 8, 104, 1), (257, 72, 40, 2)])
+def test_tensor_core_sizes(ops, dtype, l, p, n, k):
+    """Rows and columns that fill their tiles in part, with the 128 x 128 gradients."""
+    i = scan_inputs(l, 2, l, 2, p, n, k, dtype, carried=True, ragged=l > 200, strided=False)
+    check(ops, i, *upstream(i, 2))
