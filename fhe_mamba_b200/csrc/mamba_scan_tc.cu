@@ -18,9 +18,13 @@
 // differed from one of 63).  For the raw sums (OUT kOutRaw) and for E o w o r,
 // whose sum is the fp32 state, it is 22 bits and more: three terms of bfloat16
 // or two of float16.
-// For float16 the factors are scaled by powers of two (the chunk's largest w to
-// about 8, the state by 16) to use its range; where an operand overflows all
-// the same, a product is not finite, the kernel says so in *bad, and the
+// float16's range is brought to the operands by powers of two that follow what a
+// chunk holds: each row of G o L o w, the tile of E o w o r and the tile of S0
+// enter with their largest value in [2^14, 2^15), so that two terms are off by
+// at most 2^-39 of that (half a step of the subnormal numbers) where they do not
+// hold 22 bits of their own.  (With the state times 16 and w alone scaled, a
+// state's gradient of 1e-6 lost 3 decimal digits, one of 1e-9 all.)  Where a
+// product is not finite all the same, the kernel says so in *bad, and the
 // caller's launches of the fp32 walk, idle otherwise, take the work over.
 //
 // One CTA walks one (batch, head, tile of rows, segment).  Shared memory holds
@@ -199,6 +203,14 @@ __device__ __forceinline__ float scale_of(float v) {
   return e - 1u < 226u ? __uint_as_float((254u - e) << 23) : 1.f;
 }
 
+// The power of two that brings the bits of a |v| into [2^14, 2^15), at most
+// 2^`most`; 1 for 0, NaN and infinities.
+__device__ __forceinline__ float range_of(uint32_t bits, int most) {
+  const int e = (int)(bits >> 23);
+  if (bits == 0 || e == 255) return 1.f;
+  return __uint_as_float((uint32_t)(127 + min(141 - e, most)) << 23);
+}
+
 // One lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
   uint32_t one;
@@ -216,7 +228,7 @@ struct Small {
   float cols[96];   // column factor for rows of other blocks of 32: tail (reversed: head) times w
   float col8[kQ];   // and for rows of other blocks of 8 in its block of 32
   float total[4];   // product over each block of 32
-  float most[4];    // largest |w| in each block of 32 (float16)
+  uint32_t state[8];  // bits of the largest |S0| of each warp (float16)
   uint64_t bars[5];  // G and q S0, S', O; k and q have arrived, r has
   uint32_t tslot;
   // no row lies beyond the last (reversed: before the first) block of 32
@@ -253,8 +265,6 @@ __device__ __forceinline__ Token make_token(Small<REV>& g, uint32_t t, uint32_t 
     if (REV ? blk > 0 : blk < 3) g.col(blk)[lane] = (REV ? head : tail) * w;
     g.col8[t] = (REV ? head8 : tail8) * w;
     if (lane == 31) g.total[blk] = head;
-    const uint32_t most = __reduce_max_sync(~0u, __float_as_uint(fabsf(w)));
-    if (lane == 0) g.most[blk] = __uint_as_float(most);
   }
   return Token{a, w, head, tail};
 }
@@ -375,7 +385,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
   const uint32_t quarter = warp & 3, half = warp >> 2;
   const uint32_t t = quarter * 32 + lane;  // this thread's token, and column of S
   constexpr bool kHalf = std::is_same_v<T, __half>;
-  constexpr float kStateScale = kHalf ? 16.f : 1.f;  // of S0 in shared memory
+  float sigma = 1.f;  // float16: scale of S0 in shared memory
   uint64_t poison = 0;  // a sum of 0 times every product: NaN once one is not finite (float16)
 
   if (warp == 0) {
@@ -443,7 +453,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const uint64_t x = kHalf ? mul2(s[4 * v + e], pair(kStateScale, kStateScale)) : s[4 * v + e];
+        const uint64_t x = kHalf ? mul2(s[4 * v + e], pair(sigma, sigma)) : s[4 * v + e];
         split2<T>(x, hi[e], lo[e]);
       }
       const uint32_t at = ss - sq + (piece >> 1) * kTileS + swz(t, (piece & 1) * 4 + v);
@@ -451,19 +461,56 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
       *reinterpret_cast<uint4*>(smem + at + kBytesS) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
   };
+  // float16: the tile's scale from its largest value; a barrier in between
+  [[maybe_unused]] auto find_sigma = [&](uint32_t bits) {
+    bits = __reduce_max_sync(~0u, bits);
+    if (lane == 0) gate.state[warp] = bits;
+    __syncthreads();
+    bits = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) bits = max(bits, gate.state[i]);
+    sigma = range_of(bits, 126);
+  };
+  [[maybe_unused]] auto state_bits = [&] {
+    uint32_t bits = 0;
+    if (t < g.cols) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float a, c;
+        unpair(s[i], a, c);
+        bits = max(bits, __float_as_uint(fmaxf(fabsf(a), fabsf(c))));
+      }
+    }
+    return bits;
+  };
   if constexpr (OUT == kOutRaw) {
     // rows run along memory here (st_row 1): a warp takes a column's 128 rows
     // at a time, four to a lane
     const float* in = g.state_in + bh * g.in_bh + seg * g.in_seg;
+    constexpr uint32_t kLoads = COLS * ROWS / 4 / kThreadsTc, per = ROWS / 4;  // groups of four rows
+    float4 own[kHalf ? kLoads : 1];  // (float16: all of them, for their scale)
+    auto fetch = [&](uint32_t j) {
+      const uint32_t e = j * kThreadsTc + tid, c = e / per, row = row0 + e % per * 4;
+      return c < g.cols && row < g.rows ? *reinterpret_cast<const float4*>(in + (int64_t)c * g.st_col + row)
+                                        : make_float4(0, 0, 0, 0);
+    };
+    if constexpr (kHalf) {
+      uint32_t bits = 0;
 #pragma unroll
-    for (uint32_t j = 0; j < COLS * ROWS / 4 / kThreadsTc; ++j) {
-      const uint32_t e = j * kThreadsTc + tid, per = ROWS / 4;  // groups of four rows
-      const uint32_t c = e / per, n = e % per * 4, row = row0 + n;
-      float4 x = make_float4(0, 0, 0, 0);
-      if (c < g.cols && row < g.rows) x = *reinterpret_cast<const float4*>(in + (int64_t)c * g.st_col + row);
+      for (uint32_t j = 0; j < kLoads; ++j) {
+        own[j] = fetch(j);
+        bits = max(bits, __float_as_uint(fmaxf(fmaxf(fabsf(own[j].x), fabsf(own[j].y)),
+                                               fmaxf(fabsf(own[j].z), fabsf(own[j].w)))));
+      }
+      find_sigma(bits);
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kLoads; ++j) {
+      const uint32_t e = j * kThreadsTc + tid, c = e / per, n = e % per * 4;
+      const float4 x = kHalf ? own[kHalf ? j : 0] : fetch(j);
       uint2 hi, lo;
-      split2<T>(pair(kStateScale * x.x, kStateScale * x.y), hi.x, lo.x);
-      split2<T>(pair(kStateScale * x.z, kStateScale * x.w), hi.y, lo.y);
+      split2<T>(pair(sigma * x.x, sigma * x.y), hi.x, lo.x);
+      split2<T>(pair(sigma * x.z, sigma * x.w), hi.y, lo.y);
       const uint32_t at = ss - sq + (n >> 6) * kTileS + swz(c, n >> 3 & 7) + (n & 4) * 2;
       *reinterpret_cast<uint2*>(smem + at) = hi;
       *reinterpret_cast<uint2*>(smem + at + kBytesS) = lo;
@@ -483,7 +530,10 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
       s[i] = pair(in && row < g.rows ? in[row * g.st_row] : 0.f,
                   in && row + 1 < g.rows ? in[(row + 1) * g.st_row] : 0.f);
     }
-    if constexpr (OUT != kOutNone) put_state(half);
+    if constexpr (OUT != kOutNone) {
+      if constexpr (kHalf) find_sigma(state_bits());
+      put_state(half);
+    }
   }
 
   float decay = 1.f;
@@ -505,12 +555,10 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
     float rho = 1.f, up = 1.f;
     if constexpr (OUT == kOutDx || (REV && OUT == kOutRaw)) {
       const float w = row_w;
-      rho = OUT == kOutRaw || kHalf ? w * scale_of(w) : w;
+      rho = OUT == kOutRaw ? w * scale_of(w) : w;
       if constexpr (OUT == kOutRaw) {
         if (fabsf(rho) < 1.f) rho = 1.f;  // 0 or denormal
         up = 1.f / rho;
-      } else if constexpr (kHalf) {
-        up = 1.f / scale_of(w);
       }
     }
     if (i > 0) {  // (the barriers are initialised before the first)
@@ -567,15 +615,9 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
       if (u < quarter) before *= gate.total[u];
       if (u > quarter) after *= gate.total[u];
     }
-    if constexpr (kHalf) {  // w of the chunk scaled to at most 16
-      const float sw = 8.f * scale_of(fmaxf(fmaxf(gate.most[0], gate.most[1]), fmaxf(gate.most[2], gate.most[3])));
-      rho *= sw;
-      up /= sw;
-    }
-    const float back = kHalf ? 1.f / (8.f * scale_of(fmaxf(fmaxf(gate.most[0], gate.most[1]), fmaxf(gate.most[2], gate.most[3])))) : 1.f;
-    const float pt = (REV ? me.tail * after : me.head * before) * (rho / kStateScale);
-    const float et = (REV ? me.head * before : me.tail * after) * me.w / back;
-    const float keep = skip / up;  // the skip term in the products' scale
+    const float pt = (REV ? me.tail * after : me.head * before) * rho;
+    float et = (REV ? me.head * before : me.tail * after) * me.w;
+    float keep = skip / up;  // the skip term in the products' scale
     const float all = gate.total[0] * gate.total[1] * gate.total[2] * gate.total[3];
     decay *= all;
     const bool owner = half == (quarter == 1 || quarter == 2 ? 1u : 0u);  // half 0: blocks 0 and 3, half 1: 1 and 2
@@ -590,6 +632,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
       if (ok && tid == 0) load_rows(t0);
       __syncwarp();
     }
+    [[maybe_unused]] float largest = 0.f;  // of this row's products in its two blocks (float16)
     if constexpr (OUT != kOutNone) {
       if (ok) {
 #pragma unroll
@@ -610,13 +653,21 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
               ld_wait();
               if (blk == quarter) weigh_own(v, &gate.col8[blk * 32 + n * 16], ob, lane, 2 * n);
               else weigh(v, gate.col(blk) + n * 16, row);
+              if constexpr (kHalf) {  // as they are; the row's scale is found first
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const uint64_t p = pair(v[2 * e], v[2 * e + 1]);
-                split2<T>(p, x[e], x[8 + e]);
-                if constexpr (kThirds)
-                  third[e] =
-                      pack2<T>(fma2(unpack2<T>(x[8 + e]), pair(-1.f, -1.f), fma2(unpack2<T>(x[e]), pair(-1.f, -1.f), p)));
+                for (int e = 0; e < 16; ++e) {
+                  largest = fmaxf(largest, fabsf(v[e]));
+                  x[e] = __float_as_uint(v[e]);
+                }
+              } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  const uint64_t p = pair(v[2 * e], v[2 * e + 1]);
+                  split2<T>(p, x[e], x[8 + e]);
+                  if constexpr (kThirds)
+                    third[e] =
+                        pack2<T>(fma2(unpack2<T>(x[8 + e]), pair(-1.f, -1.f), fma2(unpack2<T>(x[e]), pair(-1.f, -1.f), p)));
+                }
               }
             } else {
 #pragma unroll
@@ -635,6 +686,61 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
     }
     ok = __all_sync(~0u, wait(bar_r, par)) && ok;
     if (!live && t_end < t_hi) clear(sr, kRowTiles);
+    float back = 1.f, scale = 1.f;  // float16: undoes the scale of E o w o r; S0's to the row's
+    if constexpr (kHalf) {
+      // The scales of this row's products and of the tile of E o w o r: the row's
+      // other half and the other warps are told over S0's place, which is free.
+      uint32_t* told = reinterpret_cast<uint32_t*>(smem + (ss - sq));
+      if (OUT != kOutNone) told[half * kQ + t] = __float_as_uint(largest);
+      if constexpr (CARRY) {
+        __half2 most = __half2half2(__ushort_as_half(0));
+#pragma unroll
+        for (uint32_t v = 0; v < 4; ++v) {
+          const uint4 q4 = *reinterpret_cast<const uint4*>(smem + (sr - sq) + swz(t, half * 4 + v));
+          const uint32_t q[4] = {q4.x, q4.y, q4.z, q4.w};
+#pragma unroll
+          for (int f = 0; f < 4; ++f) most = __hmax2(most, __habs2(*reinterpret_cast<const __half2*>(&q[f])));
+        }
+        const float2 m = __half22float2(most);
+        const uint32_t bits = __reduce_max_sync(~0u, __float_as_uint(fabsf(et) * fmaxf(m.x, m.y)));
+        if (lane == 0) told[2 * kQ + warp] = bits;
+      }
+      __syncthreads();
+      if constexpr (CARRY) {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) bits = max(bits, told[2 * kQ + i]);
+        const float up_r = range_of(bits, 100);
+        et *= up_r;
+        back = 1.f / up_r;
+      }
+      if constexpr (OUT != kOutNone) {
+        // (at most 2^60: the row's other terms, of the state, stay in fp32's range)
+        const float f = range_of(max(__float_as_uint(largest), told[(half ^ 1u) * kQ + t]), 60);
+        scale = f / sigma;
+        keep *= f;
+        up /= f;
+        if (ok) {
+          st_wait();
+#pragma unroll
+          for (uint32_t u = 0; u < 2; ++u) {
+            const uint32_t blk = half ? 1 + u : 3 * u;
+            if (REV ? blk < quarter : blk > quarter) continue;
+#pragma unroll
+            for (uint32_t n = 0; n < 2; ++n) {
+              const uint32_t at = tmem + lanes + blk * 32 + n * 16;
+              float v[16];
+              uint32_t x[16];
+              tmem_ld16(at, v);
+              ld_wait();
+#pragma unroll
+              for (int e = 0; e < 8; ++e) split2<T>(mul2(pair(v[2 * e], v[2 * e + 1]), pair(f, f)), x[e], x[8 + e]);
+              tmem_st16(at, x);
+            }
+          }
+        }
+      }
+    }
     if (ok) {
       // O starts from P_t (q S0) and the skip term; the scaled r, in two terms, goes over q
 #pragma unroll
@@ -675,6 +781,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
             if constexpr (OUT != kOutNone) {
               float *o = v + 8 * e + 2 * f;
               uint64_t a = mul2(pair(pt, pt), pair(o[0], o[1]));
+              if constexpr (kHalf) a = mul2(pair(scale, scale), a);
               if constexpr (OUT == kOutY || OUT == kOutDx) a = fma2(pair(keep, keep), xx, a);
               unpair(a, o[0], o[1]);
             }
@@ -748,8 +855,14 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
           s[e] = fma2(pair(all, all), s[e], x);
         }
         if constexpr (OUT != kOutNone) {
-          if (i + 1 < chunks) put_state(half);
+          if (!kHalf && i + 1 < chunks) put_state(half);
         }
+      }
+    }
+    if constexpr (kHalf && CARRY && OUT != kOutNone) {
+      if (i + 1 < chunks) {  // the same for all threads
+        find_sigma(state_bits());
+        if (ok) put_state(half);
       }
     }
     if constexpr (OUT == kOutNone) {

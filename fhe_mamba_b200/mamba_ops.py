@@ -194,8 +194,9 @@ def ssm_scan(x, write, log_decay, B, C, D=None, initial_state=None, lengths=None
     Rows of 64 tokens and more in 16 bits run on the tensor cores, whose operands
     are split into two or three terms of that type: outputs of the type are off by
     their own rounding and 16 bits of each product, the final state and the gates'
-    gradients keep 22 bits and more of every product; in bfloat16 a NaN or an
-    infinity may reach earlier tokens of its 128."""
+    gradients keep 22 bits and more of every product (in float16 of those within
+    2^-17 of the largest of 128 tokens, and 2^-39 of that of the others); in
+    bfloat16 a NaN or an infinity may reach earlier tokens of its 128."""
     if not _scan_fits(x, write, log_decay, B, C, D, initial_state, lengths):
         _check_scan("ssm_scan", x, write, log_decay, B, C, D, initial_state, lengths)
     args = (_inner(x), write, log_decay, _inner(B), _inner(C), _dense(D), _dense(initial_state), _dense(lengths))
