@@ -329,11 +329,12 @@ __global__ void __launch_bounds__(kThreads) k_step(const StepArgs g) {
 // forward, slot s + 1 holds segment s's state from zero and becomes the state
 // at its end, slot 0 the initial state; reversed, slot s holds what segment s
 // passes back from zero and becomes the gradient of the state before it,
-// slot nseg the final state's gradient.  `end` receives the last slot written.
+// slot nseg the final state's gradient.  `end` receives the last slot written;
+// `bad` (or nullptr) is cleared for the walks to come.
 template <bool REV>
 __global__ void k_join(float* slots, const float* seg_decay, const float* start, float* end, uint32_t nseg,
-                       uint32_t size, const int* only_if) {
-  if (only_if && *only_if == 0) return;
+                       uint32_t size, int* bad) {
+  if (bad && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *bad = 0;
   const uint32_t e = blockIdx.x * blockDim.x + threadIdx.x;
   const int64_t bh = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
   if (e >= size) return;
@@ -621,7 +622,7 @@ bool launch_rec(RecArgs g, uint32_t batch, cudaStream_t st, bool fp32) {
 }
 
 void launch_join(bool rev, float* slots, const float* dec, const float* start, float* end, uint32_t nseg,
-                 uint32_t size, uint32_t bh, const int* only_if, cudaStream_t st) {
+                 uint32_t size, uint32_t bh, int* bad, cudaStream_t st) {
   const uint32_t y = std::min(bh, 32768u);
   // bh < 2^24; whole rows of y blocks, then the rest
   for (uint32_t at = 0; at < bh; at += y) {
@@ -631,8 +632,8 @@ void launch_join(bool rev, float* slots, const float* dec, const float* start, f
     const float* de = dec + (int64_t)at * nseg;
     const float* b0 = start ? start + (int64_t)at * size : nullptr;
     float* e0 = end ? end + (int64_t)at * size : nullptr;
-    if (rev) k_join<true><<<grid, 256, 0, st>>>(sl, de, b0, e0, nseg, size, only_if);
-    else k_join<false><<<grid, 256, 0, st>>>(sl, de, b0, e0, nseg, size, only_if);
+    if (rev) k_join<true><<<grid, 256, 0, st>>>(sl, de, b0, e0, nseg, size, bad);
+    else k_join<false><<<grid, 256, 0, st>>>(sl, de, b0, e0, nseg, size, bad);
     note_launch();
   }
   FHE_CUDA(cudaGetLastError());
@@ -691,17 +692,19 @@ RecArgs rec_args(const fhe_ssm_scan_args& a, const Cut& cut) {
 namespace {
 struct ForwardSpace {
   int* bad;
-  float *slots, *dec;
+  float *slots, *dec, *start;
   uint64_t bytes;
 };
 ForwardSpace forward_space(const fhe_ssm_scan_args& a, const Cut& cut, void* base) {
   const uint64_t bh = (uint64_t)a.batch * a.heads;
   Carver w(base);
   ForwardSpace s{};
-  if (a.dtype == FHE_F16 && tc_type(a)) s.bad = w.take<int>(1);
+  if (tc_type(a)) s.bad = w.take<int>(1);
   if (cut.nseg > 1) {
     s.slots = w.take<float>(bh * (cut.nseg + 1) * a.head_dim * a.d_state);
     s.dec = w.take<float>(bh * cut.nseg);
+  } else if (tc_type(a) && a.initial_state && a.initial_state == a.final_state) {
+    s.start = w.take<float>(bh * a.head_dim * a.d_state);  // a second walk must not start from the first one's end
   }
   s.bytes = w.used;
   return s;
@@ -749,37 +752,33 @@ void ssm_scan(const fhe_ssm_scan_args& a) {
     using T = decltype(v);
     if (a.length == 1 && step_ok(a, one)) return launch_step<T>(one, st);
     const ForwardSpace sp = forward_space(a, cut, a.workspace);
-    auto walk = [&](bool fp32, const int* only_if) {
-      RecArgs r = g;
-      r.only_if = only_if;
-      r.bad = sp.bad;
-      bool tc = false;
-      if (cut.nseg > 1) {
-        r.seg_decay = sp.dec;
-        r.out_bh = (int64_t)(cut.nseg + 1) * size;
-        r.out_seg = size;
-        r.state_out = sp.slots + size;
-        tc |= launch_rec<T, false, kOutNone>(r, a.batch, st, fp32);
-        launch_join(false, sp.slots, sp.dec, a.initial_state, a.final_state, cut.nseg, size, bh, only_if, st);
-        r.state_in = sp.slots;
-        r.in_bh = r.out_bh;
-        r.in_seg = size;
-        r.state_out = nullptr;
-      } else {
-        r.state_in = a.initial_state;
-        r.state_out = a.final_state;
-        r.in_bh = r.out_bh = size;
-      }
-      tc |= launch_rec<T, false, kOutY>(r, a.batch, st, fp32);
-      return tc;
-    };
-    if (!sp.bad) {
-      walk(false, nullptr);
-    } else if (a.initial_state == a.final_state) {
-      walk(true, nullptr);  // a second walk would start from the first one's end
+    const float* start = a.initial_state;
+    if (sp.start) {
+      FHE_CUDA(cudaMemcpyAsync(sp.start, start, (size_t)bh * size * 4, cudaMemcpyDeviceToDevice, st));
+      start = sp.start;
+    }
+    RecArgs r = g;
+    r.bad = sp.bad;
+    if (cut.nseg > 1) {
+      r.seg_decay = sp.dec;
+      r.out_bh = (int64_t)(cut.nseg + 1) * size;
+      r.out_seg = size;
+      r.state_out = sp.slots + size;
+      launch_rec<T, false, kOutNone>(r, a.batch, st, false);
+      launch_join(false, sp.slots, sp.dec, start, a.final_state, cut.nseg, size, bh, sp.bad, st);
+      r.state_in = sp.slots;
+      r.in_bh = r.out_bh;
+      r.in_seg = size;
+      r.state_out = nullptr;
     } else {
-      FHE_CUDA(cudaMemsetAsync(sp.bad, 0, sizeof(int), st));
-      if (walk(false, nullptr)) walk(true, sp.bad);
+      if (sp.bad) FHE_CUDA(cudaMemsetAsync(sp.bad, 0, sizeof(int), st));
+      r.state_in = start;
+      r.state_out = a.final_state;
+      r.in_bh = r.out_bh = size;
+    }
+    if (launch_rec<T, false, kOutY>(r, a.batch, st, false)) {
+      r.only_if = sp.bad;
+      launch_rec<T, false, kOutY>(r, a.batch, st, true);
     }
   });
 }
@@ -806,7 +805,7 @@ BackwardSpace backward_space(const fhe_ssm_scan_grad_args& g, const Cut& cut, vo
   s.diff = w.take<float>(tok);
   s.skip = w.take<float>(tok);
   s.dd_part = w.take<float>(bh * cut.nseg);
-  if (a.dtype == FHE_F16 && tc_type(a)) s.bad = w.take<int>(1);
+  if (tc_type(a)) s.bad = w.take<int>(1);
   s.bytes = w.used;
   return s;
 }
@@ -844,67 +843,58 @@ void ssm_scan_backward(const fhe_ssm_scan_grad_args& g) {
   const int64_t slot_bh = (int64_t)(cut.nseg + 1) * size;
   with_type(a.dtype, [&](auto v) {
     using T = decltype(v);
+    RecArgs base = rec_args(a, cut);
+    base.bad = s.bad;
+    base.in_bh = base.out_bh = slot_bh;
+    base.in_seg = base.out_seg = size;
+    base.rows = a.head_dim;
+    base.cols = a.d_state;
+    base.st_row = a.d_state;
+    base.st_col = 1;
+    {  // states at the segments' ends
+      RecArgs r = base;
+      r.r = x; r.k = b; r.q = c;
+      r.write = write;
+      r.state_out = s.s_slots + size;
+      r.seg_decay = s.dec_f;
+      launch_rec<T, false, kOutNone>(r, a.batch, st, false);
+      launch_join(false, s.s_slots, s.dec_f, a.initial_state, nullptr, cut.nseg, size, bh, s.bad, st);
+    }
+    {  // gradients of the states before the segments
+      RecArgs r = base;
+      r.r = dy; r.k = c; r.q = b;
+      r.state_out = s.d_slots;
+      r.seg_decay = s.dec_r;
+      launch_rec<T, true, kOutNone>(r, a.batch, st, false);
+      launch_join(true, s.d_slots, s.dec_r, g.dfinal, g.dinitial, cut.nseg, size, bh, nullptr, st);
+    }
     auto walks = [&](bool fp32, const int* only_if) {
       bool tc = false;
-      RecArgs base = rec_args(a, cut);
-      base.only_if = only_if;
-      base.bad = s.bad;
-      base.in_bh = base.out_bh = slot_bh;
-      base.in_seg = base.out_seg = size;
-      base.rows = a.head_dim;
-      base.cols = a.d_state;
-      base.st_row = a.d_state;
-      base.st_col = 1;
-      {  // states at the segments' ends
-        RecArgs r = base;
-        r.r = x; r.k = b; r.q = c;
-        r.write = write;
-        r.state_out = s.s_slots + size;
-        r.seg_decay = s.dec_f;
-        tc |= launch_rec<T, false, kOutNone>(r, a.batch, st, fp32);
-        launch_join(false, s.s_slots, s.dec_f, a.initial_state, nullptr, cut.nseg, size, bh, only_if, st);
-      }
-      {  // gradients of the states before the segments
-        RecArgs r = base;
-        r.r = dy; r.k = c; r.q = b;
-        r.state_out = s.d_slots;
-        r.seg_decay = s.dec_r;
-        tc |= launch_rec<T, true, kOutNone>(r, a.batch, st, fp32);
-        launch_join(true, s.d_slots, s.dec_r, g.dfinal, g.dinitial, cut.nseg, size, bh, only_if, st);
-      }
-      {
-        RecArgs r = base;
-        r.r = dy; r.k = c; r.q = b;
-        r.state_in = s.d_slots + size;
-        r.out_scale = write;
-        r.d = a.d;
-        r.out = g.dx;
-        tc |= launch_rec<T, true, kOutDx>(r, a.batch, st, fp32);
-      }
-      base.rows = a.d_state;
-      base.cols = a.head_dim;
-      base.st_row = 1;
-      base.st_col = a.d_state;
-      {
-        RecArgs r = base;
-        r.r = c; r.k = dy; r.q = x;
-        r.state_in = s.d_slots + size;
-        r.out_scale = write;  // for the tensor-core form's roundings alone
-        r.out = s.u;
-        tc |= launch_rec<T, true, kOutRaw>(r, a.batch, st, fp32);
-      }
-      {
-        RecArgs r = base;
-        r.r = b; r.k = x; r.q = dy;
-        r.write = write;
-        r.state_in = s.s_slots;
-        r.out = s.dch;
-        tc |= launch_rec<T, false, kOutRaw>(r, a.batch, st, fp32);
-      }
+      RecArgs r = base;
+      r.only_if = only_if;
+      r.r = dy; r.k = c; r.q = b;
+      r.state_in = s.d_slots + size;
+      r.out_scale = write;
+      r.d = a.d;
+      r.out = g.dx;
+      tc |= launch_rec<T, true, kOutDx>(r, a.batch, st, fp32);
+      r.d = nullptr;
+      r.rows = a.d_state;
+      r.cols = a.head_dim;
+      r.st_row = 1;
+      r.st_col = a.d_state;
+      r.r = c; r.k = dy; r.q = x;  // out_scale: for the tensor-core form's roundings alone
+      r.out = s.u;
+      tc |= launch_rec<T, true, kOutRaw>(r, a.batch, st, fp32);
+      r.r = b; r.k = x; r.q = dy;
+      r.out_scale = Gate{};
+      r.write = write;
+      r.state_in = s.s_slots;
+      r.out = s.dch;
+      tc |= launch_rec<T, false, kOutRaw>(r, a.batch, st, fp32);
       return tc;
     };
-    if (s.bad) FHE_CUDA(cudaMemsetAsync(s.bad, 0, sizeof(int), st));
-    if (walks(false, nullptr) && s.bad) walks(true, s.bad);
+    if (walks(false, nullptr)) walks(true, s.bad);
     k_anchor<<<bh * cut.nseg, 256, 0, st>>>(s.s_slots, s.d_slots, s.gamma, cut.nseg, size);
     note_launch();
     SumArgs u{x, b, c, write, g.dy, a.lengths, a.length, a.heads, a.head_dim, a.d_state, a.groups,

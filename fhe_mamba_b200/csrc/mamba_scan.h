@@ -33,7 +33,7 @@ struct RecArgs {
   float* seg_decay;  // STATE pass: product of the segment's decays [bh][nseg]
   void* out;
   bool vec;  // r, k and q may be read four elements at a time
-  int* bad;            // set by the float16 tensor-core form when a product overflowed
+  int* bad;            // set by the tensor-core form when a product of an output is not finite
   const int* only_if;  // the fp32 walk does nothing while it is 0 (nullptr: always runs)
 };
 

@@ -23,9 +23,12 @@
 // enter with their largest value in [2^14, 2^15), so that two terms are off by
 // at most 2^-39 of that (half a step of the subnormal numbers) where they do not
 // hold 22 bits of their own.  (With the state times 16 and w alone scaled, a
-// state's gradient of 1e-6 lost 3 decimal digits, one of 1e-9 all.)  Where a
-// product is not finite all the same, the kernel says so in *bad, and the
-// caller's launches of the fp32 walk, idle otherwise, take the work over.
+// state's gradient of 1e-6 lost 3 decimal digits, one of 1e-9 all.)  
+// A NaN or an infinity among the operands would be carried to all tokens of its
+// chunk by the products, zeros of L or not: where an output's product is not
+// finite, the kernel says so in *bad, and the caller's launches of the fp32 walk,
+// idle otherwise, take those outputs over.  (The states between segments hold no
+// more NaN than the recurrence's own.)
 //
 // One CTA walks one (batch, head, tile of rows, segment).  Shared memory holds
 // q, k, r and S0's two terms in 128-byte-swizzled tiles of 64 columns; the
@@ -386,7 +389,12 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
   const uint32_t t = quarter * 32 + lane;  // this thread's token, and column of S
   constexpr bool kHalf = std::is_same_v<T, __half>;
   float sigma = 1.f;  // float16: scale of S0 in shared memory
-  uint64_t poison = 0;  // a sum of 0 times every product: NaN once one is not finite (float16)
+  // A sum of 0 times every product: NaN once one is not finite.
+  auto report = [&](uint64_t poison) {
+    float a, c;
+    unpair(poison, a, c);
+    if (!(a == 0.f && c == 0.f)) *g.bad = 1;
+  };
 
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&gate.tslot)),
@@ -845,16 +853,16 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
         float v[32];
         tmem_ld32(tmem + lanes + kColS + half * 32, v);
         ld_wait();
+        [[maybe_unused]] uint64_t poison = 0;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           uint64_t x = pair(v[2 * e], v[2 * e + 1]);
-          if constexpr (kHalf) {
-            poison = fma2(x, 0, poison);
-            x = mul2(x, pair(back, back));
-          }
+          if constexpr (kHalf) x = mul2(x, pair(back, back));
           s[e] = fma2(pair(all, all), s[e], x);
+          if constexpr (OUT != kOutNone) poison = fma2(s[e], 0, poison);
         }
         if constexpr (OUT != kOutNone) {
+          report(poison);
           if (!kHalf && i + 1 < chunks) put_state(half);
         }
       }
@@ -879,14 +887,14 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
           auto load = [&](uint32_t n, float (&v)[16]) {  // 16 of its rows
             tmem_ld16(tmem + lanes + kColO + piece * 32 + n * 16, v);
             ld_wait();
-            if constexpr (kHalf || (OUT == kOutRaw && REV)) {
+            uint64_t poison = 0;
 #pragma unroll
-              for (int e = 0; e < 16; e += 2) {
-                const uint64_t x = pair(v[e], v[e + 1]);
-                if constexpr (kHalf) poison = fma2(x, 0, poison);
-                unpair(mul2(x, pair(up, up)), v[e], v[e + 1]);
-              }
+            for (int e = 0; e < 16; e += 2) {
+              const uint64_t x = pair(v[e], v[e + 1]);
+              poison = fma2(x, 0, poison);
+              if constexpr (kHalf || (OUT == kOutRaw && REV)) unpair(mul2(x, pair(up, up)), v[e], v[e + 1]);
             }
+            report(poison);
           };
           // Four lanes hold words of four tokens each; transposed among them,
           // every store covers whole 64-byte runs of eight tokens.
@@ -949,11 +957,6 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
         }
       }
     }
-  }
-  if constexpr (kHalf) {
-    float a, c;
-    unpair(poison, a, c);
-    if (!(a == 0.f && c == 0.f)) *g.bad = 1;
   }
   if (ok) {
     if (CARRY && g.state_out && t < g.cols) {

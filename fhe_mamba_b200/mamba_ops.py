@@ -195,8 +195,12 @@ def ssm_scan(x, write, log_decay, B, C, D=None, initial_state=None, lengths=None
     are split into two or three terms of that type: outputs of the type are off by
     their own rounding and 16 bits of each product, the final state and the gates'
     gradients keep 22 bits and more of every product (in float16 of those within
-    2^-17 of the largest of 128 tokens, and 2^-39 of that of the others); in
-    bfloat16 a NaN or an infinity may reach earlier tokens of its 128."""
+    2^-17 of the largest of 128 tokens, and 2^-39 of that of the others).  Where
+    a product is not finite, y, dx, dB and dC are computed again in float32, so
+    that a NaN or an infinity reaches the tokens that the formula says and no
+    others; only log_decay's gradient, a running sum from the end of each 128
+    tokens, may carry it to the others of those.  log_decay is at most 0, or at
+    least the product of the decays of any run of tokens fits float32."""
     if not _scan_fits(x, write, log_decay, B, C, D, initial_state, lengths):
         _check_scan("ssm_scan", x, write, log_decay, B, C, D, initial_state, lengths)
     args = (_inner(x), write, log_decay, _inner(B), _inner(C), _dense(D), _dense(initial_state), _dense(lengths))

@@ -532,10 +532,11 @@ int fhe_rescale_noalloc(fhe_ctx* ctx, const uint64_t* in, uint32_t ncomp, uint32
  * log_decay = -inf clears the state before its token.  Tokens at or past
  * lengths[batch] (clamped to [0, length]) change no state, are not read, and
  * get y = 0.  head_dim <= 128, d_state <= 256.
- * Rows of 64 tokens and more with 16-bit activations run on the tensor cores,
- * 128 tokens at a time: there a NaN or an infinity in x, b or c may also reach
- * earlier tokens of its 128 (fp16 rows are then redone in fp32, where it does
- * not). */
+ * Rows of 64 tokens and more with 16-bit activations run on the tensor cores;
+ * where a product of theirs is not finite, y (and dx, db, dc) is computed again
+ * in fp32, by launches that are idle otherwise.  The product of the decays of any
+ * run of tokens must fit fp32 (log_decay is at most 0 as a rule).  final_state may
+ * be initial_state's memory. */
 typedef struct fhe_ssm_scan_args {
   int32_t device, dtype;
   uint32_t batch, length, heads, head_dim, d_state, groups;

@@ -167,3 +167,61 @@ def test_rows_of_different_sizes(ops, dtype):
     i["C"] = i["C"] * torch.logspace(-3, 1, 300, device="cuda")[:, None, None].to(dtype)
     dy, ds = upstream(i, 5)
     check(ops, i, dy * torch.logspace(1, -3, 300, device="cuda")[:, None, None].to(dtype), ds * 1e-7)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("name", ["x", "B", "C", "write", "log_decay"])
+def test_nothing_reaches_earlier_tokens(ops, dtype, name, value):
+    """A value that is not a number at token 200 leaves the tokens before it as they are (C's leaves all others)."""
+    i = scan_inputs(24, 2, 300, 2, 64, 128, 1, dtype, strided=False)
+    wy, _, _ = reference(i)
+    my, _, _ = reference(i, absolute=True)
+    i[name] = i[name].clone()
+    i[name][1, 200] = value
+    y, s = ops.ssm_scan(**i)
+    k = scan_k(i)
+    close(y[0], wy[0], my[0], k, "y of the other row", operand(i, y.dtype))
+    close(y[1, :200], wy[1, :200], my[1, :200], k, "y", operand(i, y.dtype))
+    assert not torch.isfinite(y[1, 200]).all()
+    if name == "C":
+        close(y[1, 201:], wy[1, 201:], my[1, 201:], k, "y", operand(i, y.dtype))
+        assert torch.isfinite(s).all()
+    else:
+        assert not torch.isfinite(s[1]).all() and torch.isfinite(s[0]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_nothing_reaches_later_gradients(ops, dtype):
+    """An upstream gradient that is not a number at token 40 leaves dx, dB of the tokens after it as they are."""
+    i = scan_inputs(25, 1, 200, 2, 64, 128, 1, dtype, strided=False)
+    dy, ds = upstream(i, 6)
+    _, _, want = reference(i, dy, ds)
+    _, _, mag = reference(i, dy, ds, absolute=True)
+    dy[:, 40] = math.nan
+    leaf = {n: v.detach().requires_grad_() for n, v in i.items() if n != "lengths"}
+    got = dict(zip(leaf, torch.autograd.grad(ops.ssm_scan(**leaf), list(leaf.values()), [dy, ds])))
+    for n in ("x", "B", "C", "write"):
+        close(got[n][:, 41:], want[n][:, 41:], mag[n][:, 41:], 2 * scan_k(i), "d" + n, operand(i, got[n].dtype))
+        assert got[n][:, 40].isnan().any()
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("l, b", [(130, 2), (1100, 1)])
+@pytest.mark.parametrize("bad", [False, True])
+def test_state_in_place(ops, dtype, l, b, bad):
+    """fhe_ssm_scan with final_state on initial_state's memory: the same outputs as beside it, also where the call is
+    computed again."""
+    import ctypes
+
+    from fhe_mamba_b200 import _lib
+    i = scan_inputs(28, b, l, 2, 64, 128, 1, dtype, strided=False)
+    if bad:
+        i["x"][0, 70, 1, 5] = math.inf
+    y, s = ops.ssm_scan(**i)
+    state, out = i["initial_state"].clone(), torch.empty_like(y)
+    a = ops._scan_args(i["x"], i["write"], i["log_decay"], i["B"], i["C"], i["D"], state, None, out, state)
+    ws = ops._workspace("fhe_ssm_scan_workspace", a, state.device)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    _lib.call("fhe_ssm_scan", ctypes.byref(a))
+    assert torch.equal(out.view(torch.int16), y.view(torch.int16)) and torch.equal(state.view(torch.int32), s.view(torch.int32))
