@@ -186,6 +186,7 @@ SIGNATURES = {
     "fhe_ctx_set_giant_hoisting": [vp, i32],
     "fhe_device_trim": [i32],
     "fhe_tc_timeouts": [vp],
+    "fhe_scan_wait_limit": [u32],
     "fhe_kernel_launches": [ctypes.POINTER(ctypes.c_uint64)],
     "fhe_ntt_butterfly_ceiling": [vp, ctypes.POINTER(ctypes.c_double)],
     "fhe_refresh": [vp, vp, f64, i32, ctypes.POINTER(vp)],

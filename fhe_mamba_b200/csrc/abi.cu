@@ -784,6 +784,10 @@ int fhe_tc_timeouts(uint64_t* count) {
   });
 }
 
+int fhe_scan_wait_limit(uint32_t polls) {
+  return guarded([&] { fhe::set_scan_wait_limit(polls); });
+}
+
 int fhe_ctx_level_counts(fhe_ctx* ctx, int32_t kind, uint64_t* out, uint32_t n) {
   return guarded([&] {
     fhe::Ckks& k = ckks(ctx);

@@ -34,6 +34,7 @@ struct RecArgs {
   void* out;
   bool vec;  // r, k and q may be read four elements at a time
   int* bad;            // set by the tensor-core form when a product of an output is not finite
+  uint32_t wait_limit;  // polls of the tensor-core form's waits
   const int* only_if;  // the fp32 walk does nothing while it is 0 (nullptr: always runs)
 };
 
@@ -47,7 +48,8 @@ __device__ __forceinline__ int clamp_length(const int32_t* lengths, uint32_t b, 
 // The tensor-core form (mamba_scan_tc.cu) for bfloat16 and float16; false, with
 // nothing launched, for sizes and layouts that it does not take.
 template <class T>
-bool launch_scan_tc(const RecArgs& g, bool rev, int out, uint32_t batch, cudaStream_t st);
-unsigned scan_tc_timeouts();
+bool launch_scan_tc(RecArgs g, bool rev, int out, uint32_t batch, cudaStream_t st);
+uint64_t scan_tc_timeouts();  // over all devices
+void set_scan_wait_limit(uint32_t polls);
 
 }  // namespace fhe

@@ -51,6 +51,7 @@
 // A walk that carries no state on (CARRY false: the gradients', a segment of
 // one chunk each) leaves S' out and takes 128 rows where there are as many.
 #include <algorithm>
+#include <atomic>
 #include <cuda.h>
 
 #include "launch_count.h"
@@ -68,11 +69,17 @@ constexpr uint32_t kColO = 128, kColS = 192;
 // More than a third of an SM's shared memory: at most two CTAs are resident,
 // whose tensor memory (2 x 256 columns) fits.
 constexpr uint32_t kLeastSmem = 80 * 1024;
-// Bound on a wait for an MMA group, far above its microseconds; on expiry the
-// kernel counts the failure, leaves its outputs and frees its tensor memory.
+// Bound on a wait for loads or products, in polls of a microsecond at most: far
+// above what they take.  When one runs out, the CTA counts it, waits (bounded
+// again) for what it has in flight, frees its tensor memory and says so: its
+// outputs are computed again by the fp32 walk (*bad), a state between segments
+// becomes NaN.
 constexpr uint32_t kWaitLimit = 1u << 20;
+constexpr uint32_t kPoll = 1000;  // ns
 
 __device__ unsigned g_scan_timeouts = 0;
+std::atomic<uint32_t> g_wait_limit{kWaitLimit};
+std::atomic<uint64_t> g_used_devices{0};  // bit d: device d has run the kernel
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -109,13 +116,13 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
 __device__ __forceinline__ void commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) {
-  for (uint32_t i = 0; i < kWaitLimit; ++i) {
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, uint32_t limit) {
+  for (uint32_t i = 0; i < limit; ++i) {
     uint32_t done;
     asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(done)
-        : "r"(bar), "r"(parity)
+        : "r"(bar), "r"(parity), "r"(kPoll)
         : "memory");
     if (done) return true;
   }
@@ -234,6 +241,7 @@ struct Small {
   uint32_t state[8];  // bits of the largest |S0| of each warp (float16)
   uint64_t bars[5];  // G and q S0, S', O; k and q have arrived, r has
   uint32_t tslot;
+  uint32_t issued;  // thread 0's, by index of the barrier: whether anything was issued, and the parity of how often
   // no row lies beyond the last (reversed: before the first) block of 32
   __device__ __forceinline__ float* col(uint32_t blk) { return cols + (blk - (REV ? 1u : 0u)) * 32; }
 };
@@ -402,19 +410,23 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   if (tid == 0) {
+    gate.issued = 0;
     for (int i = 0; i < 5; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar_g + 8 * i));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
 
+  auto note = [&](int bar) { gate.issued = (gate.issued ^ 1u << bar) | 256u << bar; };
   auto first = [&](int i) { return t_lo + (int)kQ * (REV ? chunks - 1 - i : i); };
   // One thread: the boxes of a chunk.
   auto load_rows = [&](int t0) {
     expect(bar_r, kBytesR);
+    note(4);
 #pragma unroll
     for (uint32_t j = 0; j < kRowTiles; ++j) load_box(sr + j * kTile, &maps.r, row0 + 64 * j, h / g.r.share, t0, b, bar_r);
   };
   auto load_kq = [&](int t0) {
     expect(bar_kq, kBytesK * (OUT != kOutNone ? 2 : 1));
+    note(3);
 #pragma unroll
     for (uint32_t j = 0; j < kHalves; ++j) {
       load_box(sk + j * kTile, &maps.k, 64 * j, h / g.k.share, t0, b, bar_kq);
@@ -548,7 +560,6 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
   uint32_t tmem = 0;
   const uint32_t lanes = (quarter * 32) << 16;
   bool ok = true;
-  int done = 0;  // chunks whose products were issued
   for (int i = 0; i < chunks; ++i) {
     const int t0 = first(i), tok = t0 + (int)t;
     const bool live = tok < t_end;
@@ -570,7 +581,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
       }
     }
     if (i > 0) {  // (the barriers are initialised before the first)
-      ok = __all_sync(~0u, wait(bar_kq, par)) && ok;
+      ok = __all_sync(~0u, wait(bar_kq, par, g.wait_limit)) && ok;
       if (!live && t_end < t_hi) {
         clear(sk, kHalves);
         if constexpr (OUT != kOutNone) clear(sq, kHalves);
@@ -582,7 +593,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
     fence_after();
     if (!ok) break;
     if (i == 0) {
-      ok = __all_sync(~0u, wait(bar_kq, par));
+      ok = __all_sync(~0u, wait(bar_kq, par, g.wait_limit));
       if (!live && t_end < t_hi) {
         clear(sk, kHalves);
         if constexpr (OUT != kOutNone) clear(sq, kHalves);
@@ -614,6 +625,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
         commit(bar_g);
       }
       __syncwarp();
+      if (tid == 0) note(0);
     }
     if (i + 1 < chunks) load_gates(first(i + 1));
     // products over the blocks around this row's own
@@ -632,8 +644,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
     OwnBlock ob;
     if constexpr (OUT != kOutNone) {
       if (owner) ob = own_block<REV>(me, lane, rho);
-      ok = __all_sync(~0u, wait(bar_g, par));
-      done = i + 1;
+      ok = __all_sync(~0u, wait(bar_g, par, g.wait_limit));
       fence_after();
     }
     if constexpr (kThirds) {
@@ -692,7 +703,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
         }
       }
     }
-    ok = __all_sync(~0u, wait(bar_r, par)) && ok;
+    ok = __all_sync(~0u, wait(bar_r, par, g.wait_limit)) && ok;
     if (!live && t_end < t_hi) clear(sr, kRowTiles);
     float back = 1.f, scale = 1.f;  // float16: undoes the scale of E o w o r; S0's to the row's
     if constexpr (kHalf) {
@@ -842,10 +853,11 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
         }
       }
       __syncwarp();
+      if (CARRY && tid == 0) note(1);
+      if (OUT != kOutNone && tid == 0) note(2);
     }
     if constexpr (CARRY) {
-      ok = __all_sync(~0u, wait(bar_s, par));
-      done = i + 1;
+      ok = __all_sync(~0u, wait(bar_s, par, g.wait_limit));
       fence_after();
       if (ok) {
         if (i + 1 < chunks && tid == 0) load_kq(first(i + 1));  // q's and k's places are free
@@ -876,7 +888,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
     if constexpr (OUT == kOutNone) {
       if (ok && i + 1 < chunks && tid == 0) load_rows(first(i + 1));
     } else {
-      ok = __all_sync(~0u, wait(bar_o, par)) && ok;
+      ok = __all_sync(~0u, wait(bar_o, par, g.wait_limit)) && ok;
       fence_after();
       if (ok) {
         if (i + 1 < chunks && tid == 0) load_rows(first(i + 1));
@@ -958,33 +970,23 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
       }
     }
   }
-  if (ok) {
-    if (CARRY && g.state_out && t < g.cols) {
-      float* o = g.state_out + bh * g.out_bh + seg * g.out_seg + (int64_t)t * g.st_col;
+  if (CARRY && g.state_out && t < g.cols && (ok || OUT == kOutNone)) {
+    float* o = g.state_out + bh * g.out_bh + seg * g.out_seg + (int64_t)t * g.st_col;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const uint32_t row = row0 + half * 32 + 2 * i;
-        float a, c;
-        unpair(s[i], a, c);
-        if (row < g.rows) o[row * g.st_row] = a;
-        if (row + 1 < g.rows) o[(row + 1) * g.st_row] = c;
-      }
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t row = row0 + half * 32 + 2 * i;
+      float a, c;
+      unpair(s[i], a, c);
+      if (row < g.rows) o[row * g.st_row] = ok ? a : NAN;
+      if (row + 1 < g.rows) o[(row + 1) * g.st_row] = ok ? c : NAN;
     }
-    if (OUT == kOutNone && row0 == 0 && tid == 0) g.seg_decay[bh * g.nseg + seg] = decay;
-  } else if (tid == 0) {
-    // a wait ran out: count it, and let what was issued finish (bounded) before the tensor memory goes
+  }
+  if (OUT == kOutNone && row0 == 0 && tid == 0) g.seg_decay[bh * g.nseg + seg] = decay;
+  if (!ok && tid == 0) {
     atomicAdd(&g_scan_timeouts, 1u);
-    if (done) {
-      const uint32_t par = (done - 1) & 1;
-      if (OUT != kOutNone) wait(bar_g, par);
-      if (CARRY) wait(bar_s, par);
-      if (OUT != kOutNone) wait(bar_o, par);
-    }
-    // phases of the loads: the last issued completes with either parity seen
-    wait(bar_kq, 0);
-    wait(bar_kq, 1);
-    wait(bar_r, 0);
-    wait(bar_r, 1);
+    if (OUT != kOutNone) *g.bad = 1;
+    for (int i = 0; i < 5; ++i)  // what is in flight ends before its memory goes
+      if (gate.issued >> (8 + i) & 1) wait(bar_g + 8 * i, (gate.issued >> i & 1) ^ 1, kWaitLimit);
   }
   fence_before();
   __syncthreads();
@@ -1037,6 +1039,9 @@ void launch(const RecArgs& g, const Maps& maps, uint32_t batch, cudaStream_t st)
   FHE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
   const uint64_t blocks = (uint64_t)((g.rows + ROWS - 1) / ROWS) * g.heads * g.nseg * batch;
   require(blocks < (1ull << 31), "too many blocks");
+  int device = 0;
+  FHE_CUDA(cudaGetDevice(&device));
+  g_used_devices.fetch_or(1ull << (device & 63), std::memory_order_relaxed);
   kernel<<<(uint32_t)blocks, kThreadsTc, smem, st>>>(g, maps);
   note_launch();
   FHE_CUDA(cudaGetLastError());
@@ -1045,7 +1050,8 @@ void launch(const RecArgs& g, const Maps& maps, uint32_t batch, cudaStream_t st)
 }  // namespace
 
 template <class T>
-bool launch_scan_tc(const RecArgs& g, bool rev, int out, uint32_t batch, cudaStream_t st) {
+bool launch_scan_tc(RecArgs g, bool rev, int out, uint32_t batch, cudaStream_t st) {
+  g.wait_limit = g_wait_limit.load(std::memory_order_relaxed);
   constexpr bool kHalf = std::is_same_v<T, __half>;
   Maps maps{};
   if (out == kOutRaw && (g.st_row != 1 || g.st_col % 4 != 0 || reinterpret_cast<uintptr_t>(g.state_in) % 16 != 0)) return false;
@@ -1074,13 +1080,20 @@ bool launch_scan_tc(const RecArgs& g, bool rev, int out, uint32_t batch, cudaStr
   return true;
 }
 
-template bool launch_scan_tc<__nv_bfloat16>(const RecArgs&, bool, int, uint32_t, cudaStream_t);
-template bool launch_scan_tc<__half>(const RecArgs&, bool, int, uint32_t, cudaStream_t);
+template bool launch_scan_tc<__nv_bfloat16>(RecArgs, bool, int, uint32_t, cudaStream_t);
+template bool launch_scan_tc<__half>(RecArgs, bool, int, uint32_t, cudaStream_t);
 
-unsigned scan_tc_timeouts() {
-  unsigned v = 0;
-  cudaMemcpyFromSymbol(&v, g_scan_timeouts, sizeof(v));
-  return v;
+uint64_t scan_tc_timeouts() {
+  uint64_t sum = 0;
+  for (uint64_t left = g_used_devices.load(std::memory_order_relaxed); left; left &= left - 1) {
+    DeviceGuard dev(__builtin_ctzll(left));
+    unsigned v = 0;
+    FHE_CUDA(cudaMemcpyFromSymbol(&v, g_scan_timeouts, sizeof(v)));
+    sum += v;
+  }
+  return sum;
 }
+
+void set_scan_wait_limit(uint32_t polls) { g_wait_limit.store(polls, std::memory_order_relaxed); }
 
 }  // namespace fhe

@@ -362,10 +362,15 @@ int fhe_ctx_set_keyswitch_fusion(fhe_ctx* ctx, int32_t fused);
  * EvalLinearTransform performs.  Results agree within the key switching
  * noise, not word for word. */
 int fhe_ctx_set_giant_hoisting(fhe_ctx* ctx, int32_t on);
-/* Number of tensor-core blocks (basis conversions, state scans) whose bounded
- * wait for their MMA ran out (their outputs were skipped); 0 on a healthy
- * device. */
+/* Number of tensor-core blocks whose bounded wait for their loads or products
+ * ran out; 0 on a healthy device.  A basis conversion's outputs were skipped
+ * then (counted on the current device); a state scan's were computed again in
+ * fp32, or are NaN where a state between segments was lost (counted on all
+ * devices). */
 int fhe_tc_timeouts(uint64_t* count);
+/* The state scans' bound, in polls of a microsecond at most (2^20 unless set).
+ * With 0 every wait runs out, which shows what such a device would return. */
+int fhe_scan_wait_limit(uint32_t polls);
 
 /* Bootstrapping of the context's slots (full packing N/2, or sparse packing:
  * a power of two below N/2, where ModRaise is followed by the trace over the

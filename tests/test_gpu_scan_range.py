@@ -225,3 +225,50 @@ def test_state_in_place(ops, dtype, l, b, bad):
     a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
     _lib.call("fhe_ssm_scan", ctypes.byref(a))
     assert torch.equal(out.view(torch.int16), y.view(torch.int16)) and torch.equal(state.view(torch.int32), s.view(torch.int32))
+
+
+WAITS = """
+import ctypes, sys
+sys.path.insert(0, {root!r})
+sys.path.insert(0, {tests!r})
+import torch
+import test_gpu_scan_range as here
+from fhe_mamba_b200 import _lib, mamba_ops as ops
+
+def count():
+    n = ctypes.c_uint64()
+    _lib.call("fhe_tc_timeouts", ctypes.byref(n))
+    return n.value
+
+for dtype in here.HALVES:
+    i = here.scan_inputs(29, 12, 130, 16, 64, 128, 1, dtype)  # 192 blocks: no state between segments
+    long = here.scan_inputs(30, 1, 1100, 2, 64, 128, 1, dtype)
+    leaf = i["x"].requires_grad_()
+    before = count()
+    here.check(ops, dict(i, x=leaf.detach()))
+    assert count() == before
+    _lib.call("fhe_scan_wait_limit", 0)
+    here.check(ops, dict(i, x=leaf.detach()))
+    assert count() > before
+    y, s = ops.ssm_scan(**long)
+    assert y[:, 1024:].isnan().all() and s.isnan().all()
+    assert torch.autograd.grad(ops.ssm_scan(**i)[0].sum(), leaf)[0].isnan().any()
+    _lib.call("fhe_scan_wait_limit", 1 << 20)
+    before = count()
+    here.check(ops, dict(i, x=leaf.detach()))
+    here.check(ops, long)
+    assert count() == before
+print("done")
+"""
+
+
+def test_waits_that_run_out():
+    """A wait that runs out (a limit of no polls) is counted and nothing is left unwritten: the outputs are computed
+    again in float32, or NaN behind a state that was lost.  In a process of its own, whose count it moves."""
+    import os
+    import subprocess
+    import sys
+    tests = os.path.dirname(os.path.abspath(__file__))
+    code = WAITS.format(root=os.path.dirname(tests), tests=tests)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "done" in r.stdout, r.stderr[-2000:]
