@@ -499,8 +499,8 @@ __global__ void __launch_bounds__(128) k_sum(const SumArgs g, uint32_t tokens) {
 }
 
 // One warp per (batch, head, segment): the running sum of alpha - beta from
-// the segment's end (fp64: it is a difference of sums), and the segment's
-// share of dd.
+// the segment's end (fp64: it is a difference of sums), which starts anew from
+// an exact 0 at a token that clears the state, and the segment's share of dd.
 __global__ void __launch_bounds__(128)
     k_log_decay_grad(const float* diff, const float* skip, const float* gamma, Gate log_decay, const int32_t* lengths,
                      float* out, float* dd_part, uint32_t length, uint32_t heads, uint32_t seglen, uint32_t nseg,
@@ -516,16 +516,21 @@ __global__ void __launch_bounds__(128)
     const int t = hi - 1 - (int)lane;
     const bool in = t >= t_lo;
     const int64_t at = ((int64_t)b * length + (in ? t : t_lo)) * heads + h;
-    double v = in ? diff[at] : 0.0;
+    const bool live = in && t < len;
+    const float la = live ? log_decay.p[b * log_decay.sb + t * log_decay.sl + h * log_decay.sh] : 0.f;
+    bool cut = expf(la) == 0.f;  // the sum before this lane's token owes nothing to later ones
+    double v = in && !cut ? diff[at] : 0.0;
     for (int o = 1; o < 32; o <<= 1) {
       const double u = __shfl_up_sync(~0u, v, o);
-      if ((int)lane >= o) v += u;
+      const bool c = __shfl_up_sync(~0u, cut, o);
+      if ((int)lane >= o && !cut) {
+        v += u;
+        cut = c;
+      }
     }
-    v += carry;
+    if (!cut) v += carry;
     if (in) {
-      const bool live = t < len;
-      const float la = live ? log_decay.p[b * log_decay.sb + t * log_decay.sl + h * log_decay.sh] : 0.f;
-      out[at] = live && expf(la) != 0.f ? (float)v : 0.f;
+      out[at] = live ? (float)v : 0.f;
       if (skip && live) dd += skip[at];
     }
     carry = __shfl_sync(~0u, v, 31);

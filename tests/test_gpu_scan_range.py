@@ -272,3 +272,17 @@ def test_waits_that_run_out():
     code = WAITS.format(root=os.path.dirname(tests), tests=tests)
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "done" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("at", [1, 50, 127, 128, 199])
+@pytest.mark.parametrize("size", [1e-4, 1e4])
+def test_texts_of_different_sizes(ops, dtype, at, size):
+    """A cleared state cuts the gradient of log_decay too: a text's is as exact as if it stood alone."""
+    i = scan_inputs(26, 2, 200, 2, 32, 64, 1, dtype, carried=False, strided=False)
+    i["D"] = None
+    i["log_decay"] = i["log_decay"].clone()
+    i["log_decay"][:, at] = -math.inf
+    i["write"][:, at:] *= size
+    dy, ds = upstream(i, 7)
+    check(ops, i, dy, ds)
