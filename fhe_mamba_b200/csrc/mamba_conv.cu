@@ -26,14 +26,10 @@ struct ConvArgs {
   uint64_t walkers;  // threads that walk tokens; later ones copy the final state
 };
 
-__device__ __forceinline__ int clamp_length(const int32_t* lengths, uint32_t b, uint32_t length) {
-  if (!lengths) return (int)length;
-  return min(max(lengths[b], 0), (int)length);
-}
-
 // 1 / (1 + exp(-v)) with the special-function exponential and reciprocal: a
-// few units in the last place of fp32, at a quarter of the instructions of
-// expf and a division, which would bound the 16-bit forms.
+// few units in the last place of fp32 (0 from v = -87.3 down, where it is below
+// 2^-126), at a quarter of the instructions of expf and a division, which would
+// bound the 16-bit forms.
 template <int V>
 __device__ __forceinline__ void sigmoid(float (&o)[V], const float (&v)[V]) {
   float k[V], one[V];
@@ -204,8 +200,9 @@ struct ConvGradArgs {
 // tokens more: dpre_t = dy_t act'(pre_t) enters a window of taps values, and
 // drow_u = sum_i w_i dpre_(u-i) (u a row index, u - (K - 1) a token) leaves
 // it.  The taps' and bias's gradients of the run's own tokens go to `part`.
-// 8 x 1001 tokens of 1792 float32 channels: 44 us, 3.9 TB/s; registers (two
-// windows and the taps' sums) keep it to 20 warps an SM.
+// 8 x 1001 tokens of 1792 float32 channels: 44 us, 3.9 TB/s (and 5 for the sums
+// of the parts); registers (two windows and the taps' sums) keep it to 20 warps
+// an SM.
 template <class T, int V, int K, bool SILU>
 __global__ void __launch_bounds__(kThreads) k_conv_grad(const ConvGradArgs a) {
   const ConvArgs& g = a.f;
@@ -505,8 +502,8 @@ void causal_conv_backward(const fhe_causal_conv_grad_args& a) {
   }
   with_type(a.f.dtype, [&](auto tv) {
     using T = decltype(tv);
-    // 8 bytes a load: the gradients hold twice the registers (8 x 1001 tokens of
-    // 1792 float32 channels: 49 us with 2 channels, 58 with 4)
+    // 8 bytes a load: the gradients hold twice the registers (8 x 1001 tokens of 1792
+    // float32 channels, sums of the parts included: 49 us with 2 channels, 58 with 4)
     constexpr int kVec = sizeof(T) == 4 ? 2 : 4;
     uint32_t vec = conv_vec(a.f, kVec, a.dy, a.dx, a.dfinal);
     if (!aligned(a.dinitial, vec * e)) vec = 1;

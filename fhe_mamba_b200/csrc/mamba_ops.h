@@ -64,6 +64,12 @@ inline void check_workspace(const void* ws, uint64_t have, uint64_t need) {
   require(reinterpret_cast<uintptr_t>(ws) % 256 == 0, "workspace must be 256-byte aligned");
 }
 
+// Tokens of row b (lengths may be nullptr: all).
+__device__ __forceinline__ int clamp_length(const int32_t* lengths, uint32_t b, uint32_t length) {
+  if (!lengths) return (int)length;
+  return min(max(lengths[b], 0), (int)length);
+}
+
 inline uint32_t elem_size(int32_t dtype) { return dtype == FHE_F32 ? 4 : 2; }
 
 template <class T>

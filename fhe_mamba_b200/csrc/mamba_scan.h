@@ -40,11 +40,6 @@ struct RecArgs {
 
 enum { kOutNone = 0, kOutY = 1, kOutDx = 2, kOutRaw = 3 };
 
-__device__ __forceinline__ int clamp_length(const int32_t* lengths, uint32_t b, uint32_t length) {
-  if (!lengths) return (int)length;
-  return min(max(lengths[b], 0), (int)length);
-}
-
 // The tensor-core form (mamba_scan_tc.cu) for bfloat16 and float16; false, with
 // nothing launched, for sizes and layouts that it does not take.
 template <class T>

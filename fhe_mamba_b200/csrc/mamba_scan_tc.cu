@@ -23,7 +23,7 @@
 // enter with their largest value in [2^14, 2^15), so that two terms are off by
 // at most 2^-39 of that (half a step of the subnormal numbers) where they do not
 // hold 22 bits of their own.  (With the state times 16 and w alone scaled, a
-// state's gradient of 1e-6 lost 3 decimal digits, one of 1e-9 all.)  
+// state's gradient of 1e-6 lost 3 decimal digits, one of 1e-9 all.)
 // A NaN or an infinity among the operands would be carried to all tokens of its
 // chunk by the products, zeros of L or not: where an output's product is not
 // finite, the kernel says so in *bad, and the caller's launches of the fp32 walk,
@@ -40,13 +40,14 @@
 // element passes take 16 columns at a time, since spilled registers cost more
 // than their instructions (what shared memory leaves of the L1 cache is small).
 //
-// 8 x 4096 bfloat16 tokens of 24 heads x 64, state 128: 236 us (198 with one term
-// of G o L o w and S0), of which memory needs 36 and the products about 80 at
-// full rate; a chunk is a chain of products and element passes that two CTAs to
-// an SM cover in part, and 192 CTAs leave 104 of 148 SMs with one (148 CTAs take
-// 176 us, 296 take 236).  Loads by tensor maps and stores of 64-byte runs took the
-// load and store unit out of that chain (343 us with 16-byte asynchronous copies
-// and scattered stores).
+// 8 x 4096 bfloat16 tokens of 24 heads x 64, state 128: 240 us (198 with one term
+// of G o L o w and S0 and unchecked products), of which memory needs 36 and the
+// products about 80 at full rate; a chunk is a chain of products and element
+// passes that two CTAs to an SM cover in part (issue slots 45% busy, the tensor
+// pipe 29%), and 192 CTAs leave 104 of 148 SMs with one (148 CTAs take 185 us, 296
+// take 245).  Loads by tensor maps and stores of 64-byte runs took the load and
+// store unit out of that chain (343 us with 16-byte asynchronous copies and
+// scattered stores).
 //
 // A walk that carries no state on (CARRY false: the gradients', a segment of
 // one chunk each) leaves S' out and takes 128 rows where there are as many.
@@ -365,8 +366,8 @@ __global__ void __launch_bounds__(kThreadsTc, 2) k_scan_tc(const RecArgs g, cons
   constexpr uint32_t kTileS = COLS * 128, kBytesS = kRowTiles * kTileS;
   constexpr bool kThird = CARRY && !std::is_same_v<T, __half>;  // a third term of the scaled r, in S0's place
   // The raw sums' third terms: of S0 in r's place, and of the weighted G as an
-  // operand in q's and k's (dwrite of 4 x 2048 bfloat16 tokens 4e-7 off, 2.4e-6
-  // with two; 87 us a pass, 77)
+  // operand in q's and k's (dwrite of 4 x 2048 bfloat16 tokens 4e-7 to 6e-7 off,
+  // 2.4e-6 with two; 69 us a pass)
   constexpr bool kThirds = OUT == kOutRaw && !std::is_same_v<T, __half>;
   // One product gives q times both terms of S0, side by side: the second's takes
   // the place of S', not needed yet.
