@@ -1,5 +1,5 @@
 """The state scan where ranges and masks are hard: 16-bit operands, small and large factors, values that are not
-numbers, texts of different sizes in one row, growing decays.  Against 64 bits, token by token.
+numbers, texts of different sizes in one row, waits that run out.  Against 64 bits, token by token.
 
 Tolerances as in test_gpu_mamba_ops (K roundings of u = 2^-24 of the terms' magnitudes `mag`, half a step of the
 output's type), with what an operand's rounding leaves, half = finfo.eps / 2 of the activations' type:
