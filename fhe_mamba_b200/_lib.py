@@ -123,6 +123,23 @@ class TokenLogprobsGradArgs(ctypes.Structure):
     ]
 
 
+class RmsNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("device", i32), ("dtype", i32), ("stream_dtype", i32), ("rows", u32), ("width", u32), ("groups", u32),
+        ("eps", ctypes.c_float), ("scale", ctypes.c_float),
+        ("x", vp), ("x_stride", i64), ("residual", vp), ("residual_stride", i64), ("gate", vp), ("gate_stride", i64),
+        ("channel_scale", vp), ("weight", vp), ("y", vp), ("h", vp), ("rstd", vp), ("stream", vp),
+    ]
+
+
+class RmsNormGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("f", RmsNormArgs),
+        ("dy", vp), ("dh", vp), ("dx", vp), ("dresidual", vp), ("dgate", vp), ("dweight", vp), ("dchannel_scale", vp),
+        ("workspace", vp), ("workspace_bytes", u64), ("stream", vp),
+    ]
+
+
 # name -> (argtypes); all return int status.
 SIGNATURES = {
     "fhe_last_error": [ctypes.c_char_p, ctypes.c_size_t],
@@ -228,6 +245,9 @@ SIGNATURES = {
     "fhe_causal_conv_backward": [ctypes.POINTER(CausalConvGradArgs)],
     "fhe_token_logprobs": [ctypes.POINTER(TokenLogprobsArgs)],
     "fhe_token_logprobs_backward": [ctypes.POINTER(TokenLogprobsGradArgs)],
+    "fhe_rms_norm": [ctypes.POINTER(RmsNormArgs)],
+    "fhe_rms_norm_backward_workspace": [ctypes.POINTER(RmsNormGradArgs), P64],
+    "fhe_rms_norm_backward": [ctypes.POINTER(RmsNormGradArgs)],
 }
 
 _lock = threading.Lock()

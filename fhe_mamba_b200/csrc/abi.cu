@@ -1294,4 +1294,25 @@ int fhe_token_logprobs_backward(const fhe_token_logprobs_grad_args* args) {
   });
 }
 
+int fhe_rms_norm(const fhe_rms_norm_args* args) {
+  return guarded([&] {
+    fhe::require(args != nullptr, "null argument");
+    fhe::rms_norm(*args);
+  });
+}
+
+int fhe_rms_norm_backward_workspace(const fhe_rms_norm_grad_args* args, uint64_t* bytes) {
+  return guarded([&] {
+    fhe::require(args != nullptr && bytes != nullptr, "null argument");
+    *bytes = fhe::rms_norm_backward_workspace(*args);
+  });
+}
+
+int fhe_rms_norm_backward(const fhe_rms_norm_grad_args* args) {
+  return guarded([&] {
+    fhe::require(args != nullptr, "null argument");
+    fhe::rms_norm_backward(*args);
+  });
+}
+
 }  // extern "C"

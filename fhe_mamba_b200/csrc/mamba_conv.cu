@@ -26,23 +26,6 @@ struct ConvArgs {
   uint64_t walkers;  // threads that walk tokens; later ones copy the final state
 };
 
-// 1 / (1 + exp(-v)) with the special-function exponential and reciprocal: a
-// few units in the last place of fp32 (0 from v = -87.3 down, where it is below
-// 2^-126), at a quarter of the instructions of expf and a division, which would
-// bound the 16-bit forms.
-template <int V>
-__device__ __forceinline__ void sigmoid(float (&o)[V], const float (&v)[V]) {
-  float k[V], one[V];
-  vset(k, -1.4426950408889634f);
-  vset(one, 1.f);
-  vmul(o, v, k);
-#pragma unroll
-  for (int i = 0; i < V; ++i) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(o[i]) : "f"(o[i]));
-  vadd(o, o, one);
-#pragma unroll
-  for (int i = 0; i < V; ++i) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(o[i]) : "f"(o[i]));
-}
-
 // Row element: t < 0 is the initial state's entry t + K - 1.
 template <class T, int V, int K>
 __device__ __forceinline__ void load_row(const T* x, const T* init, int64_t sl, uint32_t channels, int t,

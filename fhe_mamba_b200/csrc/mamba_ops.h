@@ -1,5 +1,6 @@
-// Plaintext Mamba-2 operators behind the fhe_ssm_scan, fhe_causal_conv and
-// fhe_token_logprobs entry points: argument checks and launches.
+// Plaintext Mamba-2 operators behind the fhe_ssm_scan, fhe_causal_conv,
+// fhe_token_logprobs, fhe_rms_norm, fhe_embedding and fhe_beam_* entry points:
+// argument checks and launches.
 #pragma once
 #include <cstdint>
 #include <cuda_bf16.h>
@@ -20,6 +21,9 @@ uint64_t causal_conv_backward_workspace(const fhe_causal_conv_grad_args& g);
 void causal_conv_backward(const fhe_causal_conv_grad_args& g);
 void token_logprobs(const fhe_token_logprobs_args& a);
 void token_logprobs_backward(const fhe_token_logprobs_grad_args& g);
+void rms_norm(const fhe_rms_norm_args& a);
+uint64_t rms_norm_backward_workspace(const fhe_rms_norm_grad_args& g);
+void rms_norm_backward(const fhe_rms_norm_grad_args& g);
 
 // Makes `device` current and restores the caller's device on destruction.
 class DeviceGuard {
@@ -173,6 +177,23 @@ __device__ __forceinline__ Pack<T, V> pack(const float (&o)[V]) {
     for (int v = 0; v < V; ++v) p.v[v] = from_f<T>(o[v]);
   }
   return p;
+}
+
+// 1 / (1 + exp(-v)) with the special-function exponential and reciprocal: a
+// few units in the last place of fp32 (0 from v = -87.3 down, where it is below
+// 2^-126), at a quarter of the instructions of expf and a division, which would
+// bound the 16-bit forms.
+template <int V>
+__device__ __forceinline__ void sigmoid(float (&o)[V], const float (&v)[V]) {
+  float k[V], one[V];
+  vset(k, -1.4426950408889634f);
+  vset(one, 1.f);
+  vmul(o, v, k);
+#pragma unroll
+  for (int i = 0; i < V; ++i) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(o[i]) : "f"(o[i]));
+  vadd(o, o, one);
+#pragma unroll
+  for (int i = 0; i < V; ++i) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(o[i]) : "f"(o[i]));
 }
 
 // Calls f with a value of the element type `dtype` names.

@@ -1,13 +1,14 @@
 """The plaintext Mamba-2 operators as torch functions: the state recurrence
 (``ssm_scan``, ``ssm_step``), the causal convolution (``causal_conv``,
-``causal_conv_step``) and token scoring (``token_logprobs``).
+``causal_conv_step``), the norms with their residual or gate (``rms_norm``,
+``add_rms_norm``, ``gated_rms_norm``) and token scoring (``token_logprobs``).
 
 They run on CUDA tensors through the C ABI (fhe_ssm_scan and the others in
 include/fhe_b200.h), on the current stream of the tensors' device, and can be
-captured into CUDA graphs; the scan, the convolution and the scores have
+captured into CUDA graphs; all but the steps have
 gradients (to capture a backward pass, hold no eager autograd graph of the same
 leaves: torch would make the capture wait for that graph's stream, and refuses).
-Activations are float32, bfloat16 or float16; gates, states and
+Activations are float32, bfloat16 or float16; gates, states, norm weights and
 scores are float32.  Arguments that do not fit raise ValueError before any GPU
 work.
 """
@@ -24,7 +25,7 @@ from . import _lib
 from ._lib import call
 
 _TYPES = {torch.float32: _lib.FHE_F32, torch.bfloat16: _lib.FHE_BF16, torch.float16: _lib.FHE_F16}
-MAX_HEAD_DIM, MAX_STATE, MAX_TAPS, MAX_TOP = 128, 256, 8, 64
+MAX_HEAD_DIM, MAX_STATE, MAX_TAPS, MAX_TOP, MAX_NORM_WIDTH = 128, 256, 8, 64, 16384
 
 
 def _need(ok, message):
@@ -376,6 +377,146 @@ def causal_conv_step(state, x, weight, bias=None, activation="silu", out=None):
                                                     activation == "silu", y, out)))
     increment_version(out)
     return y, out
+
+
+# ---- norms --------------------------------------------------------------------------------------
+
+
+def _rows(t):
+    """t as [rows, width] with a contiguous innermost axis (a view where its strides allow one)."""
+    return _inner(t if t.dim() == 2 else t.reshape(-1, t.shape[-1]))
+
+
+def _check_norm(op, x, weight, eps, others, dtype, groups=1):
+    _need(x.dim() >= 1 and x.shape[-1] >= 1, f"{op}: x must be [..., width]")
+    _need(x.dtype in _TYPES, f"{op}: x must be float32, bfloat16 or float16")
+    width = x.shape[-1]
+    _need(isinstance(groups, int) and groups >= 1 and width % groups == 0,
+          f"{op}: width ({width}) must be a multiple of groups ({groups})")
+    _need(width // groups <= MAX_NORM_WIDTH, f"{op}: at most {MAX_NORM_WIDTH} channels are normalised together")
+    _check(op, "weight", weight, (width,), torch.float32)
+    for name, t, types in others:
+        _need(t.shape == x.shape, f"{op}: {name} must have shape {tuple(x.shape)}, got {tuple(t.shape)}")
+        _need(t.dtype in types, f"{op}: {name} must be {' or '.join(str(v) for v in types)}, got {t.dtype}")
+    _need(dtype == x.dtype or (x.dtype == torch.float32 and dtype in _TYPES),
+          f"{op}: dtype must be x's, or a smaller one of a float32 x")
+    _need(0 < eps < float("inf"), f"{op}: eps must be positive")
+    _check_devices(op, x, weight, *(t for _, t, _ in others))
+
+
+def _norm_args(x, residual, gate, weight, channel_scale, eps, scale, groups, dtype, y, h, rstd):
+    """x, residual and gate as [rows, width]; x may be None in a backward pass that does not read it."""
+    first = x if x is not None else h
+    stream = h if h is not None else x
+    return _lib.RmsNormArgs(
+        first.device.index, _TYPES[dtype], _TYPES[stream.dtype] if gate is None else _TYPES[dtype],
+        first.shape[0], first.shape[1], groups, eps, scale,
+        _ptr(x), x.stride(0) if x is not None else 0, _ptr(residual), residual.stride(0) if residual is not None else 0,
+        _ptr(gate), gate.stride(0) if gate is not None else 0, _ptr(channel_scale), weight.data_ptr(),
+        _ptr(y), _ptr(h), _ptr(rstd), _stream_of(first.device.index))
+
+
+def _run_norm(x, residual, gate, weight, channel_scale, eps, scale, groups, dtype, grad):
+    d = x.device
+    y = torch.empty(x.shape, dtype=dtype, device=d)
+    h = torch.empty(x.shape, dtype=residual.dtype, device=d) if residual is not None else None
+    x2, r2, g2 = _rows(x), None if residual is None else _rows(residual), None if gate is None else _rows(gate)
+    rstd = torch.empty((x2.shape[0], groups), dtype=torch.float32, device=d) if grad else None
+    a = _norm_args(x2, r2, g2, weight, channel_scale, eps, scale, groups, dtype, y, None, rstd)
+    if h is not None:
+        a.h, a.stream_dtype = h.data_ptr(), _TYPES[h.dtype]
+    call("fhe_rms_norm", ctypes.byref(a))
+    return y, h, rstd
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, gate, weight, channel_scale, eps, scale, groups, dtype):
+        y, h, rstd = _run_norm(x, residual, gate, weight, channel_scale, eps, scale, groups, dtype, True)
+        ctx.set_materialize_grads(False)
+        ctx.rest = eps, scale, groups, dtype, x.dtype
+        ctx.save_for_backward(x if residual is None or channel_scale is not None else None, gate, weight,
+                              channel_scale, h, rstd)
+        return y if h is None else (y, h)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh=None):
+        x, gate, weight, channel_scale, h, rstd = ctx.saved_tensors
+        eps, scale, groups, dtype, x_dtype = ctx.rest
+        like = x if x is not None else h
+        new = lambda shape, t: torch.empty(shape, dtype=t, device=like.device)  # noqa: E731
+        wants = ctx.needs_input_grad
+        dy = torch.zeros(like.shape, dtype=dtype, device=like.device) if dy is None else dy.contiguous()
+        dh = None if dh is None else dh.contiguous()
+        # a branch added as it is has the stream's own gradient
+        shared = h is not None and channel_scale is None and scale == 1.0 and x_dtype == h.dtype
+        dres = new(like.shape, h.dtype) if h is not None and (wants[1] or (shared and wants[0])) else None
+        dx = new(like.shape, x_dtype) if wants[0] and not shared else None
+        dgate = new(like.shape, dtype) if gate is not None and wants[2] else None
+        dw = new(weight.shape, torch.float32) if wants[3] else None
+        dcs = new(weight.shape, torch.float32) if channel_scale is not None and wants[4] else None
+        x2, g2, h2 = (None if t is None else _rows(t) for t in (x, gate, h))
+        f = _norm_args(x2, h2, g2, weight, channel_scale, eps, scale, groups, dtype, None, h2, rstd)
+        g = _lib.RmsNormGradArgs(f, dy.data_ptr(), _ptr(dh), _ptr(dx), _ptr(dres), _ptr(dgate), _ptr(dw), _ptr(dcs),
+                                 None, 0, f.stream)
+        ws = _workspace("fhe_rms_norm_backward_workspace", g, like.device)
+        if ws is not None:
+            g.workspace, g.workspace_bytes = ws.data_ptr(), ws.numel()
+        call("fhe_rms_norm_backward", ctypes.byref(g))
+        return dres if shared else dx, dres if wants[1] else None, dgate, dw, dcs, None, None, None, None
+
+
+def rms_norm(x, weight, eps=1e-5, dtype=None):
+    """x / sqrt(mean(x^2) + eps) weight over the last axis.
+
+    x [..., width] float32, bfloat16 or float16, width at most 16384; weight
+    [width] float32.  The result has x's type, or the 16-bit `dtype` if x is
+    float32.  Only the last axis must be contiguous and the others evenly spaced
+    (a slice of wider rows will do), else x is copied.  Sums are float32; rows
+    whose squares pass its range are scaled.  Gradients reach x and weight."""
+    dtype = dtype or x.dtype
+    _check_norm("rms_norm", x, weight, eps, (), dtype)
+    args = (x, None, None, _dense(weight), None, float(eps), 1.0, 1, dtype)
+    if _wants_grad(x, weight):
+        return _RmsNorm.apply(*args)
+    return _run_norm(*args, False)[0]
+
+
+def add_rms_norm(residual, x, weight, eps=1e-5, scale=1.0):
+    """A residual stream's next value and its norm: h = residual + scale x, kept
+    in residual's type, and y = h / sqrt(mean(h^2) + eps) weight in x's type, the
+    norm of h as it is kept.
+
+    residual [..., width] of x's type or float32; x and weight as in ``rms_norm``;
+    scale a number, or [width] float32 for a factor of each channel.  Returns
+    (y, h).  Gradients reach every tensor."""
+    op = "add_rms_norm"
+    _check_norm(op, x, weight, eps, (("residual", residual, (x.dtype, torch.float32)),), x.dtype)
+    channel_scale, factor = None, scale
+    if torch.is_tensor(scale):
+        _check(op, "scale", scale, weight.shape, torch.float32)
+        _check_devices(op, x, scale)
+        channel_scale, factor = _dense(scale), 1.0
+    _need(abs(float(factor)) < float("inf"), f"{op}: scale must be finite")
+    args = (x, residual, None, _dense(weight), channel_scale, float(eps), float(factor), 1, x.dtype)
+    if _wants_grad(x, residual, weight, channel_scale):
+        return _RmsNorm.apply(*args)
+    return _run_norm(*args, False)[:2]
+
+
+def gated_rms_norm(x, gate, weight, eps=1e-5, groups=1):
+    """The norm behind the recurrence: u = x SiLU(gate), then u / sqrt(mean(u^2) +
+    eps) weight with the mean over each of `groups` equal parts of the last axis.
+
+    x and gate [..., width] of one type, gate usually a slice of the layer's wider
+    projection; weight [width] float32; a part has at most 16384 channels.
+    Products x SiLU(gate) must fit float32.  Gradients reach every tensor."""
+    _check_norm("gated_rms_norm", x, weight, eps, (("gate", gate, (x.dtype,)),), x.dtype, groups)
+    args = (x, None, gate, _dense(weight), None, float(eps), 1.0, groups, x.dtype)
+    if _wants_grad(x, gate, weight):
+        return _RmsNorm.apply(*args)
+    return _run_norm(*args, False)[0]
 
 
 # ---- token scores -------------------------------------------------------------------------------

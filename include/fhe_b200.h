@@ -661,6 +661,54 @@ typedef struct fhe_token_logprobs_grad_args {
 } fhe_token_logprobs_grad_args;
 int fhe_token_logprobs_backward(const fhe_token_logprobs_grad_args* args);
 
+/* Root-mean-square norm of rows, in one of three forms:
+ *   h = x                                          (neither residual nor gate)
+ *   h = residual + scale x, stored in stream_dtype (residual)
+ *   h = x SiLU(gate)                               (gate)
+ *   y = h / sqrt(mean(h^2) + eps) weight, the mean over each of `groups` equal
+ * parts of the row (groups = 1 without a gate).  The norm is that of h as it is
+ * stored; sums run in fp32.  Without a gate stream_dtype is dtype or FHE_F32 and
+ * is the type of residual, h, and of x when there is no residual; everything
+ * else has `dtype`.  A group has at most 16384 channels.  y and h may be x's,
+ * residual's or gate's memory where rows and types agree. */
+typedef struct fhe_rms_norm_args {
+  int32_t device, dtype, stream_dtype;
+  uint32_t rows, width, groups;
+  float eps, scale;
+  const void* x;              /* [rows][width] */
+  int64_t x_stride;           /* between rows, as the other strides */
+  const void* residual;       /* [rows][width], or NULL */
+  int64_t residual_stride;
+  const void* gate;           /* [rows][width], or NULL */
+  int64_t gate_stride;
+  const float* channel_scale; /* [width], multiplies scale, or NULL (only with a residual) */
+  const float* weight;        /* [width] */
+  void* y;                    /* [rows][width], contiguous */
+  void* h;                    /* [rows][width], contiguous; only with a residual */
+  float* rstd;                /* [rows][groups]: 1 / sqrt(mean + eps), or NULL */
+  void* stream;
+} fhe_rms_norm_args;
+int fhe_rms_norm(const fhe_rms_norm_args* args);
+
+/* Gradients of fhe_rms_norm.  `f` holds the forward call's inputs with its h
+ * (only with a residual) and rstd as inputs; its y is not used.  Every output
+ * may be NULL where it is not wanted; sums over rows run in a fixed order. */
+typedef struct fhe_rms_norm_grad_args {
+  fhe_rms_norm_args f;
+  const void* dy;             /* [rows][width], dtype, contiguous */
+  const void* dh;             /* [rows][width], stream_dtype, contiguous, or NULL for zeros (only with a residual) */
+  void* dx;                   /* [rows][width], x's type */
+  void* dresidual;            /* [rows][width], stream_dtype (only with a residual) */
+  void* dgate;                /* [rows][width] (only with a gate) */
+  float* dweight;             /* [width] */
+  float* dchannel_scale;      /* [width] (only with channel_scale) */
+  void* workspace;
+  uint64_t workspace_bytes;
+  void* stream;
+} fhe_rms_norm_grad_args;
+int fhe_rms_norm_backward_workspace(const fhe_rms_norm_grad_args* args, uint64_t* bytes);
+int fhe_rms_norm_backward(const fhe_rms_norm_grad_args* args);
+
 #ifdef __cplusplus
 }
 #endif

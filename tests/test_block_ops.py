@@ -1,0 +1,104 @@
+"""Refused arguments of the operators around the layers (norms, embedding,
+beams), of the Python functions and of the C entry points: none of them reaches
+a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+from fhe_mamba_b200 import _lib, mamba_ops as ops
+
+F16, BF16, F32, F64 = torch.float16, torch.bfloat16, torch.float32, torch.float64
+z = torch.zeros
+
+
+@pytest.mark.parametrize("args, message", [
+    ((z(()), z(1)), "width"),
+    ((z(2, 0), z(0)), "width"),
+    ((z(2, 4, dtype=F64), z(4)), "float32, bfloat16 or float16"),
+    ((z(2, 4), z(5)), "weight must have shape"),
+    ((z(2, 4), z(4, dtype=BF16)), "weight must be"),
+    ((z(1, 16385), z(16385)), "at most 16384"),
+    ((z(2, 4), z(4), 0.0), "eps"),
+    ((z(2, 4), z(4), float("nan")), "eps"),
+    ((z(2, 4), z(4), 1e-5, F64), "dtype"),
+    ((z(2, 4, dtype=BF16), z(4), 1e-5, F32), "dtype"),
+    ((z(2, 4), z(4)), "CUDA tensors expected"),
+])
+def test_norm_refusals(args, message):
+    with pytest.raises(ValueError, match=message):
+        ops.rms_norm(*args)
+
+
+@pytest.mark.parametrize("args, message", [
+    ((z(2, 5), z(2, 4), z(4)), "residual must have shape"),
+    ((z(4), z(2, 4), z(4)), "residual must have shape"),
+    ((z(2, 4, dtype=F16), z(2, 4, dtype=BF16), z(4)), "residual must be"),
+    ((z(2, 4, dtype=F16), z(2, 4), z(4)), "residual must be"),
+    ((z(2, 4), z(2, 4), z(4), 1e-5, z(5)), "scale must have shape"),
+    ((z(2, 4), z(2, 4), z(4), 1e-5, z(())), "scale must have shape"),
+    ((z(2, 4), z(2, 4), z(4), 1e-5, z(4, dtype=BF16)), "scale must be"),
+    ((z(2, 4), z(2, 4), z(4), 1e-5, float("inf")), "scale must be finite"),
+    ((z(2, 4), z(2, 4), z(4)), "CUDA tensors expected"),
+])
+def test_add_norm_refusals(args, message):
+    with pytest.raises(ValueError, match=message):
+        ops.add_rms_norm(*args)
+
+
+@pytest.mark.parametrize("args, message", [
+    ((z(2, 4), z(2, 5), z(4)), "gate must have shape"),
+    ((z(2, 4), z(2, 4, dtype=BF16), z(4)), "gate must be"),
+    ((z(2, 4), z(2, 4), z(4), 1e-5, 3), "multiple of groups"),
+    ((z(2, 4), z(2, 4), z(4), 1e-5, 0), "multiple of groups"),
+    ((z(1, 32770), z(1, 32770), z(32770), 1e-5, 2), "at most 16384"),
+    ((z(2, 4), z(2, 4), z(4)), "CUDA tensors expected"),
+])
+def test_gated_norm_refusals(args, message):
+    with pytest.raises(ValueError, match=message):
+        ops.gated_rms_norm(*args)
+
+
+def norm_struct(**kw):
+    """A C argument block whose pointers are never followed: each call below is refused before."""
+    s = dict(dtype=0, stream_dtype=0, rows=2, width=8, groups=1, eps=1e-5, scale=1.0, x=256, weight=256, y=256)
+    s.update(kw)
+    return _lib.RmsNormArgs(**s)
+
+
+@pytest.mark.parametrize("kw, message", [
+    (dict(dtype=7), "dtype"), (dict(dtype=1, stream_dtype=2), "stream_dtype"), (dict(gate=256, residual=256), "not both"),
+    (dict(gate=256, groups=3), "multiple of groups"), (dict(gate=256, groups=0), "multiple of groups"),
+    (dict(width=0), "multiple of groups"), (dict(groups=2), "groups need a gate"), (dict(width=16385), "16384"),
+    (dict(eps=0.0), "eps"), (dict(channel_scale=256), "channel_scale needs"), (dict(scale=float("inf")), "scale"),
+    (dict(rows=1 << 31), "too large"), (dict(gate=256, width=1 << 16, groups=1 << 16), "too large"),
+    (dict(x=None), "null"), (dict(y=None), "null"), (dict(weight=None), "null"), (dict(residual=256), "null"),
+])
+def test_norm_c_refusals(kw, message):
+    lib = _lib.load()
+    assert lib.fhe_rms_norm(ctypes.byref(norm_struct(**kw))) == _lib.FHE_ERR_INVALID
+    assert message in _lib.last_error()
+
+
+def test_norm_backward_c_refusals():
+    lib = _lib.load()
+    n = ctypes.c_uint64()
+
+    def refused(message, f, **kw):
+        g = _lib.RmsNormGradArgs(f=f, **kw)
+        assert lib.fhe_rms_norm_backward(ctypes.byref(g)) == _lib.FHE_ERR_INVALID and message in _lib.last_error()
+        return g
+    refused("null", norm_struct(), dy=256, dx=256)
+    refused("null", norm_struct(rstd=256), dx=256)
+    refused("null", norm_struct(rstd=256, residual=256), dy=256, dx=256)
+    refused("null", norm_struct(rstd=256, residual=256, h=256, channel_scale=256, x=None), dy=256, dx=256)
+    refused("dgate", norm_struct(rstd=256), dy=256, dgate=256)
+    refused("residual", norm_struct(rstd=256), dy=256, dresidual=256)
+    refused("residual", norm_struct(rstd=256), dy=256, dh=256)
+    refused("channel_scale", norm_struct(rstd=256), dy=256, dchannel_scale=256)
+    g = refused("workspace too small", norm_struct(rstd=256), dy=256, dweight=256)
+    assert lib.fhe_rms_norm_backward_workspace(ctypes.byref(g), ctypes.byref(n)) == 0 and n.value >= 32
+    refused("aligned", norm_struct(rstd=256), dy=256, dweight=256, workspace=257, workspace_bytes=1 << 30)
+    for name in ("fhe_rms_norm", "fhe_rms_norm_backward", "fhe_rms_norm_backward_workspace"):
+        args = (None,) if name != "fhe_rms_norm_backward_workspace" else (None, None)
+        assert getattr(lib, name)(*args) == _lib.FHE_ERR_INVALID and "null" in _lib.last_error()
