@@ -387,7 +387,7 @@ def _rows(t):
     return _inner(t if t.dim() == 2 else t.reshape(-1, t.shape[-1]))
 
 
-def _check_norm(op, x, weight, eps, others, dtype, groups=1):
+def _check_norm(op, x, weight, eps, others, dtype, groups=1, scale=1.0):
     _need(x.dim() >= 1 and x.shape[-1] >= 1, f"{op}: x must be [..., width]")
     _need(x.dtype in _TYPES, f"{op}: x must be float32, bfloat16 or float16")
     width = x.shape[-1]
@@ -401,7 +401,11 @@ def _check_norm(op, x, weight, eps, others, dtype, groups=1):
     _need(dtype == x.dtype or (x.dtype == torch.float32 and dtype in _TYPES),
           f"{op}: dtype must be x's, or a smaller one of a float32 x")
     _need(0 < eps < float("inf"), f"{op}: eps must be positive")
-    _check_devices(op, x, weight, *(t for _, t, _ in others))
+    if torch.is_tensor(scale):
+        _check(op, "scale", scale, (width,), torch.float32)
+    else:
+        _need(abs(scale) < float("inf"), f"{op}: scale must be finite")
+    _check_devices(op, x, weight, scale if torch.is_tensor(scale) else None, *(t for _, t, _ in others))
 
 
 def _norm_args(x, residual, gate, weight, channel_scale, eps, scale, groups, dtype, y, h, rstd):
@@ -492,13 +496,8 @@ def add_rms_norm(residual, x, weight, eps=1e-5, scale=1.0):
     scale a number, or [width] float32 for a factor of each channel.  Returns
     (y, h).  Gradients reach every tensor."""
     op = "add_rms_norm"
-    _check_norm(op, x, weight, eps, (("residual", residual, (x.dtype, torch.float32)),), x.dtype)
-    channel_scale, factor = None, scale
-    if torch.is_tensor(scale):
-        _check(op, "scale", scale, weight.shape, torch.float32)
-        _check_devices(op, x, scale)
-        channel_scale, factor = _dense(scale), 1.0
-    _need(abs(float(factor)) < float("inf"), f"{op}: scale must be finite")
+    _check_norm(op, x, weight, eps, (("residual", residual, (x.dtype, torch.float32)),), x.dtype, scale=scale)
+    channel_scale, factor = (_dense(scale), 1.0) if torch.is_tensor(scale) else (None, scale)
     args = (x, residual, None, _dense(weight), channel_scale, float(eps), float(factor), 1, x.dtype)
     if _wants_grad(x, residual, weight, channel_scale):
         return _RmsNorm.apply(*args)
