@@ -140,6 +140,20 @@ class RmsNormGradArgs(ctypes.Structure):
     ]
 
 
+class EmbeddingArgs(ctypes.Structure):
+    _fields_ = [
+        ("device", i32), ("dtype", i32), ("out_dtype", i32), ("wide_ids", i32),
+        ("count", u32), ("vocab", u32), ("width", u32), ("scale", ctypes.c_float),
+        ("ids", vp), ("table", vp), ("table_stride", i64), ("out", vp), ("stream", vp),
+    ]
+
+
+class EmbeddingGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("f", EmbeddingArgs), ("dout", vp), ("dtable", vp), ("workspace", vp), ("workspace_bytes", u64), ("stream", vp),
+    ]
+
+
 # name -> (argtypes); all return int status.
 SIGNATURES = {
     "fhe_last_error": [ctypes.c_char_p, ctypes.c_size_t],
@@ -248,6 +262,9 @@ SIGNATURES = {
     "fhe_rms_norm": [ctypes.POINTER(RmsNormArgs)],
     "fhe_rms_norm_backward_workspace": [ctypes.POINTER(RmsNormGradArgs), P64],
     "fhe_rms_norm_backward": [ctypes.POINTER(RmsNormGradArgs)],
+    "fhe_embedding": [ctypes.POINTER(EmbeddingArgs)],
+    "fhe_embedding_backward_workspace": [ctypes.POINTER(EmbeddingGradArgs), P64],
+    "fhe_embedding_backward": [ctypes.POINTER(EmbeddingGradArgs)],
 }
 
 _lock = threading.Lock()

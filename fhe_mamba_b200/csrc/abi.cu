@@ -1315,4 +1315,25 @@ int fhe_rms_norm_backward(const fhe_rms_norm_grad_args* args) {
   });
 }
 
+int fhe_embedding(const fhe_embedding_args* args) {
+  return guarded([&] {
+    fhe::require(args != nullptr, "null argument");
+    fhe::embedding(*args);
+  });
+}
+
+int fhe_embedding_backward_workspace(const fhe_embedding_grad_args* args, uint64_t* bytes) {
+  return guarded([&] {
+    fhe::require(args != nullptr && bytes != nullptr, "null argument");
+    *bytes = fhe::embedding_backward_workspace(*args);
+  });
+}
+
+int fhe_embedding_backward(const fhe_embedding_grad_args* args) {
+  return guarded([&] {
+    fhe::require(args != nullptr, "null argument");
+    fhe::embedding_backward(*args);
+  });
+}
+
 }  // extern "C"

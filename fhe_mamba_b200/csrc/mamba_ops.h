@@ -24,6 +24,9 @@ void token_logprobs_backward(const fhe_token_logprobs_grad_args& g);
 void rms_norm(const fhe_rms_norm_args& a);
 uint64_t rms_norm_backward_workspace(const fhe_rms_norm_grad_args& g);
 void rms_norm_backward(const fhe_rms_norm_grad_args& g);
+void embedding(const fhe_embedding_args& a);
+uint64_t embedding_backward_workspace(const fhe_embedding_grad_args& g);
+void embedding_backward(const fhe_embedding_grad_args& g);
 
 // Makes `device` current and restores the caller's device on destruction.
 class DeviceGuard {

@@ -1,7 +1,8 @@
 """The plaintext Mamba-2 operators as torch functions: the state recurrence
 (``ssm_scan``, ``ssm_step``), the causal convolution (``causal_conv``,
 ``causal_conv_step``), the norms with their residual or gate (``rms_norm``,
-``add_rms_norm``, ``gated_rms_norm``) and token scoring (``token_logprobs``).
+``add_rms_norm``, ``gated_rms_norm``), the token embedding (``embedding``) and
+token scoring (``token_logprobs``).
 
 They run on CUDA tensors through the C ABI (fhe_ssm_scan and the others in
 include/fhe_b200.h), on the current stream of the tensors' device, and can be
@@ -516,6 +517,66 @@ def gated_rms_norm(x, gate, weight, eps=1e-5, groups=1):
     if _wants_grad(x, gate, weight):
         return _RmsNorm.apply(*args)
     return _run_norm(*args, False)[0]
+
+
+# ---- embedding ----------------------------------------------------------------------------------
+
+
+def _embedding_args(tokens, weight, scale, dtype, out):
+    return _lib.EmbeddingArgs(
+        weight.device.index, _TYPES[weight.dtype], _TYPES[dtype], tokens.dtype == torch.int64, tokens.numel(),
+        weight.shape[0], weight.shape[1], scale, tokens.data_ptr(), weight.data_ptr(), weight.stride(0), _ptr(out),
+        _stream_of(weight.device.index))
+
+
+def _run_embedding(tokens, weight, scale, dtype):
+    out = torch.empty((*tokens.shape, weight.shape[1]), dtype=dtype, device=weight.device)
+    call("fhe_embedding", ctypes.byref(_embedding_args(tokens, weight, scale, dtype, out)))
+    return out
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, tokens, scale, dtype):
+        ctx.rest = scale, dtype
+        ctx.save_for_backward(weight, tokens)
+        return _run_embedding(tokens, weight, scale, dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        weight, tokens = ctx.saved_tensors
+        dout = dout.contiguous()
+        dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
+        g = _lib.EmbeddingGradArgs(_embedding_args(tokens, weight, *ctx.rest, None), dout.data_ptr(), dw.data_ptr(),
+                                   None, 0, _stream_of(weight.device.index))
+        ws = _workspace("fhe_embedding_backward_workspace", g, weight.device)
+        if ws is not None:
+            g.workspace, g.workspace_bytes = ws.data_ptr(), ws.numel()
+        call("fhe_embedding_backward", ctypes.byref(g))
+        return dw, None, None, None
+
+
+def embedding(tokens, weight, scale=1.0, dtype=None):
+    """scale weight[tokens], rounded once.
+
+    tokens [...] int64 or int32, negative for a position without a token (0, no
+    gradient); a token past the vocabulary gives NaN and has no gradient.
+    weight [vocab, width] float32, bfloat16 or float16; the result [..., width]
+    has its type, or `dtype` float32.  The gradient is that of every row of
+    weight, summed in float32 over the row's positions in their order."""
+    op, dtype = "embedding", dtype or weight.dtype
+    _need(tokens.dtype in (torch.int64, torch.int32), f"{op}: tokens must be int64 or int32, got {tokens.dtype}")
+    _need(weight.dim() == 2 and weight.dtype in _TYPES and weight.shape[1] >= 1,
+          f"{op}: weight must be [vocab, width] float32, bfloat16 or float16")
+    _need(weight.shape[1] <= 1 << 20, f"{op}: width must be at most 2^20")
+    _need(dtype in (weight.dtype, torch.float32), f"{op}: dtype must be weight's or float32")
+    _need(abs(scale) < float("inf"), f"{op}: scale must be finite")
+    _check_devices(op, weight, tokens)
+    tokens, rows = _dense(tokens), _inner(weight)
+    if _wants_grad(weight):
+        return _Embedding.apply(rows, tokens, float(scale), dtype)
+    return _run_embedding(tokens, rows, float(scale), dtype)
 
 
 # ---- token scores -------------------------------------------------------------------------------

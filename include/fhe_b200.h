@@ -709,6 +709,38 @@ typedef struct fhe_rms_norm_grad_args {
 int fhe_rms_norm_backward_workspace(const fhe_rms_norm_grad_args* args, uint64_t* bytes);
 int fhe_rms_norm_backward(const fhe_rms_norm_grad_args* args);
 
+/* Rows of a table by token, times scale: out[i] = scale table[ids[i]], rounded
+ * once.  A negative id is a position without a token (0), an id >= vocab gives
+ * NaN. */
+typedef struct fhe_embedding_args {
+  int32_t device, dtype;
+  int32_t out_dtype;          /* dtype or FHE_F32 */
+  int32_t wide_ids;           /* ids are int64_t, else int32_t */
+  uint32_t count, vocab, width;
+  float scale;
+  const void* ids;            /* [count] */
+  const void* table;          /* [vocab][width], dtype */
+  int64_t table_stride;       /* between rows */
+  void* out;                  /* [count][width], out_dtype, contiguous */
+  void* stream;
+} fhe_embedding_args;
+int fhe_embedding(const fhe_embedding_args* args);
+
+/* dtable[v] = scale times the sum of dout over the positions of token v, 0 for
+ * tokens without one: summed in fp32 in a fixed order, rounded once, the whole
+ * table written.  Positions without a token or past the vocabulary pass
+ * nothing.  `f` as in the forward call (its table and out are not used). */
+typedef struct fhe_embedding_grad_args {
+  fhe_embedding_args f;
+  const void* dout;           /* [count][width], out_dtype, contiguous */
+  void* dtable;               /* [vocab][width], dtype, contiguous */
+  void* workspace;
+  uint64_t workspace_bytes;
+  void* stream;
+} fhe_embedding_grad_args;
+int fhe_embedding_backward_workspace(const fhe_embedding_grad_args* args, uint64_t* bytes);
+int fhe_embedding_backward(const fhe_embedding_grad_args* args);
+
 #ifdef __cplusplus
 }
 #endif

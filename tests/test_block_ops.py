@@ -102,3 +102,48 @@ def test_norm_backward_c_refusals():
     for name in ("fhe_rms_norm", "fhe_rms_norm_backward", "fhe_rms_norm_backward_workspace"):
         args = (None,) if name != "fhe_rms_norm_backward_workspace" else (None, None)
         assert getattr(lib, name)(*args) == _lib.FHE_ERR_INVALID and "null" in _lib.last_error()
+
+
+I64 = torch.int64
+
+
+@pytest.mark.parametrize("args, message", [
+    ((z(3), z(5, 4)), "tokens must be"),
+    ((z(3, dtype=torch.int16), z(5, 4)), "tokens must be"),
+    ((z(3, dtype=I64), z(5)), "weight must be"),
+    ((z(3, dtype=I64), z(5, 0)), "weight must be"),
+    ((z(3, dtype=I64), z(5, 4, dtype=F64)), "weight must be"),
+    ((z(3, dtype=I64), z(1, (1 << 20) + 1)), "width"),
+    ((z(3, dtype=I64), z(5, 4), 1.0, BF16), "dtype"),
+    ((z(3, dtype=I64), z(5, 4, dtype=F16), 1.0, BF16), "dtype"),
+    ((z(3, dtype=I64), z(5, 4), float("nan")), "scale"),
+    ((z(3, dtype=I64), z(5, 4)), "CUDA tensors expected"),
+])
+def test_embedding_refusals(args, message):
+    with pytest.raises(ValueError, match=message):
+        ops.embedding(*args)
+
+
+@pytest.mark.parametrize("kw, message", [
+    (dict(dtype=9), "dtype"), (dict(dtype=1, out_dtype=2), "out_dtype"), (dict(count=1 << 31), "2^31"),
+    (dict(vocab=1 << 31), "2^31"), (dict(width=0), "width"), (dict(width=(1 << 20) + 1), "width"),
+    (dict(scale=float("inf")), "scale"), (dict(ids=None), "null"), (dict(table=None), "null"), (dict(out=None), "null"),
+])
+def test_embedding_c_refusals(kw, message):
+    lib = _lib.load()
+    base = dict(dtype=0, out_dtype=0, count=4, vocab=5, width=8, scale=1.0, ids=256, table=256, table_stride=8, out=256)
+    a = _lib.EmbeddingArgs(**{**base, **kw})
+    assert lib.fhe_embedding(ctypes.byref(a)) == _lib.FHE_ERR_INVALID and message in _lib.last_error()
+
+
+def test_embedding_backward_c_refusals():
+    lib = _lib.load()
+    f = _lib.EmbeddingArgs(dtype=0, out_dtype=0, count=4, vocab=5, width=8, scale=1.0, ids=256)
+    for kw, message in ((dict(dtable=256), "null input"), (dict(dout=256), "null output"),
+                        (dict(dout=256, dtable=256), "workspace too small"),
+                        (dict(dout=256, dtable=256, workspace=257, workspace_bytes=1 << 30), "aligned")):
+        g = _lib.EmbeddingGradArgs(f=f, **kw)
+        assert lib.fhe_embedding_backward(ctypes.byref(g)) == _lib.FHE_ERR_INVALID and message in _lib.last_error()
+    n = ctypes.c_uint64()
+    assert lib.fhe_embedding_backward_workspace(ctypes.byref(g), ctypes.byref(n)) == 0 and n.value >= 32
+    assert lib.fhe_embedding(None) == lib.fhe_embedding_backward(None) == _lib.FHE_ERR_INVALID
