@@ -154,6 +154,22 @@ class EmbeddingGradArgs(ctypes.Structure):
     ]
 
 
+class BeamSelectArgs(ctypes.Structure):
+    _fields_ = [
+        ("device", i32), ("dtype", i32), ("batch", u32), ("beams", u32), ("vocab", u32), ("width", u32),
+        ("keep_slots", i32), ("reserved", u32),
+        ("logits", vp), ("logits_stride", i64), ("scores", vp), ("finished", vp), ("eos", i64),
+        ("out_scores", vp), ("parents", vp), ("tokens", vp), ("out_finished", vp), ("stream", vp),
+    ]
+
+
+class BeamReorderArgs(ctypes.Structure):
+    _fields_ = [
+        ("device", i32), ("batch", u32), ("beams", u32), ("count", u32),
+        ("states", ctypes.POINTER(vp)), ("row_bytes", P64), ("parents", vp), ("stream", vp),
+    ]
+
+
 # name -> (argtypes); all return int status.
 SIGNATURES = {
     "fhe_last_error": [ctypes.c_char_p, ctypes.c_size_t],
@@ -265,6 +281,8 @@ SIGNATURES = {
     "fhe_embedding": [ctypes.POINTER(EmbeddingArgs)],
     "fhe_embedding_backward_workspace": [ctypes.POINTER(EmbeddingGradArgs), P64],
     "fhe_embedding_backward": [ctypes.POINTER(EmbeddingGradArgs)],
+    "fhe_beam_select": [ctypes.POINTER(BeamSelectArgs)],
+    "fhe_beam_reorder": [ctypes.POINTER(BeamReorderArgs)],
 }
 
 _lock = threading.Lock()

@@ -1336,4 +1336,18 @@ int fhe_embedding_backward(const fhe_embedding_grad_args* args) {
   });
 }
 
+int fhe_beam_select(const fhe_beam_select_args* args) {
+  return guarded([&] {
+    fhe::require(args != nullptr, "null argument");
+    fhe::beam_select(*args);
+  });
+}
+
+int fhe_beam_reorder(const fhe_beam_reorder_args* args) {
+  return guarded([&] {
+    fhe::require(args != nullptr, "null argument");
+    fhe::beam_reorder(*args);
+  });
+}
+
 }  // extern "C"

@@ -1,0 +1,554 @@
+// Beam search's selection (fhe_beam_select): the `width` best of score_i + z_iv -
+// log sum exp z_i over the beams i and tokens v of each batch item.
+//
+// A cluster of up to eight CTAs takes a batch item, a row or a share of a row to a
+// CTA at a time, in one read: sums of exp(z - m) around a running shift m, and the
+// share's best entries (a lower bound from its first loads, then only the loads that
+// reach it, ranked by counting).  The first CTA puts the shares together over
+// distributed shared memory and ranks them.  Within a beam the order is that of the
+// logits; between beams it hangs on the beams' sums, which fp32 knows to a few
+// 2^-20.  Where neighbours of different beams among the best lie closer than that,
+// the cluster sums those beams again in 64 bits, so that the choice is always that of
+// the formula.  The read bounds it.
+#include <algorithm>
+#include <cfloat>
+#include <cooperative_groups.h>
+
+#include "launch_count.h"
+#include "logit_rows.h"
+
+namespace fhe {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kGroups = 64;   // groups of 4 threads
+constexpr int kAhead = 4;     // 16-byte loads in flight per thread
+constexpr int kCap = 1024;    // candidates held
+constexpr int kHits = 512;    // turns of a thread that hold candidates
+constexpr uint32_t kMaxBeams = 64, kMaxWidth = 64, kMaxCluster = 8;
+static_assert(kMaxWidth <= kGroups, "the bound is the width-th of the groups' maxima");
+
+// One share of a row: sum of exp(z - m), and its best entries in order.
+struct Share {
+  double s;
+  float m;
+  uint32_t raises, count, pad;
+};
+
+// Dynamic shared memory: this CTA's shares, and (first CTA) every share's entries.
+struct Layout {
+  Share* share;
+  uint32_t *key, *idx;
+  double* total;
+  uint32_t *lkey, *lidx;
+  uint32_t bytes;
+  __host__ __device__ Layout(uint8_t* p, uint32_t slots, uint32_t lists, uint32_t kk) {
+    uint8_t* at = p;
+    auto take = [&](uint32_t n) {
+      uint8_t* r = at;
+      at += (n + 15) / 16 * 16;
+      return r;
+    };
+    share = reinterpret_cast<Share*>(take(slots * sizeof(Share)));
+    total = reinterpret_cast<double*>(take(lists * kk * 8));
+    key = reinterpret_cast<uint32_t*>(take(slots * kk * 4));
+    idx = reinterpret_cast<uint32_t*>(take(slots * kk * 4));
+    lkey = reinterpret_cast<uint32_t*>(take(lists * kk * 4));
+    lidx = reinterpret_cast<uint32_t*>(take(lists * kk * 4));
+    bytes = (uint32_t)(at - p);
+  }
+};
+
+struct SelectArgs {
+  fhe_beam_select_args a;
+  uint32_t cluster, kk;  // CTAs per item; entries of a row that count
+};
+
+// exp(z - m) summed over the elements of a load, m finite.
+template <class T>
+__device__ __forceinline__ uint64_t add_exps(const Quad<T>& q, uint64_t acc, uint64_t minus_m) {
+  using Q = Quad<T>;
+  const uint64_t k = pair(kLog2e, kLog2e);
+#pragma unroll
+  for (int i = 0; i < Q::kElems / 2; ++i) {
+    float f[2];
+    if constexpr (Q::kPer == 2) {
+      Q::floats(q.w[i], f);
+    } else {
+      f[0] = __uint_as_float(q.w[2 * i]);
+      f[1] = __uint_as_float(q.w[2 * i + 1]);
+    }
+    float d0, d1;
+    unpair(mul2(add2(pair(f[0], f[1]), minus_m), k), d0, d1);
+    acc = add2(acc, pair(exp2_fast(d0), exp2_fast(d1)));
+  }
+  return acc;
+}
+
+struct Scratch {
+  float fred[kWarps];
+  double dred[kWarps];
+  __align__(16) uint32_t gmax[kGroups];
+  uint32_t ckey[kCap], cidx[kCap], hit[kHits];
+  uint32_t hits, bound, count, raises;
+};
+
+__device__ __forceinline__ double block_sum(double v, double (&red)[kWarps]) {
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.;
+  for (int i = 0; i < kWarps; ++i) v += red[i];
+  return v;
+}
+
+// Share `part` of `parts` of the row z: 16-byte words between the row's first and
+// last 16-byte boundaries; the elements before and after go with the first share.
+template <class T>
+__device__ void scan_share(const T* z, uint32_t vocab, uint32_t part, uint32_t parts, uint32_t k, Scratch& sm, Share& out,
+                           uint32_t* key_out, uint32_t* idx_out) {
+  using Q = Quad<T>;
+  constexpr uint32_t V = Q::kElems;
+  const uint32_t tid = threadIdx.x;
+  const uint32_t head = min(vocab, (uint32_t)((0 - reinterpret_cast<uintptr_t>(z)) % 16 / sizeof(T)));
+  const T* body = z + head;
+  const uint32_t all = (vocab - head) / V, loose = part == 0 ? vocab - all * V : 0;
+  const uint32_t each = (all + parts - 1) / parts, first = min(part * each, all), packs = min(first + each, all);
+  const uint32_t mine = (packs - first) * V + loose;  // elements of this share
+  __syncthreads();
+  if (tid == 0) sm.hits = sm.count = sm.raises = 0;
+  __syncthreads();
+  float m = -INFINITY;
+  double s = 0.;
+  uint32_t raises = 0;
+  auto raise = [&](float top) {  // rare: the sum so far moves to a new shift
+    s *= m == -INFINITY ? 0.f : exp2_fast((m - top) * kLog2e);
+    m = top;
+    ++raises;
+  };
+  auto shift = [&] {
+    const float v = -fmaxf(m, -FLT_MAX);
+    return pair(v, v);
+  };
+  constexpr float kSlack = 4.f;  // a sum may hold terms up to e^4 before its shift moves
+  float fbnd = -INFINITY;
+  Q p[kAhead], next[kAhead];
+  auto fetch = [&](uint32_t turn) {
+    const T* at = body + (uint64_t)(turn + tid) * V;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      next[j].clear();
+      if (turn + tid + j * kThreads < packs) next[j].load(at + j * kThreads * V);
+    }
+  };
+  bool sampled = false;
+  fetch(first);
+  for (uint32_t turn = first; turn < packs; turn += kAhead * kThreads) {  // the whole CTA takes each turn
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) p[j] = next[j];
+    if (turn + kAhead * kThreads < packs) fetch(turn + kAhead * kThreads);
+    uint32_t top_word = p[0].max_word();
+#pragma unroll
+    for (int j = 1; j < kAhead; ++j) top_word = Q::max_words(top_word, p[j].max_word());
+    const float top = Q::max_of(top_word);
+    if (!(top <= m + kSlack)) raise(top);
+    uint64_t acc = 0;
+    const uint64_t minus_m = shift();
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) acc = add_exps<T>(p[j], acc, minus_m);
+    float a, b;
+    unpair(acc, a, b);
+    s += (double)(a + b);
+    if (!sampled) {  // the first turn's maxima bound the k-th largest from below
+      sampled = true;
+      float most = isnan(top) ? -INFINITY : top;
+      for (int o = kThreads / kGroups / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, o));
+      if (tid % (kThreads / kGroups) == 0) sm.gmax[tid / (kThreads / kGroups)] = order_key(most);
+      __syncthreads();
+      if (tid < kGroups) {
+        const uint32_t own = sm.gmax[tid];
+        uint32_t above = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < kGroups; j += 4) {
+          const uint4 o = *reinterpret_cast<const uint4*>(&sm.gmax[j]);
+          above += before(o.x, j, own, tid) + before(o.y, j + 1, own, tid) + before(o.z, j + 2, own, tid) +
+                   before(o.w, j + 3, own, tid);
+        }
+        if (above == k - 1) sm.bound = own;
+      }
+      __syncthreads();
+      // at or below -inf (few numbers in the sample) it lets all in
+      if (sm.bound > order_key(-INFINITY)) fbnd = key_value(sm.bound);
+    }
+    if (!(top < fbnd)) {  // this thread's loads of the turn hold a candidate
+      const uint32_t at = atomicAdd(&sm.hits, 1u);
+      if (at < kHits) sm.hit[at] = turn + tid;
+    }
+  }
+  if (tid < loose) {
+    const float f = to_f(z[tid < head ? tid : all * V + tid]);
+    if (!(f <= m + kSlack)) raise(f);
+    s += (double)exp2_fast((f - fmaxf(m, -FLT_MAX)) * kLog2e);
+  }
+  // the candidates' loads once more, from the cache, spread over the threads
+  __syncthreads();
+  if (raises > 1) atomicMax(&sm.raises, raises);
+  const uint32_t bnd = fbnd > -INFINITY ? order_key(fbnd) : 0u;
+  auto offer = [&](float f, uint32_t i) {
+    if (f < fbnd) return;
+    const uint32_t key = order_key(f);
+    if (key < bnd) return;  // a NaN
+    const uint32_t at = atomicAdd(&sm.count, 1u);
+    if (at < kCap) {
+      sm.ckey[at] = key;
+      sm.cidx[at] = i;
+    }
+  };
+  const uint32_t hits = sm.hits;
+  if (hits <= kHits) {
+    for (uint32_t c = tid; c < hits * kAhead; c += kThreads) {
+      const uint32_t i = sm.hit[c / kAhead] + c % kAhead * kThreads;
+      if (i >= packs) continue;
+      Q q;
+      q.load(body + (uint64_t)i * V);
+#pragma unroll
+      for (uint32_t v = 0; v < V; ++v) offer(q.element(v), head + i * V + v);
+    }
+    if (tid < loose) {
+      const uint32_t e = tid < head ? tid : all * V + tid;
+      offer(to_f(z[e]), e);
+    }
+  }
+  // the sums of the threads, each moved to the largest shift
+  float most = m;
+  for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, o));
+  if ((tid & 31) == 0) sm.fred[tid >> 5] = most;
+  __syncthreads();
+  most = sm.fred[0];
+  for (int i = 1; i < kWarps; ++i) most = fmaxf(most, sm.fred[i]);
+  if (m != most && s != 0.) s *= exp2_fast((m - most) * kLog2e);
+  s = block_sum(s, sm.dred);
+  const uint32_t n = hits <= kHits ? sm.count : kCap + 1, want = min(k, mine);
+  if (tid == 0) {
+    out.m = most;
+    out.s = s;
+    out.raises = sm.raises;
+    out.count = want;
+  }
+  if (n <= kCap) {
+    for (uint32_t c = tid; c < n; c += kThreads) {
+      const uint32_t key = sm.ckey[c], i = sm.cidx[c];
+      uint32_t above = 0;
+      for (uint32_t j = 0; j < n && above < k; ++j) above += before(sm.ckey[j], sm.cidx[j], key, i);
+      if (above < k) {
+        key_out[above] = key;
+        idx_out[above] = i;
+      }
+    }
+  } else {
+    // too many candidates (many equal entries): the next entry after the last, one rank at a time
+    uint32_t lk = ~0u, li = 0;
+    for (uint32_t r = 0; r < want; ++r) {
+      uint32_t bk = 0, bi = ~0u;
+      for (uint32_t c = tid; c < mine; c += kThreads) {
+        uint32_t e = head + first * V + c;  // the share's words, then the loose elements
+        if (c >= (packs - first) * V) {
+          e = c - (packs - first) * V;
+          if (e >= head) e += all * V;
+        }
+        const uint32_t key = order_key(to_f(z[e]));
+        if ((r == 0 || before(lk, li, key, e)) && before(key, e, bk, bi)) {
+          bk = key;
+          bi = e;
+        }
+      }
+      for (int o = 16; o; o >>= 1) {
+        const uint32_t ok = __shfl_xor_sync(~0u, bk, o), oi = __shfl_xor_sync(~0u, bi, o);
+        if (before(ok, oi, bk, bi)) {
+          bk = ok;
+          bi = oi;
+        }
+      }
+      __syncthreads();
+      if ((tid & 31) == 0) {
+        sm.ckey[tid >> 5] = bk;
+        sm.cidx[tid >> 5] = bi;
+      }
+      __syncthreads();
+      bk = sm.ckey[0];
+      bi = sm.cidx[0];
+      for (int w = 1; w < kWarps; ++w)
+        if (before(sm.ckey[w], sm.cidx[w], bk, bi)) {
+          bk = sm.ckey[w];
+          bi = sm.cidx[w];
+        }
+      lk = bk;
+      li = bi;
+      if (tid == 0) {
+        key_out[r] = bk;
+        idx_out[r] = bi;
+      }
+    }
+  }
+  __syncthreads();
+}
+
+template <class T>
+__global__ void __launch_bounds__(kThreads) k_select(const SelectArgs g) {
+  extern __shared__ __align__(16) uint8_t dynamic[];
+  __shared__ Scratch sm;
+  __shared__ float score[kMaxBeams];
+  __shared__ uint32_t live[kMaxBeams], ended[kMaxBeams], lives;
+  __shared__ double lse[kMaxBeams], err[kMaxBeams], top[kMaxBeams], again[kMaxBeams];
+  __shared__ uint32_t lcount[kMaxBeams + kMaxCluster], lbeam[kMaxBeams + kMaxCluster];
+  __shared__ double rtotal[kMaxWidth];
+  __shared__ uint32_t rbeam[kMaxWidth], rtok[kMaxWidth];
+  __shared__ uint64_t unsure, agreed, taken;  // beams to sum again (first CTA's, all CTAs'); beams with a child
+  const fhe_beam_select_args& a = g.a;
+  const uint32_t tid = threadIdx.x, C = g.cluster, rank = blockIdx.x % C, item = blockIdx.x / C;
+  const uint32_t B = a.beams, k = a.width, kk = g.kk;
+  cg::cluster_group cluster = cg::this_cluster();
+  if (tid < B) {
+    score[tid] = a.scores[(int64_t)item * B + tid];
+    ended[tid] = a.finished && a.finished[(int64_t)item * B + tid];
+  }
+  __syncthreads();
+  if (tid == 0) {
+    uint32_t n = 0;
+    for (uint32_t i = 0; i < B; ++i)
+      if (!ended[i] && isfinite(score[i])) live[n++] = i;
+    lives = n;
+  }
+  __syncthreads();
+  const uint32_t parts = lives ? max(1u, C / lives) : 1, units = lives * parts;
+  const Layout l(dynamic, (B + C - 1) / C, B + C, kk);
+  auto row_of = [&](uint32_t beam) {
+    return static_cast<const T*>(a.logits) + ((int64_t)item * B + beam) * a.logits_stride;
+  };
+  for (uint32_t u = rank; u < units; u += C) {
+    const uint32_t slot = u / C;
+    scan_share<T>(row_of(live[u / parts]), a.vocab, u % parts, parts, kk, sm, l.share[slot], l.key + slot * kk,
+                  l.idx + slot * kk);
+  }
+  auto meet = [&] {
+    if (C > 1) cluster.sync();
+    else __syncthreads();
+  };
+  auto of = [&](auto* p, uint32_t r) { return C == 1 ? p : cluster.map_shared_rank(p, r); };
+  meet();
+  uint32_t lists = 0;
+  if (rank == 0) {
+    // sums of the live beams
+    if (tid < lives) {
+      float m = -INFINITY;
+      uint32_t raises = 0;
+      bool bad = false;
+      for (uint32_t p = 0; p < parts; ++p) {
+        const uint32_t u = tid * parts + p;
+        const Share* s = of(l.share, u % C) + u / C;
+        m = fmaxf(m, s->m);
+        raises = max(raises, s->raises);
+        bad = bad || !isfinite(s->s);
+      }
+      double sum = 0.;
+      for (uint32_t p = 0; p < parts && !bad && m > -INFINITY; ++p) {
+        const uint32_t u = tid * parts + p;
+        const Share* s = of(l.share, u % C) + u / C;
+        if (s->s != 0.) sum += s->s * exp((double)s->m - (double)m);
+      }
+      const uint32_t i = live[tid];
+      const bool fine = !bad && isfinite(m) && sum > 0.;
+      lse[i] = fine ? (double)m + log(sum) : -INFINITY;
+      top[i] = m;
+      // Roundings of u = 2^-24: three of an exponent d = (z - m) log2 e, whose mean over
+      // the sum is at most log2(vocab / sum) and twice the slack, the exponential's four,
+      // at most 16 additions; 8 u for each time that the shift moved
+      err[i] = fine ? 0x1p-24 * (2.2 * (log2((double)a.vocab) - log2(sum) + 12.) + 24. + 8. * raises) : 0.;
+    }
+    // every share's entries; then, in place of those, the entries of beams that offer none
+    for (uint32_t c = tid; c < units * kk; c += kThreads) {
+      const uint32_t u = c / kk, j = c % kk;
+      if (j < (of(l.share, u % C) + u / C)->count) {
+        l.lkey[c] = of(l.key, u % C)[u / C * kk + j];
+        l.lidx[c] = of(l.idx, u % C)[u / C * kk + j];
+      }
+    }
+    __syncthreads();
+    if (tid < units) {
+      const uint32_t i = live[tid / parts];
+      const bool fine = isfinite(lse[i]);
+      lbeam[tid] = i;
+      lcount[tid] = fine ? (of(l.share, tid % C) + tid / C)->count : tid % parts == 0 ? kk : 0;
+    }
+    lists = units;
+    for (uint32_t i = 0; i < B; ++i) {
+      if (!ended[i] && isfinite(score[i])) continue;
+      if (tid == 0) {
+        lbeam[lists] = i;
+        lcount[lists] = kk;
+        lse[i] = -INFINITY;
+        err[i] = 0.;
+      }
+      ++lists;
+    }
+    if (tid == 0) taken = 0;
+    __syncthreads();
+  }
+  for (;;) {
+    if (rank == 0) {
+      if (tid == 0) unsure = 0;
+      for (uint32_t c = tid; c < lists * kk; c += kThreads) {
+        const uint32_t u = c / kk, j = c % kk, i = lbeam[u];
+        if (j >= lcount[u]) continue;
+        if (isfinite(lse[i])) {
+          l.total[c] = (double)score[i] + (double)key_value(l.lkey[c]) - lse[i];
+        } else {
+          // a finished beam: its end, then the impossible tokens; others impossible alone
+          const bool end = ended[i] && isfinite(score[i]);
+          const uint32_t eos = (uint32_t)a.eos;
+          l.lkey[c] = 0;
+          l.lidx[c] = !end ? j : j == 0 ? eos : j - 1 < eos ? j - 1 : j;
+          l.total[c] = end && j == 0 ? (double)score[i] : -INFINITY;
+        }
+      }
+      __syncthreads();
+      // Ranks: larger total, lower beam, larger logit, lower token.  An entry of another
+      // beam may belong before one of the best if the next of its list is too close to
+      // that one.
+      for (uint32_t c = tid; c < lists * kk; c += kThreads) {
+        const uint32_t u = c / kk, j = c % kk, i = lbeam[u];
+        if (j >= lcount[u]) continue;
+        const double t = l.total[c];
+        const uint32_t key = l.lkey[c], id = l.lidx[c];
+        uint32_t above = j;
+        uint64_t close = 0;
+        for (uint32_t v = 0; v < lists && above < k; ++v) {
+          if (v == u) continue;
+          const uint32_t w = lbeam[v], end = lcount[v];
+          uint32_t lo = 0, n = end;
+          while (n) {
+            const uint32_t half = n / 2, e = v * kk + lo + half;
+            const double o = l.total[e];
+            const bool first = o > t || (o == t && (w < i || (w == i && before(l.lkey[e], l.lidx[e], key, id))));
+            lo = first ? lo + half + 1 : lo;
+            n = first ? n - half - 1 : half;
+          }
+          above += lo;
+          const double e = err[i] + err[w];
+          if (w != i && e > 0. && lo < end && t - l.total[v * kk + lo] <= e)  // false for impossible entries
+            close |= (err[i] > 0. ? 1ull << i : 0ull) | (err[w] > 0. ? 1ull << w : 0ull);
+        }
+        if (above < k) {
+          rtotal[above] = t;
+          rbeam[above] = i;
+          rtok[above] = id;
+          if (close) atomicOr(reinterpret_cast<unsigned long long*>(&unsure), (unsigned long long)close);
+        }
+      }
+      __syncthreads();
+      if (tid < C) *of(&agreed, tid) = unsure;
+    }
+    meet();
+    const uint64_t todo = agreed;
+    if (todo == 0) break;
+    // those beams' sums in 64 bits, in an order that does not hang on alignment: equal rows give equal sums
+    for (uint32_t i = 0; i < B; ++i) {
+      if (!(todo >> i & 1)) continue;
+      const T* z = row_of(i);
+      const double m = *of(&top[i], 0);
+      double s = 0.;
+      for (uint32_t e = rank * kThreads + tid; e < a.vocab; e += C * kThreads) s += exp((double)to_f(z[e]) - m);
+      s = block_sum(s, sm.dred);
+      if (tid == 0) again[i] = s;
+    }
+    meet();
+    if (rank == 0 && tid < B && (todo >> tid & 1)) {
+      double s = 0.;
+      for (uint32_t r = 0; r < C; ++r) s += of(again, r)[tid];
+      lse[tid] = top[tid] + log(s);
+      err[tid] = 0.;
+    }
+    __syncthreads();
+  }
+  if (rank != 0) return;
+  // the best child of a beam takes its place, the others the free places in turn
+  uint32_t place = tid;
+  if (a.keep_slots) {
+    uint32_t later = 0;  // children before this one that do not take their beam's place
+    bool first = true;
+    if (tid < k) {
+      for (uint32_t r = 0; r < tid; ++r) {
+        bool one = true;
+        for (uint32_t q = 0; q < r; ++q) one = one && rbeam[q] != rbeam[r];
+        later += !one;
+        first = first && rbeam[r] != rbeam[tid];
+      }
+      atomicOr(reinterpret_cast<unsigned long long*>(&taken), 1ull << rbeam[tid]);
+    }
+    __syncthreads();
+    if (tid < k) {
+      place = rbeam[tid];
+      if (!first) {
+        place = 0;
+        for (uint32_t n = 0;; ++place)
+          if (!(taken >> place & 1) && n++ == later) break;
+      }
+    }
+  }
+  if (tid < k) {
+    const uint32_t i = rbeam[tid], t = rtok[tid];
+    const int64_t at = (int64_t)item * k + place;
+    a.out_scores[at] = (float)rtotal[tid];
+    a.parents[at] = i;
+    a.tokens[at] = t;
+    if (a.out_finished) a.out_finished[at] = ended[i] || (a.eos >= 0 && t == (uint64_t)a.eos);
+  }
+}
+
+}  // namespace
+
+void beam_select(const fhe_beam_select_args& a) {
+  require(a.dtype == FHE_F32 || a.dtype == FHE_BF16 || a.dtype == FHE_F16, "dtype must be FHE_F32, FHE_BF16 or FHE_F16");
+  require(a.beams >= 1 && a.beams <= kMaxBeams, "beams must be in [1, 64]");
+  require(a.vocab >= 1 && a.vocab <= (1u << 30), "vocab must be in [1, 2^30]");
+  require(a.width >= 1 && a.width <= kMaxWidth && (uint64_t)a.width <= (uint64_t)a.beams * a.vocab,
+          "width must be in [1, 64] and at most beams * vocab");
+  require(a.batch < (1u << 24), "batch must be below 2^24");
+  require(a.eos < (int64_t)a.vocab, "eos past the vocabulary");
+  require(!a.finished || a.eos >= 0, "finished beams need an eos token");
+  require(!a.keep_slots || a.width == a.beams, "keep_slots needs a width of beams");
+  if (a.batch == 0) return;
+  require(a.logits && a.scores && a.out_scores && a.parents && a.tokens, "null input or output");
+  DeviceGuard dev(a.device);
+  with_type(a.dtype, [&](auto t) {
+    using T = decltype(t);
+    // As many CTAs to an item as the device takes at once, and a turn of loads for each
+    const uint64_t packs = (uint64_t)a.beams * (a.vocab / Quad<T>::kElems);
+    SelectArgs g{a, 1, std::min(a.width, a.vocab)};
+    while (g.cluster < kMaxCluster && (uint64_t)a.batch * g.cluster * 2 <= 148 * 4 &&
+           packs >= (uint64_t)g.cluster * 2 * kAhead * kThreads)
+      g.cluster *= 2;
+    const uint32_t shared = Layout(nullptr, (a.beams + g.cluster - 1) / g.cluster, a.beams + g.cluster, g.kk).bytes;
+    if (shared > 32768)
+      FHE_CUDA(cudaFuncSetAttribute(k_select<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(a.batch * g.cluster);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = shared;
+    cfg.stream = static_cast<cudaStream_t>(a.stream);
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = g.cluster;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    FHE_CUDA(cudaLaunchKernelEx(&cfg, k_select<T>, g));
+  });
+  note_launch();
+  FHE_CUDA(cudaGetLastError());
+}
+
+}  // namespace fhe

@@ -27,6 +27,8 @@ void rms_norm_backward(const fhe_rms_norm_grad_args& g);
 void embedding(const fhe_embedding_args& a);
 uint64_t embedding_backward_workspace(const fhe_embedding_grad_args& g);
 void embedding_backward(const fhe_embedding_grad_args& g);
+void beam_select(const fhe_beam_select_args& a);
+void beam_reorder(const fhe_beam_reorder_args& a);
 
 // Makes `device` current and restores the caller's device on destruction.
 class DeviceGuard {

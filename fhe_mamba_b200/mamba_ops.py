@@ -1,12 +1,13 @@
 """The plaintext Mamba-2 operators as torch functions: the state recurrence
 (``ssm_scan``, ``ssm_step``), the causal convolution (``causal_conv``,
 ``causal_conv_step``), the norms with their residual or gate (``rms_norm``,
-``add_rms_norm``, ``gated_rms_norm``), the token embedding (``embedding``) and
-token scoring (``token_logprobs``).
+``add_rms_norm``, ``gated_rms_norm``), the token embedding (``embedding``),
+token scoring (``token_logprobs``) and beam search's selection and reordering of
+states (``beam_select``, ``beam_reorder``).
 
 They run on CUDA tensors through the C ABI (fhe_ssm_scan and the others in
 include/fhe_b200.h), on the current stream of the tensors' device, and can be
-captured into CUDA graphs; all but the steps have
+captured into CUDA graphs; all but the steps and the beams have
 gradients (to capture a backward pass, hold no eager autograd graph of the same
 leaves: torch would make the capture wait for that graph's stream, and refuses).
 Activations are float32, bfloat16 or float16; gates, states, norm weights and
@@ -27,6 +28,7 @@ from ._lib import call
 
 _TYPES = {torch.float32: _lib.FHE_F32, torch.bfloat16: _lib.FHE_BF16, torch.float16: _lib.FHE_F16}
 MAX_HEAD_DIM, MAX_STATE, MAX_TAPS, MAX_TOP, MAX_NORM_WIDTH = 128, 256, 8, 64, 16384
+MAX_BEAMS = 64
 
 
 def _need(ok, message):
@@ -654,3 +656,94 @@ def token_logprobs(logits, targets, top_k=0):
     if _wants_grad(logits):
         return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, top_k))
     return TokenLogprobs(*_run_logprobs(logits, targets, top_k)[:4])
+
+
+# ---- beam search --------------------------------------------------------------------------------
+
+
+class BeamStep(NamedTuple):
+    scores: torch.Tensor    # [batch, width] float32
+    parents: torch.Tensor   # [batch, width] int64, beams
+    tokens: torch.Tensor    # [batch, width] int64
+    finished: torch.Tensor  # [batch, width] bool
+
+
+def beam_select(logits, scores, finished=None, eos=None, width=None, keep_slots=False):
+    """One step of beam search: for each batch item the `width` (default: the
+    number of beams; at most 64) best of scores_i + log softmax(logits_i)_v over
+    its beams i and tokens v, best first, the lower beam and then the lower token
+    first among equals.
+
+    logits [batch * beams, vocab] or [batch, beams, vocab] float32, bfloat16 or
+    float16; scores [batch, beams] float32, -inf for a beam that does not count
+    (all but the first of equal ones at the start); beams at most 64.  A beam of
+    `finished` [batch, beams] bool goes on as it is, with the token `eos`.  Beams
+    whose score is not finite or whose logits hold a NaN or +inf offer nothing:
+    candidates of score -inf fill up what possible ones leave.  With keep_slots
+    (width = beams) a beam's best child keeps its beam's place and the others
+    take the free places in order, so that few states have to move.
+
+    Returns a ``BeamStep``: scores, parents (beams), tokens, and which beams have
+    ended.  Totals are compared in 64 bits where 32 do not tell them apart."""
+    op = "beam_select"
+    _need(scores.dim() == 2 and 1 <= scores.shape[1] <= MAX_BEAMS, f"{op}: scores must be [batch, 1 to {MAX_BEAMS} beams]")
+    _need(scores.dtype == torch.float32, f"{op}: scores must be {torch.float32}, got {scores.dtype}")
+    b, k = scores.shape
+    _need(logits.dtype in _TYPES, f"{op}: logits must be float32, bfloat16 or float16")
+    _need(logits.dim() in (2, 3) and logits.shape[:-1] in ((b * k,), (b, k)) and logits.shape[-1] >= 1,
+          f"{op}: logits must be [batch * beams, vocab] or [batch, beams, vocab]")
+    v, width = logits.shape[-1], k if width is None else width
+    _need(1 <= width <= min(MAX_BEAMS, k * v), f"{op}: width must be in [1, {min(MAX_BEAMS, k * v)}]")
+    _need(eos is None or 0 <= eos < v, f"{op}: eos must be a token")
+    if finished is not None:
+        _check(op, "finished", finished, (b, k), torch.bool)
+        _need(eos is not None, f"{op}: finished beams need an eos")
+    _need(not keep_slots or width == k, f"{op}: keep_slots needs a width of the number of beams")
+    _check_devices(op, logits, scores, finished)
+    _need(not _wants_grad(logits, scores), f"{op} has no gradient")
+    rows, scores, finished, d = _rows(logits), _dense(scores), _dense(finished), logits.device
+    out = torch.empty((b, width), dtype=torch.float32, device=d)
+    parents = torch.empty((b, width), dtype=torch.int64, device=d)
+    tokens = torch.empty_like(parents)
+    ended = torch.empty((b, width), dtype=torch.bool, device=d)
+    a = _lib.BeamSelectArgs(
+        d.index, _TYPES[logits.dtype], b, k, v, width, bool(keep_slots), 0, rows.data_ptr(), rows.stride(0),
+        scores.data_ptr(), _ptr(finished), -1 if eos is None else int(eos), out.data_ptr(), parents.data_ptr(),
+        tokens.data_ptr(), ended.data_ptr(), _stream_of(d.index))
+    call("fhe_beam_select", ctypes.byref(a))
+    return BeamStep(out, parents, tokens, ended)
+
+
+def beam_reorder(states, parents):
+    """Moves the states of beams in place: row i of each batch item becomes what
+    its row parents[:, i] was, in every tensor of `states`.
+
+    parents [batch, beams] int64 (at most 64 beams); a parent outside the beams
+    leaves its row.  states: contiguous tensors [batch * beams, ...] or [batch,
+    beams, ...] of any types, no two of them on the same memory.  Rows that
+    keep their place are neither read nor written."""
+    op = "beam_reorder"
+    _need(parents.dim() == 2 and 1 <= parents.shape[1] <= MAX_BEAMS, f"{op}: parents must be [batch, 1 to {MAX_BEAMS} beams]")
+    _need(parents.dtype == torch.int64, f"{op}: parents must be {torch.int64}, got {parents.dtype}")
+    _need(parents.shape[0] <= 65535, f"{op}: batch must be at most 65535")
+    b, k = parents.shape
+    states = list(states)
+    for t in states:
+        _need(t.dim() >= 1 and (t.shape[0] == b * k or t.shape[:2] == (b, k)),
+              f"{op}: states must be [batch * beams, ...] or [batch, beams, ...], got {tuple(t.shape)}")
+        _need(t.is_contiguous(), f"{op}: states must be contiguous")
+    _check_devices(op, parents, *states)
+    _need(not _wants_grad(*states), f"{op} has no gradient")
+    sizes = [t.numel() * t.element_size() for t in states]
+    spans = sorted((t.data_ptr(), n) for t, n in zip([*states, parents], [*sizes, parents.numel() * 8]) if n)
+    _need(all(p + n <= q for (p, n), (q, _) in zip(spans, spans[1:])), f"{op}: states share memory")
+    if b == 0:
+        return
+    n, parents = len(states), _dense(parents)
+    a = _lib.BeamReorderArgs(
+        parents.device.index, b, k, n, (ctypes.c_void_p * n)(*(t.data_ptr() for t in states)),
+        (ctypes.c_uint64 * n)(*(size // (b * k) for size in sizes)), parents.data_ptr(),
+        _stream_of(parents.device.index))
+    call("fhe_beam_reorder", ctypes.byref(a))
+    for t in states:
+        increment_version(t)

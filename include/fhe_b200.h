@@ -741,6 +741,49 @@ typedef struct fhe_embedding_grad_args {
 int fhe_embedding_backward_workspace(const fhe_embedding_grad_args* args, uint64_t* bytes);
 int fhe_embedding_backward(const fhe_embedding_grad_args* args);
 
+/* Beam search's selection: for each batch item the `width` best of
+ *   total(i, v) = scores[i] + logits[i][v] - log sum exp(logits[i])
+ * over its beams i and the tokens v, best first; equal totals by the lower beam
+ * and then the lower token.  The choice is that of the totals in 64 bits (within a
+ * beam that of the logits).  A finished beam has one candidate, the token eos at
+ * scores[i].  Beams whose score is not finite, or whose logits hold a NaN or
+ * +inf or nothing but -inf, have no possible token; impossible candidates (-inf
+ * logits too) have score -inf and are taken last.  With keep_slots (width ==
+ * beams) the best child of a beam comes out at its beam's place and the others
+ * at the free places in order, so that fhe_beam_reorder moves least. */
+typedef struct fhe_beam_select_args {
+  int32_t device, dtype;
+  uint32_t batch, beams;      /* beams in [1, 64] */
+  uint32_t vocab, width;      /* width in [1, 64], at most beams * vocab */
+  int32_t keep_slots;
+  uint32_t reserved;
+  const void* logits;         /* [batch * beams][vocab] */
+  int64_t logits_stride;      /* between rows */
+  const float* scores;        /* [batch][beams] */
+  const uint8_t* finished;    /* [batch][beams], 0 or 1, or NULL for none */
+  int64_t eos;                /* the ending token, -1 for none (then finished is NULL) */
+  float* out_scores;          /* [batch][width] */
+  int64_t* parents;           /* [batch][width]: beams */
+  int64_t* tokens;            /* [batch][width] */
+  uint8_t* out_finished;      /* [batch][width]: the parent is finished or the token is eos; or NULL */
+  void* stream;
+} fhe_beam_select_args;
+int fhe_beam_select(const fhe_beam_select_args* args);
+
+/* Rows [batch][beams] of every tensor moved in place: row (b, i) becomes what row
+ * (b, parents[b][i]) was; a parent outside [0, beams) leaves its row.  Tensors are
+ * contiguous, any type, and share no memory with each other or with parents. */
+typedef struct fhe_beam_reorder_args {
+  int32_t device;
+  uint32_t batch, beams;      /* beams in [1, 64] */
+  uint32_t count;             /* tensors */
+  void* const* states;        /* host array of device pointers, [count] */
+  const uint64_t* row_bytes;  /* host array, [count]: bytes of one row */
+  const int64_t* parents;     /* [batch][beams], device */
+  void* stream;
+} fhe_beam_reorder_args;
+int fhe_beam_reorder(const fhe_beam_reorder_args* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -147,3 +147,61 @@ def test_embedding_backward_c_refusals():
     n = ctypes.c_uint64()
     assert lib.fhe_embedding_backward_workspace(ctypes.byref(g), ctypes.byref(n)) == 0 and n.value >= 32
     assert lib.fhe_embedding(None) == lib.fhe_embedding_backward(None) == _lib.FHE_ERR_INVALID
+
+
+def select_args(**kw):
+    return {**dict(logits=z(6, 9), scores=z(2, 3)), **kw}
+
+
+@pytest.mark.parametrize("kw, message", [
+    (dict(scores=z(6)), "scores must be"), (dict(scores=z(2, 65)), "scores must be"), (dict(scores=z(2, 0)), "scores must be"),
+    (dict(scores=z(2, 3, dtype=F64)), "scores must be"), (dict(logits=z(6, 9, dtype=F64)), "logits must be float32"),
+    (dict(logits=z(5, 9)), "logits must be"), (dict(logits=z(3, 2, 9)), "logits must be"), (dict(logits=z(6)), "logits must be"),
+    (dict(logits=z(6, 0)), "logits must be"), (dict(width=0), "width"), (dict(width=28), "width"),
+    (dict(logits=z(6, 99), width=65), "width"), (dict(eos=9), "eos must be a token"), (dict(eos=-1), "eos must be a token"),
+    (dict(finished=z(2, 3, dtype=torch.bool)), "need an eos"), (dict(finished=z(2, 3), eos=0), "finished must be"),
+    (dict(finished=z(6, dtype=torch.bool), eos=0), "finished must have shape"), (dict(keep_slots=True, width=2), "keep_slots"),
+    ({}, "CUDA tensors expected"),
+])
+def test_select_refusals(kw, message):
+    with pytest.raises(ValueError, match=message):
+        ops.beam_select(**select_args(**kw))
+
+
+@pytest.mark.parametrize("states, parents, message", [
+    ([z(6, 4)], z(6, dtype=I64), "parents must be"), ([z(6, 4)], z(2, 65, dtype=I64), "parents must be"),
+    ([z(6, 4)], z(2, 3, dtype=torch.int32), "parents must be"), ([z(5, 4)], z(2, 3, dtype=I64), "states must be"),
+    ([z(3, 2, 4)], z(2, 3, dtype=I64), "states must be"), ([z(())], z(2, 3, dtype=I64), "states must be"),
+    ([z(4, 6).t()], z(2, 3, dtype=I64), "contiguous"), ([z(6, 4)], z(2, 3, dtype=I64), "CUDA tensors expected"),
+    ([z(65536, 1)], z(65536, 1, dtype=I64), "batch"),
+])
+def test_reorder_refusals(states, parents, message):
+    with pytest.raises(ValueError, match=message):
+        ops.beam_reorder(states, parents)
+
+
+def test_reorder_shared_memory(monkeypatch):
+    """One tensor twice, a view beside its base, and the parents among the states are refused (no GPU is asked)."""
+    monkeypatch.setattr(ops, "_check_devices", lambda *a: None)
+    t, parents = z(6, 4), z(2, 3, dtype=I64)
+    for states in ([t, t], [t, z(6, 4), t.view(2, 3, 4)], [t, t.view(-1)[6:12]], [parents]):
+        with pytest.raises(ValueError, match="share memory"):
+            ops.beam_reorder(states, parents)
+
+
+def test_beam_c_refusals():
+    lib = _lib.load()
+    base = dict(dtype=0, batch=2, beams=3, vocab=9, width=3, logits=256, logits_stride=9, scores=256, eos=-1, out_scores=256,
+                parents=256, tokens=256)
+    for kw, message in ((dict(dtype=5), "dtype"), (dict(beams=0), "beams"), (dict(beams=65), "beams"), (dict(vocab=0), "vocab"),
+                        (dict(width=0), "width"), (dict(width=65), "width"), (dict(width=28), "width"),
+                        (dict(batch=1 << 24), "batch"), (dict(eos=9), "eos"), (dict(finished=256), "eos"),
+                        (dict(keep_slots=1, width=2), "keep_slots"), (dict(logits=None), "null"), (dict(tokens=None), "null")):
+        a = _lib.BeamSelectArgs(**{**base, **kw})
+        assert lib.fhe_beam_select(ctypes.byref(a)) == _lib.FHE_ERR_INVALID and message in _lib.last_error(), kw
+    one, size = (ctypes.c_void_p * 1)(None), (ctypes.c_uint64 * 1)(8)
+    for kw, message in ((dict(beams=65), "beams"), (dict(beams=0), "beams"), (dict(batch=65536), "batch"),
+                        (dict(states=None), "null"), (dict(parents=None), "null"), ({}, "null state")):
+        a = _lib.BeamReorderArgs(**{**dict(batch=2, beams=3, count=1, states=one, row_bytes=size, parents=256), **kw})
+        assert lib.fhe_beam_reorder(ctypes.byref(a)) == _lib.FHE_ERR_INVALID and message in _lib.last_error(), kw
+    assert lib.fhe_beam_select(None) == lib.fhe_beam_reorder(None) == _lib.FHE_ERR_INVALID
