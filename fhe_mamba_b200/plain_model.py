@@ -3,13 +3,15 @@
 ``Mamba2Model`` evaluates its layers token by token in float64 on the host, as
 the reference for the encrypted loop.  ``PlainMamba2`` runs the same layers
 with the exact nonlinearities (``exact_step``) over batches of sequences at
-once: the in and out projections are library matrix products, the convolution,
-the recurrence and the scores the operators of ``mamba_ops``.  It scores long
-texts, prefills prompts of different lengths, continues token by token from
-the carried states, and has gradients, so a model can be tuned before it is
-calibrated and encrypted.
+once: the in and out projections are library matrix products, everything else
+the operators of ``mamba_ops``.  It scores long texts, prefills prompts of
+different lengths, continues token by token from the carried states or by beam
+search, and has gradients, so a model can be tuned before it is calibrated and
+encrypted.
 """
 from __future__ import annotations
+
+from typing import NamedTuple
 
 import torch
 
@@ -17,9 +19,10 @@ from . import mamba_ops as ops
 from .mamba_ops import TokenLogprobs
 
 
-def _rms(x, weight, eps):
-    x = x.float()
-    return x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps) * weight
+class BeamTexts(NamedTuple):
+    tokens: torch.Tensor   # [batch, beams, length] int64, best first; `eos` behind an end
+    scores: torch.Tensor   # [batch, beams] float32, sums of log-probabilities
+    lengths: torch.Tensor  # [batch, beams] int64, an end included
 
 
 class PlainMamba2(torch.nn.Module):
@@ -47,8 +50,13 @@ class PlainMamba2(torch.nn.Module):
         return [(torch.zeros(batch, W.conv_kernel - 1, W.conv_dim, dtype=self.dtype, device=d),
                  torch.zeros(batch, W.heads, W.head_dim, W.d_state, device=d)) for W in self.weights]
 
-    def _project(self, W, p, h):
-        u = _rms(h, p["norm_w"], W.eps).to(self.dtype)
+    def _norm(self, h, branch, weight, eps):
+        """The residual stream with the last layer's output added (None: as it is), and its norm."""
+        if branch is None:
+            return ops.rms_norm(h, weight, eps, self.dtype), h
+        return ops.add_rms_norm(h, branch, weight, eps)
+
+    def _project(self, W, p, u):
         z, xbc, dt = (u @ p["w_in"].T).split([W.d_inner, W.conv_dim, W.heads], -1)
         write = torch.nn.functional.softplus(dt.float() + p["dt_bias"])
         return z, xbc, write, p["a"] * write
@@ -57,9 +65,11 @@ class PlainMamba2(torch.nn.Module):
         x, B, C = xa.split([W.d_inner, W.d_state, W.d_state], -1)
         return x.unflatten(-1, (W.heads, W.head_dim)), B.unsqueeze(-2), C.unsqueeze(-2)
 
-    def _finish(self, W, p, h, y, z):
-        g = y.flatten(-2).float() * torch.nn.functional.silu(z.float())
-        return h + (_rms(g, p["gn_w"], W.eps).to(self.dtype) @ p["w_out"].T).float()
+    def _finish(self, W, p, y, z):
+        return ops.gated_rms_norm(y.flatten(-2), z, p["gn_w"], W.eps) @ p["w_out"].T
+
+    def _embed(self, tokens):
+        return ops.embedding(tokens.to(self.embedding.device), self.embedding, dtype=torch.float32)
 
     def forward(self, tokens, state=None, lengths=None):
         """The normalised final hidden vectors [batch, length, d_model] of the
@@ -68,28 +78,68 @@ class PlainMamba2(torch.nn.Module):
         if tokens.dim() != 2:
             raise ValueError("tokens must be [batch, length]")
         state = state if state is not None else self.initial_state(tokens.shape[0])
-        h, new = self.embedding[tokens].float(), []
+        h, branch, new = self._embed(tokens), None, []
         for W, p, (window, s) in zip(self.weights, self.layers, state):
-            z, xbc, write, log_decay = self._project(W, p, h)
+            u, h = self._norm(h, branch, p["norm_w"], W.eps)
+            z, xbc, write, log_decay = self._project(W, p, u)
             xa, window = ops.causal_conv(xbc, p["conv_w"], p["conv_b"], initial_state=window, lengths=lengths)
             x, B, C = self._parts(W, xa)
             y, s = ops.ssm_scan(x, write, log_decay, B, C, D=p["d"], initial_state=s, lengths=lengths)
-            h = self._finish(W, p, h, y, z)
+            branch = self._finish(W, p, y, z)
             new.append((window, s))
-        return _rms(h, self.norm_f, self.weights[0].eps).to(self.dtype), new
+        return self._norm(h, branch, self.norm_f, self.weights[0].eps)[0], new
 
     @torch.no_grad()
     def step(self, tokens, state):
         """One token of each sequence ([batch]): its hidden vectors [batch,
         d_model].  `state` moves on in place."""
-        h = self.embedding[tokens].float()
+        h, branch = self._embed(tokens), None
         for W, p, (window, s) in zip(self.weights, self.layers, state):
-            z, xbc, write, log_decay = self._project(W, p, h)
+            u, h = self._norm(h, branch, p["norm_w"], W.eps)
+            z, xbc, write, log_decay = self._project(W, p, u)
             xa, _ = ops.causal_conv_step(window, xbc, p["conv_w"], p["conv_b"])
             x, B, C = self._parts(W, xa)
             y, _ = ops.ssm_step(s, x, write, log_decay, B, C, D=p["d"])
-            h = self._finish(W, p, h, y, z)
-        return _rms(h, self.norm_f, self.weights[0].eps).to(self.dtype)
+            branch = self._finish(W, p, y, z)
+        return self._norm(h, branch, self.norm_f, self.weights[0].eps)[0]
+
+    @torch.no_grad()
+    def beam_search(self, tokens, beams, length, eos=None, lengths=None, length_penalty=0.0):
+        """The `beams` best continuations of each prompt [batch, at least 1] by at
+        most `length` tokens (``BeamTexts``): beam search over the sums of
+        log-probabilities, a text ending with `eos` if that is given, ordered by
+        score / text length ** length_penalty.  `lengths` int32 [batch] are those
+        of padded prompts, at least 1."""
+        if tokens.dim() != 2 or tokens.shape[1] < 1:
+            raise ValueError("tokens must be [batch, at least 1]")
+        if not (1 <= beams <= min(ops.MAX_BEAMS, self.embedding.shape[0]) and length >= 1):
+            raise ValueError(f"beams must be in [1, {min(ops.MAX_BEAMS, self.embedding.shape[0])}], length at least 1")
+        if lengths is not None and lengths.numel() and int(lengths.min()) < 1:
+            raise ValueError("every prompt needs a token")
+        b, d = tokens.shape[0], self.embedding.device
+        hidden, state = self(tokens, lengths=lengths)
+        last = torch.full((b,), tokens.shape[1] - 1, device=d) if lengths is None else \
+            lengths.long().clamp(max=tokens.shape[1]) - 1
+        logits = self.logits(hidden[torch.arange(b, device=d), last])
+        state = [tuple(v.repeat_interleave(beams, 0) for v in pair) for pair in state]
+        texts = torch.zeros(b, beams, length, dtype=torch.int64, device=d)
+        moved = [texts, *(v for pair in state for v in pair)]
+        found = ops.beam_select(logits, torch.zeros(b, 1, device=d), eos=eos, width=beams)
+        for i in range(length):
+            if i:
+                found = ops.beam_select(self.logits(self.step(found.tokens.flatten(), state)), found.scores,
+                                        found.finished if eos is not None else None, eos, keep_slots=True)
+                ops.beam_reorder(moved, found.parents)
+            texts[:, :, i] = found.tokens
+            if eos is not None and bool(found.finished.all()):
+                texts[:, :, i + 1:] = eos
+                break
+        n = torch.full((b, beams), length, device=d)
+        if eos is not None:
+            n = torch.minimum(n, (texts != eos).cumprod(-1).sum(-1) + 1)
+        order = torch.sort(found.scores / n ** length_penalty, dim=1, descending=True, stable=True)[1]
+        return BeamTexts(texts.gather(1, order[..., None].expand_as(texts)), found.scores.gather(1, order),
+                         n.gather(1, order))
 
     def logits(self, hidden):
         return hidden @ self.embedding.T
