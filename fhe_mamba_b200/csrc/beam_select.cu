@@ -3,13 +3,14 @@
 //
 // A cluster of up to eight CTAs takes a batch item, a row or a share of a row to a
 // CTA at a time, in one read: sums of exp(z - m) around a running shift m, and the
-// share's best entries (a lower bound from its first loads, then only the loads that
-// reach it, ranked by counting).  The first CTA puts the shares together over
-// distributed shared memory and ranks them.  Within a beam the order is that of the
-// logits; between beams it hangs on the beams' sums, which fp32 knows to a few
-// 2^-20.  Where neighbours of different beams among the best lie closer than that,
-// the cluster sums those beams again in 64 bits, so that the choice is always that of
-// the formula.  The read bounds it.
+// largest entry of each thread.  The `width`-th largest of 64 groups' maxima is a lower
+// bound on the share's best entries; the loads of the threads that reach it come once
+// more, from the cache, and what reaches it is ranked by counting.  Shares go to the
+// first CTA over distributed shared memory, which ranks them together.  Within a beam
+// the order is that of the logits; between beams it hangs on the beams' sums, which
+// fp32 knows to a few 2^-20.  Where a beam's entry lies closer than that to one of the
+// best of another, the cluster sums those beams again in 64 bits, so that the choice
+// is always that of the formula.
 #include <algorithm>
 #include <cfloat>
 #include <cooperative_groups.h>
@@ -26,7 +27,6 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kGroups = 64;   // groups of 4 threads
 constexpr int kAhead = 4;     // 16-byte loads in flight per thread
 constexpr int kCap = 1024;    // candidates held
-constexpr int kHits = 512;    // turns of a thread that hold candidates
 constexpr uint32_t kMaxBeams = 64, kMaxWidth = 64, kMaxCluster = 8;
 static_assert(kMaxWidth <= kGroups, "the bound is the width-th of the groups' maxima");
 
@@ -37,26 +37,23 @@ struct Share {
   uint32_t raises, count, pad;
 };
 
-// Dynamic shared memory: this CTA's shares, and (first CTA) every share's entries.
+// Dynamic shared memory, of the first CTA: every share with its entries.
 struct Layout {
   Share* share;
-  uint32_t *key, *idx;
   double* total;
-  uint32_t *lkey, *lidx;
+  uint32_t *key, *idx;
   uint32_t bytes;
-  __host__ __device__ Layout(uint8_t* p, uint32_t slots, uint32_t lists, uint32_t kk) {
+  __host__ __device__ Layout(uint8_t* p, uint32_t lists, uint32_t kk) {
     uint8_t* at = p;
     auto take = [&](uint32_t n) {
       uint8_t* r = at;
       at += (n + 15) / 16 * 16;
       return r;
     };
-    share = reinterpret_cast<Share*>(take(slots * sizeof(Share)));
+    share = reinterpret_cast<Share*>(take(lists * sizeof(Share)));
     total = reinterpret_cast<double*>(take(lists * kk * 8));
-    key = reinterpret_cast<uint32_t*>(take(slots * kk * 4));
-    idx = reinterpret_cast<uint32_t*>(take(slots * kk * 4));
-    lkey = reinterpret_cast<uint32_t*>(take(lists * kk * 4));
-    lidx = reinterpret_cast<uint32_t*>(take(lists * kk * 4));
+    key = reinterpret_cast<uint32_t*>(take(lists * kk * 4));
+    idx = reinterpret_cast<uint32_t*>(take(lists * kk * 4));
     bytes = (uint32_t)(at - p);
   }
 };
@@ -91,7 +88,7 @@ struct Scratch {
   float fred[kWarps];
   double dred[kWarps];
   __align__(16) uint32_t gmax[kGroups];
-  uint32_t ckey[kCap], cidx[kCap], hit[kHits];
+  uint32_t ckey[kCap], cidx[kCap], hit[kThreads];
   uint32_t hits, bound, count, raises;
 };
 
@@ -108,7 +105,7 @@ __device__ __forceinline__ double block_sum(double v, double (&red)[kWarps]) {
 // Share `part` of `parts` of the row z: 16-byte words between the row's first and
 // last 16-byte boundaries; the elements before and after go with the first share.
 template <class T>
-__device__ void scan_share(const T* z, uint32_t vocab, uint32_t part, uint32_t parts, uint32_t k, Scratch& sm, Share& out,
+__device__ void scan_share(const T* z, uint32_t vocab, uint32_t part, uint32_t parts, uint32_t k, Scratch& sm, Share* out,
                            uint32_t* key_out, uint32_t* idx_out) {
   using Q = Quad<T>;
   constexpr uint32_t V = Q::kElems;
@@ -134,7 +131,7 @@ __device__ void scan_share(const T* z, uint32_t vocab, uint32_t part, uint32_t p
     return pair(v, v);
   };
   constexpr float kSlack = 4.f;  // a sum may hold terms up to e^4 before its shift moves
-  float fbnd = -INFINITY;
+  float best = -INFINITY;  // NaN left out
   Q p[kAhead], next[kAhead];
   auto fetch = [&](uint32_t turn) {
     const T* at = body + (uint64_t)(turn + tid) * V;
@@ -144,7 +141,6 @@ __device__ void scan_share(const T* z, uint32_t vocab, uint32_t part, uint32_t p
       if (turn + tid + j * kThreads < packs) next[j].load(at + j * kThreads * V);
     }
   };
-  bool sampled = false;
   fetch(first);
   for (uint32_t turn = first; turn < packs; turn += kAhead * kThreads) {  // the whole CTA takes each turn
 #pragma unroll
@@ -162,81 +158,73 @@ __device__ void scan_share(const T* z, uint32_t vocab, uint32_t part, uint32_t p
     float a, b;
     unpair(acc, a, b);
     s += (double)(a + b);
-    if (!sampled) {  // the first turn's maxima bound the k-th largest from below
-      sampled = true;
-      float most = isnan(top) ? -INFINITY : top;
-      for (int o = kThreads / kGroups / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, o));
-      if (tid % (kThreads / kGroups) == 0) sm.gmax[tid / (kThreads / kGroups)] = order_key(most);
-      __syncthreads();
-      if (tid < kGroups) {
-        const uint32_t own = sm.gmax[tid];
-        uint32_t above = 0;
-#pragma unroll
-        for (uint32_t j = 0; j < kGroups; j += 4) {
-          const uint4 o = *reinterpret_cast<const uint4*>(&sm.gmax[j]);
-          above += before(o.x, j, own, tid) + before(o.y, j + 1, own, tid) + before(o.z, j + 2, own, tid) +
-                   before(o.w, j + 3, own, tid);
-        }
-        if (above == k - 1) sm.bound = own;
-      }
-      __syncthreads();
-      // at or below -inf (few numbers in the sample) it lets all in
-      if (sm.bound > order_key(-INFINITY)) fbnd = key_value(sm.bound);
-    }
-    if (!(top < fbnd)) {  // this thread's loads of the turn hold a candidate
-      const uint32_t at = atomicAdd(&sm.hits, 1u);
-      if (at < kHits) sm.hit[at] = turn + tid;
-    }
+    best = fmaxf(best, top);
   }
   if (tid < loose) {
     const float f = to_f(z[tid < head ? tid : all * V + tid]);
     if (!(f <= m + kSlack)) raise(f);
     s += (double)exp2_fast((f - fmaxf(m, -FLT_MAX)) * kLog2e);
+    best = fmaxf(best, f);
   }
-  // the candidates' loads once more, from the cache, spread over the threads
-  __syncthreads();
+  // a lower bound on the k-th largest, and the threads that reach it
+  float group = best;
+  for (int o = kThreads / kGroups / 2; o; o >>= 1) group = fmaxf(group, __shfl_xor_sync(~0u, group, o));
+  float most = m;
+  for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, o));
+  if (tid % (kThreads / kGroups) == 0) sm.gmax[tid / (kThreads / kGroups)] = order_key(group);
+  if ((tid & 31) == 0) sm.fred[tid >> 5] = most;
   if (raises > 1) atomicMax(&sm.raises, raises);
-  const uint32_t bnd = fbnd > -INFINITY ? order_key(fbnd) : 0u;
+  __syncthreads();
+  if (tid < kGroups) {
+    const uint32_t own = sm.gmax[tid];
+    uint32_t above = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < kGroups; j += 4) {
+      const uint4 o = *reinterpret_cast<const uint4*>(&sm.gmax[j]);
+      above += before(o.x, j, own, tid) + before(o.y, j + 1, own, tid) + before(o.z, j + 2, own, tid) +
+               before(o.w, j + 3, own, tid);
+    }
+    if (above == k - 1) sm.bound = own;
+  }
+  // meanwhile the sums of the threads, each moved to the largest shift
+  most = sm.fred[0];
+  for (int i = 1; i < kWarps; ++i) most = fmaxf(most, sm.fred[i]);
+  if (m != most && s != 0.) s *= exp2_fast((m - most) * kLog2e);
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+  if ((tid & 31) == 0) sm.dred[tid >> 5] = s;
+  __syncthreads();
+  const uint32_t bnd = sm.bound;
+  if (order_key(best) >= bnd) sm.hit[atomicAdd(&sm.hits, 1u)] = tid;
+  __syncthreads();
   auto offer = [&](float f, uint32_t i) {
-    if (f < fbnd) return;
     const uint32_t key = order_key(f);
-    if (key < bnd) return;  // a NaN
+    if (key < bnd) return;
     const uint32_t at = atomicAdd(&sm.count, 1u);
     if (at < kCap) {
       sm.ckey[at] = key;
       sm.cidx[at] = i;
     }
   };
-  const uint32_t hits = sm.hits;
-  if (hits <= kHits) {
-    for (uint32_t c = tid; c < hits * kAhead; c += kThreads) {
-      const uint32_t i = sm.hit[c / kAhead] + c % kAhead * kThreads;
-      if (i >= packs) continue;
-      Q q;
-      q.load(body + (uint64_t)i * V);
+  const uint32_t loads = (packs - first + kThreads - 1) / kThreads;  // of a thread
+  for (uint32_t c = tid; c < sm.hits * loads; c += kThreads) {
+    const uint32_t i = first + c % loads * kThreads + sm.hit[c / loads];
+    if (i >= packs) continue;
+    Q q;
+    q.load(body + (uint64_t)i * V);
+    if (order_key(Q::max_of(q.max_word())) < bnd) continue;
 #pragma unroll
-      for (uint32_t v = 0; v < V; ++v) offer(q.element(v), head + i * V + v);
-    }
-    if (tid < loose) {
-      const uint32_t e = tid < head ? tid : all * V + tid;
-      offer(to_f(z[e]), e);
-    }
+    for (uint32_t v = 0; v < V; ++v) offer(q.element(v), head + i * V + v);
   }
-  // the sums of the threads, each moved to the largest shift
-  float most = m;
-  for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, o));
-  if ((tid & 31) == 0) sm.fred[tid >> 5] = most;
+  if (tid < loose) {
+    const uint32_t e = tid < head ? tid : all * V + tid;
+    offer(to_f(z[e]), e);
+  }
   __syncthreads();
-  most = sm.fred[0];
-  for (int i = 1; i < kWarps; ++i) most = fmaxf(most, sm.fred[i]);
-  if (m != most && s != 0.) s *= exp2_fast((m - most) * kLog2e);
-  s = block_sum(s, sm.dred);
-  const uint32_t n = hits <= kHits ? sm.count : kCap + 1, want = min(k, mine);
+  const uint32_t n = sm.count, want = min(k, mine);
   if (tid == 0) {
-    out.m = most;
-    out.s = s;
-    out.raises = sm.raises;
-    out.count = want;
+    double sum = 0.;
+    for (int i = 0; i < kWarps; ++i) sum += sm.dred[i];
+    *out = Share{sum, most, sm.raises, want, 0};
   }
   if (n <= kCap) {
     for (uint32_t c = tid; c < n; c += kThreads) {
@@ -306,11 +294,12 @@ __global__ void __launch_bounds__(kThreads) k_select(const SelectArgs g) {
   __shared__ uint32_t lcount[kMaxBeams + kMaxCluster], lbeam[kMaxBeams + kMaxCluster];
   __shared__ double rtotal[kMaxWidth];
   __shared__ uint32_t rbeam[kMaxWidth], rtok[kMaxWidth];
-  __shared__ uint64_t unsure, agreed, taken;  // beams to sum again (first CTA's, all CTAs'); beams with a child
+  __shared__ uint64_t unsure, agreed;  // beams to sum again: the first CTA's, all CTAs'
   const fhe_beam_select_args& a = g.a;
   const uint32_t tid = threadIdx.x, C = g.cluster, rank = blockIdx.x % C, item = blockIdx.x / C;
   const uint32_t B = a.beams, k = a.width, kk = g.kk;
   cg::cluster_group cluster = cg::this_cluster();
+  if (C > 1) cluster.barrier_arrive();  // every CTA has to run before another's memory is written
   if (tid < B) {
     score[tid] = a.scores[(int64_t)item * B + tid];
     ended[tid] = a.finished && a.finished[(int64_t)item * B + tid];
@@ -324,20 +313,19 @@ __global__ void __launch_bounds__(kThreads) k_select(const SelectArgs g) {
   }
   __syncthreads();
   const uint32_t parts = lives ? max(1u, C / lives) : 1, units = lives * parts;
-  const Layout l(dynamic, (B + C - 1) / C, B + C, kk);
+  const Layout l(dynamic, B + C, kk);
   auto row_of = [&](uint32_t beam) {
     return static_cast<const T*>(a.logits) + ((int64_t)item * B + beam) * a.logits_stride;
   };
-  for (uint32_t u = rank; u < units; u += C) {
-    const uint32_t slot = u / C;
-    scan_share<T>(row_of(live[u / parts]), a.vocab, u % parts, parts, kk, sm, l.share[slot], l.key + slot * kk,
-                  l.idx + slot * kk);
-  }
+  auto of = [&](auto* p, uint32_t r) { return C == 1 ? p : cluster.map_shared_rank(p, r); };
   auto meet = [&] {
     if (C > 1) cluster.sync();
     else __syncthreads();
   };
-  auto of = [&](auto* p, uint32_t r) { return C == 1 ? p : cluster.map_shared_rank(p, r); };
+  if (C > 1) cluster.barrier_wait();
+  for (uint32_t u = rank; u < units; u += C)
+    scan_share<T>(row_of(live[u / parts]), a.vocab, u % parts, parts, kk, sm, of(l.share, 0) + u, of(l.key, 0) + u * kk,
+                  of(l.idx, 0) + u * kk);
   meet();
   uint32_t lists = 0;
   if (rank == 0) {
@@ -346,18 +334,17 @@ __global__ void __launch_bounds__(kThreads) k_select(const SelectArgs g) {
       float m = -INFINITY;
       uint32_t raises = 0;
       bool bad = false;
+      const Share* s = l.share + tid * parts;
       for (uint32_t p = 0; p < parts; ++p) {
-        const uint32_t u = tid * parts + p;
-        const Share* s = of(l.share, u % C) + u / C;
-        m = fmaxf(m, s->m);
-        raises = max(raises, s->raises);
-        bad = bad || !isfinite(s->s);
+        m = fmaxf(m, s[p].m);
+        raises = max(raises, s[p].raises);
+        bad = bad || !isfinite(s[p].s);
       }
-      double sum = 0.;
-      for (uint32_t p = 0; p < parts && !bad && m > -INFINITY; ++p) {
-        const uint32_t u = tid * parts + p;
-        const Share* s = of(l.share, u % C) + u / C;
-        if (s->s != 0.) sum += s->s * exp((double)s->m - (double)m);
+      double sum = s[0].s;
+      if (parts > 1 && !bad && m > -INFINITY) {
+        sum = 0.;
+        for (uint32_t p = 0; p < parts; ++p)
+          if (s[p].s != 0.) sum += s[p].s * exp((double)s[p].m - (double)m);
       }
       const uint32_t i = live[tid];
       const bool fine = !bad && isfinite(m) && sum > 0.;
@@ -368,20 +355,12 @@ __global__ void __launch_bounds__(kThreads) k_select(const SelectArgs g) {
       // at most 16 additions; 8 u for each time that the shift moved
       err[i] = fine ? 0x1p-24 * (2.2 * (log2((double)a.vocab) - log2(sum) + 12.) + 24. + 8. * raises) : 0.;
     }
-    // every share's entries; then, in place of those, the entries of beams that offer none
-    for (uint32_t c = tid; c < units * kk; c += kThreads) {
-      const uint32_t u = c / kk, j = c % kk;
-      if (j < (of(l.share, u % C) + u / C)->count) {
-        l.lkey[c] = of(l.key, u % C)[u / C * kk + j];
-        l.lidx[c] = of(l.idx, u % C)[u / C * kk + j];
-      }
-    }
     __syncthreads();
     if (tid < units) {
       const uint32_t i = live[tid / parts];
       const bool fine = isfinite(lse[i]);
       lbeam[tid] = i;
-      lcount[tid] = fine ? (of(l.share, tid % C) + tid / C)->count : tid % parts == 0 ? kk : 0;
+      lcount[tid] = fine ? l.share[tid].count : tid % parts == 0 ? kk : 0;  // its impossible tokens, once
     }
     lists = units;
     for (uint32_t i = 0; i < B; ++i) {
@@ -394,7 +373,6 @@ __global__ void __launch_bounds__(kThreads) k_select(const SelectArgs g) {
       }
       ++lists;
     }
-    if (tid == 0) taken = 0;
     __syncthreads();
   }
   for (;;) {
@@ -404,13 +382,13 @@ __global__ void __launch_bounds__(kThreads) k_select(const SelectArgs g) {
         const uint32_t u = c / kk, j = c % kk, i = lbeam[u];
         if (j >= lcount[u]) continue;
         if (isfinite(lse[i])) {
-          l.total[c] = (double)score[i] + (double)key_value(l.lkey[c]) - lse[i];
+          l.total[c] = (double)score[i] + (double)key_value(l.key[c]) - lse[i];
         } else {
           // a finished beam: its end, then the impossible tokens; others impossible alone
           const bool end = ended[i] && isfinite(score[i]);
           const uint32_t eos = (uint32_t)a.eos;
-          l.lkey[c] = 0;
-          l.lidx[c] = !end ? j : j == 0 ? eos : j - 1 < eos ? j - 1 : j;
+          l.key[c] = 0;
+          l.idx[c] = !end ? j : j == 0 ? eos : j - 1 < eos ? j - 1 : j;
           l.total[c] = end && j == 0 ? (double)score[i] : -INFINITY;
         }
       }
@@ -418,33 +396,43 @@ __global__ void __launch_bounds__(kThreads) k_select(const SelectArgs g) {
       // Ranks: larger total, lower beam, larger logit, lower token.  An entry of another
       // beam may belong before one of the best if the next of its list is too close to
       // that one.
-      for (uint32_t c = tid; c < lists * kk; c += kThreads) {
-        const uint32_t u = c / kk, j = c % kk, i = lbeam[u];
-        if (j >= lcount[u]) continue;
-        const double t = l.total[c];
-        const uint32_t key = l.lkey[c], id = l.lidx[c];
-        uint32_t above = j;
+      uint32_t lanes = 1;  // that share an entry, a list each at a time
+      while (lanes < 32 && lanes < lists && lanes * lists * kk < kThreads * 2) lanes *= 2;
+      const uint32_t turns = (lists * kk * lanes + kThreads - 1) / kThreads;
+      for (uint32_t n = 0; n < turns; ++n) {
+        const uint32_t c = (n * kThreads + tid) / lanes, lane = tid % lanes;
+        const uint32_t u = c / kk, j = c % kk;
+        uint32_t above = k;
         uint64_t close = 0;
-        for (uint32_t v = 0; v < lists && above < k; ++v) {
-          if (v == u) continue;
-          const uint32_t w = lbeam[v], end = lcount[v];
-          uint32_t lo = 0, n = end;
-          while (n) {
-            const uint32_t half = n / 2, e = v * kk + lo + half;
-            const double o = l.total[e];
-            const bool first = o > t || (o == t && (w < i || (w == i && before(l.lkey[e], l.lidx[e], key, id))));
-            lo = first ? lo + half + 1 : lo;
-            n = first ? n - half - 1 : half;
+        if (u < lists && j < lcount[u]) {
+          const uint32_t i = lbeam[u], key = l.key[c], id = l.idx[c];
+          const double t = l.total[c];
+          above = lane == 0 ? j : 0;
+          for (uint32_t v = lane; v < lists && above < k; v += lanes) {
+            if (v == u) continue;
+            const uint32_t w = lbeam[v], end = lcount[v];
+            uint32_t lo = 0, len = end;
+            while (len) {
+              const uint32_t half = len / 2, e = v * kk + lo + half;
+              const double o = l.total[e];
+              const bool first = o > t || (o == t && (w < i || (w == i && before(l.key[e], l.idx[e], key, id))));
+              lo = first ? lo + half + 1 : lo;
+              len = first ? len - half - 1 : half;
+            }
+            above += lo;
+            const double e = err[i] + err[w];
+            if (w != i && e > 0. && lo < end && t - l.total[v * kk + lo] <= e)  // false for impossible entries
+              close |= (err[i] > 0. ? 1ull << i : 0ull) | (err[w] > 0. ? 1ull << w : 0ull);
           }
-          above += lo;
-          const double e = err[i] + err[w];
-          if (w != i && e > 0. && lo < end && t - l.total[v * kk + lo] <= e)  // false for impossible entries
-            close |= (err[i] > 0. ? 1ull << i : 0ull) | (err[w] > 0. ? 1ull << w : 0ull);
         }
-        if (above < k) {
-          rtotal[above] = t;
-          rbeam[above] = i;
-          rtok[above] = id;
+        for (uint32_t o = lanes / 2; o; o /= 2) {
+          above += __shfl_xor_sync(~0u, above, o);
+          close |= __shfl_xor_sync(~0u, close, o);
+        }
+        if (lane == 0 && above < k) {
+          rtotal[above] = l.total[c];
+          rbeam[above] = lbeam[u];
+          rtok[above] = l.idx[c];
           if (close) atomicOr(reinterpret_cast<unsigned long long*>(&unsure), (unsigned long long)close);
         }
       }
@@ -476,26 +464,20 @@ __global__ void __launch_bounds__(kThreads) k_select(const SelectArgs g) {
   if (rank != 0) return;
   // the best child of a beam takes its place, the others the free places in turn
   uint32_t place = tid;
-  if (a.keep_slots) {
+  if (a.keep_slots && tid < k) {
+    uint64_t seen = 0, before_me = 0;
     uint32_t later = 0;  // children before this one that do not take their beam's place
-    bool first = true;
-    if (tid < k) {
-      for (uint32_t r = 0; r < tid; ++r) {
-        bool one = true;
-        for (uint32_t q = 0; q < r; ++q) one = one && rbeam[q] != rbeam[r];
-        later += !one;
-        first = first && rbeam[r] != rbeam[tid];
-      }
-      atomicOr(reinterpret_cast<unsigned long long*>(&taken), 1ull << rbeam[tid]);
+    for (uint32_t r = 0; r < k; ++r) {
+      const uint64_t bit = 1ull << rbeam[r];
+      if (r == tid) before_me = seen;
+      later += r < tid && (seen & bit) != 0;
+      seen |= bit;
     }
-    __syncthreads();
-    if (tid < k) {
-      place = rbeam[tid];
-      if (!first) {
-        place = 0;
-        for (uint32_t n = 0;; ++place)
-          if (!(taken >> place & 1) && n++ == later) break;
-      }
+    place = rbeam[tid];
+    if (before_me >> place & 1) {
+      uint64_t open = ~seen;
+      for (uint32_t n = 0; n < later; ++n) open &= open - 1;
+      place = __ffsll((long long)open) - 1;
     }
   }
   if (tid < k) {
@@ -531,7 +513,7 @@ void beam_select(const fhe_beam_select_args& a) {
     while (g.cluster < kMaxCluster && (uint64_t)a.batch * g.cluster * 2 <= 148 * 4 &&
            packs >= (uint64_t)g.cluster * 2 * kAhead * kThreads)
       g.cluster *= 2;
-    const uint32_t shared = Layout(nullptr, (a.beams + g.cluster - 1) / g.cluster, a.beams + g.cluster, g.kk).bytes;
+    const uint32_t shared = Layout(nullptr, a.beams + g.cluster, g.kk).bytes;
     if (shared > 32768)
       FHE_CUDA(cudaFuncSetAttribute(k_select<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
     cudaLaunchConfig_t cfg{};
