@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import os
 import re
+import struct
 import threading
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
@@ -170,6 +171,19 @@ class BeamReorderArgs(ctypes.Structure):
     ]
 
 
+def packer(block):
+    """The bytes of an argument block from its values in order (pointers as integers, 0 for none; a block within it
+    as its values): a quarter of the time that making the ctypes structure takes.  Functions of these blocks are
+    declared with a plain pointer, which bytes and ``byref`` both are."""
+    codes = {i32: "i", u32: "I", i64: "q", u64: "Q", ctypes.c_float: "f", vp: "P"}
+
+    def fields(b):
+        return "".join(codes[t] if t in codes else fields(t) for _, t in b._fields_)
+    s = struct.Struct("@" + fields(block))
+    assert s.size == ctypes.sizeof(block)
+    return s.pack
+
+
 # name -> (argtypes); all return int status.
 SIGNATURES = {
     "fhe_last_error": [ctypes.c_char_p, ctypes.c_size_t],
@@ -275,13 +289,13 @@ SIGNATURES = {
     "fhe_causal_conv_backward": [ctypes.POINTER(CausalConvGradArgs)],
     "fhe_token_logprobs": [ctypes.POINTER(TokenLogprobsArgs)],
     "fhe_token_logprobs_backward": [ctypes.POINTER(TokenLogprobsGradArgs)],
-    "fhe_rms_norm": [ctypes.POINTER(RmsNormArgs)],
-    "fhe_rms_norm_backward_workspace": [ctypes.POINTER(RmsNormGradArgs), P64],
-    "fhe_rms_norm_backward": [ctypes.POINTER(RmsNormGradArgs)],
-    "fhe_embedding": [ctypes.POINTER(EmbeddingArgs)],
-    "fhe_embedding_backward_workspace": [ctypes.POINTER(EmbeddingGradArgs), P64],
-    "fhe_embedding_backward": [ctypes.POINTER(EmbeddingGradArgs)],
-    "fhe_beam_select": [ctypes.POINTER(BeamSelectArgs)],
+    "fhe_rms_norm": [vp],
+    "fhe_rms_norm_backward_workspace": [vp, P64],
+    "fhe_rms_norm_backward": [vp],
+    "fhe_embedding": [vp],
+    "fhe_embedding_backward_workspace": [vp, P64],
+    "fhe_embedding_backward": [vp],
+    "fhe_beam_select": [vp],
     "fhe_beam_reorder": [ctypes.POINTER(BeamReorderArgs)],
 }
 

@@ -29,6 +29,7 @@ from ._lib import call
 _TYPES = {torch.float32: _lib.FHE_F32, torch.bfloat16: _lib.FHE_BF16, torch.float16: _lib.FHE_F16}
 MAX_HEAD_DIM, MAX_STATE, MAX_TAPS, MAX_TOP, MAX_NORM_WIDTH = 128, 256, 8, 64, 16384
 MAX_BEAMS = 64
+_INF = float("inf")
 
 
 def _need(ok, message):
@@ -411,28 +412,46 @@ def _check_norm(op, x, weight, eps, others, dtype, groups=1, scale=1.0):
     _check_devices(op, x, weight, scale if torch.is_tensor(scale) else None, *(t for _, t, _ in others))
 
 
-def _norm_args(x, residual, gate, weight, channel_scale, eps, scale, groups, dtype, y, h, rstd):
-    """x, residual and gate as [rows, width]; x may be None in a backward pass that does not read it."""
-    first = x if x is not None else h
-    stream = h if h is not None else x
-    return _lib.RmsNormArgs(
-        first.device.index, _TYPES[dtype], _TYPES[stream.dtype] if gate is None else _TYPES[dtype],
-        first.shape[0], first.shape[1], groups, eps, scale,
-        _ptr(x), x.stride(0) if x is not None else 0, _ptr(residual), residual.stride(0) if residual is not None else 0,
-        _ptr(gate), gate.stride(0) if gate is not None else 0, _ptr(channel_scale), weight.data_ptr(),
-        _ptr(y), _ptr(h), _ptr(rstd), _stream_of(first.device.index))
+_norm_block, _norm_grad_block = _lib.packer(_lib.RmsNormArgs), _lib.packer(_lib.RmsNormGradArgs)
+
+
+def _at(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _new(t, dtype):
+    """An uninitialised contiguous tensor of t's shape."""
+    if t.is_contiguous():
+        return torch.empty_like(t) if t.dtype == dtype else torch.empty_like(t, dtype=dtype)
+    return torch.empty(t.shape, dtype=dtype, device=t.device)
+
+
+def _spaced(t):
+    """t, or evenly spaced rows of it, and the distance between rows (None: None, 0)."""
+    if t is None:
+        return None, 0
+    if t.is_contiguous():
+        return t, t.shape[-1]
+    t = _rows(t)
+    return t, t.stride(0)
+
+
+def _norm_values(like, stream, dtype, groups, eps, scale, x, residual, gate, channel_scale, weight, y, h, rstd):
+    """The argument block's values; what is made here is to be kept until the call."""
+    (x, xs), (residual, rs), (gate, gs) = _spaced(x), _spaced(residual), _spaced(gate)
+    width, device = like.shape[-1], like.get_device()
+    return (device, _TYPES[dtype], _TYPES[stream], like.numel() // width, width, groups, eps, scale, _at(x), xs,
+            _at(residual), rs, _at(gate), gs, _at(channel_scale), weight.data_ptr(), _at(y), _at(h), _at(rstd),
+            _stream_of(device)), (x, residual, gate)
 
 
 def _run_norm(x, residual, gate, weight, channel_scale, eps, scale, groups, dtype, grad):
-    d = x.device
-    y = torch.empty(x.shape, dtype=dtype, device=d)
-    h = torch.empty(x.shape, dtype=residual.dtype, device=d) if residual is not None else None
-    x2, r2, g2 = _rows(x), None if residual is None else _rows(residual), None if gate is None else _rows(gate)
-    rstd = torch.empty((x2.shape[0], groups), dtype=torch.float32, device=d) if grad else None
-    a = _norm_args(x2, r2, g2, weight, channel_scale, eps, scale, groups, dtype, y, None, rstd)
-    if h is not None:
-        a.h, a.stream_dtype = h.data_ptr(), _TYPES[h.dtype]
-    call("fhe_rms_norm", ctypes.byref(a))
+    y = _new(x, dtype)
+    h = None if residual is None else _new(x, residual.dtype)
+    stream = x.dtype if residual is None else residual.dtype
+    rstd = torch.empty((x.numel() // x.shape[-1], groups), dtype=torch.float32, device=x.device) if grad else None
+    values, kept = _norm_values(x, stream, dtype, groups, eps, scale, x, residual, gate, channel_scale, weight, y, h, rstd)
+    call("fhe_rms_norm", _norm_block(*values))
     return y, h, rstd
 
 
@@ -451,27 +470,41 @@ class _RmsNorm(torch.autograd.Function):
     def backward(ctx, dy, dh=None):
         x, gate, weight, channel_scale, h, rstd = ctx.saved_tensors
         eps, scale, groups, dtype, x_dtype = ctx.rest
-        like = x if x is not None else h
-        new = lambda shape, t: torch.empty(shape, dtype=t, device=like.device)  # noqa: E731
-        wants = ctx.needs_input_grad
+        like, wants = x if h is None else h, ctx.needs_input_grad
+        stream = like.dtype
         dy = torch.zeros(like.shape, dtype=dtype, device=like.device) if dy is None else dy.contiguous()
         dh = None if dh is None else dh.contiguous()
         # a branch added as it is has the stream's own gradient
-        shared = h is not None and channel_scale is None and scale == 1.0 and x_dtype == h.dtype
-        dres = new(like.shape, h.dtype) if h is not None and (wants[1] or (shared and wants[0])) else None
-        dx = new(like.shape, x_dtype) if wants[0] and not shared else None
-        dgate = new(like.shape, dtype) if gate is not None and wants[2] else None
-        dw = new(weight.shape, torch.float32) if wants[3] else None
-        dcs = new(weight.shape, torch.float32) if channel_scale is not None and wants[4] else None
-        x2, g2, h2 = (None if t is None else _rows(t) for t in (x, gate, h))
-        f = _norm_args(x2, h2, g2, weight, channel_scale, eps, scale, groups, dtype, None, h2, rstd)
-        g = _lib.RmsNormGradArgs(f, dy.data_ptr(), _ptr(dh), _ptr(dx), _ptr(dres), _ptr(dgate), _ptr(dw), _ptr(dcs),
-                                 None, 0, f.stream)
-        ws = _workspace("fhe_rms_norm_backward_workspace", g, like.device)
-        if ws is not None:
-            g.workspace, g.workspace_bytes = ws.data_ptr(), ws.numel()
-        call("fhe_rms_norm_backward", ctypes.byref(g))
+        shared = h is not None and channel_scale is None and scale == 1.0 and x_dtype == stream
+        dres = _new(like, stream) if h is not None and (wants[1] or (shared and wants[0])) else None
+        dx = _new(like, x_dtype) if wants[0] and not shared else None
+        dgate = _new(like, dtype) if gate is not None and wants[2] else None
+        dw = torch.empty_like(weight) if wants[3] else None
+        dcs = torch.empty_like(weight) if channel_scale is not None and wants[4] else None
+        f, kept = _norm_values(like, stream, dtype, groups, eps, scale, x, h, gate, channel_scale, weight, None, h, rstd)
+        outs = tuple(map(_at, (dy, dh, dx, dres, dgate, dw, dcs)))
+        if dw is not None or dcs is not None:
+            ws = _space("fhe_rms_norm_backward_workspace", _norm_grad_block(*f, *outs, 0, 0, 0), like.device)
+            outs += ws.data_ptr(), ws.numel()
+        else:
+            outs += 0, 0
+        call("fhe_rms_norm_backward", _norm_grad_block(*f, *outs, f[-1]))
         return dres if shared else dx, dres if wants[1] else None, dgate, dw, dcs, None, None, None, None
+
+
+def _space(name, block, device):
+    """The workspace that a packed argument block asks for."""
+    n = ctypes.c_uint64()
+    call(name, block, ctypes.byref(n))
+    return torch.empty(n.value, dtype=torch.uint8, device=device)
+
+
+def _norm_fits(x, weight, eps, dtype):
+    """Whether the arguments that all norms share pass ``_check_norm``."""
+    t, w = x.dtype, x.shape[-1] if x.dim() else 0
+    return (x.is_cuda and t in _TYPES and 1 <= w <= MAX_NORM_WIDTH and weight.shape == (w,)
+            and weight.dtype == torch.float32 and weight.get_device() == x.get_device() and 0 < eps < _INF
+            and (dtype == t or (t == torch.float32 and dtype in _TYPES)))
 
 
 def rms_norm(x, weight, eps=1e-5, dtype=None):
@@ -483,7 +516,8 @@ def rms_norm(x, weight, eps=1e-5, dtype=None):
     (a slice of wider rows will do), else x is copied.  Sums are float32; rows
     whose squares pass its range are scaled.  Gradients reach x and weight."""
     dtype = dtype or x.dtype
-    _check_norm("rms_norm", x, weight, eps, (), dtype)
+    if not _norm_fits(x, weight, eps, dtype):
+        _check_norm("rms_norm", x, weight, eps, (), dtype)
     args = (x, None, None, _dense(weight), None, float(eps), 1.0, 1, dtype)
     if _wants_grad(x, weight):
         return _RmsNorm.apply(*args)
@@ -499,8 +533,13 @@ def add_rms_norm(residual, x, weight, eps=1e-5, scale=1.0):
     scale a number, or [width] float32 for a factor of each channel.  Returns
     (y, h).  Gradients reach every tensor."""
     op = "add_rms_norm"
-    _check_norm(op, x, weight, eps, (("residual", residual, (x.dtype, torch.float32)),), x.dtype, scale=scale)
-    channel_scale, factor = (_dense(scale), 1.0) if torch.is_tensor(scale) else (None, scale)
+    t, r = x.dtype, residual.dtype
+    channel_scale, factor = (_dense(scale), 1.0) if isinstance(scale, torch.Tensor) else (None, scale)
+    if not (_norm_fits(x, weight, eps, t) and residual.shape == x.shape and (r == t or r == torch.float32)
+            and residual.get_device() == x.get_device() and -_INF < factor < _INF
+            and (channel_scale is None or (channel_scale.shape == weight.shape and channel_scale.dtype == torch.float32
+                                           and channel_scale.get_device() == x.get_device()))):
+        _check_norm(op, x, weight, eps, (("residual", residual, (t, torch.float32)),), t, scale=scale)
     args = (x, residual, None, _dense(weight), channel_scale, float(eps), float(factor), 1, x.dtype)
     if _wants_grad(x, residual, weight, channel_scale):
         return _RmsNorm.apply(*args)
@@ -514,7 +553,9 @@ def gated_rms_norm(x, gate, weight, eps=1e-5, groups=1):
     x and gate [..., width] of one type, gate usually a slice of the layer's wider
     projection; weight [width] float32; a part has at most 16384 channels.
     Products x SiLU(gate) must fit float32.  Gradients reach every tensor."""
-    _check_norm("gated_rms_norm", x, weight, eps, (("gate", gate, (x.dtype,)),), x.dtype, groups)
+    if not (groups == 1 and _norm_fits(x, weight, eps, x.dtype) and gate.shape == x.shape and gate.dtype == x.dtype
+            and gate.get_device() == x.get_device()):
+        _check_norm("gated_rms_norm", x, weight, eps, (("gate", gate, (x.dtype,)),), x.dtype, groups)
     args = (x, None, gate, _dense(weight), None, float(eps), 1.0, groups, x.dtype)
     if _wants_grad(x, gate, weight):
         return _RmsNorm.apply(*args)
@@ -524,16 +565,18 @@ def gated_rms_norm(x, gate, weight, eps=1e-5, groups=1):
 # ---- embedding ----------------------------------------------------------------------------------
 
 
-def _embedding_args(tokens, weight, scale, dtype, out):
-    return _lib.EmbeddingArgs(
-        weight.device.index, _TYPES[weight.dtype], _TYPES[dtype], tokens.dtype == torch.int64, tokens.numel(),
-        weight.shape[0], weight.shape[1], scale, tokens.data_ptr(), weight.data_ptr(), weight.stride(0), _ptr(out),
-        _stream_of(weight.device.index))
+_embedding_block, _embedding_grad_block = _lib.packer(_lib.EmbeddingArgs), _lib.packer(_lib.EmbeddingGradArgs)
+
+
+def _embedding_values(tokens, weight, scale, dtype, out):
+    device = weight.get_device()
+    return (device, _TYPES[weight.dtype], _TYPES[dtype], tokens.dtype == torch.int64, tokens.numel(), *weight.shape, scale,
+            tokens.data_ptr(), weight.data_ptr(), weight.stride(0), _at(out), _stream_of(device))
 
 
 def _run_embedding(tokens, weight, scale, dtype):
     out = torch.empty((*tokens.shape, weight.shape[1]), dtype=dtype, device=weight.device)
-    call("fhe_embedding", ctypes.byref(_embedding_args(tokens, weight, scale, dtype, out)))
+    call("fhe_embedding", _embedding_block(*_embedding_values(tokens, weight, scale, dtype, out)))
     return out
 
 
@@ -548,14 +591,11 @@ class _Embedding(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         weight, tokens = ctx.saved_tensors
-        dout = dout.contiguous()
-        dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
-        g = _lib.EmbeddingGradArgs(_embedding_args(tokens, weight, *ctx.rest, None), dout.data_ptr(), dw.data_ptr(),
-                                   None, 0, _stream_of(weight.device.index))
-        ws = _workspace("fhe_embedding_backward_workspace", g, weight.device)
-        if ws is not None:
-            g.workspace, g.workspace_bytes = ws.data_ptr(), ws.numel()
-        call("fhe_embedding_backward", ctypes.byref(g))
+        dout, dw = dout.contiguous(), _new(weight, weight.dtype)
+        f = _embedding_values(tokens, weight, *ctx.rest, None)
+        outs = dout.data_ptr(), dw.data_ptr()
+        ws = _space("fhe_embedding_backward_workspace", _embedding_grad_block(*f, *outs, 0, 0, 0), weight.device)
+        call("fhe_embedding_backward", _embedding_grad_block(*f, *outs, ws.data_ptr(), ws.numel(), f[-1]))
         return dw, None, None, None
 
 
@@ -686,6 +726,40 @@ def beam_select(logits, scores, finished=None, eos=None, width=None, keep_slots=
     Returns a ``BeamStep``: scores, parents (beams), tokens, and which beams have
     ended.  Totals are compared in 64 bits where 32 do not tell them apart."""
     op = "beam_select"
+    if not _select_fits(logits, scores, finished, eos, width, keep_slots):
+        _check_select(op, logits, scores, finished, eos, width, keep_slots)
+    if _wants_grad(logits, scores):
+        _need(False, f"{op} has no gradient")
+    (rows, stride), scores, finished = _spaced(logits), _dense(scores), _dense(finished)
+    (b, k), v, device = scores.shape, logits.shape[-1], logits.get_device()
+    width = k if width is None else width
+    out = torch.empty((b, width), dtype=torch.float32, device=logits.device)
+    parents = torch.empty_like(out, dtype=torch.int64)
+    tokens, ended = torch.empty_like(parents), torch.empty_like(out, dtype=torch.bool)
+    call("fhe_beam_select", _select_block(
+        device, _TYPES[logits.dtype], b, k, v, width, bool(keep_slots), 0, rows.data_ptr(), stride, scores.data_ptr(),
+        _at(finished), -1 if eos is None else int(eos), out.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
+        ended.data_ptr(), _stream_of(device)))
+    return BeamStep(out, parents, tokens, ended)
+
+
+_select_block = _lib.packer(_lib.BeamSelectArgs)
+
+
+def _select_fits(logits, scores, finished, eos, width, keep):
+    """Whether the arguments pass every test of ``_check_select``."""
+    if scores.dim() != 2 or logits.dim() not in (2, 3):
+        return False
+    (b, k), v, d = scores.shape, logits.shape[-1], logits.get_device()
+    w = k if width is None else width
+    return (1 <= k <= MAX_BEAMS and v >= 1 and (logits.shape[0] == b * k if logits.dim() == 2 else logits.shape[:2] == (b, k))
+            and logits.is_cuda and logits.dtype in _TYPES and scores.dtype == torch.float32 and scores.get_device() == d
+            and 1 <= w <= min(MAX_BEAMS, k * v) and (eos is None or 0 <= eos < v) and (not keep or w == k)
+            and (finished is None or (eos is not None and finished.shape == (b, k) and finished.dtype == torch.bool
+                                      and finished.get_device() == d)))
+
+
+def _check_select(op, logits, scores, finished, eos, width, keep_slots):
     _need(scores.dim() == 2 and 1 <= scores.shape[1] <= MAX_BEAMS, f"{op}: scores must be [batch, 1 to {MAX_BEAMS} beams]")
     _need(scores.dtype == torch.float32, f"{op}: scores must be {torch.float32}, got {scores.dtype}")
     b, k = scores.shape
@@ -700,18 +774,6 @@ def beam_select(logits, scores, finished=None, eos=None, width=None, keep_slots=
         _need(eos is not None, f"{op}: finished beams need an eos")
     _need(not keep_slots or width == k, f"{op}: keep_slots needs a width of the number of beams")
     _check_devices(op, logits, scores, finished)
-    _need(not _wants_grad(logits, scores), f"{op} has no gradient")
-    rows, scores, finished, d = _rows(logits), _dense(scores), _dense(finished), logits.device
-    out = torch.empty((b, width), dtype=torch.float32, device=d)
-    parents = torch.empty((b, width), dtype=torch.int64, device=d)
-    tokens = torch.empty_like(parents)
-    ended = torch.empty((b, width), dtype=torch.bool, device=d)
-    a = _lib.BeamSelectArgs(
-        d.index, _TYPES[logits.dtype], b, k, v, width, bool(keep_slots), 0, rows.data_ptr(), rows.stride(0),
-        scores.data_ptr(), _ptr(finished), -1 if eos is None else int(eos), out.data_ptr(), parents.data_ptr(),
-        tokens.data_ptr(), ended.data_ptr(), _stream_of(d.index))
-    call("fhe_beam_select", ctypes.byref(a))
-    return BeamStep(out, parents, tokens, ended)
 
 
 def beam_reorder(states, parents):
@@ -727,23 +789,30 @@ def beam_reorder(states, parents):
     _need(parents.dtype == torch.int64, f"{op}: parents must be {torch.int64}, got {parents.dtype}")
     _need(parents.shape[0] <= 65535, f"{op}: batch must be at most 65535")
     b, k = parents.shape
-    states = list(states)
+    states, device = list(states), parents.get_device()
+    rows, spans, sizes = b * k, [(parents.data_ptr(), parents.numel() * 8)], []
     for t in states:
-        _need(t.dim() >= 1 and (t.shape[0] == b * k or t.shape[:2] == (b, k)),
-              f"{op}: states must be [batch * beams, ...] or [batch, beams, ...], got {tuple(t.shape)}")
-        _need(t.is_contiguous(), f"{op}: states must be contiguous")
-    _check_devices(op, parents, *states)
-    _need(not _wants_grad(*states), f"{op} has no gradient")
-    sizes = [t.numel() * t.element_size() for t in states]
-    spans = sorted((t.data_ptr(), n) for t, n in zip([*states, parents], [*sizes, parents.numel() * 8]) if n)
-    _need(all(p + n <= q for (p, n), (q, _) in zip(spans, spans[1:])), f"{op}: states share memory")
-    if b == 0:
+        if not (t.is_contiguous() and t.get_device() == device and t.dim() and (t.shape[0] == rows or t.shape[:2] == (b, k))):
+            _need(t.dim() >= 1 and (t.shape[0] == rows or t.shape[:2] == (b, k)),
+                  f"{op}: states must be [batch * beams, ...] or [batch, beams, ...], got {tuple(t.shape)}")
+            _need(t.is_contiguous(), f"{op}: states must be contiguous")
+            _check_devices(op, parents, t)
+        n = t.nbytes
+        sizes.append(n // rows if rows else 0)
+        spans.append((t.data_ptr(), n))
+    if not parents.is_cuda:
+        _check_devices(op, parents)
+    at = [p for p, _ in spans[1:]]
+    end = 0
+    for p, n in sorted(spans):
+        _need(p >= end or not n, f"{op}: states share memory")
+        end = max(end, p + n)
+    if _wants_grad(*states):
+        _need(False, f"{op} has no gradient")
+    if not rows:
         return
     n, parents = len(states), _dense(parents)
-    a = _lib.BeamReorderArgs(
-        parents.device.index, b, k, n, (ctypes.c_void_p * n)(*(t.data_ptr() for t in states)),
-        (ctypes.c_uint64 * n)(*(size // (b * k) for size in sizes)), parents.data_ptr(),
-        _stream_of(parents.device.index))
+    a = _lib.BeamReorderArgs(device, b, k, n, (ctypes.c_void_p * n)(*at), (ctypes.c_uint64 * n)(*sizes), parents.data_ptr(),
+                             _stream_of(device))
     call("fhe_beam_reorder", ctypes.byref(a))
-    for t in states:
-        increment_version(t)
+    increment_version(states)
