@@ -33,54 +33,51 @@ __global__ void __launch_bounds__(512) k_norm(const NormArgs g) {
     }
   }
   const float n = 1.f / (float)gw;
-  for (uint32_t row = blockIdx.x * blockDim.y + threadIdx.y; row < g.rows; row += gridDim.x * blockDim.y) {
-    float h[N][8];
+  // the next row's words come while this one is summed and written
+  constexpr bool kTwo = MODE != kNormPlain;
+  using Y = std::conditional_t<MODE == kNormGate, A, H>;  // gate or residual
+  Eight<X> e[N];
+  Eight<Y> f[kTwo ? N : 1];
+  auto fetch = [&](uint32_t row) {
     const X* x = static_cast<const X*>(g.x) + (int64_t)row * g.xs + c0;
-    if constexpr (MODE == kNormPlain) {
-      Eight<X> e[N];
+    const Y* y = MODE == kNormGate ? static_cast<const Y*>(g.gate) + (int64_t)row * g.gs + c0
+                                   : static_cast<const Y*>(g.res) + (int64_t)row * g.rs + c0;
 #pragma unroll
-      for (int c = 0; c < N; ++c) load_chunk<VEC>(e[c], x, c, gw);
+    for (int c = 0; c < N; ++c) {
+      load_chunk<VEC>(e[c], x, c, gw);
+      if constexpr (kTwo) load_chunk<VEC>(f[c], y, c, gw);
+    }
+  };
+  const uint32_t step = gridDim.x * blockDim.y;
+  uint32_t row = blockIdx.x * blockDim.y + threadIdx.y;
+  if (row < g.rows) fetch(row);
+  for (; row < g.rows; row += step) {
+    float h[N][8];
+    [[maybe_unused]] H* out = static_cast<H*>(g.h) + (int64_t)row * g.width + c0;
 #pragma unroll
-      for (int c = 0; c < N; ++c) e[c].floats(h[c]);
-    } else if constexpr (MODE == kNormGate) {
-      const A* z = static_cast<const A*>(g.gate) + (int64_t)row * g.gs + c0;
-      Eight<A> e[N], f[N];
-#pragma unroll
-      for (int c = 0; c < N; ++c) {
-        load_chunk<VEC>(e[c], x, c, gw);
-        load_chunk<VEC>(f[c], z, c, gw);
-      }
-#pragma unroll
-      for (int c = 0; c < N; ++c) {
+    for (int c = 0; c < N; ++c) {
+      if constexpr (MODE == kNormPlain) {
+        e[c].floats(h[c]);
+      } else if constexpr (MODE == kNormGate) {
         float q[8], zf[8];
         f[c].floats(zf);
         sigmoid(q, zf);
         e[c].floats(h[c]);
         vmul(q, q, zf);
         vmul(h[c], h[c], q);
-      }
-    } else {
-      const H* r = static_cast<const H*>(g.res) + (int64_t)row * g.rs + c0;
-      H* out = static_cast<H*>(g.h) + (int64_t)row * g.width + c0;
-      Eight<A> e[N];
-      Eight<H> f[N];
-#pragma unroll
-      for (int c = 0; c < N; ++c) {
-        load_chunk<VEC>(f[c], r, c, gw);
-        load_chunk<VEC>(e[c], x, c, gw);
-      }
-#pragma unroll
-      for (int c = 0; c < N; ++c) {
+      } else {
         float xf[8], rf[8], s[8];
         e[c].floats(xf);
         f[c].floats(rf);
         if constexpr (MODE == kNormAddScaled) vfma(h[c], cs[c], xf, rf);
         else vset(s, g.scale), vfma(h[c], s, xf, rf);
-        f[c].set(h[c]);
-        store_chunk<VEC>(f[c], out, c, gw);
-        f[c].floats(h[c]);
+        Eight<H> kept;
+        kept.set(h[c]);
+        store_chunk<VEC>(kept, out, c, gw);
+        kept.floats(h[c]);
       }
     }
+    if (row + step < g.rows) fetch(row + step);
     float part[2] = {0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < N; ++c)
@@ -166,7 +163,7 @@ void rms_norm(const fhe_rms_norm_args& a) {
   const bool vec = g.gw % 8 == 0 && norm_aligned(a.x, a.x_stride, ex) && norm_aligned(a.residual, a.residual_stride, eh) &&
                    norm_aligned(a.gate, a.gate_stride, ea) && norm_aligned(a.channel_scale, 0, 4) &&
                    norm_aligned(a.weight, 0, 4) && norm_aligned(a.y, 0, ea) && norm_aligned(a.h, 0, eh);
-  const NormShape s = norm_shape(g.gw, (uint64_t)a.rows * a.groups, vec, false);
+  const NormShape s = norm_shape(g.gw, (uint64_t)a.rows * a.groups, vec);
   const uint32_t blocks = std::min((a.rows + s.rows_per_block - 1) / s.rows_per_block,
                                    std::max(1u, 148 * 12 / a.groups));
   with_norm(a, s.chunks, vec, [&](auto mode, auto act, auto str, auto chunks, auto words) {

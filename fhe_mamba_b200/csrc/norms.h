@@ -21,6 +21,7 @@ struct NormArgs {
   float* part;  // sums of each block: [grid.x][width] for the weight, then as much for the channel scale
   uint32_t rows, width, gw, groups;
   float eps, scale;
+  int stages;  // rows in the gradients' ring
 };
 
 // Eight elements as 16-byte words (or, where alignment does not allow that,
@@ -99,16 +100,15 @@ struct RowSum {
 
 // Warps per row and chunks of eight channels per thread.  Few rows are spread over
 // as many warps as have a chunk.  Else a thread takes three chunks where that fills
-// every lane, four (the gradients and single elements, which need more registers:
-// two), and rows past 16 warps of that take four.  Four rows of one warp share a
-// block, a longer row has its own.
+// every lane, else four (single elements, which need more registers: two); at most 16
+// warps.  Four rows of one warp share a block, a longer row has its own.
 struct NormShape {
   uint32_t warps, chunks, rows_per_block;
 };
-inline NormShape norm_shape(uint32_t gw, uint64_t rows, bool vec, bool grad) {
+inline NormShape norm_shape(uint32_t gw, uint64_t rows, bool vec) {
   const uint32_t all = (gw + 7) / 8;
   const bool whole = vec && all % 96 == 0 && all / 96 <= 8;
-  const uint32_t want = rows < 2 * 148 ? 1 : whole ? 3 : vec && !grad ? 4 : 2;
+  const uint32_t want = rows < 2 * 148 ? 1 : whole ? 3 : vec ? 4 : 2;
   NormShape s;
   s.warps = std::min(16u, (all + 32 * want - 1) / (32 * want));
   s.chunks = (all + 32 * s.warps - 1) / (32 * s.warps);

@@ -1,20 +1,43 @@
 // Gradients of the root-mean-square norms (fhe_rms_norm_backward).
 //
 // With a = dy w and u = h r: dh = r (a - u mean(a u)) (+ the gradient that h
-// itself has), dweight = sum over rows of dy u.  Like the norm, a row lies in
-// registers and is read once; a block keeps its share of the sums over rows in
-// registers from row to row, and a second launch adds the blocks' shares in a
-// fixed order.
+// itself has), dweight = sum over rows of dy u.  Like the norm, a row is spread
+// over one to sixteen warps and read once.  Its words come by asynchronous copies
+// through each thread's own part of shared memory, rows ahead, and are taken from
+// there twice, for the mean and for the gradients; single elements are held in
+// registers.  A block keeps its share of the sums over rows in registers from row
+// to row, and a second launch adds the blocks' shares in a fixed order.
 #include "launch_count.h"
 #include "norms.h"
 
 namespace fhe {
 namespace {
 
+// Through the first cache where a thread's two words of float32 lie in one sector,
+// past it otherwise.
+template <bool TWO>
+__device__ __forceinline__ void copy16(void* to, const void* from) {
+  const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
+  if constexpr (TWO) asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+  else asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+}
+
+// A thread's share of a row in shared memory, in 16-byte words: what is read twice
+// stays out of the registers, and the loads of the next rows run behind the
+// arithmetic of this one.
+template <int MODE, class A, class H, int N>
+struct GradRing {
+  static constexpr bool kAdd = MODE == kNormAdd || MODE == kNormAddScaled;
+  static constexpr int kWa = sizeof(A) / 2, kWs = (MODE == kNormGate ? sizeof(A) : sizeof(H)) / 2, kWh = sizeof(H) / 2;
+  static constexpr int kS = 0, kDy = kS + N * kWs, kZ = kDy + N * kWa,
+                       kDh = kZ + (MODE == kNormGate || MODE == kNormAddScaled ? N * kWa : 0),
+                       kWords = kDh + (kAdd ? N * kWh : 0);
+};
+
 template <int MODE, class A, class H, int N, bool VEC>
 __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs g) {
   __shared__ float red[2][16];
-  extern __shared__ float sums[];  // [channels of the group]
+  extern __shared__ __align__(16) float sums[];  // the ring of rows; then sums over a block's rows
   RowSum row_sum{red};
   constexpr bool kAdd = MODE == kNormAdd || MODE == kNormAddScaled, kScaled = MODE == kNormAddScaled;
   using X = std::conditional_t<MODE == kNormPlain, H, A>;  // x
@@ -35,30 +58,91 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
     }
   }
   const float n = 1.f / (float)gw;
-  for (uint32_t row = blockIdx.x * blockDim.y + threadIdx.y; row < g.rows; row += gridDim.x * blockDim.y) {
+  // what a row is read from: h or x, dy, gate or (for the channel scale) x, dh
+  constexpr bool kThird = MODE == kNormGate || kScaled;
+  using Ring = GradRing<MODE, A, H, N>;
+  Eight<S> s[VEC ? 1 : N];
+  Eight<A> dy[VEC ? 1 : N], z[kThird && !VEC ? N : 1];
+  Eight<H> dh[kAdd && !VEC ? N : 1];
+  uint8_t* ring = reinterpret_cast<uint8_t*>(sums) + (threadIdx.y * blockDim.x + threadIdx.x) * 16;
+  auto visit = [&](uint32_t row, int stage, auto&& f_s, auto&& f_dy, auto&& f_z, auto&& f_dh) {
     const int64_t out = (int64_t)row * g.width + c0;
     const S* src = kAdd ? static_cast<const S*>(g.h) + out : static_cast<const S*>(g.x) + (int64_t)row * g.xs + c0;
-    const A* dyp = static_cast<const A*>(g.dy) + out;
-    Eight<S> s[N];
-    Eight<A> dy[N], z[MODE == kNormGate || kScaled ? N : 1];
-    Eight<H> dh[kAdd ? N : 1];
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-      load_chunk<VEC>(s[c], src, c, gw);
-      load_chunk<VEC>(dy[c], dyp, c, gw);
-      if constexpr (MODE == kNormGate) load_chunk<VEC>(z[c], static_cast<const A*>(g.gate) + (int64_t)row * g.gs + c0, c, gw);
-      if constexpr (kScaled) load_chunk<VEC>(z[c], static_cast<const A*>(g.x) + (int64_t)row * g.xs + c0, c, gw);
+      f_s(src, c);
+      f_dy(static_cast<const A*>(g.dy) + out, c);
+      if constexpr (MODE == kNormGate) f_z(static_cast<const A*>(g.gate) + (int64_t)row * g.gs + c0, c);
+      if constexpr (kScaled) f_z(static_cast<const A*>(g.x) + (int64_t)row * g.xs + c0, c);
       if constexpr (kAdd)
-        if (g.dh) load_chunk<VEC>(dh[c], static_cast<const H*>(g.dh) + out, c, gw);
+        if (g.dh) f_dh(static_cast<const H*>(g.dh) + out, c);
+    }
+  };
+  const uint32_t step = gridDim.x * blockDim.y, row0 = blockIdx.x * blockDim.y + threadIdx.y;
+  const uint32_t threads = blockDim.x * blockDim.y;
+  auto fetch = [&](uint32_t row, int stage) {
+    if constexpr (VEC) {
+      if (row < g.rows) {
+        auto copy = [&](int first) {
+          return [&, first](const auto* p, int c) {
+            constexpr int W = sizeof(*p) / 2;  // 16-byte words of a chunk
+            const uint32_t at = channel<true>(c, 0);
+#pragma unroll
+            for (int k = 0; k < W; ++k)
+              if (at < gw) copy16<W == 2>(ring + (uint64_t)(stage * Ring::kWords + first + c * W + k) * threads * 16, p + at + k * (8 / W));
+          };
+        };
+        visit(row, stage, copy(Ring::kS), copy(Ring::kDy), copy(Ring::kZ), copy(Ring::kDh));
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    } else if (row < g.rows) {
+      visit(row, 0, [&](const S* p, int c) { load_chunk<VEC>(s[c], p, c, gw); },
+            [&](const A* p, int c) { load_chunk<VEC>(dy[c], p, c, gw); },
+            [&](const A* p, int c) { load_chunk<VEC>(z[c], p, c, gw); },
+            [&](const H* p, int c) { load_chunk<VEC>(dh[c], p, c, gw); });
+    }
+  };
+  const int stages = g.stages;
+  int stage = 0;
+  // chunk c of an array, from the ring or the registers; lanes past the row hold 0
+  auto take = [&](auto* held, int first, int c, float (&o)[8]) {
+    using T = std::remove_pointer_t<decltype(held)>;
+    if constexpr (VEC) {
+      constexpr int W = sizeof(T) / 16;
+      T e;
+#pragma unroll
+      for (int k = 0; k < W; ++k)
+        reinterpret_cast<uint4*>(&e)[k] = channel<true>(c, 0) < gw
+            ? *reinterpret_cast<const uint4*>(ring + (uint64_t)(stage * Ring::kWords + first + c * W + k) * threads * 16)
+            : make_uint4(0, 0, 0, 0);
+      e.floats(o);
+    } else {
+      held[c].floats(o);
+    }
+  };
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (i + 1 < stages) fetch(row0 + i * step, i);
+  }
+  for (uint32_t row = row0; row < g.rows; row += step) {
+    const int64_t out = (int64_t)row * g.width + c0;
+    if constexpr (VEC) {
+      fetch(row + (stages - 1) * step, stage ? stage - 1 : stages - 1);
+      if (stages == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+      else if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+      else asm volatile("cp.async.wait_group 0;" ::: "memory");
+    } else {
+      fetch(row, 0);
     }
     const float r = g.rstd[(int64_t)row * g.groups + blockIdx.y];
     float rr[8];
     vset(rr, r);
     // u = h r; with a gate also p = SiLU(gate)
     auto unit = [&](int c, float (&u)[8], float (&xf)[8], float (&p)[8], float (&q)[8], float (&zf)[8]) {
-      s[c].floats(xf);
+      take(s, Ring::kS, c, xf);
       if constexpr (MODE == kNormGate) {
-        z[c].floats(zf);
+        take(z, Ring::kZ, c, zf);
         sigmoid(q, zf);
         vmul(p, q, zf);
         vmul(u, xf, p);
@@ -72,7 +156,7 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
     for (int c = 0; c < N; ++c) {
       float u[8], xf[8], p[8], q[8], zf[8], d[8], a[8];
       unit(c, u, xf, p, q, zf);
-      dy[c].floats(d);
+      take(dy, Ring::kDy, c, d);
       vmul(a, d, u);
       vadd(dw[c], dw[c], a);
 #pragma unroll
@@ -88,13 +172,13 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
     for (int c = 0; c < N; ++c) {
       float u[8], xf[8], p[8], q[8], zf[8], d[8];
       unit(c, u, xf, p, q, zf);
-      dy[c].floats(d);
+      take(dy, Ring::kDy, c, d);
       vmul(d, d, w[c]);
       vfma(d, u, mm, d);
       if constexpr (kAdd) {
         float e[8];
         vset(e, 0.f);
-        if (g.dh) dh[c].floats(e);
+        if (g.dh) take(dh, Ring::kDh, c, e);
         vfma(d, d, rr, e);
       } else {
         vmul(d, d, rr);
@@ -116,7 +200,7 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
       } else {
         if constexpr (kScaled) {
           float xg[8];
-          z[c].floats(xg);
+          take(z, Ring::kZ, c, xg);
           vfma(dcs[c], d, xg, dcs[c]);
         }
         if constexpr (kAdd) {
@@ -133,7 +217,9 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
         if (g.dx) store_chunk<VEC>(e, static_cast<X*>(g.dx) + out, c, gw);
       }
     }
+    stage = stage + 1 == stages ? 0 : stage + 1;
   }
+  if constexpr (VEC) asm volatile("cp.async.wait_all;" ::: "memory");
   // the block's rows together, one after the other
   auto gather = [&](float (&v)[N][8], float* to, float k) {
     for (uint32_t turn = 0; turn < blockDim.y; ++turn) {
@@ -158,25 +244,25 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
   }
 }
 
-// Adds the blocks' shares: 32 channels x 16 strands of blocks.
-__global__ void __launch_bounds__(512) k_norm_sum(const float* part, uint32_t blocks, uint32_t width, float* dweight,
-                                                  float* dcscale) {
-  __shared__ float s[16][33];
+// Adds the blocks' shares: 32 channels x 32 strands of blocks.
+__global__ void __launch_bounds__(1024) k_norm_sum(const float* part, uint32_t blocks, uint32_t width, float* dweight,
+                                                   float* dcscale) {
+  __shared__ float s[32][33];
   const uint32_t c = blockIdx.x * 32 + threadIdx.x;
   float* out = blockIdx.y ? dcscale : dweight;
   if (!out) return;
   part += (int64_t)blockIdx.y * blocks * width;
   float v = 0.f;
   if (c < width) {
-#pragma unroll 8
-    for (uint32_t b = threadIdx.y; b < blocks; b += 16) v += part[(int64_t)b * width + c];
+#pragma unroll 10
+    for (uint32_t b = threadIdx.y; b < blocks; b += 32) v += part[(int64_t)b * width + c];
   }
   s[threadIdx.y][threadIdx.x] = v;
   __syncthreads();
-  if (threadIdx.y == 0 && c < width) {
-    for (int i = 1; i < 16; ++i) v += s[i][threadIdx.x];
-    out[c] = v;
-  }
+  v = s[threadIdx.x][threadIdx.y];  // strand x of channel y
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  if (threadIdx.x == 0 && blockIdx.x * 32 + threadIdx.y < width) out[blockIdx.x * 32 + threadIdx.y] = v;
 }
 
 bool words(const fhe_rms_norm_grad_args& a) {
@@ -191,15 +277,41 @@ bool words(const fhe_rms_norm_grad_args& a) {
          norm_aligned(a.dgate, 0, ea);
 }
 
-NormShape grad_shape(const fhe_rms_norm_grad_args& a) {
-  return norm_shape(a.f.width / a.f.groups, (uint64_t)a.f.rows * a.f.groups, words(a), true);
-}
-
-// Blocks that go from row to row: 16 warps an SM.
-uint32_t grad_blocks(const fhe_rms_norm_grad_args& a, const NormShape& s) {
-  const uint32_t resident = std::max(1u, 16 / (s.warps * s.rows_per_block));
-  return std::max(1u, std::min((a.f.rows + s.rows_per_block - 1) / s.rows_per_block,
-                               std::max(1u, 148 * resident / a.f.groups)));
+// How a call is laid out: shape, rows of the ring (up to three, as far as 12 warps
+// still fit an SM), shared memory, and blocks that go from row to row, as many as
+// are resident.
+struct GradPlan {
+  NormShape shape;
+  bool vec;
+  uint32_t stages, shared, blocks;
+};
+GradPlan grad_plan(const fhe_rms_norm_grad_args& a) {
+  constexpr uint32_t kShared = 227 * 1024, kOwn = 1024 + 128;  // of an SM; of a block beside its ring
+  const fhe_rms_norm_args& f = a.f;
+  const uint32_t gw = f.width / f.groups;
+  const uint32_t wa = elem_size(f.dtype) / 2, wh = f.gate ? wa : elem_size(f.stream_dtype) / 2;
+  const uint32_t per_chunk = (f.gate ? wa : wh) + wa + (f.gate || f.channel_scale ? wa : 0) + (f.residual ? wh : 0);
+  GradPlan p{};
+  p.vec = words(a);
+  for (;; p.vec = false) {
+    p.shape = norm_shape(gw, (uint64_t)f.rows * f.groups, p.vec);
+    const uint32_t warps = p.shape.warps * p.shape.rows_per_block;
+    uint32_t resident = std::max(1u, 16 / warps);
+    p.shared = p.shape.rows_per_block > 1 ? gw * sizeof(float) : 0;  // one warp's channels, at most 1024
+    if (p.vec) {
+      const uint32_t row = p.shape.chunks * per_chunk * 16 * 32 * warps;
+      if (row + kOwn > kShared) continue;
+      for (p.stages = 3; p.stages > 1; --p.stages) {
+        const uint32_t fit = kShared / (p.stages * row + kOwn);
+        if (fit && fit * warps >= 12) break;
+      }
+      p.shared = std::max(p.shared, p.stages * row);
+      resident = std::max(1u, std::min(resident, kShared / (p.shared + kOwn)));
+    }
+    p.blocks = std::max(1u, std::min((f.rows + p.shape.rows_per_block - 1) / p.shape.rows_per_block,
+                                     std::max(1u, 148 * resident / f.groups)));
+    return p;
+  }
 }
 
 bool sums_wanted(const fhe_rms_norm_grad_args& a) { return a.dweight || a.dchannel_scale; }
@@ -209,7 +321,7 @@ bool sums_wanted(const fhe_rms_norm_grad_args& a) { return a.dweight || a.dchann
 uint64_t rms_norm_backward_workspace(const fhe_rms_norm_grad_args& a) {
   check_norm(a.f);
   if (!sums_wanted(a)) return 0;
-  return (uint64_t)grad_blocks(a, grad_shape(a)) * a.f.width * sizeof(float) * (a.f.channel_scale ? 2 : 1);
+  return (uint64_t)grad_plan(a).blocks * a.f.width * sizeof(float) * (a.f.channel_scale ? 2 : 1);
 }
 
 void rms_norm_backward(const fhe_rms_norm_grad_args& a) {
@@ -235,18 +347,18 @@ void rms_norm_backward(const fhe_rms_norm_grad_args& a) {
   g.dres = a.dresidual;
   g.dgate = a.dgate;
   g.part = sums_wanted(a) ? static_cast<float*>(a.workspace) : nullptr;
-  const bool vec = words(a);
-  const NormShape s = grad_shape(a);
-  const uint32_t blocks = grad_blocks(a, s);
-  const size_t shared = s.rows_per_block > 1 ? g.gw * sizeof(float) : 0;  // at most 1024 channels: one warp's
-  with_norm(f, s.chunks, vec, [&](auto mode, auto act, auto str, auto chunks, auto words) {
-    k_norm_grad<decltype(mode)::value, decltype(act), decltype(str), decltype(chunks)::value, decltype(words)::value>
-        <<<dim3(blocks, f.groups), dim3(32 * s.warps, s.rows_per_block), shared, st>>>(g);
+  const GradPlan p = grad_plan(a);
+  g.stages = (int)p.stages;
+  with_norm(f, p.shape.chunks, p.vec, [&](auto mode, auto act, auto str, auto chunks, auto words) {
+    auto k = k_norm_grad<decltype(mode)::value, decltype(act), decltype(str), decltype(chunks)::value,
+                         decltype(words)::value>;
+    if (p.shared > 48000) FHE_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.shared));
+    k<<<dim3(p.blocks, f.groups), dim3(32 * p.shape.warps, p.shape.rows_per_block), p.shared, st>>>(g);
   });
   note_launch();
   if (g.part) {
-    k_norm_sum<<<dim3((f.width + 31) / 32, f.channel_scale ? 2 : 1), dim3(32, 16), 0, st>>>(
-        g.part, blocks, f.width, a.dweight, a.dchannel_scale);
+    k_norm_sum<<<dim3((f.width + 31) / 32, f.channel_scale ? 2 : 1), dim3(32, 32), 0, st>>>(
+        g.part, p.blocks, f.width, a.dweight, a.dchannel_scale);
     note_launch();
   }
   FHE_CUDA(cudaGetLastError());
