@@ -15,79 +15,117 @@ namespace {
 template <int MODE, class A, class H, int N, bool VEC>
 __global__ void __launch_bounds__(512) k_norm(const NormArgs g) {
   __shared__ float red[2][16];
+  extern __shared__ __align__(16) uint8_t shared[];
   RowSum row_sum{red};
+  constexpr bool kTwo = MODE != kNormPlain, kRing = MODE == kNormGate && VEC;
   using X = std::conditional_t<MODE == kNormPlain, H, A>;
-  const uint32_t gw = g.gw, c0 = blockIdx.y * gw;
-  float w[N][8];
-  float cs[MODE == kNormAddScaled ? N : 1][8];
+  using Y = std::conditional_t<MODE == kNormGate, A, H>;  // gate or residual
+  const uint32_t c0 = blockIdx.y * g.gw + from<N, VEC>();
+  const int left = (int)g.gw - (int)from<N, VEC>();
+  const X* xp = static_cast<const X*>(g.x) + c0;
+  const Y* yp = static_cast<const Y*>(MODE == kNormGate ? g.gate : g.res) + c0;
+  const int64_t ys = MODE == kNormGate ? g.gs : g.rs;
+  Eight<float> w[N], cs[MODE == kNormAddScaled ? N : 1];
 #pragma unroll
   for (int c = 0; c < N; ++c) {
-    Eight<float> e;
-    load_chunk<VEC>(e, g.weight + c0, c, gw);
-    e.floats(w[c]);
+    w[c].clear();
+    load_chunk<VEC>(w[c], g.weight + c0, c, left);
     if constexpr (MODE == kNormAddScaled) {
-      load_chunk<VEC>(e, g.cscale + c0, c, gw);
-      e.floats(cs[c]);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) cs[c][i] *= g.scale;
+      cs[c].clear();
+      load_chunk<VEC>(cs[c], g.cscale + c0, c, left);
     }
   }
-  const float n = 1.f / (float)gw;
-  // the next row's words come while this one is summed and written
-  constexpr bool kTwo = MODE != kNormPlain;
-  using Y = std::conditional_t<MODE == kNormGate, A, H>;  // gate or residual
-  Eight<X> e[N];
-  Eight<Y> f[kTwo ? N : 1];
-  auto fetch = [&](uint32_t row) {
-    const X* x = static_cast<const X*>(g.x) + (int64_t)row * g.xs + c0;
-    const Y* y = MODE == kNormGate ? static_cast<const Y*>(g.gate) + (int64_t)row * g.gs + c0
-                                   : static_cast<const Y*>(g.res) + (int64_t)row * g.rs + c0;
-#pragma unroll
-    for (int c = 0; c < N; ++c) {
-      load_chunk<VEC>(e[c], x, c, gw);
-      if constexpr (kTwo) load_chunk<VEC>(f[c], y, c, gw);
-    }
-  };
+  const float n = 1.f / (float)g.gw;
   const uint32_t step = gridDim.x * blockDim.y;
   uint32_t row = blockIdx.x * blockDim.y + threadIdx.y;
-  if (row < g.rows) fetch(row);
+  // The next row's words come while this one is summed and written: into registers,
+  // or with a gate, whose sigmoids take longer, one or two rows ahead through a ring.
+  Eight<X> e[N];
+  Eight<Y> f[kTwo ? N : 1];
+  constexpr int kQ = Eight<A>::kQuads;
+  const Ring<2 * N * kQ> ring(shared, g.stages);
+  int stage = 0;
+  auto fetch = [&](uint32_t at, [[maybe_unused]] int to) {
+    if (at < g.rows) {
+      const X* x = xp + (int64_t)at * g.xs;
+      const Y* y = yp + (int64_t)at * ys;
+#pragma unroll
+      for (int c = 0; c < N; ++c) {
+        if constexpr (kRing) {
+          ring.copy(to, 0, x, c, left);
+          ring.copy(to, N * kQ, y, c, left);
+        } else {
+          load_chunk<VEC>(e[c], x, c, left);
+          if constexpr (kTwo) load_chunk<VEC>(f[c], y, c, left);
+        }
+      }
+    }
+    if constexpr (kRing) asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if constexpr (kRing) {
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      ring.blank(g.stages, 0, xp, c, left);
+      ring.blank(g.stages, N * kQ, yp, c, left);
+    }
+    for (int i = 0; i + 1 < g.stages; ++i) fetch(row + i * step, i);
+  } else {
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      e[c].clear();
+      if constexpr (kTwo) f[c].clear();
+    }
+    fetch(row, 0);
+  }
   for (; row < g.rows; row += step) {
+    if constexpr (kRing) {
+      fetch(row + (g.stages - 1) * step, stage ? stage - 1 : g.stages - 1);
+      wait_copies(g.stages);
+#pragma unroll
+      for (int c = 0; c < N; ++c) {
+        ring.take(e[c], stage, 0, c);
+        ring.take(f[c], stage, N * kQ, c);
+      }
+      stage = stage + 1 == g.stages ? 0 : stage + 1;
+    }
     float h[N][8];
     [[maybe_unused]] H* out = static_cast<H*>(g.h) + (int64_t)row * g.width + c0;
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-      if constexpr (MODE == kNormPlain) {
-        e[c].floats(h[c]);
-      } else if constexpr (MODE == kNormGate) {
+      e[c].floats(h[c]);
+      if constexpr (MODE == kNormGate) {
         float q[8], zf[8];
         f[c].floats(zf);
         sigmoid(q, zf);
-        e[c].floats(h[c]);
         vmul(q, q, zf);
         vmul(h[c], h[c], q);
-      } else {
-        float xf[8], rf[8], s[8];
-        e[c].floats(xf);
+      } else if constexpr (kTwo) {
+        float rf[8], s[8];
         f[c].floats(rf);
-        if constexpr (MODE == kNormAddScaled) vfma(h[c], cs[c], xf, rf);
-        else vset(s, g.scale), vfma(h[c], s, xf, rf);
+        vset(s, g.scale);
+        if constexpr (MODE == kNormAddScaled) {
+          float v[8];
+          cs[c].floats(v);
+          vmul(s, s, v);
+        }
+        vfma(h[c], s, h[c], rf);
         Eight<H> kept;
         kept.set(h[c]);
-        store_chunk<VEC>(kept, out, c, gw);
+        store_chunk<VEC>(kept, out, c, left);
         kept.floats(h[c]);
       }
     }
-    if (row + step < g.rows) fetch(row + step);
-    float part[2] = {0.f, 0.f};
+    if constexpr (!kRing) fetch(row + step, 0);
+    float part[2][2] = {};
 #pragma unroll
     for (int c = 0; c < N; ++c)
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
         const float p[2] = {h[c][i], h[c][i + 1]};
-        vfma(part, p, p, part);
+        vfma(part[i / 2 % 2], p, p, part[i / 2 % 2]);
       }
-    const float ss = row_sum(part[0] + part[1]);
-    float r = 1.f / sqrtf(fmaf(ss, n, g.eps));
+    const float ss = row_sum((part[0][0] + part[0][1]) + (part[1][0] + part[1][1]));
+    float r = rsqrtf(fmaf(ss, n, g.eps));
     // squares past fp32's range: the row again, scaled (an infinity of the row itself gives r = 0)
     if (ss == INFINITY) {
       const float k = 0x1p-80f;
@@ -102,15 +140,17 @@ __global__ void __launch_bounds__(512) k_norm(const NormArgs g) {
     A* y = static_cast<A*>(g.y) + (int64_t)row * g.width + c0;
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-      float o[8], rr[8];
+      float o[8], rr[8], wf[8];
+      w[c].floats(wf);
       vset(rr, r);
       vmul(o, h[c], rr);
-      vmul(o, o, w[c]);
-      Eight<A> e;
-      e.set(o);
-      store_chunk<VEC>(e, y, c, gw);
+      vmul(o, o, wf);
+      Eight<A> to;
+      to.set(o);
+      store_chunk<VEC>(to, y, c, left);
     }
   }
+  if constexpr (kRing) asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 }  // namespace
@@ -157,18 +197,30 @@ void rms_norm(const fhe_rms_norm_args& a) {
   if (a.rows == 0) return;
   require(a.x && a.weight && a.y && (!a.residual || a.h), "null input or output");
   DeviceGuard dev(a.device);
-  const NormArgs g = norm_args(a);
+  NormArgs g = norm_args(a);
   const uint32_t ea = elem_size(a.dtype), eh = a.gate ? ea : elem_size(a.stream_dtype);
   const uint32_t ex = a.gate || a.residual ? ea : eh;
   const bool vec = g.gw % 8 == 0 && norm_aligned(a.x, a.x_stride, ex) && norm_aligned(a.residual, a.residual_stride, eh) &&
                    norm_aligned(a.gate, a.gate_stride, ea) && norm_aligned(a.channel_scale, 0, 4) &&
                    norm_aligned(a.weight, 0, 4) && norm_aligned(a.y, 0, ea) && norm_aligned(a.h, 0, eh);
   const NormShape s = norm_shape(g.gw, (uint64_t)a.rows * a.groups, vec);
+  // blocks that go from row to row: with a ring as many as are resident
+  uint32_t resident = 12, shared = 0;
+  if (a.gate && vec) {
+    const uint32_t warps = s.warps * s.rows_per_block, row = s.chunks * ea * 16 * 32 * warps;
+    for (g.stages = 3; g.stages > 1; --g.stages) {
+      const uint32_t fit = kSmShared / (g.stages * row + kBlockShared);
+      if (fit && fit * warps >= 20) break;
+    }
+    shared = g.stages * row;
+    resident = std::max(1u, std::min(24 / warps, kSmShared / (shared + kBlockShared)));
+  }
   const uint32_t blocks = std::min((a.rows + s.rows_per_block - 1) / s.rows_per_block,
-                                   std::max(1u, 148 * 12 / a.groups));
+                                   std::max(1u, 148 * resident / a.groups));
   with_norm(a, s.chunks, vec, [&](auto mode, auto act, auto str, auto chunks, auto words) {
-    k_norm<decltype(mode)::value, decltype(act), decltype(str), decltype(chunks)::value, decltype(words)::value>
-        <<<dim3(blocks, a.groups), dim3(32 * s.warps, s.rows_per_block), 0, static_cast<cudaStream_t>(a.stream)>>>(g);
+    auto k = k_norm<decltype(mode)::value, decltype(act), decltype(str), decltype(chunks)::value, decltype(words)::value>;
+    if (shared > 48000) FHE_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
+    k<<<dim3(blocks, a.groups), dim3(32 * s.warps, s.rows_per_block), shared, static_cast<cudaStream_t>(a.stream)>>>(g);
   });
   note_launch();
   FHE_CUDA(cudaGetLastError());

@@ -21,62 +21,153 @@ struct NormArgs {
   float* part;  // sums of each block: [grid.x][width] for the weight, then as much for the channel scale
   uint32_t rows, width, gw, groups;
   float eps, scale;
-  int stages;  // rows in the gradients' ring
+  int stages;  // rows in the ring
 };
 
-// Eight elements as 16-byte words (or, where alignment does not allow that,
-// element by element).
+// Eight elements as 32-bit words, in memory's order.
 template <class T>
 struct alignas(16) Eight {
-  T v[8];
+  static constexpr int kWords = sizeof(T) * 2, kQuads = kWords / 4;  // of 4 and of 16 bytes
+  uint32_t w[kWords];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+  }
   __device__ __forceinline__ void floats(float (&o)[8]) const {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = to_f(v[i]);
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        o[i] = __uint_as_float(w[i]);
+      } else if constexpr (std::is_same_v<T, __half>) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        o[2 * i] = f.x, o[2 * i + 1] = f.y;
+      } else {
+        o[2 * i] = __uint_as_float(w[i] << 16), o[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    }
   }
   __device__ __forceinline__ void set(const float (&f)[8]) {
-    const Pack<T, 8> p = pack<T, 8>(f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = p.v[i];
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        w[i] = __float_as_uint(f[i]);
+      } else if constexpr (std::is_same_v<T, __half>) {
+        const __half2 p = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&p);
+      } else {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&p);
+      }
+    }
   }
 };
 
-// A row's (or group's) channels over T = blockDim.x threads: chunk c of thread t
-// holds channels (c T + t) 8 .. + 8 where words are loaded, (c 8 + i) T + t
-// otherwise; both read consecutive memory across a warp.
+// A row's (or group's) channels over warps: N chunks of 256 to a warp.  Chunk c of a
+// lane holds the channels from(): + c 256 .. + 8 where 16-byte words are loaded,
+// + (c 8 + i) 32 otherwise; both read consecutive memory across a warp, at constant
+// distances.
+template <int N, bool VEC>
+__device__ __forceinline__ uint32_t from() {
+  return (threadIdx.x >> 5) * (N * 256) + (threadIdx.x & 31) * (VEC ? 8 : 1);
+}
 template <bool VEC>
-__device__ __forceinline__ uint32_t channel(int c, int i) {
-  return VEC ? (c * blockDim.x + threadIdx.x) * 8 + i : (c * 8 + i) * blockDim.x + threadIdx.x;
+__host__ __device__ constexpr int away(int c, int i) {
+  return VEC ? c * 256 + i : (c * 8 + i) * 32;
 }
+// Chunk c of the lane's channels at p; `left` of them are before the row's end, the
+// others stay as they are.
 template <bool VEC, class T>
-__device__ __forceinline__ void load_chunk(Eight<T>& e, const T* p, int c, uint32_t gw) {
+__device__ __forceinline__ void load_chunk(Eight<T>& e, const T* p, int c, int left) {
   if constexpr (VEC) {
-    const uint32_t at = channel<true>(c, 0);
-    if (at < gw) {
-      const uint4* s = reinterpret_cast<const uint4*>(p + at);
+    if (away<true>(c, 0) < left) {
 #pragma unroll
-      for (int k = 0; k < (int)sizeof(T) / 2; ++k) reinterpret_cast<uint4*>(&e)[k] = s[k];
-      return;
+      for (int k = 0; k < Eight<T>::kQuads; ++k)
+        reinterpret_cast<uint4*>(e.w)[k] = reinterpret_cast<const uint4*>(p + away<true>(c, 0))[k];
     }
-#pragma unroll
-    for (int k = 0; k < (int)sizeof(T) / 2; ++k) reinterpret_cast<uint4*>(&e)[k] = make_uint4(0, 0, 0, 0);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e.v[i] = channel<false>(c, i) < gw ? p[channel<false>(c, i)] : from_f<T>(0.f);
-  }
-}
-template <bool VEC, class T>
-__device__ __forceinline__ void store_chunk(const Eight<T>& e, T* p, int c, uint32_t gw) {
-  if constexpr (VEC) {
-    const uint32_t at = channel<true>(c, 0);
-    if (at >= gw) return;
-#pragma unroll
-    for (int k = 0; k < (int)sizeof(T) / 2; ++k)
-      reinterpret_cast<uint4*>(p + at)[k] = reinterpret_cast<const uint4*>(&e)[k];
-  } else {
+  } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (channel<false>(c, i) < gw) p[channel<false>(c, i)] = e.v[i];
+      if (away<false>(c, i) < left) e.w[i] = reinterpret_cast<const uint32_t*>(p)[away<false>(c, i)];
+  } else {
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+    uint32_t v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = away<false>(c, i) < left ? q[away<false>(c, i)] : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e.w[i] = v[2 * i] | v[2 * i + 1] << 16;
   }
+}
+template <bool VEC, class T>
+__device__ __forceinline__ void store_chunk(const Eight<T>& e, T* p, int c, int left) {
+  if constexpr (VEC) {
+    if (away<true>(c, 0) < left) {
+#pragma unroll
+      for (int k = 0; k < Eight<T>::kQuads; ++k)
+        reinterpret_cast<uint4*>(p + away<true>(c, 0))[k] = reinterpret_cast<const uint4*>(e.w)[k];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (away<false>(c, i) >= left) continue;
+      if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(p)[away<false>(c, i)] = e.w[i];
+      else reinterpret_cast<uint16_t*>(p)[away<false>(c, i)] = (uint16_t)(e.w[i / 2] >> (i % 2 * 16));
+    }
+  }
+}
+
+// A lane's part of its warp's ring in shared memory: rows of `words` 16-byte words a
+// lane, filled by asynchronous copies (through the first cache where two words lie in
+// one sector, past it otherwise) and read by the lane that asked for them.  Words past
+// the row's end hold 0.
+template <int WORDS>
+struct Ring {
+  uint32_t base;
+  static constexpr uint32_t kRow = WORDS * 512;  // bytes of a warp's row
+  __device__ __forceinline__ Ring(const void* shared, int stages) {
+    const uint32_t warp = threadIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    base = (uint32_t)__cvta_generic_to_shared(shared) + warp * stages * kRow + (threadIdx.x & 31) * 16;
+  }
+  // Chunk c of an array whose words start at `first`.
+  template <class T>
+  __device__ __forceinline__ void copy(int stage, int first, const T* p, int c, int left) const {
+    constexpr int Q = Eight<T>::kQuads;
+    if (away<true>(c, 0) < left) {
+#pragma unroll
+      for (int k = 0; k < Q; ++k) {
+        const uint32_t to = base + stage * kRow + (first + c * Q + k) * 512;
+        const T* at = p + away<true>(c, 0) + k * (16 / sizeof(T));
+        if constexpr (Q == 2) asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(to), "l"(at) : "memory");
+        else asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(at) : "memory");
+      }
+    }
+  }
+  template <class T>
+  __device__ __forceinline__ void take(Eight<T>& e, int stage, int first, int c) const {
+    constexpr int Q = Eight<T>::kQuads;
+#pragma unroll
+    for (int k = 0; k < Q; ++k)
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(e.w[4 * k]), "=r"(e.w[4 * k + 1]), "=r"(e.w[4 * k + 2]), "=r"(e.w[4 * k + 3])
+                   : "r"(base + stage * kRow + (first + c * Q + k) * 512) : "memory");
+  }
+  // 0 where no copy of chunk c goes, in every row.
+  template <class T>
+  __device__ __forceinline__ void blank(int stages, int first, const T*, int c, int left) const {
+    constexpr int Q = Eight<T>::kQuads;
+    if (away<true>(c, 0) < left) return;
+    for (int stage = 0; stage < stages; ++stage)
+#pragma unroll
+      for (int k = 0; k < Q; ++k)
+        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(base + stage * kRow + (first + c * Q + k) * 512), "r"(0)
+                     : "memory");
+  }
+};
+
+// Waits until all but the last `stages` - 1 groups of copies are there.
+__device__ __forceinline__ void wait_copies(int stages) {
+  if (stages == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // Sum over the threads of a row, one value for all of them: a warp, or all warps
@@ -116,6 +207,8 @@ inline NormShape norm_shape(uint32_t gw, uint64_t rows, bool vec) {
   s.rows_per_block = s.warps == 1 ? 4 : 1;
   return s;
 }
+
+constexpr uint32_t kSmShared = 227 * 1024, kBlockShared = 1024 + 256;  // of an SM; of a block beside its ring
 
 inline bool norm_aligned(const void* p, int64_t stride, uint32_t elem) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % (int64_t)(16 / elem) == 0;

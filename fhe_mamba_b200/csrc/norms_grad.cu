@@ -13,25 +13,15 @@
 namespace fhe {
 namespace {
 
-// Through the first cache where a thread's two words of float32 lie in one sector,
-// past it otherwise.
-template <bool TWO>
-__device__ __forceinline__ void copy16(void* to, const void* from) {
-  const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
-  if constexpr (TWO) asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
-  else asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
-}
-
-// A thread's share of a row in shared memory, in 16-byte words: what is read twice
-// stays out of the registers, and the loads of the next rows run behind the
-// arithmetic of this one.
+// A lane's words of a row in the ring: h or x, dy, gate or (for the channel scale) x,
+// dh.  What is read twice stays out of the registers, and the loads of the next rows
+// run behind the arithmetic of this one.
 template <int MODE, class A, class H, int N>
-struct GradRing {
-  static constexpr bool kAdd = MODE == kNormAdd || MODE == kNormAddScaled;
-  static constexpr int kWa = sizeof(A) / 2, kWs = (MODE == kNormGate ? sizeof(A) : sizeof(H)) / 2, kWh = sizeof(H) / 2;
-  static constexpr int kS = 0, kDy = kS + N * kWs, kZ = kDy + N * kWa,
-                       kDh = kZ + (MODE == kNormGate || MODE == kNormAddScaled ? N * kWa : 0),
-                       kWords = kDh + (kAdd ? N * kWh : 0);
+struct GradWords {
+  using S = std::conditional_t<MODE == kNormGate, A, H>;
+  static constexpr bool kAdd = MODE == kNormAdd || MODE == kNormAddScaled, kThird = MODE == kNormGate || MODE == kNormAddScaled;
+  static constexpr int kS = 0, kDy = kS + N * Eight<S>::kQuads, kZ = kDy + N * Eight<A>::kQuads,
+                       kDh = kZ + (kThird ? N * Eight<A>::kQuads : 0), kAll = kDh + (kAdd ? N * Eight<H>::kQuads : 0);
 };
 
 template <int MODE, class A, class H, int N, bool VEC>
@@ -39,82 +29,64 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
   __shared__ float red[2][16];
   extern __shared__ __align__(16) float sums[];  // the ring of rows; then sums over a block's rows
   RowSum row_sum{red};
-  constexpr bool kAdd = MODE == kNormAdd || MODE == kNormAddScaled, kScaled = MODE == kNormAddScaled;
+  using W = GradWords<MODE, A, H, N>;
+  constexpr bool kAdd = W::kAdd, kScaled = MODE == kNormAddScaled, kThird = W::kThird;
   using X = std::conditional_t<MODE == kNormPlain, H, A>;  // x
-  using S = std::conditional_t<MODE == kNormGate, A, H>;   // what h is made from
-  const uint32_t gw = g.gw, c0 = blockIdx.y * gw;
-  float w[N][8], dw[N][8];
-  float cs[kScaled ? N : 1][8], dcs[kScaled ? N : 1][8];
+  using S = typename W::S;                                 // what h is made from
+  const uint32_t c0 = blockIdx.y * g.gw + from<N, VEC>();
+  const int left = (int)g.gw - (int)from<N, VEC>();
+  Eight<float> w[N], cs[kScaled ? N : 1];
+  float dw[N][8], dcs[kScaled ? N : 1][8];
 #pragma unroll
   for (int c = 0; c < N; ++c) {
-    Eight<float> e;
-    load_chunk<VEC>(e, g.weight + c0, c, gw);
-    e.floats(w[c]);
+    w[c].clear();
+    load_chunk<VEC>(w[c], g.weight + c0, c, left);
     vset(dw[c], 0.f);
     if constexpr (kScaled) {
-      load_chunk<VEC>(e, g.cscale + c0, c, gw);
-      e.floats(cs[c]);
+      cs[c].clear();
+      load_chunk<VEC>(cs[c], g.cscale + c0, c, left);
       vset(dcs[c], 0.f);
     }
   }
-  const float n = 1.f / (float)gw;
-  // what a row is read from: h or x, dy, gate or (for the channel scale) x, dh
-  constexpr bool kThird = MODE == kNormGate || kScaled;
-  using Ring = GradRing<MODE, A, H, N>;
+  const float n = 1.f / (float)g.gw;
+  const Ring<W::kAll> ring(sums, g.stages);
   Eight<S> s[VEC ? 1 : N];
   Eight<A> dy[VEC ? 1 : N], z[kThird && !VEC ? N : 1];
   Eight<H> dh[kAdd && !VEC ? N : 1];
-  uint8_t* ring = reinterpret_cast<uint8_t*>(sums) + (threadIdx.y * blockDim.x + threadIdx.x) * 16;
-  auto visit = [&](uint32_t row, int stage, auto&& f_s, auto&& f_dy, auto&& f_z, auto&& f_dh) {
-    const int64_t out = (int64_t)row * g.width + c0;
-    const S* src = kAdd ? static_cast<const S*>(g.h) + out : static_cast<const S*>(g.x) + (int64_t)row * g.xs + c0;
-#pragma unroll
-    for (int c = 0; c < N; ++c) {
-      f_s(src, c);
-      f_dy(static_cast<const A*>(g.dy) + out, c);
-      if constexpr (MODE == kNormGate) f_z(static_cast<const A*>(g.gate) + (int64_t)row * g.gs + c0, c);
-      if constexpr (kScaled) f_z(static_cast<const A*>(g.x) + (int64_t)row * g.xs + c0, c);
-      if constexpr (kAdd)
-        if (g.dh) f_dh(static_cast<const H*>(g.dh) + out, c);
-    }
-  };
   const uint32_t step = gridDim.x * blockDim.y, row0 = blockIdx.x * blockDim.y + threadIdx.y;
-  const uint32_t threads = blockDim.x * blockDim.y;
-  auto fetch = [&](uint32_t row, int stage) {
-    if constexpr (VEC) {
-      if (row < g.rows) {
-        auto copy = [&](int first) {
-          return [&, first](const auto* p, int c) {
-            constexpr int W = sizeof(*p) / 2;  // 16-byte words of a chunk
-            const uint32_t at = channel<true>(c, 0);
-#pragma unroll
-            for (int k = 0; k < W; ++k)
-              if (at < gw) copy16<W == 2>(ring + (uint64_t)(stage * Ring::kWords + first + c * W + k) * threads * 16, p + at + k * (8 / W));
-          };
-        };
-        visit(row, stage, copy(Ring::kS), copy(Ring::kDy), copy(Ring::kZ), copy(Ring::kDh));
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    } else if (row < g.rows) {
-      visit(row, 0, [&](const S* p, int c) { load_chunk<VEC>(s[c], p, c, gw); },
-            [&](const A* p, int c) { load_chunk<VEC>(dy[c], p, c, gw); },
-            [&](const A* p, int c) { load_chunk<VEC>(z[c], p, c, gw); },
-            [&](const H* p, int c) { load_chunk<VEC>(dh[c], p, c, gw); });
-    }
-  };
-  const int stages = g.stages;
   int stage = 0;
-  // chunk c of an array, from the ring or the registers; lanes past the row hold 0
-  auto take = [&](auto* held, int first, int c, float (&o)[8]) {
-    using T = std::remove_pointer_t<decltype(held)>;
-    if constexpr (VEC) {
-      constexpr int W = sizeof(T) / 16;
-      T e;
+  auto fetch = [&](uint32_t row, [[maybe_unused]] int to) {
+    if (row < g.rows) {
+      const int64_t out = (int64_t)row * g.width + c0;
+      const S* sp = kAdd ? static_cast<const S*>(g.h) + out : static_cast<const S*>(g.x) + (int64_t)row * g.xs + c0;
+      const A* dyp = static_cast<const A*>(g.dy) + out;
+      const A* zp = MODE == kNormGate ? static_cast<const A*>(g.gate) + (int64_t)row * g.gs + c0
+                                      : static_cast<const A*>(g.x) + (int64_t)row * g.xs + c0;
+      const H* dhp = static_cast<const H*>(g.dh) + out;
 #pragma unroll
-      for (int k = 0; k < W; ++k)
-        reinterpret_cast<uint4*>(&e)[k] = channel<true>(c, 0) < gw
-            ? *reinterpret_cast<const uint4*>(ring + (uint64_t)(stage * Ring::kWords + first + c * W + k) * threads * 16)
-            : make_uint4(0, 0, 0, 0);
+      for (int c = 0; c < N; ++c) {
+        if constexpr (VEC) {
+          ring.copy(to, W::kS, sp, c, left);
+          ring.copy(to, W::kDy, dyp, c, left);
+          if constexpr (kThird) ring.copy(to, W::kZ, zp, c, left);
+          if constexpr (kAdd)
+            if (g.dh) ring.copy(to, W::kDh, dhp, c, left);
+        } else {
+          load_chunk<VEC>(s[c], sp, c, left);
+          load_chunk<VEC>(dy[c], dyp, c, left);
+          if constexpr (kThird) load_chunk<VEC>(z[c], zp, c, left);
+          if constexpr (kAdd)
+            if (g.dh) load_chunk<VEC>(dh[c], dhp, c, left);
+        }
+      }
+    }
+    if constexpr (VEC) asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // chunk c of an array, from the ring or the registers; 0 past the row's end
+  auto take = [&](auto& held, int first, int c, float (&o)[8]) {
+    if constexpr (VEC) {
+      std::remove_reference_t<decltype(held[0])> e;
+      ring.take(e, stage, first, c);
       e.floats(o);
     } else {
       held[c].floats(o);
@@ -122,63 +94,78 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
   };
   if constexpr (VEC) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (i + 1 < stages) fetch(row0 + i * step, i);
+    for (int c = 0; c < N; ++c) {
+      ring.blank(g.stages, W::kS, (const S*)nullptr, c, left);
+      ring.blank(g.stages, W::kDy, (const A*)nullptr, c, left);
+      if constexpr (kThird) ring.blank(g.stages, W::kZ, (const A*)nullptr, c, left);
+      if constexpr (kAdd) ring.blank(g.stages, W::kDh, (const H*)nullptr, c, left);
+    }
+    for (int i = 0; i + 1 < g.stages; ++i) fetch(row0 + i * step, i);
+  } else {
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      s[c].clear();
+      dy[c].clear();
+      if constexpr (kThird) z[c].clear();
+      if constexpr (kAdd) dh[c].clear();
+    }
   }
   for (uint32_t row = row0; row < g.rows; row += step) {
     const int64_t out = (int64_t)row * g.width + c0;
+    const float r = g.rstd[(int64_t)row * g.groups + blockIdx.y];
     if constexpr (VEC) {
-      fetch(row + (stages - 1) * step, stage ? stage - 1 : stages - 1);
-      if (stages == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
-      else if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
-      else asm volatile("cp.async.wait_group 0;" ::: "memory");
+      fetch(row + (g.stages - 1) * step, stage ? stage - 1 : g.stages - 1);
+      wait_copies(g.stages);
     } else {
       fetch(row, 0);
     }
-    const float r = g.rstd[(int64_t)row * g.groups + blockIdx.y];
     float rr[8];
     vset(rr, r);
-    // u = h r; with a gate also p = SiLU(gate)
-    auto unit = [&](int c, float (&u)[8], float (&xf)[8], float (&p)[8], float (&q)[8], float (&zf)[8]) {
-      take(s, Ring::kS, c, xf);
+    // u = h r; with a gate also p = SiLU(gate), from its sigmoid, which is kept
+    float q[MODE == kNormGate ? N : 1][8];
+    auto unit = [&](int c, bool first, float (&u)[8], float (&xf)[8], float (&p)[8]) {
+      take(s, W::kS, c, xf);
       if constexpr (MODE == kNormGate) {
-        take(z, Ring::kZ, c, zf);
-        sigmoid(q, zf);
-        vmul(p, q, zf);
+        float zf[8];
+        take(z, W::kZ, c, zf);
+        if (first) sigmoid(q[c], zf);
+        vmul(p, q[c], zf);
         vmul(u, xf, p);
         vmul(u, u, rr);
       } else {
         vmul(u, xf, rr);
       }
     };
-    float part[2] = {0.f, 0.f};
+    float part[2][2] = {};
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-      float u[8], xf[8], p[8], q[8], zf[8], d[8], a[8];
-      unit(c, u, xf, p, q, zf);
-      take(dy, Ring::kDy, c, d);
-      vmul(a, d, u);
-      vadd(dw[c], dw[c], a);
+      float u[8], xf[8], p[8], d[8], wf[8];
+      unit(c, true, u, xf, p);
+      take(dy, W::kDy, c, d);
+      w[c].floats(wf);
+      vmul(d, d, u);
+      vadd(dw[c], dw[c], d);
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
-        const float aa[2] = {a[i], a[i + 1]}, ww[2] = {w[c][i], w[c][i + 1]};
-        vfma(part, aa, ww, part);
+        const float aa[2] = {d[i], d[i + 1]}, ww[2] = {wf[i], wf[i + 1]};
+        vfma(part[i / 2 % 2], aa, ww, part[i / 2 % 2]);
       }
     }
-    const float m = row_sum(part[0] + part[1]) * n;
+    const float m = row_sum((part[0][0] + part[0][1]) + (part[1][0] + part[1][1])) * n;
     float mm[8];
     vset(mm, -m);
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-      float u[8], xf[8], p[8], q[8], zf[8], d[8];
-      unit(c, u, xf, p, q, zf);
-      take(dy, Ring::kDy, c, d);
-      vmul(d, d, w[c]);
+      float u[8], xf[8], p[8], d[8], wf[8];
+      unit(c, false, u, xf, p);
+      take(dy, W::kDy, c, d);
+      w[c].floats(wf);
+      vmul(d, d, wf);
       vfma(d, u, mm, d);
       if constexpr (kAdd) {
         float e[8];
         vset(e, 0.f);
-        if (g.dh) take(dh, Ring::kDh, c, e);
+        if (g.dh) take(dh, W::kDh, c, e);
         vfma(d, d, rr, e);
       } else {
         vmul(d, d, rr);
@@ -188,40 +175,44 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
         Eight<A> e;
         vmul(o, d, p);
         e.set(o);
-        if (g.dx) store_chunk<VEC>(e, static_cast<A*>(g.dx) + out, c, gw);
+        if (g.dx) store_chunk<VEC>(e, static_cast<A*>(g.dx) + out, c, left);
         // SiLU' = q (1 + z (1 - q)) = q + p (1 - q)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) one[i] = 1.f - q[i];
-        vfma(o, p, one, q);
+        for (int i = 0; i < 8; ++i) one[i] = 1.f - q[c][i];
+        vfma(o, p, one, q[c]);
         vmul(d, d, xf);
         vmul(o, o, d);
         e.set(o);
-        if (g.dgate) store_chunk<VEC>(e, static_cast<A*>(g.dgate) + out, c, gw);
+        if (g.dgate) store_chunk<VEC>(e, static_cast<A*>(g.dgate) + out, c, left);
       } else {
         if constexpr (kScaled) {
           float xg[8];
-          take(z, Ring::kZ, c, xg);
+          take(z, W::kZ, c, xg);
           vfma(dcs[c], d, xg, dcs[c]);
         }
         if constexpr (kAdd) {
           Eight<H> e;
           e.set(d);
-          if (g.dres) store_chunk<VEC>(e, static_cast<H*>(g.dres) + out, c, gw);
+          if (g.dres) store_chunk<VEC>(e, static_cast<H*>(g.dres) + out, c, left);
           float sc[8];
           vset(sc, g.scale);
           vmul(d, d, sc);
-          if constexpr (kScaled) vmul(d, d, cs[c]);
+          if constexpr (kScaled) {
+            cs[c].floats(sc);
+            vmul(d, d, sc);
+          }
         }
         Eight<X> e;
         e.set(d);
-        if (g.dx) store_chunk<VEC>(e, static_cast<X*>(g.dx) + out, c, gw);
+        if (g.dx) store_chunk<VEC>(e, static_cast<X*>(g.dx) + out, c, left);
       }
     }
-    stage = stage + 1 == stages ? 0 : stage + 1;
+    stage = stage + 1 == g.stages ? 0 : stage + 1;
   }
   if constexpr (VEC) asm volatile("cp.async.wait_all;" ::: "memory");
   // the block's rows together, one after the other
   auto gather = [&](float (&v)[N][8], float* to, float k) {
+    float* sum = sums + from<N, VEC>();
     for (uint32_t turn = 0; turn < blockDim.y; ++turn) {
       __syncthreads();
       if (threadIdx.y != turn) continue;
@@ -229,11 +220,11 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
       for (int c = 0; c < N; ++c)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const uint32_t at = channel<VEC>(c, i);
-          if (at >= gw) continue;
-          const float sum = turn ? sums[at] + v[c][i] : v[c][i];
-          if (turn + 1 == blockDim.y) to[at] = sum * k;
-          else sums[at] = sum;
+          const int at = away<VEC>(c, i);
+          if (at >= left) continue;
+          const float all = turn ? sum[at] + v[c][i] : v[c][i];
+          if (turn + 1 == blockDim.y) to[at] = all * k;
+          else sum[at] = all;
         }
     }
   };
@@ -286,7 +277,6 @@ struct GradPlan {
   uint32_t stages, shared, blocks;
 };
 GradPlan grad_plan(const fhe_rms_norm_grad_args& a) {
-  constexpr uint32_t kShared = 227 * 1024, kOwn = 1024 + 128;  // of an SM; of a block beside its ring
   const fhe_rms_norm_args& f = a.f;
   const uint32_t gw = f.width / f.groups;
   const uint32_t wa = elem_size(f.dtype) / 2, wh = f.gate ? wa : elem_size(f.stream_dtype) / 2;
@@ -300,13 +290,13 @@ GradPlan grad_plan(const fhe_rms_norm_grad_args& a) {
     p.shared = p.shape.rows_per_block > 1 ? gw * sizeof(float) : 0;  // one warp's channels, at most 1024
     if (p.vec) {
       const uint32_t row = p.shape.chunks * per_chunk * 16 * 32 * warps;
-      if (row + kOwn > kShared) continue;
+      if (row + kBlockShared > kSmShared) continue;
       for (p.stages = 3; p.stages > 1; --p.stages) {
-        const uint32_t fit = kShared / (p.stages * row + kOwn);
+        const uint32_t fit = kSmShared / (p.stages * row + kBlockShared);
         if (fit && fit * warps >= 12) break;
       }
       p.shared = std::max(p.shared, p.stages * row);
-      resident = std::max(1u, std::min(resident, kShared / (p.shared + kOwn)));
+      resident = std::max(1u, std::min(resident, kSmShared / (p.shared + kBlockShared)));
     }
     p.blocks = std::max(1u, std::min((f.rows + p.shape.rows_per_block - 1) / p.shape.rows_per_block,
                                      std::max(1u, 148 * resident / f.groups)));
