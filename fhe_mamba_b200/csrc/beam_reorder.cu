@@ -1,11 +1,12 @@
 // Reordering of states after a selection (fhe_beam_reorder): row i of each batch
 // item's beams becomes its row parents[i], in place, for every tensor at once.
 //
-// A thread owns the same 16 bytes of all of an item's rows: it brings the rows that
-// others take into its own part of shared memory by asynchronous copies, waits for
-// them, and then writes the rows that change.  So no thread reads what another
-// writes, nothing waits for another thread, and only rows that change are written,
-// only their parents read.  Memory bounds it.
+// A thread owns the same 16 bytes of all of an item's rows, and the next 16 of the
+// block's after them: it brings the rows that others take into its own part of shared
+// memory by asynchronous copies, up to three steps ahead, waits for them, and then
+// writes the rows that change.  So no thread reads what another writes, nothing waits
+// for another thread, and only rows that change are written, only their parents read.
+// Memory bounds it.
 #include <algorithm>
 
 #include "launch_count.h"
@@ -14,7 +15,8 @@
 namespace fhe {
 namespace {
 
-constexpr uint32_t kMaxBeams = 64, kTable = 64;
+constexpr uint32_t kMaxBeams = 64, kTable = 64, kThreads = 128, kStep = kThreads * 16;  // bytes of a row in a step
+constexpr uint32_t kSlots = 16;  // rows' steps in shared memory, as many as beams where those are more
 
 struct State {
   uint8_t* p;
@@ -24,7 +26,7 @@ struct State {
 };
 struct ReorderArgs {
   State state[kTable];
-  uint32_t n, beams;
+  uint32_t n, beams, steps;  // steps of a block
   const int64_t* parents;
 };
 
@@ -38,34 +40,46 @@ __device__ __forceinline__ void bring(W* to, const W* from) {
   }
 }
 
-// The block's 16 bytes a thread of each row, as words of type W.
-template <class W>
-__device__ __forceinline__ void move(uint8_t* base, uint64_t row, uint64_t at, uint32_t beams, const uint8_t* parent,
+// The block's steps from byte `at` of each row, as words of type W, D - 1 steps ahead.
+template <class W, int D>
+__device__ __forceinline__ void move(uint8_t* base, uint64_t row, uint64_t at, uint32_t steps, const uint8_t* parent,
                                      uint64_t wanted, uint64_t changed, uint8_t* shared) {
   constexpr int N = 16 / sizeof(W);
-  const uint32_t threads = blockDim.x, tid = threadIdx.x;
+  const uint32_t tid = threadIdx.x, each_step = __popcll(wanted);
   auto each = [&](uint64_t rows, auto&& f) {
     for (; rows; rows &= rows - 1) f((uint32_t)__ffsll((long long)rows) - 1);
   };
-  auto here = [&](uint32_t slot, int i) { return reinterpret_cast<W*>(shared) + ((uint64_t)slot * N + i) * threads + tid; };
-  auto there = [&](int i) { return at + ((uint64_t)i * threads + tid) * sizeof(W); };
-  uint32_t slot = 0;
-  each(wanted, [&](uint32_t r) {
+  auto here = [&](uint32_t step, uint32_t slot, int i) {
+    return reinterpret_cast<W*>(shared + (step % D * each_step + slot) * kStep) + i * kThreads + tid;
+  };
+  auto there = [&](uint32_t step, int i) { return at + step * kStep + (i * kThreads + tid) * sizeof(W); };
+  auto fetch = [&](uint32_t step) {
+    uint32_t slot = 0;
+    if (step < steps)
+      each(wanted, [&](uint32_t r) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (there(i) < row) bring(here(slot, i), reinterpret_cast<const W*>(base + r * row + there(i)));
-    ++slot;
-  });
+        for (int i = 0; i < N; ++i)
+          if (there(step, i) < row) bring(here(step, slot, i), reinterpret_cast<const W*>(base + r * row + there(step, i)));
+        ++slot;
+      });
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < D - 1; ++i) fetch(i);
+  for (uint32_t step = 0; step < steps && at + step * kStep < row; ++step) {
+    fetch(step + D - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
+    each(changed, [&](uint32_t r) {
+      const uint32_t from = __popcll(wanted & ((1ull << parent[r]) - 1));
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (there(step, i) < row) *reinterpret_cast<W*>(base + r * row + there(step, i)) = *here(step, from, i);
+    });
+  }
   asm volatile("cp.async.wait_all;" ::: "memory");
-  each(changed, [&](uint32_t r) {
-    const uint32_t from = __popcll(wanted & ((1ull << parent[r]) - 1));
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (there(i) < row) *reinterpret_cast<W*>(base + r * row + there(i)) = *here(from, i);
-  });
 }
 
-__global__ void __launch_bounds__(256) k_reorder(const __grid_constant__ ReorderArgs g) {
+__global__ void __launch_bounds__(kThreads) k_reorder(const __grid_constant__ ReorderArgs g) {
   extern __shared__ __align__(16) uint8_t shared[];
   __shared__ uint8_t parent[kMaxBeams];
   __shared__ uint64_t wanted, changed;
@@ -89,13 +103,20 @@ __global__ void __launch_bounds__(256) k_reorder(const __grid_constant__ Reorder
     else hi = mid;
   }
   const State& s = g.state[lo];
-  const uint64_t at = (uint64_t)(blockIdx.x - s.first) * blockDim.x * 16;
+  const uint64_t at = (uint64_t)(blockIdx.x - s.first) * g.steps * kStep;
   uint8_t* base = s.p + (uint64_t)item * K * s.row;
-  if (s.word == 16) move<uint4>(base, s.row, at, K, parent, wanted, changed, shared);
-  else if (s.word == 8) move<uint2>(base, s.row, at, K, parent, wanted, changed, shared);
-  else if (s.word == 4) move<uint32_t>(base, s.row, at, K, parent, wanted, changed, shared);
-  else if (s.word == 2) move<uint16_t>(base, s.row, at, K, parent, wanted, changed, shared);
-  else move<uint8_t>(base, s.row, at, K, parent, wanted, changed, shared);
+  const uint32_t n = __popcll(wanted), slots = max(K, kSlots);
+  auto with = [&](auto w) {
+    using W = decltype(w);
+    if (n * 4 <= slots) move<W, 4>(base, s.row, at, g.steps, parent, wanted, changed, shared);
+    else if (n * 2 <= slots) move<W, 2>(base, s.row, at, g.steps, parent, wanted, changed, shared);
+    else move<W, 1>(base, s.row, at, g.steps, parent, wanted, changed, shared);
+  };
+  if (s.word == 16) with(uint4{});
+  else if (s.word == 8) with(uint2{});
+  else if (s.word == 4) with(uint32_t{});
+  else if (s.word == 2) with(uint16_t{});
+  else with(uint8_t{});
 }
 
 }  // namespace
@@ -110,27 +131,31 @@ void beam_reorder(const fhe_beam_reorder_args& a) {
     require(a.row_bytes[i] < (1ull << 36), "row too large");
   }
   DeviceGuard dev(a.device);
-  // 16 bytes a thread and beam: 32 to 64 KB of shared memory to a block
-  const uint32_t threads = a.beams <= 8 ? 256 : a.beams <= 16 ? 128 : 64;
-  const uint32_t shared = threads * 16 * a.beams;
+  const uint32_t shared = std::max(a.beams, kSlots) * kStep;
   if (shared > 32768)
     FHE_CUDA(cudaFuncSetAttribute(k_reorder, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
+  // up to 16 steps to a block, fewer where that leaves places on the SMs empty
+  uint64_t all = 0;
+  for (uint32_t i = 0; i < a.count; ++i) all += (a.row_bytes[i] + kStep - 1) / kStep;
+  uint32_t steps = 16;
+  while (steps > 1 && all * a.batch / steps < 148 * 7) steps /= 2;
   for (uint32_t i = 0; i < a.count;) {
     ReorderArgs g{};
     g.beams = a.beams;
+    g.steps = steps;
     g.parents = a.parents;
     uint64_t blocks = 0;
     for (; i < a.count && g.n < kTable; ++i) {
       const uint64_t row = a.row_bytes[i];
       if (row == 0) continue;
-      const uint64_t more = (row + threads * 16 - 1) / (threads * 16);
+      const uint64_t more = (row + steps * kStep - 1) / (steps * kStep);
       if (blocks + more >= (1ull << 31)) break;
       const uint64_t bits = row | reinterpret_cast<uintptr_t>(a.states[i]) | 16;
       g.state[g.n++] = State{static_cast<uint8_t*>(a.states[i]), row, (uint32_t)blocks, (uint32_t)(bits & (0 - bits))};
       blocks += more;
     }
     if (g.n == 0) continue;
-    k_reorder<<<dim3((uint32_t)blocks, a.batch), threads, shared, static_cast<cudaStream_t>(a.stream)>>>(g);
+    k_reorder<<<dim3((uint32_t)blocks, a.batch), kThreads, shared, static_cast<cudaStream_t>(a.stream)>>>(g);
     note_launch();
     FHE_CUDA(cudaGetLastError());
   }

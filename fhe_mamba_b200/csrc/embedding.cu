@@ -2,13 +2,13 @@
 //
 // The lookup moves rows: a warp a row, 16 bytes a lane.  The gradient of a table
 // row is the sum over the positions that hold its token, so positions are sorted
-// by token: runs of 2048 in shared memory, then groups of 32 runs put together by
-// rank (an element's place is its own index plus, for every other run, how many of
-// its elements come before, found by halving), which waits for nothing and keeps
-// equal tokens in the order of their positions.  Blocks of equally many sorted
-// positions then sum the rows; a token that reaches past its block leaves partial
-// sums, which a last launch adds in order.  No atomics: the same call gives the same
-// bits.  Rows without a position are cleared by blocks beside those that sort.
+// by token: runs of 256 by counting, then groups of 32 runs put together by rank
+// (an element's place is its own index plus, for every other run, how many of its
+// elements come before, found by halving), which waits for nothing and keeps equal
+// tokens in the order of their positions.  Blocks of equally many sorted positions
+// then sum the rows; a token that reaches past its block leaves partial sums, which a
+// last launch adds in order.  No atomics: the same call gives the same bits.  Rows
+// without a position are cleared by blocks beside those that sort.
 #include <algorithm>
 
 #include "launch_count.h"
@@ -17,7 +17,7 @@
 namespace fhe {
 namespace {
 
-constexpr uint32_t kRun = 2048, kMerge = 32, kSortThreads = 1024;
+constexpr uint32_t kRun = 256, kMerge = 32, kMergeWarps = 8;
 constexpr uint32_t kNone = ~0u;  // sorts behind every token
 constexpr int kAhead = 8;        // rows in flight
 
@@ -30,38 +30,43 @@ __device__ __forceinline__ uint32_t token_of(const void* ids, bool wide, uint32_
   return wide ? token_at<int64_t>(ids, i, vocab) : token_at<int32_t>(ids, i, vocab);
 }
 
-// One warp a position.  VEC: eight elements a lane and turn.
-template <class T, class Y, bool VEC>
+// A warp takes R positions at a time, all their loads before the first store.  V
+// elements a lane: as many as make 16 bytes of the output, so that a warp's stores
+// are whole lines; 1 where alignment does not allow that.
+template <class T, class Y, int V, int R>
 __global__ void __launch_bounds__(128) k_embed(const fhe_embedding_args g) {
-  const uint32_t i = blockIdx.x * 4 + threadIdx.x / 32, lane = threadIdx.x % 32;
-  if (i >= g.count) return;
-  const uint32_t t = token_of(g.ids, g.wide_ids, i, g.vocab);
-  Y* out = static_cast<Y*>(g.out) + (int64_t)i * g.width;
-  if (t == kNone) {
-    const bool past = g.wide_ids ? static_cast<const int64_t*>(g.ids)[i] >= 0 : static_cast<const int32_t*>(g.ids)[i] >= 0;
-    for (uint32_t c = lane; c < g.width; c += 32) out[c] = from_f<Y>(past ? NAN : 0.f);
-    return;
-  }
-  const T* row = static_cast<const T*>(g.table) + (int64_t)t * g.table_stride;
-  if constexpr (VEC) {
-#pragma unroll 4
-    for (uint32_t c = lane * 8; c < g.width; c += 256) {
-      float f[8];
-      Pack<T, 8> p;
+  constexpr int kCols = V > 1 ? 2 : 4;  // loads of a lane and position in a turn
+  const uint32_t lane = threadIdx.x % 32, i0 = (blockIdx.x * 4 + threadIdx.x / 32) * R;
+  uint32_t t[R];
 #pragma unroll
-      for (int k = 0; k < (int)sizeof(T) / 2; ++k)
-        reinterpret_cast<uint4*>(&p)[k] = reinterpret_cast<const uint4*>(row + c)[k];
-      unpack(p, f);
+  for (int r = 0; r < R; ++r) t[r] = i0 + r < g.count ? token_of(g.ids, g.wide_ids, i0 + r, g.vocab) : kNone;
+  const T* table = static_cast<const T*>(g.table);
+  Y* out = static_cast<Y*>(g.out) + (int64_t)i0 * g.width;
+  for (uint32_t c0 = lane * V; c0 < g.width; c0 += kCols * 32 * V) {
+    Pack<T, V> p[R][kCols];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] *= g.scale;
-      const Pack<Y, 8> q = pack<Y, 8>(f);
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int k = 0; k < (int)sizeof(Y) / 2; ++k)
-        reinterpret_cast<uint4*>(out + c)[k] = reinterpret_cast<const uint4*>(&q)[k];
+      for (int j = 0; j < kCols; ++j)
+        if (t[r] != kNone && c0 + j * 32 * V < g.width)
+          p[r][j] = *reinterpret_cast<const Pack<T, V>*>(table + (int64_t)t[r] * g.table_stride + c0 + j * 32 * V);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (i0 + r >= g.count) break;
+      float none = 0.f;
+      if (t[r] == kNone)
+        none = (g.wide_ids ? static_cast<const int64_t*>(g.ids)[i0 + r] >= 0
+                           : static_cast<const int32_t*>(g.ids)[i0 + r] >= 0) ? NAN : 0.f;
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) {
+        if (c0 + j * 32 * V >= g.width) break;
+        float f[V];
+        unpack(p[r][j], f);
+#pragma unroll
+        for (int k = 0; k < V; ++k) f[k] = t[r] == kNone ? none : f[k] * g.scale;
+        *reinterpret_cast<Pack<Y, V>*>(out + (int64_t)r * g.width + c0 + j * 32 * V) = pack<Y, V>(f);
+      }
     }
-  } else {
-#pragma unroll 4
-    for (uint32_t c = lane; c < g.width; c += 32) out[c] = from_f<Y>(to_f(row[c]) * g.scale);
   }
 }
 
@@ -87,64 +92,74 @@ struct Fill {
   uint32_t blocks;  // behind the launch's own
 };
 
-// Blocks [0, runs) sort a run of positions by (token, position), the others clear.
-__global__ void __launch_bounds__(kSortThreads) k_sort(const void* ids, bool wide, uint32_t count, uint32_t vocab,
-                                                       uint32_t runs, Sorted out, Fill fill) {
-  __shared__ uint64_t key[kRun];
+// Blocks [0, runs) sort a run of positions by (token, position), a thread a position
+// whose place is the number of those before it; the other blocks clear.
+__global__ void __launch_bounds__(kRun) k_sort(const void* ids, bool wide, uint32_t count, uint32_t vocab, uint32_t runs,
+                                               Sorted out, Fill fill) {
+  __shared__ __align__(16) uint32_t token[kRun];
   if (blockIdx.x >= runs) return clear(fill.p, fill.bytes, blockIdx.x - runs, fill.blocks);
-  const uint32_t first = blockIdx.x * kRun, n = min(kRun, count - first);
-  uint32_t size = 2;
-  while (size < n) size *= 2;
-  for (uint32_t i = threadIdx.x; i < size; i += kSortThreads)
-    key[i] = i < n ? (uint64_t)token_of(ids, wide, first + i, vocab) << 32 | (first + i) : ~0ull;
-  for (uint32_t span = 2; span <= size; span *= 2) {
-    for (uint32_t step = span / 2; step; step /= 2) {
-      __syncthreads();
-      const uint32_t t = threadIdx.x;
-      if (t >= size / 2) continue;
-      const uint32_t a = 2 * t - (t & (step - 1)), b = a + step;
-      const uint64_t x = key[a], y = key[b];
-      if ((x > y) == ((a & span) == 0)) {
-        key[a] = y;
-        key[b] = x;
+  const uint32_t first = blockIdx.x * kRun, i = threadIdx.x, n = min(kRun, count - first);
+  const uint32_t t = i < n ? token_of(ids, wide, first + i, vocab) : kNone;
+  token[i] = t;
+  __syncthreads();
+  uint32_t at = 0;
+#pragma unroll 16
+  for (uint32_t j = 0; j < kRun; j += 4) {
+    const uint4 o = *reinterpret_cast<const uint4*>(&token[j]);
+    at += (o.x < t) + (o.y < t) + (o.z < t) + (o.w < t);
+    at += (o.x == t && j < i) + (o.y == t && j + 1 < i) + (o.z == t && j + 2 < i) + (o.w == t && j + 3 < i);
+  }
+  if (i < n) {
+    out.token[first + at] = t;
+    out.pos[first + at] = first + i;
+  }
+}
+
+// Puts groups of kMerge sorted runs of `run` (a power of two) elements together, 32
+// elements to a block: its warps share the other runs, four searches of a lane at a
+// time.  Blocks past `own` clear.
+__global__ void __launch_bounds__(32 * kMergeWarps) k_merge(Sorted in, Sorted out, uint32_t count, uint32_t run_log,
+                                                            uint32_t own, Fill fill) {
+  __shared__ uint32_t places[kMergeWarps][32];
+  if (blockIdx.x >= own) return clear(fill.p, fill.bytes, blockIdx.x - own, fill.blocks);
+  const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, e = blockIdx.x * 32 + lane;
+  const bool live = e < count;
+  const uint32_t t = live ? in.token[e] : 0;
+  const uint64_t group = (uint64_t)kMerge << run_log, at0 = (uint64_t)blockIdx.x * 32, base = at0 / group * group;
+  const uint32_t mine = (uint32_t)((at0 - base) >> run_log);  // the block's elements lie in one run
+  const uint32_t runs = (uint32_t)min((uint64_t)kMerge, ((uint64_t)count - base + ((uint64_t)1 << run_log) - 1) >> run_log);
+  uint32_t before_me = 0;
+  for (uint32_t r0 = warp; r0 < runs; r0 += 4 * kMergeWarps) {
+    const uint32_t* p[4];
+    uint32_t n[4], lo[4], top[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t r = r0 + k * kMergeWarps;
+      const uint64_t first = base + ((uint64_t)r << run_log);
+      const bool other = r < runs && r != mine;
+      p[k] = in.token + (other ? first : 0);
+      n[k] = other ? (uint32_t)min((uint64_t)1 << run_log, (uint64_t)count - first) : 0;
+      lo[k] = 0;
+      top[k] = t + (r < mine);  // equal tokens of earlier runs come before (kNone wraps: see below)
+    }
+    for (uint32_t step = 1u << run_log; step; step >>= 1) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t at = lo[k] + step;
+        if (at <= n[k] && p[k][at - 1] < top[k]) lo[k] = at;
       }
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) before_me += t == kNone && top[k] == 0 ? n[k] : lo[k];  // nothing is past kNone
   }
+  places[warp][lane] = before_me;
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < n; i += kSortThreads) {
-    out.token[first + i] = (uint32_t)(key[i] >> 32);
-    out.pos[first + i] = (uint32_t)key[i];
+  if (warp == 0 && live) {
+    uint64_t at = base + (e - base - ((uint64_t)mine << run_log));
+    for (uint32_t w = 0; w < kMergeWarps; ++w) at += places[w][lane];
+    out.token[at] = t;
+    out.pos[at] = in.pos[e];
   }
-}
-
-// Tokens of p[0, n) below t, or not above it.
-__device__ __forceinline__ uint32_t below(const uint32_t* p, uint32_t n, uint32_t t, bool or_equal) {
-  uint32_t lo = 0;
-  while (n) {
-    const uint32_t half = n / 2, v = p[lo + half];
-    const bool in = v < t || (or_equal && v == t);
-    lo = in ? lo + half + 1 : lo;
-    n = in ? n - half - 1 : half;
-  }
-  return lo;
-}
-
-// Puts groups of kMerge sorted runs of `run` elements together; blocks past `own` clear.
-__global__ void __launch_bounds__(256) k_merge(Sorted in, Sorted out, uint32_t count, uint64_t run, uint32_t own, Fill fill) {
-  if (blockIdx.x >= own) return clear(fill.p, fill.bytes, blockIdx.x - own, fill.blocks);
-  const uint32_t e = blockIdx.x * 256 + threadIdx.x;
-  if (e >= count) return;
-  const uint64_t base = e / (run * kMerge) * (run * kMerge);
-  const uint32_t mine = (uint32_t)((e - base) / run), t = in.token[e];
-  uint64_t at = e - mine * run;
-#pragma unroll 4
-  for (uint32_t r = 0; r < kMerge; ++r) {
-    const uint64_t first = base + r * run;
-    if (first >= count) break;
-    if (r != mine) at += below(in.token + first, (uint32_t)min(run, count - first), t, r < mine);
-  }
-  out.token[at] = t;
-  out.pos[at] = in.pos[e];
 }
 
 // blockDim.y blocks of `chunk` sorted positions, V columns to a thread.  A token
@@ -204,32 +219,55 @@ __global__ void __launch_bounds__(256) k_sum(const fhe_embedding_grad_args a, So
 }
 
 // Adds the partial sums of the token that begins in a block of positions and
-// reaches past it: strand y takes every eighth block, the strands follow in order.
-template <class T>
+// reaches past it: 64 columns of four, strand y takes every fourth block, the strands
+// follow in order.
+template <class T, bool VEC>
 __global__ void __launch_bounds__(256) k_join(const fhe_embedding_grad_args a, Sorted s, uint32_t chunk, uint32_t chunks,
                                               const float* part) {
-  __shared__ float sums[8][33];
+  __shared__ float4 sums[4][64];
   const uint32_t c = blockIdx.x, count = a.f.count, width = a.f.width;
   const uint32_t first = c * chunk, next = first + chunk;
   if (next >= count) return;
   const uint32_t t = s.token[next - 1];
-  if (t == kNone || s.token[next] != t) return;
-  if (s.token[first] == t && first && s.token[first - 1] == t) return;  // began earlier
-  const uint32_t end = next + below(s.token + next, count - next, t, true);
-  const uint32_t stop = (end - 1) / chunk;  // the last block with a share
-  for (uint32_t base = blockIdx.y * 32; base < width; base += gridDim.y * 32) {
-    const uint32_t col = base + threadIdx.x;
-    float v = 0.f;
-    if (col < width) {
+  const uint32_t after = s.token[next], begin = s.token[first], prior = first ? s.token[first - 1] : kNone;
+  if (t == kNone || after != t || (begin == t && prior == t)) return;  // ends here, or began earlier
+  uint32_t stop = c + 1;  // the last block with a share: its first position has the token
+  for (;;) {
+    const uint32_t b = stop + 1 + threadIdx.x % 32;
+    const uint32_t same = __ballot_sync(~0u, b < chunks && s.token[b * chunk] == t);
+    const uint32_t run = __ffs((int)~same);  // 1 + the number of blocks in a row, 0 for all 32
+    stop += run ? run - 1 : 32;
+    if (run) break;
+  }
+  const uint32_t x = threadIdx.x % 64, y = threadIdx.x / 64;
+  for (uint32_t base = blockIdx.y * 256; base < width; base += gridDim.y * 256) {
+    const uint32_t col = base + x * 4;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-      for (uint32_t b = c + threadIdx.y; b <= stop; b += 8) v += part[((int64_t)b * 2 + (b == c)) * width + col];
+    for (uint32_t b = c + y; b <= stop; b += 4) {
+      const float* p = part + ((int64_t)b * 2 + (b == c)) * width + col;
+      if constexpr (VEC) {
+        if (col < width) {
+          const float4 q = *reinterpret_cast<const float4*>(p);
+          v[0] += q.x, v[1] += q.y, v[2] += q.z, v[3] += q.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (col + i < width) v[i] += p[i];
+      }
     }
     __syncthreads();
-    sums[threadIdx.y][threadIdx.x] = v;
+    sums[y][x] = make_float4(v[0], v[1], v[2], v[3]);
     __syncthreads();
-    if (threadIdx.y == 0 && col < width) {
-      for (int i = 1; i < 8; ++i) v += sums[i][threadIdx.x];
-      static_cast<T*>(a.dtable)[(int64_t)t * width + col] = from_f<T>(v * a.f.scale);
+    if (y == 0) {
+      for (int i = 1; i < 4; ++i) {
+        const float4 q = sums[i][x];
+        v[0] += q.x, v[1] += q.y, v[2] += q.z, v[3] += q.w;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (col + i < width) static_cast<T*>(a.dtable)[(int64_t)t * width + col + i] = from_f<T>(v[i] * a.f.scale);
     }
   }
 }
@@ -254,7 +292,7 @@ void with_types(const fhe_embedding_args& a, F&& f) {
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // Sorted positions to a block: fewer when there are few, so that every SM has some.
-uint32_t chunk_of(uint32_t count) { return count >= 16384 ? 32 : 8; }
+uint32_t chunk_of(uint32_t count) { return count >= 16384 ? 16 : 8; }
 
 struct GradPlan {
   Sorted a, b;
@@ -284,10 +322,17 @@ void embedding(const fhe_embedding_args& a) {
   with_types(a, [&](auto t, auto y) {
     using T = decltype(t);
     using Y = decltype(y);
-    const bool vec = a.width % 8 == 0 && aligned16(a.table) && aligned16(a.out) && a.table_stride % (16 / sizeof(T)) == 0;
-    const uint32_t blocks = (a.count + 3) / 4;
-    if (vec) k_embed<T, Y, true><<<blocks, 128, 0, static_cast<cudaStream_t>(a.stream)>>>(a);
-    else k_embed<T, Y, false><<<blocks, 128, 0, static_cast<cudaStream_t>(a.stream)>>>(a);
+    constexpr int V = 16 / sizeof(Y);
+    cudaStream_t st = static_cast<cudaStream_t>(a.stream);
+    const bool vec = a.width % V == 0 && reinterpret_cast<uintptr_t>(a.table) % (V * sizeof(T)) == 0 && aligned16(a.out) &&
+                     a.table_stride % V == 0;
+    // four positions a warp once every SM has 32 warps
+    const bool many = a.count >= 148 * 32 * 4;
+    const uint32_t blocks = many ? (a.count + 15) / 16 : (a.count + 3) / 4;
+    if (vec && many) k_embed<T, Y, V, 4><<<blocks, 128, 0, st>>>(a);
+    else if (vec) k_embed<T, Y, V, 1><<<blocks, 128, 0, st>>>(a);
+    else if (many) k_embed<T, Y, 1, 4><<<blocks, 128, 0, st>>>(a);
+    else k_embed<T, Y, 1, 1><<<blocks, 128, 0, st>>>(a);
   });
   note_launch();
   FHE_CUDA(cudaGetLastError());
@@ -314,20 +359,23 @@ void embedding_backward(const fhe_embedding_grad_args& a) {
   }
   GradPlan p = plan_of(f, a.workspace);
   const uint32_t runs = (f.count + kRun - 1) / kRun;
-  // half of the table is cleared beside each of the first two launches
+  // the table is cleared beside the launches that sort, a share each
   uint8_t* table = static_cast<uint8_t*>(a.dtable);
-  const uint64_t here = runs == 1 ? bytes : bytes / 2 / 16 * 16;
-  auto fill = [&](uint8_t* at, uint64_t n) {
-    return Fill{at, n, (uint32_t)std::min<uint64_t>(148 * 2, (n + 65535) / 65536)};
+  uint32_t sorts = 1, share = 0;
+  for (uint64_t run = kRun; run < f.count; run *= kMerge) ++sorts;
+  auto fill = [&] {
+    const uint64_t each = bytes / sorts / 16 * 16, from = each * share++, to = share == sorts ? bytes : each * share;
+    return Fill{table + from, to - from, (uint32_t)std::min<uint64_t>(148 * 4, (to - from + 65535) / 65536)};
   };
-  const Fill one = fill(table, here), two = fill(table + here, bytes - here);
-  k_sort<<<runs + one.blocks, kSortThreads, 0, st>>>(f.ids, f.wide_ids, f.count, f.vocab, runs, p.a, one);
+  const Fill one = fill();
+  k_sort<<<runs + one.blocks, kRun, 0, st>>>(f.ids, f.wide_ids, f.count, f.vocab, runs, p.a, one);
   note_launch();
   Sorted s = p.a, other = p.b;
-  const uint32_t own = (f.count + 255) / 256;
-  for (uint64_t run = kRun; run < f.count; run *= kMerge) {
-    const Fill more = run == kRun ? two : Fill{};
-    k_merge<<<own + more.blocks, 256, 0, st>>>(s, other, f.count, run, own, more);
+  const uint32_t own = (f.count + 31) / 32;
+  static_assert(kRun == 1u << 8 && kMerge == 1u << 5, "powers of two");
+  for (uint32_t log = 8; (1ull << log) < f.count; log += 5) {
+    const Fill more = fill();
+    k_merge<<<own + more.blocks, 32 * kMergeWarps, 0, st>>>(s, other, f.count, log, own, more);
     note_launch();
     std::swap(s, other);
   }
@@ -343,7 +391,9 @@ void embedding_backward(const fhe_embedding_grad_args& a) {
     else k_sum<T, Y, 1><<<grid, block, 0, st>>>(a, s, p.chunk, p.chunks, p.part);
     note_launch();
     if (p.chunks > 1) {
-      k_join<T><<<dim3(p.chunks, std::min(8u, (f.width + 31) / 32)), dim3(32, 8), 0, st>>>(a, s, p.chunk, p.chunks, p.part);
+      const dim3 cover(p.chunks, std::min(4u, (f.width + 255) / 256));
+      if (f.width % 4 == 0) k_join<T, true><<<cover, 256, 0, st>>>(a, s, p.chunk, p.chunks, p.part);
+      else k_join<T, false><<<cover, 256, 0, st>>>(a, s, p.chunk, p.chunks, p.part);
       note_launch();
     }
   });
