@@ -175,7 +175,7 @@ def packer(block):
     """The bytes of an argument block from its values in order (pointers as integers, 0 for none; a block within it
     as its values): a quarter of the time that making the ctypes structure takes.  Functions of these blocks are
     declared with a plain pointer, which bytes and ``byref`` both are."""
-    codes = {i32: "i", u32: "I", i64: "q", u64: "Q", ctypes.c_float: "f", vp: "P"}
+    codes = {i32: "i", u32: "I", i64: "q", u64: "Q", ctypes.c_float: "f", vp: "P", ctypes.POINTER(vp): "P", P64: "P"}
 
     def fields(b):
         return "".join(codes[t] if t in codes else fields(t) for _, t in b._fields_)
@@ -296,7 +296,7 @@ SIGNATURES = {
     "fhe_embedding_backward_workspace": [vp, P64],
     "fhe_embedding_backward": [vp],
     "fhe_beam_select": [vp],
-    "fhe_beam_reorder": [ctypes.POINTER(BeamReorderArgs)],
+    "fhe_beam_reorder": [vp],
 }
 
 _lock = threading.Lock()

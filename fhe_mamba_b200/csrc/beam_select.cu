@@ -1,7 +1,7 @@
 // Beam search's selection (fhe_beam_select): the `width` best of score_i + z_iv -
 // log sum exp z_i over the beams i and tokens v of each batch item.
 //
-// A cluster of up to eight CTAs takes a batch item, a row or a share of a row to a
+// A cluster of up to sixteen CTAs takes a batch item, a row or a share of a row to a
 // CTA at a time, in one read: sums of exp(z - m) around a running shift m, and the
 // largest entry of each thread.  The `width`-th largest of 64 groups' maxima is a lower
 // bound on the share's best entries; the loads of the threads that reach it come once
@@ -27,7 +27,7 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kGroups = 64;   // groups of 4 threads
 constexpr int kAhead = 4;     // 16-byte loads in flight per thread
 constexpr int kCap = 1024;    // candidates held
-constexpr uint32_t kMaxBeams = 64, kMaxWidth = 64, kMaxCluster = 8;
+constexpr uint32_t kMaxBeams = 64, kMaxWidth = 64, kMaxCluster = 16;
 static_assert(kMaxWidth <= kGroups, "the bound is the width-th of the groups' maxima");
 
 // One share of a row: sum of exp(z - m), and its best entries in order.
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kThreads) k_select(const SelectArgs g) {
   extern __shared__ __align__(16) uint8_t dynamic[];
   __shared__ Scratch sm;
   __shared__ float score[kMaxBeams];
-  __shared__ uint32_t live[kMaxBeams], ended[kMaxBeams], lives;
+  __shared__ uint32_t live[kMaxBeams], ended[kMaxBeams], alive[2];
   __shared__ double lse[kMaxBeams], err[kMaxBeams], top[kMaxBeams], again[kMaxBeams];
   __shared__ uint32_t lcount[kMaxBeams + kMaxCluster], lbeam[kMaxBeams + kMaxCluster];
   __shared__ double rtotal[kMaxWidth];
@@ -300,17 +300,23 @@ __global__ void __launch_bounds__(kThreads) k_select(const SelectArgs g) {
   const uint32_t B = a.beams, k = a.width, kk = g.kk;
   cg::cluster_group cluster = cg::this_cluster();
   if (C > 1) cluster.barrier_arrive();  // every CTA has to run before another's memory is written
-  if (tid < B) {
-    score[tid] = a.scores[(int64_t)item * B + tid];
-    ended[tid] = a.finished && a.finished[(int64_t)item * B + tid];
+  if (tid < 64) {  // the live beams, in order
+    const bool mine = tid < B;
+    const float v = mine ? a.scores[(int64_t)item * B + tid] : 0.f;
+    const bool end = mine && a.finished && a.finished[(int64_t)item * B + tid];
+    const uint32_t on = __ballot_sync(~0u, mine && !end && isfinite(v));
+    if (mine) {
+      score[tid] = v;
+      ended[tid] = end;
+    }
+    if (tid % 32 == 0) alive[tid / 32] = on;
   }
   __syncthreads();
-  if (tid == 0) {
-    uint32_t n = 0;
-    for (uint32_t i = 0; i < B; ++i)
-      if (!ended[i] && isfinite(score[i])) live[n++] = i;
-    lives = n;
+  if (tid < 64) {
+    const uint32_t w = tid / 32, on = alive[w], skip = w ? __popc(alive[0]) : 0;
+    if (on >> tid % 32 & 1) live[skip + __popc(on & ((1u << tid % 32) - 1))] = tid;
   }
+  const uint32_t lives = __popc(alive[0]) + __popc(alive[1]);
   __syncthreads();
   const uint32_t parts = lives ? max(1u, C / lives) : 1, units = lives * parts;
   const Layout l(dynamic, B + C, kk);
@@ -362,16 +368,13 @@ __global__ void __launch_bounds__(kThreads) k_select(const SelectArgs g) {
       lbeam[tid] = i;
       lcount[tid] = fine ? l.share[tid].count : tid % parts == 0 ? kk : 0;  // its impossible tokens, once
     }
-    lists = units;
-    for (uint32_t i = 0; i < B; ++i) {
-      if (!ended[i] && isfinite(score[i])) continue;
-      if (tid == 0) {
-        lbeam[lists] = i;
-        lcount[lists] = kk;
-        lse[i] = -INFINITY;
-        err[i] = 0.;
-      }
-      ++lists;
+    lists = units + B - lives;
+    if (tid < B && !(alive[tid / 32] >> tid % 32 & 1)) {  // the others offer what is impossible, or their end
+      const uint32_t at = units + tid - (tid >= 32 ? __popc(alive[0]) : 0) - __popc(alive[tid / 32] & ((1u << tid % 32) - 1));
+      lbeam[at] = tid;
+      lcount[at] = kk;
+      lse[tid] = -INFINITY;
+      err[tid] = 0.;
     }
     __syncthreads();
   }
@@ -507,15 +510,18 @@ void beam_select(const fhe_beam_select_args& a) {
   DeviceGuard dev(a.device);
   with_type(a.dtype, [&](auto t) {
     using T = decltype(t);
-    // As many CTAs to an item as the device takes at once, and a turn of loads for each
+    // As many CTAs to an item as the device takes at once, and a turn of loads for each;
+    // sixteen where eight would take several beams each (1 x 10 beams of 50280 bfloat16:
+    // 17 us, 23 with eight; 1 x 4: 11 us with either)
     const uint64_t packs = (uint64_t)a.beams * (a.vocab / Quad<T>::kElems);
     SelectArgs g{a, 1, std::min(a.width, a.vocab)};
-    while (g.cluster < kMaxCluster && (uint64_t)a.batch * g.cluster * 2 <= 148 * 4 &&
+    while (g.cluster < (a.beams > 8 ? kMaxCluster : 8) && (uint64_t)a.batch * g.cluster * 2 <= 148 * 4 &&
            packs >= (uint64_t)g.cluster * 2 * kAhead * kThreads)
       g.cluster *= 2;
     const uint32_t shared = Layout(nullptr, a.beams + g.cluster, g.kk).bytes;
     if (shared > 32768)
       FHE_CUDA(cudaFuncSetAttribute(k_select<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
+    if (g.cluster > 8) FHE_CUDA(cudaFuncSetAttribute(k_select<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(a.batch * g.cluster);
     cfg.blockDim = dim3(kThreads);

@@ -17,6 +17,7 @@ work.
 from __future__ import annotations
 
 import ctypes
+from array import array
 from typing import NamedTuple
 
 import torch
@@ -787,32 +788,30 @@ def beam_reorder(states, parents):
     op = "beam_reorder"
     _need(parents.dim() == 2 and 1 <= parents.shape[1] <= MAX_BEAMS, f"{op}: parents must be [batch, 1 to {MAX_BEAMS} beams]")
     _need(parents.dtype == torch.int64, f"{op}: parents must be {torch.int64}, got {parents.dtype}")
-    _need(parents.shape[0] <= 65535, f"{op}: batch must be at most 65535")
-    b, k = parents.shape
-    states, device = list(states), parents.get_device()
-    rows, spans, sizes = b * k, [(parents.data_ptr(), parents.numel() * 8)], []
-    for t in states:
-        if not (t.is_contiguous() and t.get_device() == device and t.dim() and (t.shape[0] == rows or t.shape[:2] == (b, k))):
+    (b, k), device = parents.shape, parents.get_device()
+    _need(b <= 65535, f"{op}: batch must be at most 65535")
+    rows, states = b * k, list(states)
+    if not (device >= 0 and all([t.is_contiguous() and t.get_device() == device and t.dim() and t.size(0) == rows
+                                 for t in states])):
+        for t in states:
             _need(t.dim() >= 1 and (t.shape[0] == rows or t.shape[:2] == (b, k)),
                   f"{op}: states must be [batch * beams, ...] or [batch, beams, ...], got {tuple(t.shape)}")
             _need(t.is_contiguous(), f"{op}: states must be contiguous")
-            _check_devices(op, parents, t)
-        n = t.nbytes
-        sizes.append(n // rows if rows else 0)
-        spans.append((t.data_ptr(), n))
-    if not parents.is_cuda:
-        _check_devices(op, parents)
-    at = [p for p, _ in spans[1:]]
+        _check_devices(op, parents, *states)
+    at, sizes = [t.data_ptr() for t in states], [t.nbytes for t in states]
     end = 0
-    for p, n in sorted(spans):
-        _need(p >= end or not n, f"{op}: states share memory")
-        end = max(end, p + n)
-    if _wants_grad(*states):
+    for p, n in sorted(zip([*at, parents.data_ptr()], [*sizes, parents.nbytes])):
+        if p < end and n:
+            _need(False, f"{op}: states share memory")
+        end = p + n if n else end
+    if torch.is_grad_enabled() and any([t.requires_grad for t in states]):
         _need(False, f"{op} has no gradient")
     if not rows:
         return
-    n, parents = len(states), _dense(parents)
-    a = _lib.BeamReorderArgs(device, b, k, n, (ctypes.c_void_p * n)(*at), (ctypes.c_uint64 * n)(*sizes), parents.data_ptr(),
-                             _stream_of(device))
-    call("fhe_beam_reorder", ctypes.byref(a))
+    at, sizes, parents = array("Q", at), array("Q", [n // rows for n in sizes]), _dense(parents)
+    call("fhe_beam_reorder", _reorder_block(device, b, k, len(states), at.buffer_info()[0], sizes.buffer_info()[0],
+                                            parents.data_ptr(), _stream_of(device)))
     increment_version(states)
+
+
+_reorder_block = _lib.packer(_lib.BeamReorderArgs)
