@@ -12,16 +12,17 @@
 namespace fhe {
 namespace {
 
-template <int MODE, class A, class H, int N, bool VEC>
+template <int MODE, class A, class H, int N, int LAY>
 __global__ void __launch_bounds__(512) k_norm(const NormArgs g) {
   __shared__ float red[2][16];
   extern __shared__ __align__(16) uint8_t shared[];
-  RowSum row_sum{red};
-  constexpr bool kTwo = MODE != kNormPlain, kRing = MODE == kNormGate && VEC;
+  constexpr bool kNarrow = is_narrow(LAY);
+  RowSum<kNarrow> row_sum{red, g.lanes};
+  constexpr bool kTwo = MODE != kNormPlain, kRing = MODE == kNormGate && LAY == kWords;
   using X = std::conditional_t<MODE == kNormPlain, H, A>;
   using Y = std::conditional_t<MODE == kNormGate, A, H>;  // gate or residual
-  const uint32_t c0 = blockIdx.y * g.gw + from<N, VEC>();
-  const int left = (int)g.gw - (int)from<N, VEC>();
+  const uint32_t c0 = blockIdx.y * g.gw + from<N, LAY>(g.lanes);
+  const int left = (int)g.gw - (int)from<N, LAY>(g.lanes);
   const X* xp = static_cast<const X*>(g.x) + c0;
   const Y* yp = static_cast<const Y*>(MODE == kNormGate ? g.gate : g.res) + c0;
   const int64_t ys = MODE == kNormGate ? g.gs : g.rs;
@@ -29,15 +30,17 @@ __global__ void __launch_bounds__(512) k_norm(const NormArgs g) {
 #pragma unroll
   for (int c = 0; c < N; ++c) {
     w[c].clear();
-    load_chunk<VEC>(w[c], g.weight + c0, c, left);
+    load_chunk<LAY>(w[c], g.weight + c0, c, left);
     if constexpr (MODE == kNormAddScaled) {
       cs[c].clear();
-      load_chunk<VEC>(cs[c], g.cscale + c0, c, left);
+      load_chunk<LAY>(cs[c], g.cscale + c0, c, left);
     }
   }
   const float n = 1.f / (float)g.gw;
-  const uint32_t step = gridDim.x * blockDim.y;
-  uint32_t row = blockIdx.x * blockDim.y + threadIdx.y;
+  // a warp's first row, and this lane's among its rows
+  const uint32_t rows = kNarrow ? 32 / g.lanes : 1, sub = kNarrow ? threadIdx.x / g.lanes : 0;
+  const uint32_t step = gridDim.x * blockDim.y * rows;
+  uint32_t base = (blockIdx.x * blockDim.y + threadIdx.y) * rows;
   // The next row's words come while this one is summed and written: into registers,
   // or with a gate, whose sigmoids take longer, one or two rows ahead through a ring.
   Eight<X> e[N];
@@ -55,8 +58,8 @@ __global__ void __launch_bounds__(512) k_norm(const NormArgs g) {
           ring.copy(to, 0, x, c, left);
           ring.copy(to, N * kQ, y, c, left);
         } else {
-          load_chunk<VEC>(e[c], x, c, left);
-          if constexpr (kTwo) load_chunk<VEC>(f[c], y, c, left);
+          load_chunk<LAY>(e[c], x, c, left);
+          if constexpr (kTwo) load_chunk<LAY>(f[c], y, c, left);
         }
       }
     }
@@ -68,16 +71,18 @@ __global__ void __launch_bounds__(512) k_norm(const NormArgs g) {
       ring.blank(g.stages, 0, xp, c, left);
       ring.blank(g.stages, N * kQ, yp, c, left);
     }
-    for (int i = 0; i + 1 < g.stages; ++i) fetch(row + i * step, i);
+    for (int i = 0; i + 1 < g.stages; ++i) fetch(base + i * step, i);
   } else {
 #pragma unroll
     for (int c = 0; c < N; ++c) {
       e[c].clear();
       if constexpr (kTwo) f[c].clear();
     }
-    fetch(row, 0);
+    fetch(base + sub, 0);
   }
-  for (; row < g.rows; row += step) {
+  for (; base < g.rows; base += step) {
+    const uint32_t row = base + sub;
+    const bool live = !kNarrow || row < g.rows;
     if constexpr (kRing) {
       fetch(row + (g.stages - 1) * step, stage ? stage - 1 : g.stages - 1);
       wait_copies(g.stages);
@@ -111,7 +116,7 @@ __global__ void __launch_bounds__(512) k_norm(const NormArgs g) {
         vfma(h[c], s, h[c], rf);
         Eight<H> kept;
         kept.set(h[c]);
-        store_chunk<VEC>(kept, out, c, left);
+        if (live) store_chunk<LAY>(kept, out, c, left);
         kept.floats(h[c]);
       }
     }
@@ -127,16 +132,18 @@ __global__ void __launch_bounds__(512) k_norm(const NormArgs g) {
     const float ss = row_sum((part[0][0] + part[0][1]) + (part[1][0] + part[1][1]));
     float r = rsqrtf(fmaf(ss, n, g.eps));
     // squares past fp32's range: the row again, scaled (an infinity of the row itself gives r = 0)
-    if (ss == INFINITY) {
+    if (kNarrow ? __any_sync(~0u, ss == INFINITY) : ss == INFINITY) {
       const float k = 0x1p-80f;
       float again = 0.f;
 #pragma unroll
       for (int c = 0; c < N; ++c)
 #pragma unroll
         for (int i = 0; i < 8; ++i) again = fmaf(h[c][i] * k, h[c][i] * k, again);
-      r = k / sqrtf(row_sum(again) * n);
+      again = row_sum(again);
+      if (ss == INFINITY) r = k / sqrtf(again * n);
     }
-    if (g.rstd && threadIdx.x == 0) g.rstd[(int64_t)row * g.groups + blockIdx.y] = r;
+    if (!live) continue;
+    if (g.rstd && (kNarrow ? threadIdx.x % g.lanes : threadIdx.x) == 0) g.rstd[(int64_t)row * g.groups + blockIdx.y] = r;
     A* y = static_cast<A*>(g.y) + (int64_t)row * g.width + c0;
 #pragma unroll
     for (int c = 0; c < N; ++c) {
@@ -147,7 +154,7 @@ __global__ void __launch_bounds__(512) k_norm(const NormArgs g) {
       vmul(o, o, wf);
       Eight<A> to;
       to.set(o);
-      store_chunk<VEC>(to, y, c, left);
+      store_chunk<LAY>(to, y, c, left);
     }
   }
   if constexpr (kRing) asm volatile("cp.async.wait_all;" ::: "memory");
@@ -204,9 +211,10 @@ void rms_norm(const fhe_rms_norm_args& a) {
                    norm_aligned(a.gate, a.gate_stride, ea) && norm_aligned(a.channel_scale, 0, 4) &&
                    norm_aligned(a.weight, 0, 4) && norm_aligned(a.y, 0, ea) && norm_aligned(a.h, 0, eh);
   const NormShape s = norm_shape(g.gw, (uint64_t)a.rows * a.groups, vec);
+  g.lanes = s.lanes;
   // blocks that go from row to row: with a ring as many as are resident
   uint32_t resident = 12, shared = 0;
-  if (a.gate && vec) {
+  if (a.gate && s.layout(vec) == kWords) {
     const uint32_t warps = s.warps * s.rows_per_block, row = s.chunks * ea * 16 * 32 * warps;
     for (g.stages = 3; g.stages > 1; --g.stages) {
       const uint32_t fit = kSmShared / (g.stages * row + kBlockShared);
@@ -217,10 +225,11 @@ void rms_norm(const fhe_rms_norm_args& a) {
   }
   const uint32_t blocks = std::min((a.rows + s.rows_per_block - 1) / s.rows_per_block,
                                    std::max(1u, 148 * resident / a.groups));
-  with_norm(a, s.chunks, vec, [&](auto mode, auto act, auto str, auto chunks, auto words) {
-    auto k = k_norm<decltype(mode)::value, decltype(act), decltype(str), decltype(chunks)::value, decltype(words)::value>;
+  with_norm(a, s.chunks, s.layout(vec), [&](auto mode, auto act, auto str, auto chunks, auto layout) {
+    auto k = k_norm<decltype(mode)::value, decltype(act), decltype(str), decltype(chunks)::value, decltype(layout)::value>;
     if (shared > 48000) FHE_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
-    k<<<dim3(blocks, a.groups), dim3(32 * s.warps, s.rows_per_block), shared, static_cast<cudaStream_t>(a.stream)>>>(g);
+    const dim3 block(32 * s.warps, s.warps == 1 ? 4 : 1);
+    k<<<dim3(blocks, a.groups), block, shared, static_cast<cudaStream_t>(a.stream)>>>(g);
   });
   note_launch();
   FHE_CUDA(cudaGetLastError());

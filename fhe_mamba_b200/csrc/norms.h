@@ -21,7 +21,8 @@ struct NormArgs {
   float* part;  // sums of each block: [grid.x][width] for the weight, then as much for the channel scale
   uint32_t rows, width, gw, groups;
   float eps, scale;
-  int stages;  // rows in the ring
+  int stages;       // rows in the ring
+  uint32_t lanes;   // of a narrow row
 };
 
 // Eight elements as 32-bit words, in memory's order.
@@ -62,55 +63,61 @@ struct alignas(16) Eight {
   }
 };
 
-// A row's (or group's) channels over warps: N chunks of 256 to a warp.  Chunk c of a
-// lane holds the channels from(): + c 256 .. + 8 where 16-byte words are loaded,
-// + (c 8 + i) 32 otherwise; both read consecutive memory across a warp, at constant
-// distances.
-template <int N, bool VEC>
-__device__ __forceinline__ uint32_t from() {
-  return (threadIdx.x >> 5) * (N * 256) + (threadIdx.x & 31) * (VEC ? 8 : 1);
+// How a row's (or group's) channels lie over lanes: N chunks of 256 to a warp, or in
+// narrow rows (up to 128 channels) one of eight to each of `lanes` lanes and several
+// rows to a warp.  Chunk c of a lane holds the channels from(): + c 256 .. + 8 where
+// 16-byte words are loaded or rows are narrow, + (c 8 + i) 32 otherwise; they read
+// consecutive memory across a warp, at constant distances.
+enum { kSingles = 0, kWords = 1, kNarrowSingles = 2, kNarrowWords = 3 };
+constexpr bool is_words(int lay) { return lay & 1; }
+constexpr bool is_narrow(int lay) { return lay >= kNarrowSingles; }
+
+template <int N, int LAY>
+__device__ __forceinline__ uint32_t from(uint32_t lanes) {
+  if constexpr (is_narrow(LAY)) return (threadIdx.x & (lanes - 1)) * 8;
+  return (threadIdx.x >> 5) * (N * 256) + (threadIdx.x & 31) * (is_words(LAY) ? 8 : 1);
 }
-template <bool VEC>
+template <int LAY>
 __host__ __device__ constexpr int away(int c, int i) {
-  return VEC ? c * 256 + i : (c * 8 + i) * 32;
+  return LAY == kSingles ? (c * 8 + i) * 32 : c * 256 + i;
 }
 // Chunk c of the lane's channels at p; `left` of them are before the row's end, the
 // others stay as they are.
-template <bool VEC, class T>
+template <int LAY, class T>
 __device__ __forceinline__ void load_chunk(Eight<T>& e, const T* p, int c, int left) {
-  if constexpr (VEC) {
-    if (away<true>(c, 0) < left) {
+  if constexpr (is_words(LAY)) {
+    if (away<LAY>(c, 0) < left) {
 #pragma unroll
       for (int k = 0; k < Eight<T>::kQuads; ++k)
-        reinterpret_cast<uint4*>(e.w)[k] = reinterpret_cast<const uint4*>(p + away<true>(c, 0))[k];
+        reinterpret_cast<uint4*>(e.w)[k] = reinterpret_cast<const uint4*>(p + away<LAY>(c, 0))[k];
     }
   } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (away<false>(c, i) < left) e.w[i] = reinterpret_cast<const uint32_t*>(p)[away<false>(c, i)];
+      if (away<LAY>(c, i) < left) e.w[i] = reinterpret_cast<const uint32_t*>(p)[away<LAY>(c, i)];
   } else {
     const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
     uint32_t v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = away<false>(c, i) < left ? q[away<false>(c, i)] : 0;
+    for (int i = 0; i < 8; ++i) v[i] = away<LAY>(c, i) < left ? q[away<LAY>(c, i)] : 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) e.w[i] = v[2 * i] | v[2 * i + 1] << 16;
   }
 }
-template <bool VEC, class T>
+template <int LAY, class T>
 __device__ __forceinline__ void store_chunk(const Eight<T>& e, T* p, int c, int left) {
-  if constexpr (VEC) {
-    if (away<true>(c, 0) < left) {
+  if constexpr (is_words(LAY)) {
+    if (away<LAY>(c, 0) < left) {
 #pragma unroll
       for (int k = 0; k < Eight<T>::kQuads; ++k)
-        reinterpret_cast<uint4*>(p + away<true>(c, 0))[k] = reinterpret_cast<const uint4*>(e.w)[k];
+        reinterpret_cast<uint4*>(p + away<LAY>(c, 0))[k] = reinterpret_cast<const uint4*>(e.w)[k];
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (away<false>(c, i) >= left) continue;
-      if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(p)[away<false>(c, i)] = e.w[i];
-      else reinterpret_cast<uint16_t*>(p)[away<false>(c, i)] = (uint16_t)(e.w[i / 2] >> (i % 2 * 16));
+      if (away<LAY>(c, i) >= left) continue;
+      if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(p)[away<LAY>(c, i)] = e.w[i];
+      else reinterpret_cast<uint16_t*>(p)[away<LAY>(c, i)] = (uint16_t)(e.w[i / 2] >> (i % 2 * 16));
     }
   }
 }
@@ -131,11 +138,11 @@ struct Ring {
   template <class T>
   __device__ __forceinline__ void copy(int stage, int first, const T* p, int c, int left) const {
     constexpr int Q = Eight<T>::kQuads;
-    if (away<true>(c, 0) < left) {
+    if (away<kWords>(c, 0) < left) {
 #pragma unroll
       for (int k = 0; k < Q; ++k) {
         const uint32_t to = base + stage * kRow + (first + c * Q + k) * 512;
-        const T* at = p + away<true>(c, 0) + k * (16 / sizeof(T));
+        const T* at = p + away<kWords>(c, 0) + k * (16 / sizeof(T));
         if constexpr (Q == 2) asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(to), "l"(at) : "memory");
         else asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(at) : "memory");
       }
@@ -154,7 +161,7 @@ struct Ring {
   template <class T>
   __device__ __forceinline__ void blank(int stages, int first, const T*, int c, int left) const {
     constexpr int Q = Eight<T>::kQuads;
-    if (away<true>(c, 0) < left) return;
+    if (away<kWords>(c, 0) < left) return;
     for (int stage = 0; stage < stages; ++stage)
 #pragma unroll
       for (int k = 0; k < Q; ++k)
@@ -170,12 +177,18 @@ __device__ __forceinline__ void wait_copies(int stages) {
   else asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// Sum over the threads of a row, one value for all of them: a warp, or all warps
-// of the block by two sets of partial sums used in turn.
+// Sum over the threads of a row, one value for all of them: some lanes, a warp, or
+// all warps of the block by two sets of partial sums used in turn.
+template <bool NARROW>
 struct RowSum {
   float (*red)[16];
+  uint32_t lanes;
   int turn = 0;
   __device__ __forceinline__ float operator()(float v) {
+    if constexpr (NARROW) {
+      for (uint32_t o = lanes / 2; o; o /= 2) v += __shfl_xor_sync(~0u, v, o);
+      return v;
+    }
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
     if (blockDim.x == 32) return v;
@@ -193,11 +206,18 @@ struct RowSum {
 // as many warps as have a chunk.  Else a thread takes three chunks where that fills
 // every lane, else four (single elements, which need more registers: two); at most 16
 // warps.  Four rows of one warp share a block, a longer row has its own.
+// Narrow rows share a warp.
 struct NormShape {
-  uint32_t warps, chunks, rows_per_block;
+  uint32_t warps, chunks, rows_per_block, lanes;
+  int layout(bool words) const { return (words ? kWords : kSingles) + (lanes < 32 ? kNarrowSingles : 0); }
 };
 inline NormShape norm_shape(uint32_t gw, uint64_t rows, bool vec) {
   const uint32_t all = (gw + 7) / 8;
+  if (all <= 16) {
+    uint32_t lanes = 1;
+    while (lanes < all) lanes *= 2;
+    return {1, 1, 4 * 32 / lanes, lanes};
+  }
   const bool whole = vec && all % 96 == 0 && all / 96 <= 8;
   const uint32_t want = rows < 2 * 148 ? 1 : whole ? 3 : vec ? 4 : 2;
   NormShape s;
@@ -205,6 +225,7 @@ inline NormShape norm_shape(uint32_t gw, uint64_t rows, bool vec) {
   s.chunks = (all + 32 * s.warps - 1) / (32 * s.warps);
   if (s.chunks == 3 && (!vec || s.warps > 8)) s.chunks = 4;
   s.rows_per_block = s.warps == 1 ? 4 : 1;
+  s.lanes = 32;
   return s;
 }
 
@@ -220,21 +241,22 @@ inline int norm_mode(const fhe_rms_norm_args& a) {
   return a.gate ? kNormGate : !a.residual ? kNormPlain : a.channel_scale ? kNormAddScaled : kNormAdd;
 }
 
-// Calls f(mode, A{}, H{}, chunks, words) with constants: the activations' and the
-// stream's type, chunks per thread, whether 16-byte words are loaded.
+// Calls f(mode, A{}, H{}, chunks, layout) with constants: the activations' and the
+// stream's type, chunks per thread, the layout.
 template <class F>
-void with_norm(const fhe_rms_norm_args& a, uint32_t chunks, bool vec, F&& f) {
+void with_norm(const fhe_rms_norm_args& a, uint32_t chunks, int layout, F&& f) {
   auto shape = [&](auto mode, auto act, auto str) {
-    if (!vec) {
-      if (chunks == 1) f(mode, act, str, std::integral_constant<int, 1>{}, std::false_type{});
-      else if (chunks == 2) f(mode, act, str, std::integral_constant<int, 2>{}, std::false_type{});
-      else f(mode, act, str, std::integral_constant<int, 4>{}, std::false_type{});
-      return;
-    }
-    if (chunks == 1) f(mode, act, str, std::integral_constant<int, 1>{}, std::true_type{});
-    else if (chunks == 2) f(mode, act, str, std::integral_constant<int, 2>{}, std::true_type{});
-    else if (chunks == 3) f(mode, act, str, std::integral_constant<int, 3>{}, std::true_type{});
-    else f(mode, act, str, std::integral_constant<int, 4>{}, std::true_type{});
+    auto with = [&](auto n, auto lay) { f(mode, act, str, n, lay); };
+    using std::integral_constant;
+    if (layout == kNarrowSingles) with(integral_constant<int, 1>{}, integral_constant<int, kNarrowSingles>{});
+    else if (layout == kNarrowWords) with(integral_constant<int, 1>{}, integral_constant<int, kNarrowWords>{});
+    else if (layout == kSingles && chunks == 1) with(integral_constant<int, 1>{}, integral_constant<int, kSingles>{});
+    else if (layout == kSingles && chunks == 2) with(integral_constant<int, 2>{}, integral_constant<int, kSingles>{});
+    else if (layout == kSingles) with(integral_constant<int, 4>{}, integral_constant<int, kSingles>{});
+    else if (chunks == 1) with(integral_constant<int, 1>{}, integral_constant<int, kWords>{});
+    else if (chunks == 2) with(integral_constant<int, 2>{}, integral_constant<int, kWords>{});
+    else if (chunks == 3) with(integral_constant<int, 3>{}, integral_constant<int, kWords>{});
+    else with(integral_constant<int, 4>{}, integral_constant<int, kWords>{});
   };
   with_type(a.dtype, [&](auto act) {
     auto stream = [&](auto mode) {

@@ -24,27 +24,28 @@ struct GradWords {
                        kDh = kZ + (kThird ? N * Eight<A>::kQuads : 0), kAll = kDh + (kAdd ? N * Eight<H>::kQuads : 0);
 };
 
-template <int MODE, class A, class H, int N, bool VEC>
+template <int MODE, class A, class H, int N, int LAY>
 __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs g) {
   __shared__ float red[2][16];
   extern __shared__ __align__(16) float sums[];  // the ring of rows; then sums over a block's rows
-  RowSum row_sum{red};
+  constexpr bool kNarrow = is_narrow(LAY), VEC = LAY == kWords;  // words of wide rows come through the ring
+  RowSum<kNarrow> row_sum{red, g.lanes};
   using W = GradWords<MODE, A, H, N>;
   constexpr bool kAdd = W::kAdd, kScaled = MODE == kNormAddScaled, kThird = W::kThird;
   using X = std::conditional_t<MODE == kNormPlain, H, A>;  // x
   using S = typename W::S;                                 // what h is made from
-  const uint32_t c0 = blockIdx.y * g.gw + from<N, VEC>();
-  const int left = (int)g.gw - (int)from<N, VEC>();
+  const uint32_t c0 = blockIdx.y * g.gw + from<N, LAY>(g.lanes);
+  const int left = (int)g.gw - (int)from<N, LAY>(g.lanes);
   Eight<float> w[N], cs[kScaled ? N : 1];
   float dw[N][8], dcs[kScaled ? N : 1][8];
 #pragma unroll
   for (int c = 0; c < N; ++c) {
     w[c].clear();
-    load_chunk<VEC>(w[c], g.weight + c0, c, left);
+    load_chunk<LAY>(w[c], g.weight + c0, c, left);
     vset(dw[c], 0.f);
     if constexpr (kScaled) {
       cs[c].clear();
-      load_chunk<VEC>(cs[c], g.cscale + c0, c, left);
+      load_chunk<LAY>(cs[c], g.cscale + c0, c, left);
       vset(dcs[c], 0.f);
     }
   }
@@ -53,7 +54,9 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
   Eight<S> s[VEC ? 1 : N];
   Eight<A> dy[VEC ? 1 : N], z[kThird && !VEC ? N : 1];
   Eight<H> dh[kAdd && !VEC ? N : 1];
-  const uint32_t step = gridDim.x * blockDim.y, row0 = blockIdx.x * blockDim.y + threadIdx.y;
+  // a warp's first row, and this lane's among its rows
+  const uint32_t rows = kNarrow ? 32 / g.lanes : 1, sub = kNarrow ? threadIdx.x / g.lanes : 0;
+  const uint32_t step = gridDim.x * blockDim.y * rows, base0 = (blockIdx.x * blockDim.y + threadIdx.y) * rows;
   int stage = 0;
   auto fetch = [&](uint32_t row, [[maybe_unused]] int to) {
     if (row < g.rows) {
@@ -72,11 +75,11 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
           if constexpr (kAdd)
             if (g.dh) ring.copy(to, W::kDh, dhp, c, left);
         } else {
-          load_chunk<VEC>(s[c], sp, c, left);
-          load_chunk<VEC>(dy[c], dyp, c, left);
-          if constexpr (kThird) load_chunk<VEC>(z[c], zp, c, left);
+          load_chunk<LAY>(s[c], sp, c, left);
+          load_chunk<LAY>(dy[c], dyp, c, left);
+          if constexpr (kThird) load_chunk<LAY>(z[c], zp, c, left);
           if constexpr (kAdd)
-            if (g.dh) load_chunk<VEC>(dh[c], dhp, c, left);
+            if (g.dh) load_chunk<LAY>(dh[c], dhp, c, left);
         }
       }
     }
@@ -100,7 +103,7 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
       if constexpr (kThird) ring.blank(g.stages, W::kZ, (const A*)nullptr, c, left);
       if constexpr (kAdd) ring.blank(g.stages, W::kDh, (const H*)nullptr, c, left);
     }
-    for (int i = 0; i + 1 < g.stages; ++i) fetch(row0 + i * step, i);
+    for (int i = 0; i + 1 < g.stages; ++i) fetch(base0 + i * step, i);
   } else {
 #pragma unroll
     for (int c = 0; c < N; ++c) {
@@ -110,9 +113,11 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
       if constexpr (kAdd) dh[c].clear();
     }
   }
-  for (uint32_t row = row0; row < g.rows; row += step) {
+  for (uint32_t base = base0; base < g.rows; base += step) {
+    const uint32_t row = base + sub;
+    const bool live = !kNarrow || row < g.rows;
     const int64_t out = (int64_t)row * g.width + c0;
-    const float r = g.rstd[(int64_t)row * g.groups + blockIdx.y];
+    const float r = live ? g.rstd[(int64_t)row * g.groups + blockIdx.y] : 0.f;
     if constexpr (VEC) {
       fetch(row + (g.stages - 1) * step, stage ? stage - 1 : g.stages - 1);
       wait_copies(g.stages);
@@ -136,6 +141,13 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
         vmul(u, xf, rr);
       }
     };
+    if constexpr (kNarrow) {
+      if (!live) {  // rows past the last add nothing
+        s[0].clear();
+        dy[0].clear();
+        if constexpr (kThird) z[0].clear();
+      }
+    }
     float part[2][2] = {};
 #pragma unroll
     for (int c = 0; c < N; ++c) {
@@ -152,6 +164,7 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
       }
     }
     const float m = row_sum((part[0][0] + part[0][1]) + (part[1][0] + part[1][1])) * n;
+    if (!live) continue;
     float mm[8];
     vset(mm, -m);
 #pragma unroll
@@ -175,7 +188,7 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
         Eight<A> e;
         vmul(o, d, p);
         e.set(o);
-        if (g.dx) store_chunk<VEC>(e, static_cast<A*>(g.dx) + out, c, left);
+        if (g.dx) store_chunk<LAY>(e, static_cast<A*>(g.dx) + out, c, left);
         // SiLU' = q (1 + z (1 - q)) = q + p (1 - q)
 #pragma unroll
         for (int i = 0; i < 8; ++i) one[i] = 1.f - q[c][i];
@@ -183,7 +196,7 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
         vmul(d, d, xf);
         vmul(o, o, d);
         e.set(o);
-        if (g.dgate) store_chunk<VEC>(e, static_cast<A*>(g.dgate) + out, c, left);
+        if (g.dgate) store_chunk<LAY>(e, static_cast<A*>(g.dgate) + out, c, left);
       } else {
         if constexpr (kScaled) {
           float xg[8];
@@ -193,7 +206,7 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
         if constexpr (kAdd) {
           Eight<H> e;
           e.set(d);
-          if (g.dres) store_chunk<VEC>(e, static_cast<H*>(g.dres) + out, c, left);
+          if (g.dres) store_chunk<LAY>(e, static_cast<H*>(g.dres) + out, c, left);
           float sc[8];
           vset(sc, g.scale);
           vmul(d, d, sc);
@@ -204,15 +217,23 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
         }
         Eight<X> e;
         e.set(d);
-        if (g.dx) store_chunk<VEC>(e, static_cast<X*>(g.dx) + out, c, left);
+        if (g.dx) store_chunk<LAY>(e, static_cast<X*>(g.dx) + out, c, left);
       }
     }
     stage = stage + 1 == g.stages ? 0 : stage + 1;
   }
   if constexpr (VEC) asm volatile("cp.async.wait_all;" ::: "memory");
+  if constexpr (kNarrow) {  // the warp's rows together
+    for (uint32_t o = g.lanes; o < 32; o *= 2)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        dw[0][i] += __shfl_xor_sync(~0u, dw[0][i], o);
+        if constexpr (kScaled) dcs[0][i] += __shfl_xor_sync(~0u, dcs[0][i], o);
+      }
+  }
   // the block's rows together, one after the other
   auto gather = [&](float (&v)[N][8], float* to, float k) {
-    float* sum = sums + from<N, VEC>();
+    float* sum = sums + from<N, LAY>(g.lanes);
     for (uint32_t turn = 0; turn < blockDim.y; ++turn) {
       __syncthreads();
       if (threadIdx.y != turn) continue;
@@ -220,8 +241,8 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
       for (int c = 0; c < N; ++c)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int at = away<VEC>(c, i);
-          if (at >= left) continue;
+          const int at = away<LAY>(c, i);
+          if (at >= left || (kNarrow && sub != 0)) continue;
           const float all = turn ? sum[at] + v[c][i] : v[c][i];
           if (turn + 1 == blockDim.y) to[at] = all * k;
           else sum[at] = all;
@@ -285,10 +306,10 @@ GradPlan grad_plan(const fhe_rms_norm_grad_args& a) {
   p.vec = words(a);
   for (;; p.vec = false) {
     p.shape = norm_shape(gw, (uint64_t)f.rows * f.groups, p.vec);
-    const uint32_t warps = p.shape.warps * p.shape.rows_per_block;
+    const uint32_t warps = p.shape.warps == 1 ? 4 : p.shape.warps;  // of a block
     uint32_t resident = std::max(1u, 16 / warps);
-    p.shared = p.shape.rows_per_block > 1 ? gw * sizeof(float) : 0;  // one warp's channels, at most 1024
-    if (p.vec) {
+    p.shared = p.shape.warps == 1 ? gw * sizeof(float) : 0;  // one warp's channels, at most 1024
+    if (p.shape.layout(p.vec) == kWords) {
       const uint32_t row = p.shape.chunks * per_chunk * 16 * 32 * warps;
       if (row + kBlockShared > kSmShared) continue;
       for (p.stages = 3; p.stages > 1; --p.stages) {
@@ -339,11 +360,13 @@ void rms_norm_backward(const fhe_rms_norm_grad_args& a) {
   g.part = sums_wanted(a) ? static_cast<float*>(a.workspace) : nullptr;
   const GradPlan p = grad_plan(a);
   g.stages = (int)p.stages;
-  with_norm(f, p.shape.chunks, p.vec, [&](auto mode, auto act, auto str, auto chunks, auto words) {
+  g.lanes = p.shape.lanes;
+  with_norm(f, p.shape.chunks, p.shape.layout(p.vec), [&](auto mode, auto act, auto str, auto chunks, auto layout) {
     auto k = k_norm_grad<decltype(mode)::value, decltype(act), decltype(str), decltype(chunks)::value,
-                         decltype(words)::value>;
+                         decltype(layout)::value>;
     if (p.shared > 48000) FHE_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.shared));
-    k<<<dim3(p.blocks, f.groups), dim3(32 * p.shape.warps, p.shape.rows_per_block), p.shared, st>>>(g);
+    const dim3 block(32 * p.shape.warps, p.shape.warps == 1 ? 4 : 1);
+    k<<<dim3(p.blocks, f.groups), block, p.shared, st>>>(g);
   });
   note_launch();
   if (g.part) {

@@ -61,7 +61,7 @@ def grads_of(dy, u, r, w, groups=1):
 
 
 SHAPES = [(1, 1), (3, 7), (5, 8), (1, 768), (4, 768), (301, 768), (700, 1536), (13, 1001), (400, 333), (2, 16384), (3, 12296),
-          (300, 4096), (310, 2560), (9, 1024), (333, 64), (299, 9000)]
+          (300, 4096), (310, 2560), (9, 1024), (333, 64), (299, 9000), (1000, 1), (77, 100), (130, 128), (65, 13), (5, 130)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -119,7 +119,7 @@ def test_add_norm(ops, dtype, rows, width, scale):
         close(only[1], dh.double() * s64, (dh.double() * s64).abs(), what="dx of h alone")
 
 
-GATED = [(1, 1, 1), (3, 7, 1), (4, 1536, 1), (301, 1536, 1), (300, 1536, 8), (20, 555 * 3, 3), (700, 192, 1), (2, 40960, 5),
+GATED = [(1, 1, 1), (3, 7, 1), (999, 1, 1), (70, 104, 1), (31, 360, 3), (40, 39, 3), (4, 1536, 1), (301, 1536, 1), (300, 1536, 8), (20, 555 * 3, 3), (700, 192, 1), (2, 40960, 5),
          (299, 9000, 1), (33, 35, 5)]
 
 
