@@ -289,8 +289,8 @@ bool words(const fhe_rms_norm_grad_args& a) {
          norm_aligned(a.dgate, 0, ea);
 }
 
-// How a call is laid out: shape, rows of the ring (up to three, as far as 12 warps
-// still fit an SM), shared memory, and blocks that go from row to row, as many as
+// How a call is laid out: shape, rows of the ring (three where 16 warps still fit an
+// SM, two where 12 do), shared memory, and blocks that go from row to row, as many as
 // are resident.
 struct GradPlan {
   NormShape shape;
@@ -314,7 +314,7 @@ GradPlan grad_plan(const fhe_rms_norm_grad_args& a) {
       if (row + kBlockShared > kSmShared) continue;
       for (p.stages = 3; p.stages > 1; --p.stages) {
         const uint32_t fit = kSmShared / (p.stages * row + kBlockShared);
-        if (fit && fit * warps >= 12) break;
+        if (fit && fit * warps >= (p.stages == 3 ? 16 : 12)) break;
       }
       p.shared = std::max(p.shared, p.stages * row);
       resident = std::max(1u, std::min(resident, kSmShared / (p.shared + kBlockShared)));
