@@ -75,7 +75,7 @@ __device__ __forceinline__ void clear(uint8_t* p, uint64_t bytes, uint64_t b, ui
   const uint64_t head = min(bytes, (uint64_t)((0 - reinterpret_cast<uintptr_t>(p)) % 16)), words = (bytes - head) / 16;
   const uint64_t each = (words + blocks - 1) / blocks, first = min(words, b * each), last = min(words, first + each);
   uint4* w = reinterpret_cast<uint4*>(p + head);
-#pragma unroll 4
+#pragma unroll 8
   for (uint64_t i = first + threadIdx.x; i < last; i += blockDim.x) w[i] = make_uint4(0, 0, 0, 0);
   if (b == 0) {
     for (uint64_t i = threadIdx.x; i < head; i += blockDim.x) p[i] = 0;
@@ -89,16 +89,16 @@ struct Sorted {
 struct Fill {
   uint8_t* p;
   uint64_t bytes;
-  uint32_t blocks;  // behind the launch's own
+  uint32_t blocks;  // before the launch's own, so that they write while those wait
 };
 
-// Blocks [0, runs) sort a run of positions by (token, position), a thread a position
-// whose place is the number of those before it; the other blocks clear.
-__global__ void __launch_bounds__(kRun) k_sort(const void* ids, bool wide, uint32_t count, uint32_t vocab, uint32_t runs,
-                                               Sorted out, Fill fill) {
+// The blocks behind those that clear sort a run of positions by (token, position), a
+// thread a position whose place is the number of those before it.
+__global__ void __launch_bounds__(kRun) k_sort(const void* ids, bool wide, uint32_t count, uint32_t vocab, Sorted out,
+                                               Fill fill) {
   __shared__ __align__(16) uint32_t token[kRun];
-  if (blockIdx.x >= runs) return clear(fill.p, fill.bytes, blockIdx.x - runs, fill.blocks);
-  const uint32_t first = blockIdx.x * kRun, i = threadIdx.x, n = min(kRun, count - first);
+  if (blockIdx.x < fill.blocks) return clear(fill.p, fill.bytes, blockIdx.x, fill.blocks);
+  const uint32_t first = (blockIdx.x - fill.blocks) * kRun, i = threadIdx.x, n = min(kRun, count - first);
   const uint32_t t = i < n ? token_of(ids, wide, first + i, vocab) : kNone;
   token[i] = t;
   __syncthreads();
@@ -117,15 +117,17 @@ __global__ void __launch_bounds__(kRun) k_sort(const void* ids, bool wide, uint3
 
 // Puts groups of kMerge sorted runs of `run` (a power of two) elements together, 32
 // elements to a block: its warps share the other runs, four searches of a lane at a
-// time.  Blocks past `own` clear.
+// time.  The first blocks clear.
 __global__ void __launch_bounds__(32 * kMergeWarps) k_merge(Sorted in, Sorted out, uint32_t count, uint32_t run_log,
-                                                            uint32_t own, Fill fill) {
+                                                            Fill fill) {
   __shared__ uint32_t places[kMergeWarps][32];
-  if (blockIdx.x >= own) return clear(fill.p, fill.bytes, blockIdx.x - own, fill.blocks);
-  const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, e = blockIdx.x * 32 + lane;
+  if (blockIdx.x < fill.blocks) return clear(fill.p, fill.bytes, blockIdx.x, fill.blocks);
+  const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const uint64_t at0 = (uint64_t)(blockIdx.x - fill.blocks) * 32;
+  const uint32_t e = (uint32_t)at0 + lane;
   const bool live = e < count;
   const uint32_t t = live ? in.token[e] : 0;
-  const uint64_t group = (uint64_t)kMerge << run_log, at0 = (uint64_t)blockIdx.x * 32, base = at0 / group * group;
+  const uint64_t group = (uint64_t)kMerge << run_log, base = at0 / group * group;
   const uint32_t mine = (uint32_t)((at0 - base) >> run_log);  // the block's elements lie in one run
   const uint32_t runs = (uint32_t)min((uint64_t)kMerge, ((uint64_t)count - base + ((uint64_t)1 << run_log) - 1) >> run_log);
   uint32_t before_me = 0;
@@ -218,33 +220,54 @@ __global__ void __launch_bounds__(256) k_sum(const fhe_embedding_grad_args a, So
   put(last == count || s.token[last] != now);
 }
 
-// Adds the partial sums of the token that begins in a block of positions and
-// reaches past it: 64 columns of four, strand y takes every fourth block, the strands
-// follow in order.
+// Adds the partial sums of the tokens that begin in one of kJoin blocks of positions
+// and reach past it: each warp looks at one of the blocks.  Up to kFew shares are
+// added in order by a warp, four columns a lane, a token a warp; more by the whole
+// CTA, strand y every eighth share, the strands in order.
+constexpr uint32_t kJoin = 8, kFew = 16;
 template <class T, bool VEC>
-__global__ void __launch_bounds__(256) k_join(const fhe_embedding_grad_args a, Sorted s, uint32_t chunk, uint32_t chunks,
-                                              const float* part) {
-  __shared__ float4 sums[4][64];
-  const uint32_t c = blockIdx.x, count = a.f.count, width = a.f.width;
-  const uint32_t first = c * chunk, next = first + chunk;
-  if (next >= count) return;
-  const uint32_t t = s.token[next - 1];
-  const uint32_t after = s.token[next], begin = s.token[first], prior = first ? s.token[first - 1] : kNone;
-  if (t == kNone || after != t || (begin == t && prior == t)) return;  // ends here, or began earlier
-  uint32_t stop = c + 1;  // the last block with a share: its first position has the token
-  for (;;) {
-    const uint32_t b = stop + 1 + threadIdx.x % 32;
-    const uint32_t same = __ballot_sync(~0u, b < chunks && s.token[b * chunk] == t);
-    const uint32_t run = __ffs((int)~same);  // 1 + the number of blocks in a row, 0 for all 32
-    stop += run ? run - 1 : 32;
-    if (run) break;
+__global__ void __launch_bounds__(32 * kJoin) k_join(const fhe_embedding_grad_args a, Sorted s, uint32_t chunk,
+                                                     uint32_t chunks, const float* part) {
+  __shared__ float4 sums[kJoin][32];
+  __shared__ uint32_t tokens[kJoin], stops[kJoin];
+  const uint32_t count = a.f.count, width = a.f.width;
+  {
+    const uint32_t c = blockIdx.x * kJoin + threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t first = c * chunk, next = first + chunk;
+    uint32_t t = kNone, stop = c + 1;  // the last block with a share: its first position has the token
+    if (c < chunks && next < count) {
+      t = s.token[next - 1];
+      const uint32_t after = s.token[next], begin = s.token[first], prior = first ? s.token[first - 1] : kNone;
+      if (after != t || (begin == t && prior == t)) t = kNone;  // ends here, or began earlier
+    }
+    while (t != kNone) {  // the same for the whole warp
+      bool same[4];  // four blocks a lane, in order over the lanes
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t b = stop + 1 + k * 32 + lane;
+        same[k] = b < chunks && s.token[b * chunk] == t;
+      }
+      uint32_t run = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t some = __ballot_sync(~0u, same[k]);
+        if (run == k * 32u) run += some == ~0u ? 32 : __ffs((int)~some) - 1;
+      }
+      stop += run;
+      if (run < 128) break;
+    }
+    if (lane == 0) {
+      tokens[threadIdx.x / 32] = t;
+      stops[threadIdx.x / 32] = stop;
+    }
   }
-  const uint32_t x = threadIdx.x % 64, y = threadIdx.x / 64;
-  for (uint32_t base = blockIdx.y * 256; base < width; base += gridDim.y * 256) {
-    const uint32_t col = base + x * 4;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
+  __syncthreads();
+  const uint32_t x = threadIdx.x % 32, y = threadIdx.x / 32;
+  auto add = [&](float (&v)[4], uint32_t c, uint32_t b, uint32_t stop, uint32_t step, uint32_t col) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = 0.f;
 #pragma unroll 8
-    for (uint32_t b = c + y; b <= stop; b += 4) {
+    for (; b <= stop; b += step) {
       const float* p = part + ((int64_t)b * 2 + (b == c)) * width + col;
       if constexpr (VEC) {
         if (col < width) {
@@ -253,21 +276,43 @@ __global__ void __launch_bounds__(256) k_join(const fhe_embedding_grad_args a, S
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (col + i < width) v[i] += p[i];
+        for (int k = 0; k < 4; ++k)
+          if (col + k < width) v[k] += p[k];
       }
     }
-    __syncthreads();
-    sums[y][x] = make_float4(v[0], v[1], v[2], v[3]);
-    __syncthreads();
-    if (y == 0) {
-      for (int i = 1; i < 4; ++i) {
-        const float4 q = sums[i][x];
-        v[0] += q.x, v[1] += q.y, v[2] += q.z, v[3] += q.w;
-      }
+  };
+  auto put = [&](const float (&v)[4], uint32_t t, uint32_t col) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (col + i < width) static_cast<T*>(a.dtable)[(int64_t)t * width + col + i] = from_f<T>(v[i] * a.f.scale);
+    for (int k = 0; k < 4; ++k)
+      if (col + k < width) static_cast<T*>(a.dtable)[(int64_t)t * width + col + k] = from_f<T>(v[k] * a.f.scale);
+  };
+  bool more = false;
+  for (uint32_t i = 0; i < kJoin; ++i) more = more || (tokens[i] != kNone && stops[i] - (blockIdx.x * kJoin + i) >= kFew);
+  if (tokens[y] != kNone && stops[y] - (blockIdx.x * kJoin + y) < kFew) {
+    const uint32_t t = tokens[y], c = blockIdx.x * kJoin + y;
+    for (uint32_t base = blockIdx.y * 128; base < width; base += gridDim.y * 128) {
+      float v[4];
+      add(v, c, c, stops[y], 1, base + x * 4);
+      put(v, t, base + x * 4);
+    }
+  }
+  if (!more) return;
+  for (uint32_t i = 0; i < kJoin; ++i) {
+    const uint32_t t = tokens[i], c = blockIdx.x * kJoin + i;
+    if (t == kNone || stops[i] - c < kFew) continue;
+    for (uint32_t base = blockIdx.y * 128; base < width; base += gridDim.y * 128) {
+      float v[4];
+      add(v, c, c + y, stops[i], kJoin, base + x * 4);
+      __syncthreads();
+      sums[y][x] = make_float4(v[0], v[1], v[2], v[3]);
+      __syncthreads();
+      if (y == 0) {
+        for (int k = 1; k < (int)kJoin; ++k) {
+          const float4 q = sums[k][x];
+          v[0] += q.x, v[1] += q.y, v[2] += q.z, v[3] += q.w;
+        }
+        put(v, t, base + x * 4);
+      }
     }
   }
 }
@@ -365,17 +410,17 @@ void embedding_backward(const fhe_embedding_grad_args& a) {
   for (uint64_t run = kRun; run < f.count; run *= kMerge) ++sorts;
   auto fill = [&] {
     const uint64_t each = bytes / sorts / 16 * 16, from = each * share++, to = share == sorts ? bytes : each * share;
-    return Fill{table + from, to - from, (uint32_t)std::min<uint64_t>(148 * 4, (to - from + 65535) / 65536)};
+    return Fill{table + from, to - from, (uint32_t)std::min<uint64_t>(148 * 2, (to - from + 65535) / 65536)};
   };
   const Fill one = fill();
-  k_sort<<<runs + one.blocks, kRun, 0, st>>>(f.ids, f.wide_ids, f.count, f.vocab, runs, p.a, one);
+  k_sort<<<runs + one.blocks, kRun, 0, st>>>(f.ids, f.wide_ids, f.count, f.vocab, p.a, one);
   note_launch();
   Sorted s = p.a, other = p.b;
   const uint32_t own = (f.count + 31) / 32;
   static_assert(kRun == 1u << 8 && kMerge == 1u << 5, "powers of two");
   for (uint32_t log = 8; (1ull << log) < f.count; log += 5) {
     const Fill more = fill();
-    k_merge<<<own + more.blocks, 32 * kMergeWarps, 0, st>>>(s, other, f.count, log, own, more);
+    k_merge<<<own + more.blocks, 32 * kMergeWarps, 0, st>>>(s, other, f.count, log, more);
     note_launch();
     std::swap(s, other);
   }
@@ -391,7 +436,7 @@ void embedding_backward(const fhe_embedding_grad_args& a) {
     else k_sum<T, Y, 1><<<grid, block, 0, st>>>(a, s, p.chunk, p.chunks, p.part);
     note_launch();
     if (p.chunks > 1) {
-      const dim3 cover(p.chunks, std::min(4u, (f.width + 255) / 256));
+      const dim3 cover((p.chunks + kJoin - 1) / kJoin, std::min(8u, (f.width + 127) / 128));
       if (f.width % 4 == 0) k_join<T, true><<<cover, 256, 0, st>>>(a, s, p.chunk, p.chunks, p.part);
       else k_join<T, false><<<cover, 256, 0, st>>>(a, s, p.chunk, p.chunks, p.part);
       note_launch();

@@ -214,16 +214,18 @@ void rms_norm(const fhe_rms_norm_args& a) {
   g.lanes = s.lanes;
   // Blocks that go from row to row.  With a ring as many as are resident: 24 warps an SM
   // where two rows fit the ring, fewer rows else (32768 x 1536 bfloat16 with three rows
-  // and 22 warps 60 us, with two and 24 57 us; loads of one row in registers 65 us).
+  // and 22 warps 60 us, with two and 24 57 us; loads of one row in registers 65 us); 40
+  // for one chunk of float32 (40000 groups of 192: 19 us, 22; of bfloat16 41 us, 39).
   uint32_t resident = 12, shared = 0;
   if (a.gate && s.layout(vec) == kWords) {
     const uint32_t warps = s.warps * s.rows_per_block, row = s.chunks * ea * 16 * 32 * warps;
+    const uint32_t full = s.chunks == 1 && ea == 4 ? 40 : 24;
     for (g.stages = 3; g.stages > 1; --g.stages) {
       const uint32_t fit = kSmShared / (g.stages * row + kBlockShared);
-      if (fit && fit * warps >= 24) break;
+      if (fit && fit * warps >= full) break;
     }
     shared = g.stages * row;
-    resident = std::max(1u, std::min(24 / warps, kSmShared / (shared + kBlockShared)));
+    resident = std::max(1u, std::min(full / warps, kSmShared / (shared + kBlockShared)));
   }
   const uint32_t blocks = std::min((a.rows + s.rows_per_block - 1) / s.rows_per_block,
                                    std::max(1u, 148 * resident / a.groups));
