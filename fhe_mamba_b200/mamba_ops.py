@@ -30,7 +30,7 @@ from ._lib import call
 _TYPES = {torch.float32: _lib.FHE_F32, torch.bfloat16: _lib.FHE_BF16, torch.float16: _lib.FHE_F16}
 MAX_HEAD_DIM, MAX_STATE, MAX_TAPS, MAX_TOP, MAX_NORM_WIDTH = 128, 256, 8, 64, 16384
 MAX_BEAMS = 64
-_INF = float("inf")
+_LARGEST = torch.finfo(torch.float32).max
 
 
 def _need(ok, message):
@@ -405,11 +405,11 @@ def _check_norm(op, x, weight, eps, others, dtype, groups=1, scale=1.0):
         _need(t.dtype in types, f"{op}: {name} must be {' or '.join(str(v) for v in types)}, got {t.dtype}")
     _need(dtype == x.dtype or (x.dtype == torch.float32 and dtype in _TYPES),
           f"{op}: dtype must be x's, or a smaller one of a float32 x")
-    _need(0 < eps < float("inf"), f"{op}: eps must be positive")
+    _need(0 < eps <= _LARGEST, f"{op}: eps must be positive")
     if torch.is_tensor(scale):
         _check(op, "scale", scale, (width,), torch.float32)
     else:
-        _need(abs(scale) < float("inf"), f"{op}: scale must be finite")
+        _need(abs(scale) <= _LARGEST, f"{op}: scale must be finite")
     _check_devices(op, x, weight, scale if torch.is_tensor(scale) else None, *(t for _, t, _ in others))
 
 
@@ -504,7 +504,7 @@ def _norm_fits(x, weight, eps, dtype):
     """Whether the arguments that all norms share pass ``_check_norm``."""
     t, w = x.dtype, x.shape[-1] if x.dim() else 0
     return (x.is_cuda and t in _TYPES and 1 <= w <= MAX_NORM_WIDTH and weight.shape == (w,)
-            and weight.dtype == torch.float32 and weight.get_device() == x.get_device() and 0 < eps < _INF
+            and weight.dtype == torch.float32 and weight.get_device() == x.get_device() and 0 < eps <= _LARGEST
             and (dtype == t or (t == torch.float32 and dtype in _TYPES)))
 
 
@@ -537,7 +537,7 @@ def add_rms_norm(residual, x, weight, eps=1e-5, scale=1.0):
     t, r = x.dtype, residual.dtype
     channel_scale, factor = (_dense(scale), 1.0) if isinstance(scale, torch.Tensor) else (None, scale)
     if not (_norm_fits(x, weight, eps, t) and residual.shape == x.shape and (r == t or r == torch.float32)
-            and residual.get_device() == x.get_device() and -_INF < factor < _INF
+            and residual.get_device() == x.get_device() and -_LARGEST <= factor <= _LARGEST
             and (channel_scale is None or (channel_scale.shape == weight.shape and channel_scale.dtype == torch.float32
                                            and channel_scale.get_device() == x.get_device()))):
         _check_norm(op, x, weight, eps, (("residual", residual, (t, torch.float32)),), t, scale=scale)
@@ -584,18 +584,19 @@ def _run_embedding(tokens, weight, scale, dtype):
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, weight, tokens, scale, dtype):
-        ctx.rest = scale, dtype
-        ctx.save_for_backward(weight, tokens)
+        ctx.rest = scale, dtype, weight.shape, weight.dtype
+        ctx.save_for_backward(tokens)  # the table may change before the backward pass
         return _run_embedding(tokens, weight, scale, dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        weight, tokens = ctx.saved_tensors
-        dout, dw = dout.contiguous(), _new(weight, weight.dtype)
-        f = _embedding_values(tokens, weight, *ctx.rest, None)
+        tokens, = ctx.saved_tensors
+        scale, dtype, shape, weight_dtype = ctx.rest
+        dout, dw = dout.contiguous(), torch.empty(shape, dtype=weight_dtype, device=tokens.device)
+        f = _embedding_values(tokens, dw, scale, dtype, None)
         outs = dout.data_ptr(), dw.data_ptr()
-        ws = _space("fhe_embedding_backward_workspace", _embedding_grad_block(*f, *outs, 0, 0, 0), weight.device)
+        ws = _space("fhe_embedding_backward_workspace", _embedding_grad_block(*f, *outs, 0, 0, 0), dw.device)
         call("fhe_embedding_backward", _embedding_grad_block(*f, *outs, ws.data_ptr(), ws.numel(), f[-1]))
         return dw, None, None, None
 
@@ -614,7 +615,7 @@ def embedding(tokens, weight, scale=1.0, dtype=None):
           f"{op}: weight must be [vocab, width] float32, bfloat16 or float16")
     _need(weight.shape[1] <= 1 << 20, f"{op}: width must be at most 2^20")
     _need(dtype in (weight.dtype, torch.float32), f"{op}: dtype must be weight's or float32")
-    _need(abs(scale) < float("inf"), f"{op}: scale must be finite")
+    _need(abs(scale) <= _LARGEST, f"{op}: scale must be finite")
     _check_devices(op, weight, tokens)
     tokens, rows = _dense(tokens), _inner(weight)
     if _wants_grad(weight):

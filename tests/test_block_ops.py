@@ -21,6 +21,7 @@ z = torch.zeros
     ((z(1, 16385), z(16385)), "at most 16384"),
     ((z(2, 4), z(4), 0.0), "eps"),
     ((z(2, 4), z(4), float("nan")), "eps"),
+    ((z(2, 4), z(4), 1e39), "eps"),
     ((z(2, 4), z(4), 1e-5, F64), "dtype"),
     ((z(2, 4, dtype=BF16), z(4), 1e-5, F32), "dtype"),
     ((z(2, 4), z(4)), "CUDA tensors expected"),
@@ -39,6 +40,7 @@ def test_norm_refusals(args, message):
     ((z(2, 4), z(2, 4), z(4), 1e-5, z(())), "scale must have shape"),
     ((z(2, 4), z(2, 4), z(4), 1e-5, z(4, dtype=BF16)), "scale must be"),
     ((z(2, 4), z(2, 4), z(4), 1e-5, float("inf")), "scale must be finite"),
+    ((z(2, 4), z(2, 4), z(4), 1e-5, -1e39), "scale must be finite"),
     ((z(2, 4), z(2, 4), z(4)), "CUDA tensors expected"),
 ])
 def test_add_norm_refusals(args, message):
@@ -117,6 +119,7 @@ I64 = torch.int64
     ((z(3, dtype=I64), z(5, 4), 1.0, BF16), "dtype"),
     ((z(3, dtype=I64), z(5, 4, dtype=F16), 1.0, BF16), "dtype"),
     ((z(3, dtype=I64), z(5, 4), float("nan")), "scale"),
+    ((z(3, dtype=I64), z(5, 4), 1e39), "scale"),
     ((z(3, dtype=I64), z(5, 4)), "CUDA tensors expected"),
 ])
 def test_embedding_refusals(args, message):

@@ -95,6 +95,21 @@ def test_shapes_and_strides(ops):
     assert g.shape == leaf.shape and not g.any()
 
 
+def test_table_changed_or_empty(ops):
+    """The gradient needs no value of the table; a table without rows has nothing but absent tokens."""
+    leaf = torch.ones(5, 16, device="cuda", requires_grad=True)
+    tokens = torch.tensor([1, 1, 4], device="cuda")
+    y = ops.embedding(tokens, leaf)
+    with torch.no_grad():
+        leaf.add_(1)
+    g, = torch.autograd.grad(y.sum(), leaf)
+    assert torch.equal(g.sum(1), torch.tensor([0.0, 32, 0, 0, 16], device="cuda"))
+    none = torch.empty(0, 16, device="cuda", requires_grad=True)
+    y = ops.embedding(torch.tensor([0, -1], device="cuda"), none)
+    assert torch.isnan(y[0]).all() and (y[1] == 0).all()
+    assert torch.autograd.grad(y.sum(), none)[0].shape == (0, 16)
+
+
 def test_large_offsets(ops):
     """Rows past 2^31 elements of the table, its gradient and the outputs."""
     table = torch.zeros(40000, 1 << 16, device="cuda", dtype=torch.bfloat16)

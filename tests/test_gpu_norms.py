@@ -200,6 +200,31 @@ def test_ranges(ops, width):
     assert torch.equal(h[1::2], x.half()[1::2]) and torch.isfinite(y[1::2]).all() and torch.isnan(y[4]).all()
 
 
+def test_large_offsets(ops):
+    """Rows past 2^31 elements, wide and narrow."""
+    for rows, width in ((135000, 16384), (300_000_000, 8)):
+        x = torch.zeros(rows, width, device="cuda", dtype=torch.bfloat16)
+        g = torch.Generator(device="cuda").manual_seed(width)
+        some = torch.randn(3, width, generator=g, device="cuda").bfloat16()
+        at = torch.tensor([0, rows // 2 + 1, rows - 1], device="cuda")
+        x[at] = some
+        w = (1 + torch.randn(width, generator=g, device="cuda")).requires_grad_()
+        small = some.clone().requires_grad_()
+        want = ops.rms_norm(small, w)
+        dw_want, dx_want = torch.autograd.grad(want, (w, small), some)
+        x.requires_grad_()
+        y = ops.rms_norm(x, w)
+        assert torch.equal(y[at], want) and not y[1:9].any()
+        dw, dx = torch.autograd.grad(y, (w, x), x.detach())
+        assert torch.equal(dx[at], dx_want)
+        # every other row adds an exact 0; three terms, added in whatever order, are off by 2 u of their magnitudes each way
+        _, r = norm_of(some.double(), w.detach().double(), 1e-5)
+        mag = (some.double() * some.double() * r).abs().sum(0)
+        assert ((dw - dw_want).abs() <= 6 * U * mag).all()
+        del x, y, dx
+        torch.cuda.empty_cache()
+
+
 def test_gradients_against_differences(ops):
     """Directional derivatives against central differences of the forward calls: the differences of steps of 2^-6 are
     off by the third-order term, below a hundredth of inputs of size 1, and by 2^-24 sqrt(n) / 2^-6 of the outputs."""
