@@ -42,7 +42,8 @@ __global__ void __launch_bounds__(512) k_norm(const NormArgs g) {
   const uint32_t step = gridDim.x * blockDim.y * rows;
   uint32_t base = (blockIdx.x * blockDim.y + threadIdx.y) * rows;
   // The next row's words come while this one is summed and written: into registers,
-  // or with a gate, whose sigmoids take longer, one or two rows ahead through a ring.
+  // or with a gate, whose sigmoids take longer, a row ahead through a ring (32768 x 1536
+  // bfloat16: 50 us, 65 with loads in registers).
   Eight<X> e[N];
   Eight<Y> f[kTwo ? N : 1];
   constexpr int kQ = Eight<A>::kQuads;
@@ -84,6 +85,7 @@ __global__ void __launch_bounds__(512) k_norm(const NormArgs g) {
     const uint32_t row = base + sub;
     const bool live = !kNarrow || row < g.rows;
     if constexpr (kRing) {
+      __syncwarp();  // the row to be filled has been read
       fetch(row + (g.stages - 1) * step, stage ? stage - 1 : g.stages - 1);
       wait_copies(g.stages);
 #pragma unroll
@@ -212,20 +214,14 @@ void rms_norm(const fhe_rms_norm_args& a) {
                    norm_aligned(a.weight, 0, 4) && norm_aligned(a.y, 0, ea) && norm_aligned(a.h, 0, eh);
   const NormShape s = norm_shape(g.gw, (uint64_t)a.rows * a.groups, vec);
   g.lanes = s.lanes;
-  // Blocks that go from row to row.  With a ring as many as are resident: 24 warps an SM
-  // where two rows fit the ring, fewer rows else (32768 x 1536 bfloat16 with three rows
-  // and 22 warps 60 us, with two and 24 57 us; loads of one row in registers 65 us); 40
-  // for one chunk of float32 (40000 groups of 192: 19 us, 22; of bfloat16 41 us, 39).
+  // blocks that go from row to row
   uint32_t resident = 12, shared = 0;
   if (a.gate && s.layout(vec) == kWords) {
     const uint32_t warps = s.warps * s.rows_per_block, row = s.chunks * ea * 16 * 32 * warps;
-    const uint32_t full = s.chunks == 1 && ea == 4 ? 40 : 24;
-    for (g.stages = 3; g.stages > 1; --g.stages) {
-      const uint32_t fit = kSmShared / (g.stages * row + kBlockShared);
-      if (fit && fit * warps >= full) break;
-    }
-    shared = g.stages * row;
-    resident = std::max(1u, std::min(full / warps, kSmShared / (shared + kBlockShared)));
+    const RingPlan r = ring_plan(row, warps, 104 * 1024);
+    g.stages = (int)r.stages;
+    shared = r.stages * row;
+    resident = r.blocks;
   }
   const uint32_t blocks = std::min((a.rows + s.rows_per_block - 1) / s.rows_per_block,
                                    std::max(1u, 148 * resident / a.groups));

@@ -122,10 +122,12 @@ __device__ __forceinline__ void store_chunk(const Eight<T>& e, T* p, int c, int 
   }
 }
 
-// A lane's part of its warp's ring in shared memory: rows of `words` 16-byte words a
-// lane, filled by asynchronous copies (through the first cache where two words lie in
-// one sector, past it otherwise) and read by the lane that asked for them.  Words past
-// the row's end hold 0.
+// A warp's ring in shared memory: rows of `words` 16-byte words a lane, filled by
+// asynchronous copies.  Arrays lie in it as in memory, chunk by chunk, and each
+// copy of a warp takes whole lines: with float32 a lane copies words that its
+// neighbours read (two of its own lie in one sector, which a second copy would fetch
+// again).  So the warp meets behind its waits and before it fills a row again.
+// Words past the row's end hold 0.
 template <int WORDS>
 struct Ring {
   uint32_t base;
@@ -134,47 +136,49 @@ struct Ring {
     const uint32_t warp = threadIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5);
     base = (uint32_t)__cvta_generic_to_shared(shared) + warp * stages * kRow + (threadIdx.x & 31) * 16;
   }
+  // Word k of chunk c that this lane copies, from the lane's own channels on.
+  template <class T>
+  __device__ __forceinline__ static int word(int c, int k) {
+    return away<kWords>(c, 0) + (Eight<T>::kQuads == 2 ? k * 128 - (int)(threadIdx.x & 31) * 4 : 0);
+  }
   // Chunk c of an array whose words start at `first`.
   template <class T>
   __device__ __forceinline__ void copy(int stage, int first, const T* p, int c, int left) const {
     constexpr int Q = Eight<T>::kQuads;
-    if (away<kWords>(c, 0) < left) {
 #pragma unroll
-      for (int k = 0; k < Q; ++k) {
-        const uint32_t to = base + stage * kRow + (first + c * Q + k) * 512;
-        const T* at = p + away<kWords>(c, 0) + k * (16 / sizeof(T));
-        if constexpr (Q == 2) asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(to), "l"(at) : "memory");
-        else asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(at) : "memory");
-      }
-    }
+    for (int k = 0; k < Q; ++k)
+      if (word<T>(c, k) < left)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(base + stage * kRow + (first + c * Q + k) * 512),
+                     "l"(p + word<T>(c, k)) : "memory");
   }
   template <class T>
   __device__ __forceinline__ void take(Eight<T>& e, int stage, int first, int c) const {
     constexpr int Q = Eight<T>::kQuads;
+    const uint32_t at = base + stage * kRow + (first + c * Q) * 512 + (Q == 2 ? (threadIdx.x & 31) * 16 : 0);
 #pragma unroll
     for (int k = 0; k < Q; ++k)
       asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                    : "=r"(e.w[4 * k]), "=r"(e.w[4 * k + 1]), "=r"(e.w[4 * k + 2]), "=r"(e.w[4 * k + 3])
-                   : "r"(base + stage * kRow + (first + c * Q + k) * 512) : "memory");
+                   : "r"(at + k * 16) : "memory");
   }
   // 0 where no copy of chunk c goes, in every row.
   template <class T>
   __device__ __forceinline__ void blank(int stages, int first, const T*, int c, int left) const {
     constexpr int Q = Eight<T>::kQuads;
-    if (away<kWords>(c, 0) < left) return;
-    for (int stage = 0; stage < stages; ++stage)
 #pragma unroll
-      for (int k = 0; k < Q; ++k)
-        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(base + stage * kRow + (first + c * Q + k) * 512), "r"(0)
-                     : "memory");
+    for (int k = 0; k < Q; ++k)
+      if (word<T>(c, k) >= left)
+        for (int stage = 0; stage < stages; ++stage)
+          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(base + stage * kRow + (first + c * Q + k) * 512), "r"(0)
+                       : "memory");
   }
 };
 
-// Waits until all but the last `stages` - 1 groups of copies are there.
+// Waits until all but the last `stages` - 1 (0 or 1) groups of the warp's copies are there.
 __device__ __forceinline__ void wait_copies(int stages) {
-  if (stages == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
-  else if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+  if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
   else asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncwarp();
 }
 
 // Sum over the threads of a row, one value for all of them: some lanes, a warp, or
@@ -230,6 +234,22 @@ inline NormShape norm_shape(uint32_t gw, uint64_t rows, bool vec) {
 }
 
 constexpr uint32_t kSmShared = 227 * 1024, kBlockShared = 1024 + 256;  // of an SM; of a block beside its ring
+
+// Rows in the ring and blocks an SM for blocks of `warps` warps whose row takes `row`
+// bytes: two rows, and as many blocks as bring the rings to about `target` bytes but 8
+// warps at least.  More traffic in flight is slower, not faster: 32768 x 1536 bfloat16
+// with a gate, gradients, two rows: 93 us with 8 warps (74 KB), 80 with 12 (110 KB), 88
+// with 16, 102 with 20; forward 62, 53, 50 and 53 us.
+struct RingPlan {
+  uint32_t stages, blocks;
+};
+inline RingPlan ring_plan(uint32_t row, uint32_t warps, uint32_t target) {
+  RingPlan p{2, 1};
+  if (2 * row + kBlockShared > kSmShared) p.stages = 1;
+  const uint32_t block = p.stages * row, most = std::max(1u, kSmShared / (block + kBlockShared));
+  p.blocks = std::min(most, std::max(target / block, (8 + warps - 1) / warps));
+  return p;
+}
 
 inline bool norm_aligned(const void* p, int64_t stride, uint32_t elem) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % (int64_t)(16 / elem) == 0;

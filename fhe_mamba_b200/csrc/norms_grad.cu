@@ -119,6 +119,7 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
     const int64_t out = (int64_t)row * g.width + c0;
     const float r = live ? g.rstd[(int64_t)row * g.groups + blockIdx.y] : 0.f;
     if constexpr (VEC) {
+      __syncwarp();  // the row to be filled has been read
       fetch(row + (g.stages - 1) * step, stage ? stage - 1 : g.stages - 1);
       wait_copies(g.stages);
     } else {
@@ -289,9 +290,8 @@ bool words(const fhe_rms_norm_grad_args& a) {
          norm_aligned(a.dgate, 0, ea);
 }
 
-// How a call is laid out: shape, rows of the ring (three where 16 warps still fit an
-// SM, two where 12 do), shared memory, and blocks that go from row to row, as many as
-// are resident.
+// How a call is laid out: shape, rows of the ring, shared memory, and blocks that go
+// from row to row, as many as are resident.
 struct GradPlan {
   NormShape shape;
   bool vec;
@@ -312,12 +312,10 @@ GradPlan grad_plan(const fhe_rms_norm_grad_args& a) {
     if (p.shape.layout(p.vec) == kWords) {
       const uint32_t row = p.shape.chunks * per_chunk * 16 * 32 * warps;
       if (row + kBlockShared > kSmShared) continue;
-      for (p.stages = 3; p.stages > 1; --p.stages) {
-        const uint32_t fit = kSmShared / (p.stages * row + kBlockShared);
-        if (fit && fit * warps >= (p.stages == 3 ? 16 : 12)) break;
-      }
+      const RingPlan r = ring_plan(row, warps, 120 * 1024);
+      p.stages = r.stages;
       p.shared = std::max(p.shared, p.stages * row);
-      resident = std::max(1u, std::min(resident, kSmShared / (p.shared + kBlockShared)));
+      resident = r.blocks;
     }
     p.blocks = std::max(1u, std::min((f.rows + p.shape.rows_per_block - 1) / p.shape.rows_per_block,
                                      std::max(1u, 148 * resident / f.groups)));
