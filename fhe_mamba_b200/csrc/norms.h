@@ -208,14 +208,14 @@ struct RowSum {
 
 // Warps per row and chunks of eight channels per thread.  Few rows are spread over
 // as many warps as have a chunk.  Else a thread takes three chunks where that fills
-// every lane, else four (single elements, which need more registers: two); at most 16
-// warps.  Four rows of one warp share a block, a longer row has its own.
+// every lane, else four (single elements and gradients through a gate, which need more
+// registers: two; 40000 x 1024 bfloat16 gradients 79 us, 104); at most 16 warps.  Four rows of one warp share a block, a longer row has its own.
 // Narrow rows share a warp.
 struct NormShape {
   uint32_t warps, chunks, rows_per_block, lanes;
   int layout(bool words) const { return (words ? kWords : kSingles) + (lanes < 32 ? kNarrowSingles : 0); }
 };
-inline NormShape norm_shape(uint32_t gw, uint64_t rows, bool vec) {
+inline NormShape norm_shape(uint32_t gw, uint64_t rows, bool vec, bool heavy = false) {
   const uint32_t all = (gw + 7) / 8;
   if (all <= 16) {
     uint32_t lanes = 1;
@@ -223,7 +223,7 @@ inline NormShape norm_shape(uint32_t gw, uint64_t rows, bool vec) {
     return {1, 1, 4 * 32 / lanes, lanes};
   }
   const bool whole = vec && all % 96 == 0 && all / 96 <= 8;
-  const uint32_t want = rows < 2 * 148 ? 1 : whole ? 3 : vec ? 4 : 2;
+  const uint32_t want = rows < 2 * 148 ? 1 : whole ? 3 : vec && !heavy ? 4 : 2;
   NormShape s;
   s.warps = std::min(16u, (all + 32 * want - 1) / (32 * want));
   s.chunks = (all + 32 * s.warps - 1) / (32 * s.warps);

@@ -305,7 +305,7 @@ GradPlan grad_plan(const fhe_rms_norm_grad_args& a) {
   GradPlan p{};
   p.vec = words(a);
   for (;; p.vec = false) {
-    p.shape = norm_shape(gw, (uint64_t)f.rows * f.groups, p.vec);
+    p.shape = norm_shape(gw, (uint64_t)f.rows * f.groups, p.vec, f.gate != nullptr);
     const uint32_t warps = p.shape.warps == 1 ? 4 : p.shape.warps;  // of a block
     uint32_t resident = std::max(1u, 16 / warps);
     p.shared = p.shape.warps == 1 ? gw * sizeof(float) : 0;  // one warp's channels, at most 1024

@@ -413,6 +413,15 @@ def _check_norm(op, x, weight, eps, others, dtype, groups=1, scale=1.0):
     _check_devices(op, x, weight, scale if torch.is_tensor(scale) else None, *(t for _, t, _ in others))
 
 
+def _first_derivatives(backward):
+    """``once_differentiable`` where a graph of the backward pass is asked for, else the function as it is."""
+    guarded = once_differentiable(backward)
+
+    def call_backward(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return call_backward
+
+
 _norm_block, _norm_grad_block = _lib.packer(_lib.RmsNormArgs), _lib.packer(_lib.RmsNormGradArgs)
 
 
@@ -467,7 +476,7 @@ class _RmsNorm(torch.autograd.Function):
         return y if h is None else (y, h)
 
     @staticmethod
-    @once_differentiable
+    @_first_derivatives
     def backward(ctx, dy, dh=None):
         x, gate, weight, channel_scale, h, rstd = ctx.saved_tensors
         eps, scale, groups, dtype, x_dtype = ctx.rest
@@ -589,7 +598,7 @@ class _Embedding(torch.autograd.Function):
         return _run_embedding(tokens, weight, scale, dtype)
 
     @staticmethod
-    @once_differentiable
+    @_first_derivatives
     def backward(ctx, dout):
         tokens, = ctx.saved_tensors
         scale, dtype, shape, weight_dtype = ctx.rest

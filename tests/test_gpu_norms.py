@@ -268,6 +268,16 @@ def test_partial_gradients(ops):
             assert torch.equal(got, want[i]), i
 
 
+def test_second_derivatives_are_refused(ops):
+    """A graph of the backward pass may be asked for; using it raises, and no gradient comes out as if it were constant."""
+    x, w = normal(1, 6, 32).requires_grad_(), (1 + normal(2, 32)).requires_grad_()
+    table, tokens = normal(3, 9, 32).requires_grad_(), torch.tensor([1, 4], device="cuda")
+    for y, leaf in ((ops.rms_norm(x, w), x), (ops.gated_rms_norm(x, x, w), w), (ops.embedding(tokens, table) * x[0], table)):
+        once, = torch.autograd.grad(y.sin().sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            once.sum().backward()
+
+
 def test_streams_and_graphs(ops):
     """Another stream than the default one, and a captured call replayed on new values."""
     x, r, w = normal(1, 50, 768).bfloat16(), normal(2, 50, 768), 1 + normal(3, 768)
