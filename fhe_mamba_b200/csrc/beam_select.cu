@@ -510,13 +510,13 @@ void beam_select(const fhe_beam_select_args& a) {
   DeviceGuard dev(a.device);
   with_type(a.dtype, [&](auto t) {
     using T = decltype(t);
-    // As many CTAs to an item as the device takes at once, and a turn of loads for each;
+    // As many CTAs to an item as the device takes at once, a beam or a turn of loads for each;
     // sixteen where eight would take several beams each (1 x 10 beams of 50280 bfloat16:
     // 17 us, 23 with eight; 1 x 4: 11 us with either)
     const uint64_t packs = (uint64_t)a.beams * (a.vocab / Quad<T>::kElems);
     SelectArgs g{a, 1, std::min(a.width, a.vocab)};
     while (g.cluster < (a.beams > 8 ? kMaxCluster : 8) && (uint64_t)a.batch * g.cluster * 2 <= 148 * 4 &&
-           packs >= (uint64_t)g.cluster * 2 * kAhead * kThreads)
+           (g.cluster < a.beams || packs >= (uint64_t)g.cluster * 2 * kAhead * kThreads))
       g.cluster *= 2;
     const uint32_t shared = Layout(nullptr, a.beams + g.cluster, g.kk).bytes;
     if (shared > 32768)
