@@ -25,6 +25,8 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kGroups = 64;   // groups of 4 threads
+constexpr uint32_t kFineWidth = 32;    // more best entries than this are bounded by every thread's maximum
+constexpr uint32_t kAllRanked = 512;   // entries of an item up to which none is left out before ranking
 constexpr int kAhead = 4;     // 16-byte loads in flight per thread
 constexpr int kCap = 1024;    // candidates held
 constexpr uint32_t kMaxBeams = 64, kMaxWidth = 64, kMaxCluster = 16;
@@ -87,10 +89,19 @@ __device__ __forceinline__ uint64_t add_exps(const Quad<T>& q, uint64_t acc, uin
 struct Scratch {
   float fred[kWarps];
   double dred[kWarps];
-  __align__(16) uint32_t gmax[kGroups];
+  __align__(16) uint32_t gmax[kThreads];
   uint32_t ckey[kCap], cidx[kCap], hit[kThreads];
   uint32_t hits, bound, count, raises;
 };
+
+// A number as an unsigned integer of the same order, and back.
+__device__ __forceinline__ uint64_t ordered(double v) {
+  const uint64_t u = (uint64_t)__double_as_longlong(v);
+  return u >> 63 ? ~u : u | 1ull << 63;
+}
+__device__ __forceinline__ double number(uint64_t o) {
+  return __longlong_as_double((int64_t)(o >> 63 ? o & ~(1ull << 63) : ~o));
+}
 
 __device__ __forceinline__ double block_sum(double v, double (&red)[kWarps]) {
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
@@ -166,20 +177,25 @@ __device__ void scan_share(const T* z, uint32_t vocab, uint32_t part, uint32_t p
     s += (double)exp2_fast((f - fmaxf(m, -FLT_MAX)) * kLog2e);
     best = fmaxf(best, f);
   }
-  // a lower bound on the k-th largest, and the threads that reach it
+  // a lower bound on the k-th largest: that of the maxima of groups of threads, or of
+  // all threads where there are many to find or fewer groups have loads than there are
+  // to find; and the threads that reach it
+  const bool fine = k > kFineWidth || packs - first < 4 * k;
   float group = best;
-  for (int o = kThreads / kGroups / 2; o; o >>= 1) group = fmaxf(group, __shfl_xor_sync(~0u, group, o));
+  if (!fine)
+    for (int o = kThreads / kGroups / 2; o; o >>= 1) group = fmaxf(group, __shfl_xor_sync(~0u, group, o));
   float most = m;
   for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, o));
-  if (tid % (kThreads / kGroups) == 0) sm.gmax[tid / (kThreads / kGroups)] = order_key(group);
+  const uint32_t groups = fine ? kThreads : kGroups, per = kThreads / groups;
+  if (tid % per == 0) sm.gmax[tid / per] = order_key(group);
   if ((tid & 31) == 0) sm.fred[tid >> 5] = most;
   if (raises > 1) atomicMax(&sm.raises, raises);
   __syncthreads();
-  if (tid < kGroups) {
+  if (tid < groups) {
     const uint32_t own = sm.gmax[tid];
     uint32_t above = 0;
-#pragma unroll
-    for (uint32_t j = 0; j < kGroups; j += 4) {
+#pragma unroll 8
+    for (uint32_t j = 0; j < groups; j += 4) {
       const uint4 o = *reinterpret_cast<const uint4*>(&sm.gmax[j]);
       above += before(o.x, j, own, tid) + before(o.y, j + 1, own, tid) + before(o.z, j + 2, own, tid) +
                before(o.w, j + 3, own, tid);
@@ -294,6 +310,7 @@ __global__ void __launch_bounds__(kThreads) k_select(const SelectArgs g) {
   __shared__ uint32_t lcount[kMaxBeams + kMaxCluster], lbeam[kMaxBeams + kMaxCluster];
   __shared__ double rtotal[kMaxWidth];
   __shared__ uint32_t rbeam[kMaxWidth], rtok[kMaxWidth];
+  __shared__ uint32_t votes[kMaxBeams + kMaxCluster];
   __shared__ uint64_t unsure, agreed;  // beams to sum again: the first CTA's, all CTAs'
   const fhe_beam_select_args& a = g.a;
   const uint32_t tid = threadIdx.x, C = g.cluster, rank = blockIdx.x % C, item = blockIdx.x / C;
@@ -396,6 +413,38 @@ __global__ void __launch_bounds__(kThreads) k_select(const SelectArgs g) {
         }
       }
       __syncthreads();
+      // Many entries: the lists, which are in order, are cut behind what lies within reach
+      // of the k-th largest total, whose upper word is found bit by bit.
+      if (lists * kk > kAllRanked) {
+        auto upper = [&](double v) { return (uint32_t)(ordered(v) >> 32); };
+        auto at_least = [&](auto&& in) {  // entries of this thread's list up to the first that is not in
+          uint32_t lo = 0;
+          for (uint32_t len = tid < lists ? lcount[tid] : 0; len;) {
+            const uint32_t half = len / 2;
+            const bool f = in(l.total[tid * kk + lo + half]);
+            lo = f ? lo + half + 1 : lo;
+            len = f ? len - half - 1 : half;
+          }
+          return lo;
+        };
+        uint32_t kth = 0;
+        for (uint32_t bit = 1u << 31; bit; bit >>= 1) {
+          if (tid < lists) votes[tid] = at_least([&](double v) { return upper(v) >= (kth | bit); });
+          __syncthreads();
+          uint32_t all = 0;
+          for (uint32_t u = tid & 31; u < lists; u += 32) all += votes[u];
+          all = __reduce_add_sync(~0u, all);
+          if (all >= k) kth |= bit;
+          __syncthreads();
+        }
+        double reach = 0.;
+        for (uint32_t i = 0; i < B; ++i) reach = fmax(reach, 2. * err[i]);
+        const double least = number((uint64_t)kth << 32) - reach;
+        const uint32_t keep = at_least([&](double v) { return v >= least; });
+        __syncthreads();
+        if (tid < lists) lcount[tid] = keep;
+        __syncthreads();
+      }
       // Ranks: larger total, lower beam, larger logit, lower token.  An entry of another
       // beam may belong before one of the best if the next of its list is too close to
       // that one.

@@ -118,6 +118,12 @@ def test_ties(ops, dtype, vocab):
     apart[1] -= 7
     apart[1, 3] = torch.nextafter(apart[1, 3], apart[1, 3] + 1)
     check(ops, same, apart, width=min(20, 4 * vocab))
+    # many lists of equal entries, of possible and of impossible ones
+    wide = torch.zeros(2, 16, device="cuda")
+    check(ops, row.expand(32, vocab), wide, width=min(64, 16 * vocab))
+    wide[1, 3:] = -INF
+    check(ops, torch.full((32, vocab), -1.0, device="cuda", dtype=dtype), wide, width=min(64, 16 * vocab))
+    check(ops, torch.full((32, vocab), -INF, device="cuda", dtype=dtype), wide, width=min(64, 16 * vocab))
     few = (row * 2).round() / 2
     check(ops, few.expand(12, vocab), apart, width=min(16, 4 * vocab))
 
