@@ -439,7 +439,8 @@ __global__ void __launch_bounds__(kThreads) k_select(const SelectArgs g) {
         }
         double reach = 0.;
         for (uint32_t i = 0; i < B; ++i) reach = fmax(reach, 2. * err[i]);
-        const double least = number((uint64_t)kth << 32) - reach;
+        // (the word of -inf with zeros behind it is no number)
+        const double least = kth <= upper(-INFINITY) ? -INFINITY : number((uint64_t)kth << 32) - reach;
         const uint32_t keep = at_least([&](double v) { return v >= least; });
         __syncthreads();
         if (tid < lists) lcount[tid] = keep;
