@@ -380,8 +380,9 @@ __global__ void __launch_bounds__(kThreads) k_select(const SelectArgs g) {
       top[i] = m;
       // Roundings of u = 2^-24: three of an exponent d = (z - m) log2 e, whose mean over
       // the sum is at most log2(vocab / sum) and twice the slack, the exponential's four,
-      // at most 16 additions; 8 u for each time that the shift moved
-      err[i] = fine ? 0x1p-24 * (2.2 * (log2((double)a.vocab) - log2(sum) + 12.) + 24. + 8. * raises) : 0.;
+      // at most 17 additions, 6 for moving the threads' sums to one shift; 8 u for each
+      // time that a thread's shift moved
+      err[i] = fine ? 0x1p-24 * (2.2 * (log2((double)a.vocab) - log2(sum) + 12.) + 32. + 8. * raises) : 0.;
     }
     __syncthreads();
     if (tid < units) {

@@ -3,8 +3,9 @@
 Parents, tokens and ends have to be those of the totals score + logit - log sum
 exp in float64, also where float32 does not tell candidates apart.  A returned
 score is that total rounded to float32, from a sum of exponentials off by at
-most 2^-24 (2.2 (log2 of the vocabulary + 12) + 24) relative to itself: 8e-6 up
-to 2^30 tokens.  Moved rows are equal."""
+most 2^-24 (2.2 (log2 of the vocabulary + 12) + 32) relative to itself (5.6e-6 up
+to 2^17 tokens), and 8 2^-24 more for each time that a running shift moves: 8e-6
+with five of them.  Moved rows are equal."""
 import math
 
 import pytest

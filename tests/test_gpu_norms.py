@@ -278,6 +278,39 @@ def test_second_derivatives_are_refused(ops):
             once.sum().backward()
 
 
+def test_one_leaf_twice_and_shared_gradients(ops):
+    """A tensor that is stream and branch at once gets both gradients; leaves that share one do not share memory."""
+    w, dy, dh = 1 + normal(1, 96), normal(2, 30, 96), normal(3, 30, 96)
+    one = normal(4, 30, 96).requires_grad_()
+    r, x = (one.detach().clone().requires_grad_() for _ in range(2))
+    got, = torch.autograd.grad(ops.add_rms_norm(one, one, w), one, (dy, dh))
+    a, b = torch.autograd.grad(ops.add_rms_norm(r, x, w), (r, x), (dy, dh))
+    assert torch.equal(a, b) and torch.equal(got, a + b)
+    torch.autograd.backward(ops.add_rms_norm(r, x, w), (dy, dh))
+    r.grad.zero_()
+    assert torch.equal(x.grad, a)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows, width", [(700, 1536), (33, 1001), (500, 64), (4, 768)])
+def test_outputs_over_inputs(ops, dtype, rows, width):
+    """The C calls may write y and h over x, residual or gate."""
+    from fhe_mamba_b200._lib import call
+    w = 1 + normal(1, width)
+    r, x, z = (normal(i, rows, width).to(dtype) for i in (2, 3, 4))
+    for over in "xz":
+        a, b = x.clone(), z.clone()
+        want = ops.gated_rms_norm(a, b, w)
+        values, _ = ops._norm_values(a, dtype, dtype, 1, 1e-5, 1.0, a, None, b, None, w, a if over == "x" else b, None, None)
+        call("fhe_rms_norm", ops._norm_block(*values))
+        assert torch.equal(a if over == "x" else b, want)
+    a, b = x.clone(), r.clone()
+    want = ops.add_rms_norm(b, a, w)
+    values, _ = ops._norm_values(a, dtype, dtype, 1, 1e-5, 1.0, a, b, None, None, w, a, b, None)
+    call("fhe_rms_norm", ops._norm_block(*values))
+    assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+
+
 def test_streams_and_graphs(ops):
     """Another stream than the default one, and a captured call replayed on new values."""
     x, r, w = normal(1, 50, 768).bfloat16(), normal(2, 50, 768), 1 + normal(3, 768)
