@@ -211,14 +211,19 @@ void rms_norm(const fhe_rms_norm_args& a) {
   NormArgs g = norm_args(a);
   const uint32_t ea = elem_size(a.dtype), eh = a.gate ? ea : elem_size(a.stream_dtype);
   const uint32_t ex = a.gate || a.residual ? ea : eh;
-  const bool vec = g.gw % 8 == 0 && norm_aligned(a.x, a.x_stride, ex) && norm_aligned(a.residual, a.residual_stride, eh) &&
-                   norm_aligned(a.gate, a.gate_stride, ea) && norm_aligned(a.channel_scale, 0, 4) &&
-                   norm_aligned(a.weight, 0, 4) && norm_aligned(a.y, 0, ea) && norm_aligned(a.h, 0, eh);
-  const NormShape s = norm_shape(g.gw, (uint64_t)a.rows * a.groups, vec);
+  Together t(g.gw);
+  t.with(a.x, a.x_stride, ex);
+  if (a.residual) t.with(a.residual, a.residual_stride, eh);
+  if (a.gate) t.with(a.gate, a.gate_stride, ea);
+  t.with(a.channel_scale, 0, 4);
+  t.with(a.weight, 0, 4);
+  t.with(a.y, a.width, ea);
+  t.with(a.h, a.width, eh);
+  const NormShape s = norm_shape(g.gw, (uint64_t)a.rows * a.groups, t.n);
   g.lanes = s.lanes;
   // blocks that go from row to row
   uint32_t resident = 12, shared = 0;
-  if (a.gate && s.layout(vec) == kWords) {
+  if (a.gate && s.layout(t.n) == kWords) {
     const uint32_t warps = s.warps * s.rows_per_block, row = s.chunks * ea * 16 * 32 * warps;
     const RingPlan r = ring_plan(row, warps, 104 * 1024);
     g.stages = (int)r.stages;
@@ -227,7 +232,7 @@ void rms_norm(const fhe_rms_norm_args& a) {
   }
   const uint32_t blocks = std::min((a.rows + s.rows_per_block - 1) / s.rows_per_block,
                                    std::max(1u, 148 * resident / a.groups));
-  with_norm(a, s.chunks, s.layout(vec), [&](auto mode, auto act, auto str, auto chunks, auto layout) {
+  with_norm(a, s.chunks, s.layout(t.n), [&](auto mode, auto act, auto str, auto chunks, auto layout) {
     auto k = k_norm<decltype(mode)::value, decltype(act), decltype(str), decltype(chunks)::value, decltype(layout)::value>;
     if (shared > 48000) FHE_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
     const dim3 block(32 * s.warps, s.warps == 1 ? 4 : 1);

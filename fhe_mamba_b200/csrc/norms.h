@@ -66,20 +66,22 @@ struct alignas(16) Eight {
 // How a row's (or group's) channels lie over lanes: N chunks of 256 to a warp, or in
 // narrow rows (up to 128 channels) one of eight to each of `lanes` lanes and several
 // rows to a warp.  Chunk c of a lane holds the channels from(): + c 256 .. + 8 where
-// 16-byte words are loaded or rows are narrow, + (c 8 + i) 32 otherwise; they read
-// consecutive memory across a warp, at constant distances.
-enum { kSingles = 0, kWords = 1, kNarrowSingles = 2, kNarrowWords = 3 };
-constexpr bool is_words(int lay) { return lay & 1; }
-constexpr bool is_narrow(int lay) { return lay >= kNarrowSingles; }
+// 16-byte words are loaded or rows are narrow, four pairs 64 apart where rows and
+// widths are even, + (c 8 + i) 32 otherwise; they read consecutive memory across a
+// warp, at constant distances.  (25000 rows of 1002, bfloat16 on float32: 61 us by
+// pairs, 77 by single elements, gradients 64 and 86.)
+enum { kSingles = 0, kWords = 1, kNarrowSingles = 2, kNarrowWords = 3, kPairs = 4 };
+constexpr bool is_words(int lay) { return lay == kWords || lay == kNarrowWords; }
+constexpr bool is_narrow(int lay) { return lay == kNarrowSingles || lay == kNarrowWords; }
 
 template <int N, int LAY>
 __device__ __forceinline__ uint32_t from(uint32_t lanes) {
   if constexpr (is_narrow(LAY)) return (threadIdx.x & (lanes - 1)) * 8;
-  return (threadIdx.x >> 5) * (N * 256) + (threadIdx.x & 31) * (is_words(LAY) ? 8 : 1);
+  return (threadIdx.x >> 5) * (N * 256) + (threadIdx.x & 31) * (is_words(LAY) ? 8 : LAY == kPairs ? 2 : 1);
 }
 template <int LAY>
 __host__ __device__ constexpr int away(int c, int i) {
-  return LAY == kSingles ? (c * 8 + i) * 32 : c * 256 + i;
+  return LAY == kSingles ? (c * 8 + i) * 32 : LAY == kPairs ? (c * 4 + i / 2) * 64 + i % 2 : c * 256 + i;
 }
 // Chunk c of the lane's channels at p; `left` of them are before the row's end, the
 // others stay as they are.
@@ -90,6 +92,17 @@ __device__ __forceinline__ void load_chunk(Eight<T>& e, const T* p, int c, int l
 #pragma unroll
       for (int k = 0; k < Eight<T>::kQuads; ++k)
         reinterpret_cast<uint4*>(e.w)[k] = reinterpret_cast<const uint4*>(p + away<LAY>(c, 0))[k];
+    }
+  } else if constexpr (LAY == kPairs) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      if (away<LAY>(c, i) >= left) continue;  // a pair lies before the row's end, or behind
+      if constexpr (sizeof(T) == 4) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p + away<LAY>(c, i));
+        e.w[i] = v.x, e.w[i + 1] = v.y;
+      } else {
+        e.w[i / 2] = *reinterpret_cast<const uint32_t*>(p + away<LAY>(c, i));
+      }
     }
   } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -111,6 +124,13 @@ __device__ __forceinline__ void store_chunk(const Eight<T>& e, T* p, int c, int 
 #pragma unroll
       for (int k = 0; k < Eight<T>::kQuads; ++k)
         reinterpret_cast<uint4*>(p + away<LAY>(c, 0))[k] = reinterpret_cast<const uint4*>(e.w)[k];
+    }
+  } else if constexpr (LAY == kPairs) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      if (away<LAY>(c, i) >= left) continue;
+      if constexpr (sizeof(T) == 4) *reinterpret_cast<uint2*>(p + away<LAY>(c, i)) = make_uint2(e.w[i], e.w[i + 1]);
+      else *reinterpret_cast<uint32_t*>(p + away<LAY>(c, i)) = e.w[i / 2];
     }
   } else {
 #pragma unroll
@@ -191,17 +211,17 @@ struct RowSum {
   __device__ __forceinline__ float operator()(float v) {
     if constexpr (NARROW) {
       for (uint32_t o = lanes / 2; o; o /= 2) v += __shfl_xor_sync(~0u, v, o);
-      return v;
-    }
+    } else {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-    if (blockDim.x == 32) return v;
-    float* r = red[turn];
-    turn ^= 1;
-    if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.f;
-    for (uint32_t w = 0; w < blockDim.x / 32; ++w) v += r[w];
+      for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+      if (blockDim.x == 32) return v;
+      float* r = red[turn];
+      turn ^= 1;
+      if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
+      __syncthreads();
+      v = 0.f;
+      for (uint32_t w = 0; w < blockDim.x / 32; ++w) v += r[w];
+    }
     return v;
   }
 };
@@ -215,9 +235,13 @@ struct RowSum {
 // each).
 struct NormShape {
   uint32_t warps, chunks, rows_per_block, lanes;
-  int layout(bool words) const { return (words ? kWords : kSingles) + (lanes < 32 ? kNarrowSingles : 0); }
+  int layout(uint32_t together) const {  // elements that may be loaded together: 8, 2 or 1
+    if (lanes < 32) return together == 8 ? kNarrowWords : kNarrowSingles;
+    return together == 8 ? kWords : together == 2 ? kPairs : kSingles;
+  }
 };
-inline NormShape norm_shape(uint32_t gw, uint64_t rows, bool vec, bool heavy = false) {
+inline NormShape norm_shape(uint32_t gw, uint64_t rows, uint32_t together, bool heavy = false) {
+  const bool vec = together == 8;
   const uint32_t all = (gw + 7) / 8;
   if (all <= 16) {
     uint32_t lanes = 1;
@@ -253,9 +277,17 @@ inline RingPlan ring_plan(uint32_t row, uint32_t warps, uint32_t target) {
   return p;
 }
 
-inline bool norm_aligned(const void* p, int64_t stride, uint32_t elem) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % (int64_t)(16 / elem) == 0;
-}
+// Elements that may be loaded together from every one of these arrays: 8 (16-byte
+// words), 2 or 1.
+struct Together {
+  uint32_t n;
+  explicit Together(uint32_t gw) : n(gw % 8 == 0 ? 8 : gw % 2 == 0 ? 2 : 1) {}
+  void with(const void* p, int64_t stride, uint32_t elem) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    if (n == 8 && (at % 16 || stride % (int64_t)(16 / elem))) n = 2;
+    if (n == 2 && (at % (2 * elem) || stride % 2)) n = 1;
+  }
+};
 
 void check_norm(const fhe_rms_norm_args& a);
 NormArgs norm_args(const fhe_rms_norm_args& a);
@@ -272,6 +304,9 @@ void with_norm(const fhe_rms_norm_args& a, uint32_t chunks, int layout, F&& f) {
     using std::integral_constant;
     if (layout == kNarrowSingles) with(integral_constant<int, 1>{}, integral_constant<int, kNarrowSingles>{});
     else if (layout == kNarrowWords) with(integral_constant<int, 1>{}, integral_constant<int, kNarrowWords>{});
+    else if (layout == kPairs && chunks == 1) with(integral_constant<int, 1>{}, integral_constant<int, kPairs>{});
+    else if (layout == kPairs && chunks == 2) with(integral_constant<int, 2>{}, integral_constant<int, kPairs>{});
+    else if (layout == kPairs) with(integral_constant<int, 4>{}, integral_constant<int, kPairs>{});
     else if (layout == kSingles && chunks == 1) with(integral_constant<int, 1>{}, integral_constant<int, kSingles>{});
     else if (layout == kSingles && chunks == 2) with(integral_constant<int, 2>{}, integral_constant<int, kSingles>{});
     else if (layout == kSingles) with(integral_constant<int, 4>{}, integral_constant<int, kSingles>{});

@@ -30,7 +30,7 @@ template <int MODE, class A, class H, int N, int LAY>
 __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs g) {
   __shared__ float red[2][16];
   extern __shared__ __align__(16) float sums[];  // the ring of rows; then sums over a block's rows
-  constexpr bool kNarrow = is_narrow(LAY), VEC = LAY == kWords;  // words of wide rows come through the ring
+  constexpr bool kNarrow = is_narrow(LAY), kRing = LAY == kWords;  // words of wide rows come through the ring
   RowSum<kNarrow> row_sum{red, g.lanes};
   using W = GradWords<MODE, A, H, N>;
   constexpr bool kAdd = W::kAdd, kScaled = MODE == kNormAddScaled, kThird = W::kThird;
@@ -53,9 +53,9 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
   }
   const float n = 1.f / (float)g.gw;
   const Ring<W::kAll> ring(sums, g.stages);
-  Eight<S> s[VEC ? 1 : N];
-  Eight<A> dy[VEC ? 1 : N], z[kThird && !VEC ? N : 1];
-  Eight<H> dh[kAdd && !VEC ? N : 1];
+  Eight<S> s[kRing ? 1 : N];
+  Eight<A> dy[kRing ? 1 : N], z[kThird && !kRing ? N : 1];
+  Eight<H> dh[kAdd && !kRing ? N : 1];
   // a warp's first row, and this lane's among its rows
   const uint32_t rows = kNarrow ? 32 / g.lanes : 1, sub = kNarrow ? threadIdx.x / g.lanes : 0;
   const uint32_t step = gridDim.x * blockDim.y * rows, base0 = (blockIdx.x * blockDim.y + threadIdx.y) * rows;
@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
       const H* dhp = static_cast<const H*>(g.dh) + out;
 #pragma unroll
       for (int c = 0; c < N; ++c) {
-        if constexpr (VEC) {
+        if constexpr (kRing) {
           ring.copy(to, W::kS, sp, c, left);
           ring.copy(to, W::kDy, dyp, c, left);
           if constexpr (kThird) ring.copy(to, W::kZ, zp, c, left);
@@ -85,11 +85,11 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
         }
       }
     }
-    if constexpr (VEC) asm volatile("cp.async.commit_group;" ::: "memory");
+    if constexpr (kRing) asm volatile("cp.async.commit_group;" ::: "memory");
   };
   // chunk c of an array, from the ring or the registers; 0 past the row's end
   auto take = [&](auto& held, int first, int c, float (&o)[8]) {
-    if constexpr (VEC) {
+    if constexpr (kRing) {
       std::remove_reference_t<decltype(held[0])> e;
       ring.take(e, stage, first, c);
       e.floats(o);
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
       held[c].floats(o);
     }
   };
-  if constexpr (VEC) {
+  if constexpr (kRing) {
 #pragma unroll
     for (int c = 0; c < N; ++c) {
       ring.blank(g.stages, W::kS, (const S*)nullptr, c, left);
@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
     const bool live = !kNarrow || row < g.rows;
     const int64_t out = (int64_t)row * g.width + c0;
     const float r = live ? g.rstd[(int64_t)row * g.groups + blockIdx.y] : 0.f;
-    if constexpr (VEC) {
+    if constexpr (kRing) {
       __syncwarp();  // the row to be filled has been read
       fetch(row + (g.stages - 1) * step, stage ? stage - 1 : g.stages - 1);
       wait_copies(g.stages);
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
     }
     stage = stage + 1 == g.stages ? 0 : stage + 1;
   }
-  if constexpr (VEC) asm volatile("cp.async.wait_all;" ::: "memory");
+  if constexpr (kRing) asm volatile("cp.async.wait_all;" ::: "memory");
   if constexpr (kNarrow) {  // the warp's rows together
     for (uint32_t o = g.lanes; o < 32; o *= 2)
 #pragma unroll
@@ -280,24 +280,29 @@ __global__ void __launch_bounds__(1024) k_norm_sum(const float* part, uint32_t b
   if (threadIdx.x == 0 && blockIdx.x * 32 + threadIdx.y < width) out[blockIdx.x * 32 + threadIdx.y] = v;
 }
 
-bool words(const fhe_rms_norm_grad_args& a) {
+uint32_t together(const fhe_rms_norm_grad_args& a) {
   const fhe_rms_norm_args& f = a.f;
   const uint32_t ea = elem_size(f.dtype), eh = f.gate ? ea : elem_size(f.stream_dtype);
   const uint32_t ex = f.gate || f.residual ? ea : eh;
-  const bool x_read = !f.residual || f.channel_scale;
-  return f.width / f.groups % 8 == 0 && (!x_read || norm_aligned(f.x, f.x_stride, ex)) &&
-         (!f.residual || norm_aligned(f.h, 0, eh)) && norm_aligned(f.gate, f.gate_stride, ea) &&
-         norm_aligned(f.channel_scale, 0, 4) && norm_aligned(f.weight, 0, 4) && norm_aligned(a.dy, 0, ea) &&
-         norm_aligned(a.dh, 0, eh) && norm_aligned(a.dx, 0, ex) && norm_aligned(a.dresidual, 0, eh) &&
-         norm_aligned(a.dgate, 0, ea);
+  Together t(f.width / f.groups);
+  if (!f.residual || f.channel_scale) t.with(f.x, f.x_stride, ex);
+  if (f.residual) t.with(f.h, f.width, eh);
+  if (f.gate) t.with(f.gate, f.gate_stride, ea);
+  t.with(f.channel_scale, 0, 4);
+  t.with(f.weight, 0, 4);
+  t.with(a.dy, f.width, ea);
+  t.with(a.dh, f.width, eh);
+  t.with(a.dx, f.width, ex);
+  t.with(a.dresidual, f.width, eh);
+  t.with(a.dgate, f.width, ea);
+  return t.n;
 }
 
 // How a call is laid out: shape, rows of the ring, shared memory, and blocks that go
 // from row to row, as many as are resident.
 struct GradPlan {
   NormShape shape;
-  bool vec;
-  uint32_t stages, shared, blocks;
+  uint32_t together, stages, shared, blocks;
 };
 GradPlan grad_plan(const fhe_rms_norm_grad_args& a) {
   const fhe_rms_norm_args& f = a.f;
@@ -305,13 +310,13 @@ GradPlan grad_plan(const fhe_rms_norm_grad_args& a) {
   const uint32_t wa = elem_size(f.dtype) / 2, wh = f.gate ? wa : elem_size(f.stream_dtype) / 2;
   const uint32_t per_chunk = (f.gate ? wa : wh) + wa + (f.gate || f.channel_scale ? wa : 0) + (f.residual ? wh : 0);
   GradPlan p{};
-  p.vec = words(a);
-  for (;; p.vec = false) {
-    p.shape = norm_shape(gw, (uint64_t)f.rows * f.groups, p.vec, f.gate != nullptr);
+  p.together = together(a);
+  for (;; p.together = 2) {
+    p.shape = norm_shape(gw, (uint64_t)f.rows * f.groups, p.together, f.gate != nullptr);
     const uint32_t warps = p.shape.warps == 1 ? 4 : p.shape.warps;  // of a block
     uint32_t resident = std::max(1u, 16 / warps);
     p.shared = p.shape.warps == 1 ? gw * sizeof(float) : 0;  // one warp's channels, at most 1024
-    if (p.shape.layout(p.vec) == kWords) {
+    if (p.shape.layout(p.together) == kWords) {
       const uint32_t row = p.shape.chunks * per_chunk * 16 * 32 * warps;
       if (row + kBlockShared > kSmShared) continue;
       const RingPlan r = ring_plan(row, warps, 120 * 1024);
@@ -361,7 +366,7 @@ void rms_norm_backward(const fhe_rms_norm_grad_args& a) {
   const GradPlan p = grad_plan(a);
   g.stages = (int)p.stages;
   g.lanes = p.shape.lanes;
-  with_norm(f, p.shape.chunks, p.shape.layout(p.vec), [&](auto mode, auto act, auto str, auto chunks, auto layout) {
+  with_norm(f, p.shape.chunks, p.shape.layout(p.together), [&](auto mode, auto act, auto str, auto chunks, auto layout) {
     auto k = k_norm_grad<decltype(mode)::value, decltype(act), decltype(str), decltype(chunks)::value,
                          decltype(layout)::value>;
     if (p.shared > 48000) FHE_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.shared));

@@ -147,16 +147,21 @@ def test_gated_norm(ops, dtype, rows, width, groups):
 
 
 def test_strides_and_shapes(ops):
-    """Any leading axes, rows apart or not evenly apart, unaligned starts, broadcast inputs, no rows at all."""
+    """Any leading axes, rows apart or not evenly apart, unaligned starts, broadcast inputs, no rows at all.  How a row
+    is loaded decides the order of its sum of squares: results are held to the module's bound, not to equal bits."""
     w = 1 + normal(1, 768)
     base = normal(2, 4, 6, 900).bfloat16()
     for x in (base[..., :768], base[..., 3:771], base.transpose(0, 1)[..., :768], base[1, 2, :768], base[:, 2, 100:868],
               base[:1, :, :768].expand(5, 6, 768), base[:0, :, :768]):
-        assert torch.equal(ops.rms_norm(x, w), ops.rms_norm(x.contiguous(), w))
+        want, _ = norm_of(x.double(), w.double(), 1e-5)
+        close(ops.rms_norm(x, w), want, want.abs())
         y, h = ops.add_rms_norm(x.float(), x, w)
-        y2, h2 = ops.add_rms_norm(x.float().contiguous(), x.contiguous(), w)
-        assert torch.equal(y, y2) and torch.equal(h, h2) and h.shape == x.shape
-        assert torch.equal(ops.gated_rms_norm(x, x, w), ops.gated_rms_norm(x.contiguous(), x.contiguous(), w))
+        assert torch.equal(h, 2 * x.float())
+        want, _ = norm_of(h.double(), w.double(), 1e-5)
+        close(y, want, want.abs())
+        u = x.double() * x.double() * torch.sigmoid(x.double())
+        want, _ = norm_of(u, w.double(), 1e-5)
+        close(ops.gated_rms_norm(x, x, w), want, want.abs())
     one = base[:1, :1, :768].float().requires_grad_()
     y, h = ops.add_rms_norm(one.expand(4, 6, 768), base[..., :768], w)
     dy, dh = normal(3, 4, 6, 768).bfloat16(), normal(4, 4, 6, 768)
