@@ -8,10 +8,10 @@ import torch
 pytestmark = pytest.mark.gpu
 
 
-def build(vocab, **kw):
+def build(vocab, dtype=None):
     from fhe_mamba_b200.mamba2_layer import Mamba2Model
-    return Mamba2Model(**{**dict(layers=2, d_model=64, d_state=32, heads=4, vocab=vocab, std=0.2, calib_sequences=2,
-                                 calib_tokens=4, calib_prompt=2), **kw}).plain_sequences()
+    return Mamba2Model(layers=2, d_model=64, d_state=32, heads=4, vocab=vocab, std=0.2, calib_sequences=2, calib_tokens=4,
+                       calib_prompt=2).plain_sequences(dtype=dtype)
 
 
 @pytest.fixture(scope="module")
@@ -72,7 +72,10 @@ def test_scores_belong_to_the_texts(net, beams):
     assert (ending.lengths < 12).any()
 
 
-def test_one_beam_is_greedy(net):
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_one_beam_is_greedy(dtype):
+    """The same steps with the first of the largest logits, in every type of activations."""
+    net = build(211, dtype)
     prompt = torch.randint(0, 211, (4, 5), generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
     with torch.no_grad():
         out = net.beam_search(prompt, 1, 8)
