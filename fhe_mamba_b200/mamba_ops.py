@@ -808,6 +808,7 @@ def beam_reorder(states, parents):
                   f"{op}: states must be [batch * beams, ...] or [batch, beams, ...], got {tuple(t.shape)}")
             _need(t.is_contiguous(), f"{op}: states must be contiguous")
         _check_devices(op, parents, *states)
+    parents = _dense(parents)  # a broadcast one spans more than it holds
     at, sizes = [t.data_ptr() for t in states], [t.nbytes for t in states]
     end = 0
     for p, n in sorted(zip([*at, parents.data_ptr()], [*sizes, parents.nbytes])):
@@ -818,7 +819,7 @@ def beam_reorder(states, parents):
         _need(False, f"{op} has no gradient")
     if not rows:
         return
-    at, sizes, parents = array("Q", at), array("Q", [n // rows for n in sizes]), _dense(parents)
+    at, sizes = array("Q", at), array("Q", [n // rows for n in sizes])
     call("fhe_beam_reorder", _reorder_block(device, b, k, len(states), at.buffer_info()[0], sizes.buffer_info()[0],
                                             parents.data_ptr(), _stream_of(device)))
     increment_version(states)

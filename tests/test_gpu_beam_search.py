@@ -99,6 +99,13 @@ def test_refusals_and_small_calls(net):
     assert net.beam_search(prompt.cpu(), 2, 1).tokens.shape == (2, 2, 1)
 
 
+def test_rows_without_tokens(net):
+    """Rows of no tokens come out empty and leave the state as it was."""
+    hidden, state = net(torch.zeros(3, 0, dtype=torch.int64, device="cuda"))
+    assert hidden.shape == (3, 0, 64)
+    assert all(not w.any() and not s.any() for w, s in state)
+
+
 def test_training_pass_reaches_every_parameter(net):
     """Tied embedding included, padded rows with and without a token id in the padding."""
     tokens = torch.randint(0, 211, (2, 20), generator=torch.Generator(device="cuda").manual_seed(4), device="cuda")

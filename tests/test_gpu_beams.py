@@ -229,6 +229,17 @@ def test_reorder(ops, batch, beams):
     ops.beam_reorder([], shift)
 
 
+def test_reorder_broadcast_parents(ops):
+    """Parents that are one row for every item, and a state right behind that row in memory."""
+    flat = torch.zeros(4 + 400 * 4, dtype=torch.int64, device="cuda")
+    flat[:4] = torch.tensor([1, 1, 0, 3], device="cuda")
+    flat[4:] = torch.arange(400 * 4, device="cuda")
+    state = flat[4:].view(1600, 1)
+    ops.beam_reorder([state], flat[:4].expand(400, 4))
+    want = (torch.arange(400, device="cuda")[:, None] * 4 + flat[:4]).view(1600, 1)
+    assert torch.equal(state, want)
+
+
 def test_reorder_large_offsets(ops):
     """Rows past 2^32 bytes."""
     state = torch.zeros(6, (1 << 30) + 8, dtype=torch.uint8, device="cuda")
