@@ -567,11 +567,14 @@ void beam_select(const fhe_beam_select_args& a) {
   with_type(a.dtype, [&](auto t) {
     using T = decltype(t);
     // As many CTAs to an item as the device takes at once, a beam or a turn of loads for each;
-    // sixteen where eight would take several beams each (1 x 10 beams of 50280 bfloat16:
-    // 17 us, 23 with eight; 1 x 4: 11 us with either)
+    // as many as it takes in two rounds while a CTA has two beams (300 x 8 bfloat16 beams: 87
+    // us with four, 105 with one; but 128 x 4: 22 with four, 32 with eight); sixteen where
+    // eight would take several beams each (1 x 10 beams of 50280 bfloat16: 17 us, 23 with
+    // eight; 1 x 4: 11 us with either).
     const uint64_t packs = (uint64_t)a.beams * (a.vocab / Quad<T>::kElems);
     SelectArgs g{a, 1, std::min(a.width, a.vocab)};
-    while (g.cluster < (a.beams > 8 ? kMaxCluster : 8) && (uint64_t)a.batch * g.cluster * 2 <= 148 * 4 &&
+    while (g.cluster < (a.beams > 8 ? kMaxCluster : 8) &&
+           (uint64_t)a.batch * g.cluster * 2 <= (g.cluster * 4 <= a.beams ? 148 * 9 : 148 * 4) &&
            (g.cluster < a.beams || packs >= (uint64_t)g.cluster * 2 * kAhead * kThreads))
       g.cluster *= 2;
     const uint32_t shared = Layout(nullptr, a.beams + g.cluster, g.kk).bytes;
