@@ -181,7 +181,13 @@ def packer(block):
         return "".join(codes[t] if t in codes else fields(t) for _, t in b._fields_)
     s = struct.Struct("@" + fields(block))
     assert s.size == ctypes.sizeof(block)
-    return s.pack
+
+    def pack(*values):
+        try:
+            return s.pack(*values)
+        except struct.error as e:
+            raise ValueError(f"{block.__name__}: a size is out of range ({e})") from None
+    return pack
 
 
 # name -> (argtypes); all return int status.

@@ -208,3 +208,12 @@ def test_beam_c_refusals():
         a = _lib.BeamReorderArgs(**{**dict(batch=2, beams=3, count=1, states=one, row_bytes=size, parents=256), **kw})
         assert lib.fhe_beam_reorder(ctypes.byref(a)) == _lib.FHE_ERR_INVALID and message in _lib.last_error(), kw
     assert lib.fhe_beam_select(None) == lib.fhe_beam_reorder(None) == _lib.FHE_ERR_INVALID
+
+
+def test_sizes_past_their_fields():
+    pack = _lib.packer(_lib.RmsNormArgs)
+    fields = [0, 0, 0, 2, 8, 1, 1e-5, 1.0] + [0] * 12
+    assert pack(*fields) == bytes(_lib.RmsNormArgs(rows=2, width=8, groups=1, eps=1e-5, scale=1.0))
+    for place, value in ((3, 1 << 32), (4, -1), (0, 1 << 31)):
+        with pytest.raises(ValueError, match="RmsNormArgs: a size is out of range"):
+            pack(*fields[:place], value, *fields[place + 1:])
