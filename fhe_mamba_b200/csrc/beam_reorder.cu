@@ -135,8 +135,7 @@ void beam_reorder(const fhe_beam_reorder_args& a) {
   }
   DeviceGuard dev(a.device);
   const uint32_t shared = std::max(a.beams, kSlots) * kStep;
-  if (shared > 32768)
-    FHE_CUDA(cudaFuncSetAttribute(k_reorder, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
+  if (shared > 32768) allow_shared(k_reorder, kMaxBeams * kStep);
   // up to 16 steps to a block, fewer where that leaves places on the SMs empty
   uint64_t all = 0;
   for (uint32_t i = 0; i < a.count; ++i) all += (a.row_bytes[i] + kStep - 1) / kStep;

@@ -578,8 +578,7 @@ void beam_select(const fhe_beam_select_args& a) {
            (g.cluster < a.beams || packs >= (uint64_t)g.cluster * 2 * kAhead * kThreads))
       g.cluster *= 2;
     const uint32_t shared = Layout(nullptr, a.beams + g.cluster, g.kk).bytes;
-    if (shared > 32768)
-      FHE_CUDA(cudaFuncSetAttribute(k_select<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
+    if (shared > 32768) allow_shared(k_select<T>, Layout(nullptr, kMaxBeams + kMaxCluster, kMaxWidth).bytes);
     if (g.cluster > 8) FHE_CUDA(cudaFuncSetAttribute(k_select<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(a.batch * g.cluster);

@@ -100,6 +100,15 @@ struct alignas(sizeof(T) * N) Pack {
   T v[N];
 };
 
+// Lets a kernel have up to `bytes` of dynamic shared memory.  The limit is state of the
+// whole process and of every call of that kernel: `bytes` is the most that any launch of
+// it asks for, never the size of one launch, so that calls from other threads, of other
+// sizes, do not take it from this one.
+template <class K>
+void allow_shared(K kernel, uint32_t bytes) {
+  FHE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+}
+
 // Two fp32 operations per instruction (sm_100): elementwise over arrays of V,
 // pairs packed when V is even.
 __device__ __forceinline__ uint64_t pair(float a, float b) {

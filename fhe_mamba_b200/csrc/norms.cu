@@ -234,7 +234,7 @@ void rms_norm(const fhe_rms_norm_args& a) {
                                    std::max(1u, 148 * resident / a.groups));
   with_norm(a, s.chunks, s.layout(t.n), [&](auto mode, auto act, auto str, auto chunks, auto layout) {
     auto k = k_norm<decltype(mode)::value, decltype(act), decltype(str), decltype(chunks)::value, decltype(layout)::value>;
-    if (shared > 48000) FHE_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
+    if (shared > 48000) allow_shared(k, kSmShared - kBlockShared);
     const dim3 block(32 * s.warps, s.warps == 1 ? 4 : 1);
     k<<<dim3(blocks, a.groups), block, shared, static_cast<cudaStream_t>(a.stream)>>>(g);
   });

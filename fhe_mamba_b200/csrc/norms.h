@@ -259,7 +259,7 @@ inline NormShape norm_shape(uint32_t gw, uint64_t rows, uint32_t together, bool 
   return s;
 }
 
-constexpr uint32_t kSmShared = 227 * 1024, kBlockShared = 1024 + 256;  // of an SM; of a block beside its ring
+constexpr uint32_t kSmShared = 227 * 1024, kBlockShared = 1024 + 256;  // of an SM; of a block beside its ring, which has the rest at most
 
 // Rows in the ring and blocks an SM for blocks of `warps` warps whose row takes `row`
 // bytes: two rows, and as many blocks as bring the rings to about `target` bytes but 8

@@ -369,7 +369,7 @@ void rms_norm_backward(const fhe_rms_norm_grad_args& a) {
   with_norm(f, p.shape.chunks, p.shape.layout(p.together), [&](auto mode, auto act, auto str, auto chunks, auto layout) {
     auto k = k_norm_grad<decltype(mode)::value, decltype(act), decltype(str), decltype(chunks)::value,
                          decltype(layout)::value>;
-    if (p.shared > 48000) FHE_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.shared));
+    if (p.shared > 48000) allow_shared(k, kSmShared - kBlockShared);
     const dim3 block(32 * p.shape.warps, p.shape.warps == 1 ? 4 : 1);
     k<<<dim3(p.blocks, f.groups), block, p.shared, st>>>(g);
   });
