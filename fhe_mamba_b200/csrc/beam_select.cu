@@ -360,11 +360,12 @@ __global__ void __launch_bounds__(kThreads) k_select(const SelectArgs g) {
     // sums of the live beams
     if (tid < lives) {
       float m = -INFINITY;
-      uint32_t raises = 0;
+      uint32_t raises = 0, most = 0;
       bool bad = false;
       const Share* s = l.share + tid * parts;
       for (uint32_t p = 0; p < parts; ++p) {
         m = fmaxf(m, s[p].m);
+        if (s[p].count) most = max(most, l.key[(tid * parts + p) * kk]);
         raises = max(raises, s[p].raises);
         bad = bad || !isfinite(s[p].s);
       }
@@ -377,7 +378,7 @@ __global__ void __launch_bounds__(kThreads) k_select(const SelectArgs g) {
       const uint32_t i = live[tid];
       const bool fine = !bad && isfinite(m) && sum > 0.;
       lse[i] = fine ? (double)m + log(sum) : -INFINITY;
-      top[i] = m;
+      top[i] = key_value(most);  // the row's largest: a shift that, unlike m, is the same at any alignment
       // Roundings of u = 2^-24: three of an exponent d = (z - m) log2 e, whose mean over
       // the sum is at most log2(vocab / sum) and twice the slack, the exponential's four,
       // at most 17 additions, 6 for moving the threads' sums to one shift; 8 u for each
@@ -501,7 +502,8 @@ __global__ void __launch_bounds__(kThreads) k_select(const SelectArgs g) {
     meet();
     const uint64_t todo = agreed;
     if (todo == 0) break;
-    // those beams' sums in 64 bits, in an order that does not hang on alignment: equal rows give equal sums
+    // those beams' sums in 64 bits, from a shift and in an order that do not hang on alignment: equal rows
+    // give equal sums
     for (uint32_t i = 0; i < B; ++i) {
       if (!(todo >> i & 1)) continue;
       const T* z = row_of(i);
