@@ -37,6 +37,13 @@ constexpr int kCap = 1024;    // candidates held
 constexpr uint32_t kMaxBeams = 64, kMaxWidth = 64, kMaxCluster = 16;
 static_assert(kMaxWidth <= kGroups, "the bound is the width-th of the groups' maxima");
 
+// What a row's logits and its log sum exp are counted from.  Rows below zero are counted
+// from their largest: where the mask leaves nothing but numbers like -1e30 or the type's
+// lowest, score and log of the sum would be lost beside them and the total come out as 0,
+// the best of all.  Others from 0: logits past 2^30 are no mask, and their totals are
+// good to 2^-52 of them.
+__device__ __forceinline__ double origin(double largest) { return fmin(largest, 0.); }
+
 // One share of a row: sum of exp(z - m), and its best entries in order.
 struct Share {
   double s;
@@ -377,8 +384,8 @@ __global__ void __launch_bounds__(kThreads) k_select(const SelectArgs g) {
       }
       const uint32_t i = live[tid];
       const bool fine = !bad && isfinite(m) && sum > 0.;
-      lse[i] = fine ? (double)m + log(sum) : -INFINITY;
       top[i] = key_value(most);  // the row's largest: a shift that, unlike m, is the same at any alignment
+      lse[i] = fine ? (double)m - origin(top[i]) + log(sum) : -INFINITY;
       // Roundings of u = 2^-24: three of an exponent d = (z - m) log2 e, whose mean over
       // the sum is at most log2(vocab / sum) and twice the slack, the exponential's four,
       // at most 17 additions, 6 for moving the threads' sums to one shift; 8 u for each
@@ -409,7 +416,7 @@ __global__ void __launch_bounds__(kThreads) k_select(const SelectArgs g) {
         const uint32_t u = c / kk, j = c % kk, i = lbeam[u];
         if (j >= lcount[u]) continue;
         if (isfinite(lse[i])) {
-          l.total[c] = (double)score[i] + (double)key_value(l.key[c]) - lse[i];
+          l.total[c] = (double)score[i] + ((double)key_value(l.key[c]) - origin(top[i])) - lse[i];
         } else {
           // a finished beam: its end, then the impossible tokens; others impossible alone
           const bool end = ended[i] && isfinite(score[i]);
@@ -517,7 +524,7 @@ __global__ void __launch_bounds__(kThreads) k_select(const SelectArgs g) {
     if (rank == 0 && tid < B && (todo >> tid & 1)) {
       double s = 0.;
       for (uint32_t r = 0; r < C; ++r) s += of(again, r)[tid];
-      lse[tid] = top[tid] + log(s);
+      lse[tid] = top[tid] - origin(top[tid]) + log(s);
       err[tid] = 0.;
     }
     __syncthreads();

@@ -745,7 +745,8 @@ int fhe_embedding_backward(const fhe_embedding_grad_args* args);
  *   total(i, v) = scores[i] + logits[i][v] - log sum exp(logits[i])
  * over its beams i and the tokens v, best first; equal totals by the lower beam
  * and then the lower token.  The choice is that of the totals in 64 bits (within a
- * beam that of the logits).  A finished beam has one candidate, the token eos at
+ * beam that of the logits), good to 2^-52 of the row's largest logit where that is
+ * positive; a row of large negative numbers alone has the totals of the formula.  A finished beam has one candidate, the token eos at
  * scores[i].  Beams whose score is not finite, or whose logits hold a NaN or
  * +inf or nothing but -inf, have no possible token; impossible candidates (-inf
  * logits too) have score -inf and are taken last.  With keep_slots (width ==
