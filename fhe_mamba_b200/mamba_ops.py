@@ -10,6 +10,7 @@ include/fhe_b200.h), on the current stream of the tensors' device, and can be
 captured into CUDA graphs; all but the steps and the beams have
 gradients (to capture a backward pass, hold no eager autograd graph of the same
 leaves: torch would make the capture wait for that graph's stream, and refuses).
+Second and forward-mode derivatives are refused.
 Activations are float32, bfloat16 or float16; gates, states, norm weights and
 scores are float32.  Arguments that do not fit raise ValueError before any GPU
 work.
@@ -21,6 +22,7 @@ from array import array
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
@@ -70,6 +72,11 @@ _stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
 
 
 def _wants_grad(*tensors):
+    """Whether a backward pass may ask for gradients of these.  Tensors with a forward-mode derivative are refused:
+    the outputs would have none."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # outside a dual level no tensor has one
+        _need(all(t is None or forward_ad.unpack_dual(t).tangent is None for t in tensors),
+              "the operators have no forward-mode derivatives")
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
@@ -815,7 +822,7 @@ def beam_reorder(states, parents):
         if p < end and n:
             _need(False, f"{op}: states share memory")
         end = p + n if n else end
-    if torch.is_grad_enabled() and any([t.requires_grad for t in states]):
+    if _wants_grad(*states):
         _need(False, f"{op} has no gradient")
     if not rows:
         return
