@@ -28,7 +28,9 @@ class BeamTexts(NamedTuple):
 class PlainMamba2(torch.nn.Module):
     """`model`'s layers as parameters in `dtype` (activations and matrices; the
     norms, gates and states stay float32) on `device`.  The embedding is tied:
-    it also gives the logits."""
+    it also gives the logits.  A negative input token counts from the
+    vocabulary's end; past the vocabulary NaN comes out, before it the
+    embedding is 0."""
 
     GATES = ("norm_w", "gn_w", "dt_bias", "a", "d")  # float32 whatever the dtype
 
@@ -69,7 +71,9 @@ class PlainMamba2(torch.nn.Module):
         return ops.gated_rms_norm(y.flatten(-2), z, p["gn_w"], W.eps) @ p["w_out"].T
 
     def _embed(self, tokens):
-        return ops.embedding(tokens.to(self.embedding.device), self.embedding, dtype=torch.float32)
+        tokens = tokens.to(self.embedding.device)
+        tokens = torch.add(tokens, tokens < 0, alpha=self.embedding.shape[0])  # an index from the end, as any tensor's
+        return ops.embedding(tokens, self.embedding, dtype=torch.float32)
 
     def forward(self, tokens, state=None, lengths=None):
         """The normalised final hidden vectors [batch, length, d_model] of the
