@@ -19,6 +19,17 @@ from . import mamba_ops as ops
 from .mamba_ops import TokenLogprobs
 
 
+def _operators_take(weight, eps):
+    """Whether the norm operators take rows of this width with this eps."""
+    f = torch.finfo(torch.float32)
+    return weight.shape[0] <= ops.MAX_NORM_WIDTH and f.tiny <= eps <= f.max
+
+
+def _rms(x, weight, eps):
+    """The norm of float32 rows that the operators do not take."""
+    return x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps) * weight
+
+
 class BeamTexts(NamedTuple):
     tokens: torch.Tensor   # [batch, beams, length] int64, best first; `eos` behind an end
     scores: torch.Tensor   # [batch, beams] float32, sums of log-probabilities
@@ -53,7 +64,10 @@ class PlainMamba2(torch.nn.Module):
                  torch.zeros(batch, W.heads, W.head_dim, W.d_state, device=d)) for W in self.weights]
 
     def _norm(self, h, branch, weight, eps):
-        """The residual stream with the last layer's output added (None: as it is), and its norm."""
+        """The norm of the residual stream with the last layer's output added (None: as it is), and that stream."""
+        if not _operators_take(weight, eps):
+            h = h if branch is None else h + branch.float()
+            return _rms(h, weight, eps).to(self.dtype), h
         if branch is None:
             return ops.rms_norm(h, weight, eps, self.dtype), h
         return ops.add_rms_norm(h, branch, weight, eps)
@@ -68,7 +82,10 @@ class PlainMamba2(torch.nn.Module):
         return x.unflatten(-1, (W.heads, W.head_dim)), B.unsqueeze(-2), C.unsqueeze(-2)
 
     def _finish(self, W, p, y, z):
-        return ops.gated_rms_norm(y.flatten(-2), z, p["gn_w"], W.eps) @ p["w_out"].T
+        y, w = y.flatten(-2), p["gn_w"]
+        if _operators_take(w, W.eps):
+            return ops.gated_rms_norm(y, z, w, W.eps) @ p["w_out"].T
+        return _rms(y.float() * torch.nn.functional.silu(z.float()), w, W.eps).to(self.dtype) @ p["w_out"].T
 
     def _embed(self, tokens):
         tokens = tokens.to(self.embedding.device)
