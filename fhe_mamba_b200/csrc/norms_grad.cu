@@ -304,13 +304,13 @@ struct GradPlan {
   NormShape shape;
   uint32_t together, stages, shared, blocks;
 };
-GradPlan grad_plan(const fhe_rms_norm_grad_args& a) {
+GradPlan grad_plan(const fhe_rms_norm_grad_args& a, uint32_t together) {
   const fhe_rms_norm_args& f = a.f;
   const uint32_t gw = f.width / f.groups;
   const uint32_t wa = elem_size(f.dtype) / 2, wh = f.gate ? wa : elem_size(f.stream_dtype) / 2;
   const uint32_t per_chunk = (f.gate ? wa : wh) + wa + (f.gate || f.channel_scale ? wa : 0) + (f.residual ? wh : 0);
   GradPlan p{};
-  p.together = together(a);
+  p.together = together;
   for (;; p.together = 2) {
     p.shape = norm_shape(gw, (uint64_t)f.rows * f.groups, p.together, f.gate != nullptr);
     const uint32_t warps = p.shape.warps == 1 ? 4 : p.shape.warps;  // of a block
@@ -337,7 +337,12 @@ bool sums_wanted(const fhe_rms_norm_grad_args& a) { return a.dweight || a.dchann
 uint64_t rms_norm_backward_workspace(const fhe_rms_norm_grad_args& a) {
   check_norm(a.f);
   if (!sums_wanted(a)) return 0;
-  return (uint64_t)grad_plan(a).blocks * a.f.width * sizeof(float) * (a.f.channel_scale ? 2 : 1);
+  // enough for these sizes wherever the arrays lie: the workspace may be asked for before they exist
+  const uint32_t most = Together(a.f.width / a.f.groups).n;
+  uint32_t blocks = 0;
+  for (uint32_t n : {1u, 2u, 8u})
+    if (n <= most) blocks = std::max(blocks, grad_plan(a, n).blocks);
+  return (uint64_t)blocks * a.f.width * sizeof(float) * (a.f.channel_scale ? 2 : 1);
 }
 
 void rms_norm_backward(const fhe_rms_norm_grad_args& a) {
@@ -363,7 +368,7 @@ void rms_norm_backward(const fhe_rms_norm_grad_args& a) {
   g.dres = a.dresidual;
   g.dgate = a.dgate;
   g.part = sums_wanted(a) ? static_cast<float*>(a.workspace) : nullptr;
-  const GradPlan p = grad_plan(a);
+  const GradPlan p = grad_plan(a, together(a));
   g.stages = (int)p.stages;
   g.lanes = p.shape.lanes;
   with_norm(f, p.shape.chunks, p.shape.layout(p.together), [&](auto mode, auto act, auto str, auto chunks, auto layout) {

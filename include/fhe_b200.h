@@ -692,7 +692,9 @@ int fhe_rms_norm(const fhe_rms_norm_args* args);
 
 /* Gradients of fhe_rms_norm.  `f` holds the forward call's inputs with its h
  * (only with a residual) and rstd as inputs; its y is not used.  Every output
- * may be NULL where it is not wanted; sums over rows run in a fixed order. */
+ * may be NULL where it is not wanted; sums over rows run in a fixed order.  The
+ * workspace hangs on the sizes, the types and which pointers are NULL, not on
+ * where the others point (0 bytes without dweight and dchannel_scale). */
 typedef struct fhe_rms_norm_grad_args {
   fhe_rms_norm_args f;
   const void* dy;             /* [rows][width], dtype, contiguous */
