@@ -193,10 +193,10 @@ __device__ __forceinline__ Pack<T, V> pack(const float (&o)[V]) {
   return p;
 }
 
-// 1 / (1 + exp(-v)) with the special-function exponential and reciprocal: a
-// few units in the last place of fp32 (0 from v = -87.3 down, where it is below
-// 2^-126), at a quarter of the instructions of expf and a division, which would
-// bound the 16-bit forms.
+// 1 / (1 + exp(-v)) with the special-function exponential and reciprocal: off by
+// (6 + 3 |v|) 2^-24 relative to itself, since v log2 e is rounded before the
+// exponential (0 from v = -87.3 down, where it is below 2^-126), at a quarter of
+// the instructions of expf and a division, which would bound the 16-bit forms.
 template <int V>
 __device__ __forceinline__ void sigmoid(float (&o)[V], const float (&v)[V]) {
   float k[V], one[V];

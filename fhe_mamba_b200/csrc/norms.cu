@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(512) k_norm(const NormArgs g) {
       if constexpr (MODE == kNormGate) {
         float q[8], zf[8];
         f[c].floats(zf);
-        sigmoid(q, zf);
+        gate_sigmoid<A>(q, zf);
         vmul(q, q, zf);
         vmul(h[c], h[c], q);
       } else if constexpr (kTwo) {

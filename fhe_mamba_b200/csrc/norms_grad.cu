@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(N == 3 ? 256 : 512) k_norm_grad(const NormArgs
       if constexpr (MODE == kNormGate) {
         float zf[8];
         take(z, W::kZ, c, zf);
-        if (first) sigmoid(q[c], zf);
+        if (first) gate_sigmoid<A>(q[c], zf);
         vmul(p, q[c], zf);
         vmul(u, xf, p);
         vmul(u, u, rr);
