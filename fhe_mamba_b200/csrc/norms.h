@@ -198,8 +198,9 @@ struct Ring {
 // behind a 16-bit gate's own rounding.  float32 gates keep 8 2^-24 whatever v is: 2^d for
 // the rounded d = -v log2 e is off by the factor e^(-v - d ln 2), 1 + its exponent here
 // (5000 x 1536 float32 from memory: 18.2 us, 17.6 without; from the second cache 18.5,
-// 16.5, and 28 with expf and a rounded reciprocal).  Exponents are kept where all of that is finite; below -88.5 the reciprocal is 0 as
-// without, and an infinite or NaN v comes back with the product that SiLU is.
+// 16.5, and 28 with expf and a rounded reciprocal).  Exponents are kept where all of that
+// is finite; below -88.5 the reciprocal is 0 as without, and an infinite or NaN v comes
+// back with the product that SiLU is.
 template <class A, int V>
 __device__ __forceinline__ void gate_sigmoid(float (&o)[V], const float (&v)[V]) {
   if constexpr (sizeof(A) == 4) {

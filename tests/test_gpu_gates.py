@@ -73,3 +73,55 @@ def test_float32_gates_keep_their_bits(ops, rows, width, groups):
     v = x.double() * z.double() * torch.sigmoid(z.double())
     want = v * torch.rsqrt(mean_of(v.square(), groups) + 1e-4) * w.double()
     close(y, want, want.abs(), 46, "y")
+
+
+# the row or group that holds an infinity or a NaN, by layout: words, their groups, pairs, single elements, narrow rows
+PLACES = [(8, 1536, 1), (9, 1536, 8), (5, 1002, 1), (5, 1001, 1), (7, 104, 1), (9, 39, 3), (40, 8, 1)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows, width, groups", PLACES)
+def test_infinities_and_nan_stay_in_their_group(ops, dtype, rows, width, groups):
+    x, w = normal(1, rows, width).to(dtype), 1 + 0.1 * normal(3, width)
+    z, dy = normal(2, rows, width).to(dtype), normal(4, rows, width).to(dtype)
+    x[x == 0] = 1
+    z[z == 0] = 1
+
+    def run(x, z):
+        x, z = x.clone().requires_grad_(), z.clone().requires_grad_()
+        y = ops.gated_rms_norm(x, z, w, 1e-4, groups)
+        return [y.detach(), *torch.autograd.grad(y, (x, z), dy)]
+    fine = run(x, z)
+    each, at = width // groups, (rows // 2, width - 2 - width // 3)
+    mine = torch.zeros(rows, width, dtype=torch.bool, device="cuda")
+    mine[at[0], at[1] // each * each:(at[1] // each + 1) * each] = True
+    here = torch.zeros_like(mine)
+    here[at] = True
+    inf, nan = float("inf"), float("nan")
+    for where, value in (("z", inf), ("z", -inf), ("z", nan), ("x", inf), ("x", nan)):
+        a, b = x.clone(), z.clone()
+        (a if where == "x" else b)[at] = value
+        got = run(a, b)
+        for g, f in zip(got, fine):
+            assert torch.equal(g[~mine], f[~mine]), (where, value)
+        assert torch.isnan(got[0][at])
+        if value == inf:  # SiLU(-inf) and NaN leave nothing of the group, an infinity divides it to 0
+            assert (got[0][mine & ~here] == 0).all()
+        else:
+            assert torch.isnan(got[0][mine]).all()
+
+
+@pytest.mark.parametrize("rows, width, groups", [(5, 1536, 1), (300, 1536, 8), (5, 1001, 1), (70, 104, 1), (31, 39, 3), (600, 8, 1),
+                                                 (1000, 1, 1)])
+def test_squares_past_float32(ops, rows, width, groups):
+    """Some rows of products whose squares pass float32, among rows of ordinary ones: with and without a gate."""
+    x, z, w = normal(1, rows, width), (3 * normal(2, rows, width)).clamp(-9, 9), 1 + 0.1 * normal(3, width)
+    x[::3] *= 1e25
+    x[1::5] *= 1e-3
+    y = ops.gated_rms_norm(x, z, w, 1e-4, groups)
+    v = x.double() * z.double() * torch.sigmoid(z.double())
+    want = v * torch.rsqrt(mean_of(v.square(), groups) + 1e-4) * w.double()
+    close(y, want, want.abs(), K + 8, "gate")  # the scaled root: 8 u more
+    y = ops.rms_norm(x, w)
+    want = x.double() * torch.rsqrt(x.double().square().mean(-1, keepdim=True) + 1e-5) * w.double()
+    close(y, want, want.abs(), K + 8, "plain")
