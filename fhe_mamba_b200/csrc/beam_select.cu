@@ -15,7 +15,10 @@
 // 64 items of 8 bfloat16 beams of 50304, 15% of them finished: 24 us.  The reads come at
 // 5.8 TB/s (7.5 us, all 512 CTAs at once); then bound, candidates and ranks of each share
 // (2.7 us), the meeting, and the ranking of the item's entries while others still read.
-// One item of 4 float32 beams: 10.5 us, of which the reads 3.4.
+// One item of 4 float32 beams: 10.5 us, of which the reads 3.4.  Rows in which fewer
+// groups of threads hold a possible token than are wanted (a mask that leaves one to five
+// tokens, or thirty neighbours; rows of one value alike) have no bound above the
+// impossible ones and read their share again for each rank: 490 us and 68 us.
 #include <algorithm>
 #include <cfloat>
 #include <cooperative_groups.h>
@@ -576,8 +579,10 @@ void beam_select(const fhe_beam_select_args& a) {
   with_type(a.dtype, [&](auto t) {
     using T = decltype(t);
     // As many CTAs to an item as the device takes at once, a beam or a turn of loads for each;
-    // as many as it takes in two rounds while a CTA has two beams (300 x 8 bfloat16 beams: 87
-    // us with four, 105 with one; but 128 x 4: 22 with four, 32 with eight); sixteen where
+    // nine an SM while a CTA has two beams, up to where one round of larger shares takes as
+    // long as those and their last, part-filled round (300 x 8 bfloat16 beams: 87 us with four,
+    // 105 with one; 333 x 8: 87 with four, 94 with two; but 360 x 8 float32: 141 with four, 112
+    // with two, and 128 x 4 bfloat16: 22 with four, 32 with eight); sixteen where
     // eight would take several beams each (1 x 10 beams of 50280 bfloat16: 17 us, 23 with
     // eight; 1 x 4: 11 us with either).
     const uint64_t packs = (uint64_t)a.beams * (a.vocab / Quad<T>::kElems);

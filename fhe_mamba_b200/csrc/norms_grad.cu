@@ -4,9 +4,14 @@
 // itself has), dweight = sum over rows of dy u.  Like the norm, a row is spread
 // over one to sixteen warps and read once.  Its words come by asynchronous copies
 // through each thread's own part of shared memory, rows ahead, and are taken from
-// there twice, for the mean and for the gradients; single elements are held in
-// registers.  A block keeps its share of the sums over rows in registers from row
-// to row, and a second launch (4 to 6 us) adds the blocks' shares in a fixed order.
+// there twice, for the mean and for the gradients; pairs and single elements are held
+// in registers.  Two chunks of them fit; groups of more than 8192 channels that are not
+// loaded as words, or whose row is too large for the ring (float32 with a factor for each
+// of 16384 channels), take four, much of which the compiler spills to local memory (norm
+// and gradients of 2000 x 12290 bfloat16 on float32: 0.38 ms, of 2000 x 16384 float32
+// with factors 0.81 ms, a quarter of a copy's rate).  A block keeps its share of the sums
+// over rows in registers from row to row, and a second launch (4 to 6 us) adds the
+// blocks' shares in a fixed order.
 // 32768 rows of 768, bfloat16 and a float32 stream: 70 us, 5.8 TB/s; 32768 x 1536
 // bfloat16 with a gate: 81 us, 6.2 TB/s.
 #include "launch_count.h"
